@@ -118,6 +118,60 @@ class AdamArgs(C.Structure):
     ]
 
 
+F32, BF16, F16 = 0, 1, 2
+MOMENT_BLOCK = 128
+ADAMW_MAX_GROUPS = 1024
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("param", C.c_void_p), ("grad", C.c_void_p), ("copy", C.c_void_p),
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("block_scale", C.c_void_p),
+        ("n", C.c_int64), ("first_number", C.c_int64),
+        ("param_type", C.c_int32), ("grad_type", C.c_int32), ("copy_type", C.c_int32), ("group", C.c_int32),
+    ]
+
+
+class AdamWGroup(C.Structure):
+    _fields_ = [("lr", C.c_double), ("weight_decay", C.c_double), ("step", C.c_int64)]
+
+
+class AdamWDeviceState(C.Structure):
+    _fields_ = [("step", C.c_int64), ("lr_factor", C.c_float), ("reserved", C.c_float)]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [
+        ("tensors", C.POINTER(AdamWTensor)), ("groups", C.POINTER(AdamWGroup)),
+        ("num_tensors", C.c_int32), ("num_groups", C.c_int32),
+        ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+        ("moment_bits", C.c_int32), ("stochastic_rounding", C.c_int32),
+        ("seed", C.c_uint64),
+        ("zero_grad", C.c_int32), ("reserved", C.c_int32),
+        ("grad_scale", C.c_void_p), ("device_state", C.c_void_p),
+    ]
+
+
+class Gradient(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("n", C.c_int64), ("type", C.c_int32), ("reserved", C.c_int32)]
+
+
+class GradientNormArgs(C.Structure):
+    _fields_ = [
+        ("gradients", C.POINTER(Gradient)), ("num_gradients", C.c_int32), ("reserved", C.c_int32),
+        ("max_norm", C.c_double), ("scale", C.c_double),
+        ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class MomentTensor(C.Structure):
+    _fields_ = [
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+        ("exp_avg_code", C.c_void_p), ("exp_avg_sq_code", C.c_void_p), ("block_scale", C.c_void_p),
+        ("n", C.c_int64),
+    ]
+
+
 class PackArgs(C.Structure):
     _fields_ = [
         ("num_points", C.c_int32),
@@ -204,6 +258,12 @@ SYMBOLS = {
     "vetrast_packed_descriptor_bytes": (C.c_size_t, [C.c_int32]),
     "vetrast_pack_descriptors": (C.c_int, [C.c_void_p, C.POINTER(PackArgs), C.c_void_p]),
     "vetrast_adam_step": (C.c_int, [C.c_void_p, C.POINTER(AdamArgs), C.c_void_p]),
+    "vetrast_adamw_device_state_bytes": (C.c_size_t, [C.c_int32]),
+    "vetrast_adamw_step": (C.c_int, [C.c_void_p, C.POINTER(AdamWArgs), C.c_void_p]),
+    "vetrast_gradient_norm_workspace_bytes": (C.c_size_t, [C.POINTER(Gradient), C.c_int32]),
+    "vetrast_gradient_norm": (C.c_int, [C.c_void_p, C.POINTER(GradientNormArgs), C.c_void_p]),
+    "vetrast_pack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentTensor), C.c_int32, C.c_void_p]),
+    "vetrast_unpack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentTensor), C.c_int32, C.c_void_p]),
     "vetrast_lift_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "vetrast_lift_workspace_bytes_for_image": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     "vetrast_lift_error": (C.c_int, [C.c_void_p, C.POINTER(LiftArgs), C.c_void_p]),

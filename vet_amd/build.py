@@ -56,7 +56,7 @@ def build_torch_extension(verbose=True):
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for i in inc + ["/opt/rocm/include", sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", i]
-    cmd += [os.path.join(HERE, "torch_ext", "point_render.cpp"), "-o", TORCH_EXT_PATH,
+    cmd += [os.path.join(HERE, "torch_ext", "point_render.cpp"), os.path.join(HERE, "torch_ext", "adamw.cpp"), "-o", TORCH_EXT_PATH,
             f"-L{torch_lib}", f"-L{LIB_DIR}", "-lvetrast", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
             "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     if verbose:

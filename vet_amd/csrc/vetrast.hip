@@ -18,6 +18,7 @@
 #include "build_kernels.h"
 #include "backward_kernels.h"
 #include "lift_kernels.h"
+#include "optim_kernels.h"
 #include "region_rule.h"
 
 using namespace vetrast;
@@ -472,6 +473,15 @@ void launch_lift(const vetrast_lift_args* a, char* ws, size_t num_sums, hipStrea
     } while (y < bottom);
     hipLaunchKernelGGL(lift_plain_kernel, dim3(kLiftPlainShare, kLiftPlainAtOnce), dim3(kBlock), 0, stream, lp);
 }
+
+// Lists of tensors (optim_kernels.h)
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
+inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
+constexpr int64_t kOptimEntryElements = 1 << 30;  // a longer tensor is several entries of a launch: places inside one are 32 bits
+constexpr uint32_t kOptimGrid         = 2048;     // workgroups of a launch at most, each goes through its share of chunks
+constexpr uint32_t kNormGrid          = 1024;
+static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 
 }  // namespace
 
@@ -1314,6 +1324,243 @@ int vetrast_adam_step(vetrast_ctx* ctx, const vetrast_adam_args* a, void* stream
                        a->zero_grad);
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
+}
+
+size_t vetrast_adamw_device_state_bytes(int32_t num_groups)
+{
+    if (num_groups < 0 || num_groups > VETRAST_ADAMW_MAX_GROUPS) return 0;
+    return sizeof(vetrast_adamw_device_state) + (size_t)num_groups * sizeof(AdamWGroup);
+}
+
+int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stream_)
+{
+    if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
+    if (a->num_tensors < 0 || a->num_groups < 0 || a->num_groups > VETRAST_ADAMW_MAX_GROUPS) return VETRAST_ERR_INVALID_ARG;
+    if (a->moment_bits != 32 && a->moment_bits != 8) return VETRAST_ERR_INVALID_ARG;
+    if (!(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0)) return VETRAST_ERR_INVALID_ARG;
+    if (!((float)a->eps > 0.f) || !std::isfinite((float)a->eps)) return VETRAST_ERR_INVALID_ARG;  // a second moment of zero divides by it
+    if ((a->num_tensors > 0 && !a->tensors) || (a->num_groups > 0 && !a->groups)) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->grad_scale, 4) || !aligned_to(a->device_state, 16)) return VETRAST_ERR_INVALID_ARG;
+    for (int k = 0; k < a->num_groups; ++k)
+    {
+        const vetrast_adamw_group& g = a->groups[k];
+        if (!std::isfinite(g.lr) || !std::isfinite(g.weight_decay)) return VETRAST_ERR_INVALID_ARG;
+        if (!a->device_state && g.step < 1) return VETRAST_ERR_INVALID_ARG;
+    }
+    for (int k = 0; k < a->num_tensors; ++k)
+    {
+        const vetrast_adamw_tensor& t = a->tensors[k];
+        if (t.n < 0 || t.group < 0 || t.group >= a->num_groups) return VETRAST_ERR_INVALID_ARG;
+        if (!is_dtype(t.param_type) || !is_dtype(t.grad_type)) return VETRAST_ERR_INVALID_ARG;
+        if (t.first_number < 0 || t.first_number % kMomentBlock != 0) return VETRAST_ERR_INVALID_ARG;
+        if (t.n == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return VETRAST_ERR_INVALID_ARG;
+        if (!aligned_to(t.param, dtype_bytes(t.param_type)) || !aligned_to(t.grad, dtype_bytes(t.grad_type))) return VETRAST_ERR_INVALID_ARG;
+        if (t.copy && (t.param_type != VETRAST_F32 || (t.copy_type != VETRAST_BF16 && t.copy_type != VETRAST_F16) || !aligned_to(t.copy, 2)))
+            return VETRAST_ERR_INVALID_ARG;
+        const size_t moment_alignment = a->moment_bits == 8 ? 8 : 4;
+        if (!aligned_to(t.exp_avg, moment_alignment) || !aligned_to(t.exp_avg_sq, moment_alignment)) return VETRAST_ERR_INVALID_ARG;
+        if (a->moment_bits == 8 && (!t.block_scale || !aligned_to(t.block_scale, 2))) return VETRAST_ERR_INVALID_ARG;
+    }
+    hipStream_t stream = (hipStream_t)stream_;
+    AdamWDevice* device = static_cast<AdamWDevice*>(a->device_state);
+    if (device)
+    {
+        AdamWBegin b;
+        b.device     = device;
+        b.grad_scale = a->grad_scale;
+        b.beta1      = a->beta1;
+        b.beta2      = a->beta2;
+        b.seed       = a->seed;
+        for (b.first = 0, b.last = 0; !b.last; b.first += kBeginGroups)
+        {
+            b.groups = std::min(a->num_groups - b.first, kBeginGroups);
+            b.last   = b.first + b.groups == a->num_groups;
+            for (int k = 0; k < b.groups; ++k) b.g[k] = {a->groups[b.first + k].lr, a->groups[b.first + k].weight_decay};
+            hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(kBeginGroups), 0, stream, b);
+        }
+    }
+    AdamWLaunch l;
+    l.grad_scale      = a->grad_scale;
+    l.device          = device;
+    l.beta1           = (float)a->beta1;
+    l.one_minus_beta1 = (float)(1.0 - a->beta1);
+    l.beta2           = (float)a->beta2;
+    l.one_minus_beta2 = (float)(1.0 - a->beta2);
+    l.eps             = (float)a->eps;
+    l.zero_grad       = a->zero_grad;
+    l.stochastic      = a->stochastic_rounding;
+    l.entries = l.chunks = 0;
+    int slot_group[kAdamWGroups], slots = 0;
+    const auto launch = [&] {
+        if (l.entries == 0) return;
+        const dim3 grid(std::min(l.chunks, kOptimGrid));
+        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32>), grid, dim3(kBlock), 0, stream, l);
+        else hipLaunchKernelGGL((adamw_step_kernel<8>), grid, dim3(kBlock), 0, stream, l);
+        l.entries = l.chunks = 0;
+        slots                = 0;
+    };
+    for (int k = 0; k < a->num_tensors; ++k)
+    {
+        const vetrast_adamw_tensor& t = a->tensors[k];
+        for (int64_t from = 0; from < t.n; from += kOptimEntryElements)
+        {
+            int slot = 0;
+            while (slot < slots && slot_group[slot] != t.group) ++slot;
+            if (l.entries == (uint32_t)kAdamWEntries || slot == kAdamWGroups)
+            {
+                launch();
+                slot = 0;
+            }
+            if (slot == slots)
+            {
+                const vetrast_adamw_group& g = a->groups[t.group];
+                AdamWGroup& c                = l.g[slot];
+                slot_group[slots++]          = t.group;
+                if (device) c = {0.f, 0.f, 0.f, (uint32_t)t.group};
+                else
+                {
+                    // bias corrections in double, handed to the kernel rounded once
+                    c.step_size    = (float)(g.lr / (1.0 - std::pow(a->beta1, (double)g.step)));
+                    c.keep         = (float)(1.0 - g.lr * g.weight_decay);
+                    c.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)g.step)));
+                    c.key          = step_key(a->seed, g.step);
+                }
+            }
+            AdamWEntry& e = l.e[l.entries++];
+            const int64_t moment_bytes = a->moment_bits / 8;
+            e.param = static_cast<char*>(t.param) + from * (int64_t)dtype_bytes(t.param_type);
+            e.grad  = static_cast<char*>(t.grad) + from * (int64_t)dtype_bytes(t.grad_type);
+            e.copy  = t.copy ? static_cast<char*>(t.copy) + from * 2 : nullptr;
+            e.m     = static_cast<char*>(t.exp_avg) + from * moment_bytes;
+            e.v     = static_cast<char*>(t.exp_avg_sq) + from * moment_bytes;
+            e.scale = a->moment_bits == 8 ? t.block_scale + from / kMomentBlock * 2 : nullptr;
+            e.n     = (uint32_t)std::min(t.n - from, kOptimEntryElements);
+            e.first = l.chunks;
+            e.pair  = (uint32_t)((uint64_t)(t.first_number + from) / 2);
+            bool whole = aligned_to(e.param, 16) && aligned_to(e.grad, 16) && aligned_to(e.copy, 16);
+            if (a->moment_bits == 32) whole = whole && aligned_to(e.m, 16) && aligned_to(e.v, 16);
+            e.types = (uint32_t)t.param_type | (uint32_t)t.grad_type << 2 | (t.copy ? (uint32_t)t.copy_type << 4 | kHasCopy : 0u) |
+                      (whole ? kAligned : 0u) | (uint32_t)slot << 8;
+            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+        }
+    }
+    launch();
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+size_t vetrast_gradient_norm_workspace_bytes(const vetrast_gradient* gradients, int32_t num_gradients)
+{
+    if (num_gradients < 0 || (num_gradients > 0 && !gradients)) return 0;
+    int64_t entries = 0;
+    for (int k = 0; k < num_gradients; ++k)
+    {
+        if (gradients[k].n < 0) return 0;
+        entries += (gradients[k].n + kOptimEntryElements - 1) / kOptimEntryElements;
+    }
+    return (size_t)std::max<int64_t>((entries + kNormEntries - 1) / kNormEntries, 1) * kNormGrid * sizeof(double);
+}
+
+int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a, void* stream_)
+{
+    if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
+    if (a->num_gradients < 0 || (a->num_gradients > 0 && !a->gradients) || !a->out || !a->workspace) return VETRAST_ERR_INVALID_ARG;
+    if (!std::isfinite(a->scale) || std::isnan(a->max_norm)) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->out, 4) || !aligned_to(a->workspace, 8)) return VETRAST_ERR_INVALID_ARG;
+    for (int k = 0; k < a->num_gradients; ++k)
+    {
+        const vetrast_gradient& g = a->gradients[k];
+        if (g.n < 0 || !is_dtype(g.type)) return VETRAST_ERR_INVALID_ARG;
+        if (g.n > 0 && (!g.grad || !aligned_to(g.grad, dtype_bytes(g.type)))) return VETRAST_ERR_INVALID_ARG;
+    }
+    if (a->workspace_bytes < vetrast_gradient_norm_workspace_bytes(a->gradients, a->num_gradients)) return VETRAST_ERR_WORKSPACE_SMALL;
+    hipStream_t stream = (hipStream_t)stream_;
+    double* partial    = static_cast<double*>(a->workspace);
+    uint32_t partials  = 0;
+    NormLaunch l;
+    l.entries = l.chunks = 0;
+    const auto launch = [&] {
+        if (l.entries == 0) return;
+        const uint32_t grid = std::min(l.chunks, kNormGrid);
+        l.partial           = partial + partials;
+        hipLaunchKernelGGL(gradient_squares_kernel, dim3(grid), dim3(kBlock), 0, stream, l);
+        partials += grid;
+        l.entries = l.chunks = 0;
+    };
+    for (int k = 0; k < a->num_gradients; ++k)
+    {
+        const vetrast_gradient& g = a->gradients[k];
+        for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
+        {
+            if (l.entries == (uint32_t)kNormEntries) launch();
+            NormEntry& e = l.e[l.entries++];
+            e.grad       = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
+            e.n          = (uint32_t)std::min(g.n - from, kOptimEntryElements);
+            e.first      = l.chunks;
+            e.type       = (uint32_t)g.type;
+            e.aligned    = aligned_to(e.grad, 16) ? 1u : 0u;
+            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+        }
+    }
+    launch();
+    hipLaunchKernelGGL(gradient_norm_kernel, dim3(1), dim3(kBlock), 0, stream, partial, partials, a->max_norm, a->scale, a->out);
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+static int convert_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, hipStream_t stream, bool pack)
+{
+    if (!ctx || num_tensors < 0 || (num_tensors > 0 && !tensors)) return VETRAST_ERR_INVALID_ARG;
+    for (int k = 0; k < num_tensors; ++k)
+    {
+        const vetrast_moment_tensor& t = tensors[k];
+        if (t.n < 0) return VETRAST_ERR_INVALID_ARG;
+        if (t.n == 0) continue;
+        if (!t.exp_avg || !t.exp_avg_sq || !t.exp_avg_code || !t.exp_avg_sq_code || !t.block_scale) return VETRAST_ERR_INVALID_ARG;
+        if (!aligned_to(t.exp_avg, 4) || !aligned_to(t.exp_avg_sq, 4) || !aligned_to(t.exp_avg_code, 8) ||
+            !aligned_to(t.exp_avg_sq_code, 8) || !aligned_to(t.block_scale, 2))
+            return VETRAST_ERR_INVALID_ARG;
+    }
+    MomentLaunch l;
+    l.entries = l.chunks = 0;
+    const auto launch = [&] {
+        if (l.entries == 0) return;
+        const dim3 grid(std::min(l.chunks, kOptimGrid));
+        if (pack) hipLaunchKernelGGL((convert_moments_kernel<true>), grid, dim3(kBlock), 0, stream, l);
+        else hipLaunchKernelGGL((convert_moments_kernel<false>), grid, dim3(kBlock), 0, stream, l);
+        l.entries = l.chunks = 0;
+    };
+    for (int k = 0; k < num_tensors; ++k)
+    {
+        const vetrast_moment_tensor& t = tensors[k];
+        for (int64_t from = 0; from < t.n; from += kOptimEntryElements)
+        {
+            if (l.entries == (uint32_t)kMomentEntries) launch();
+            MomentEntry& e = l.e[l.entries++];
+            e.m            = t.exp_avg + from;
+            e.v            = t.exp_avg_sq + from;
+            e.mc           = t.exp_avg_code + from;
+            e.vc           = t.exp_avg_sq_code + from;
+            e.scale        = t.block_scale + from / kMomentBlock * 2;
+            e.n            = (uint32_t)std::min(t.n - from, kOptimEntryElements);
+            e.first        = l.chunks;
+            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+        }
+    }
+    launch();
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream)
+{
+    return convert_moments(ctx, tensors, num_tensors, (hipStream_t)stream, true);
+}
+
+int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream)
+{
+    return convert_moments(ctx, tensors, num_tensors, (hipStream_t)stream, false);
 }
 
 size_t vetrast_lift_workspace_bytes(int64_t num_cells)

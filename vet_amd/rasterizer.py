@@ -14,6 +14,9 @@ from . import abi
 from .synthetic import Scene
 
 
+_DTYPES = {torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16}
+
+
 def make_params(scene: Scene, **overrides) -> abi.Params:
     """RenderParams of the blending path with the defaults the benchmark configurations use."""
     p = abi.Params()
@@ -338,6 +341,69 @@ class Rasterizer:
         a.n, a.step = param.numel(), step
         a.lr, a.beta1, a.beta2, a.eps, a.weight_decay, a.zero_grad = lr, beta1, beta2, eps, weight_decay, int(zero_grad)
         abi.check(self.lib.vetrast_adam_step(self.ctx, C.byref(a), self._stream()), "adam_step")
+
+    def adamw_step(self, tensors, groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, stochastic_rounding=False, seed=0,
+                   zero_grad=False, grad_scale=None, device_state=None):
+        """One AdamW step in place on a list of tensors (vetrast_adamw_step). tensors: dicts of contiguous CUDA tensors param, grad,
+        exp_avg, exp_avg_sq and, as wanted, block_scale and copy, with first_number and group (0 where left out). groups:
+        (lr, weight_decay, step). device_state: a uint8 tensor of vetrast_adamw_device_state_bytes(len(groups)) bytes."""
+        ts, gs, a = (abi.AdamWTensor * max(len(tensors), 1))(), (abi.AdamWGroup * max(len(groups), 1))(), abi.AdamWArgs()
+        for t, d in zip(ts, tensors):
+            n = d["param"].numel()
+            for name in ("param", "grad", "exp_avg", "exp_avg_sq", "block_scale", "copy"):
+                x = d.get(name)
+                if x is not None:
+                    assert x.is_cuda and x.is_contiguous()
+                    setattr(t, name, x.data_ptr())
+            blocks = -(-n // abi.MOMENT_BLOCK)
+            state = n if moment_bits == 32 else blocks * abi.MOMENT_BLOCK
+            assert d["grad"].numel() == n and d["exp_avg"].numel() >= state and d["exp_avg_sq"].numel() >= state
+            assert all(d[k].dtype == (torch.float32 if moment_bits == 32 else torch.uint8) for k in ("exp_avg", "exp_avg_sq"))
+            assert moment_bits == 32 or (d["block_scale"].dtype == torch.uint8 and d["block_scale"].numel() >= 2 * blocks)
+            t.n, t.first_number, t.group = n, d.get("first_number", 0), d.get("group", 0)
+            t.param_type, t.grad_type = _DTYPES[d["param"].dtype], _DTYPES[d["grad"].dtype]
+            if d.get("copy") is not None:
+                assert d["copy"].numel() == n
+                t.copy_type = _DTYPES[d["copy"].dtype]
+        for g, (lr, weight_decay, step) in zip(gs, groups):
+            g.lr, g.weight_decay, g.step = lr, weight_decay, step
+        a.tensors, a.groups, a.num_tensors, a.num_groups = ts, gs, len(tensors), len(groups)
+        a.beta1, a.beta2, a.eps, a.moment_bits, a.seed = beta1, beta2, eps, moment_bits, seed
+        a.stochastic_rounding, a.zero_grad = int(stochastic_rounding), int(zero_grad)
+        if grad_scale is not None:
+            assert grad_scale.is_cuda and grad_scale.dtype == torch.float32
+            a.grad_scale = grad_scale.data_ptr()
+        if device_state is not None:
+            assert device_state.is_cuda and device_state.numel() >= self.lib.vetrast_adamw_device_state_bytes(len(groups))
+            a.device_state = device_state.data_ptr()
+        abi.check(self.lib.vetrast_adamw_step(self.ctx, C.byref(a), self._stream()), "adamw_step")
+
+    def gradient_norm(self, gradients, max_norm=0.0, scale=1.0, out=None, workspace=None):
+        """Norm of all gradients and the factor that clips it, float32 [2] (vetrast_gradient_norm)."""
+        gs, a = (abi.Gradient * max(len(gradients), 1))(), abi.GradientNormArgs()
+        for g, x in zip(gs, gradients):
+            assert x.is_cuda and x.is_contiguous()
+            g.grad, g.n, g.type = x.data_ptr(), x.numel(), _DTYPES[x.dtype]
+        need = self.lib.vetrast_gradient_norm_workspace_bytes(gs, len(gradients))
+        out = torch.empty(2, device="cuda") if out is None else out
+        workspace = torch.empty(need, dtype=torch.uint8, device="cuda") if workspace is None else workspace
+        a.gradients, a.num_gradients, a.max_norm, a.scale = gs, len(gradients), max_norm, scale
+        a.out, a.workspace, a.workspace_bytes = out.data_ptr(), workspace.data_ptr(), workspace.numel()
+        abi.check(self.lib.vetrast_gradient_norm(self.ctx, C.byref(a), self._stream()), "gradient_norm")
+        return out
+
+    def convert_moments(self, tensors, pack):
+        """float32 moments to 8 bits or back (vetrast_pack_moments, vetrast_unpack_moments): a list of (exp_avg, exp_avg_sq, code,
+        code_sq, block_scale), the first two float32 of the same number of elements."""
+        ts = (abi.MomentTensor * max(len(tensors), 1))()
+        for t, (m, v, mc, vc, scale) in zip(ts, tensors):
+            n, blocks = m.numel(), -(-m.numel() // abi.MOMENT_BLOCK)
+            assert all(x.is_cuda and x.is_contiguous() for x in (m, v, mc, vc, scale)) and m.dtype == v.dtype == torch.float32
+            assert v.numel() == n and min(mc.numel(), vc.numel()) >= blocks * abi.MOMENT_BLOCK and scale.numel() >= 2 * blocks
+            t.exp_avg, t.exp_avg_sq, t.n = m.data_ptr(), v.data_ptr(), n
+            t.exp_avg_code, t.exp_avg_sq_code, t.block_scale = mc.data_ptr(), vc.data_ptr(), scale.data_ptr()
+        call = self.lib.vetrast_pack_moments if pack else self.lib.vetrast_unpack_moments
+        abi.check(call(self.ctx, ts, len(tensors), self._stream()), "convert_moments")
 
     def lift_error(self, cell_bb_min, cell_bb_length, cell_value, cell_access_count, view, poses_se3, intrinsics,
                    loss_image, border_pixels=abi.LIFT_BORDER_PIXELS, workspace=None, static_scratch=False):

@@ -1,0 +1,462 @@
+// See adamw.h.
+#include "adamw.h"
+
+#include <cstring>
+#include <map>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+
+namespace vet_amd
+{
+namespace
+{
+constexpr int64_t kBlock = VETRAST_MOMENT_BLOCK;
+
+void check(int st, const char* where)
+{
+    TORCH_CHECK(st == VETRAST_OK, "vetrast ", where, " failed: ", st, " (", vetrast_status_string(st), ")");
+}
+
+// A context serves one host thread at a time and belongs to a device. The caller has made `device` the current one.
+vetrast_ctx* context_on(const torch::Device& device)
+{
+    struct Contexts
+    {
+        std::map<int, vetrast_ctx*> of;
+        ~Contexts()
+        {
+            for (auto& c : of) vetrast_destroy(c.second);
+        }
+    };
+    thread_local Contexts contexts;
+    vetrast_ctx*& ctx = contexts.of[device.index()];
+    if (!ctx) check(vetrast_create(&ctx), "create");
+    return ctx;
+}
+
+void* stream_on(const torch::Device& device)
+{
+    return (void*)c10::hip::getCurrentHIPStream(device.index()).stream();
+}
+
+int32_t type_of(const torch::Tensor& t, const char* what)
+{
+    switch (t.scalar_type())
+    {
+        case torch::kFloat32: return VETRAST_F32;
+        case torch::kBFloat16: return VETRAST_BF16;
+        case torch::kFloat16: return VETRAST_F16;
+        default: TORCH_CHECK(false, what, " must be float32, bfloat16 or float16, not ", t.scalar_type());
+    }
+}
+
+void check_on(const torch::Tensor& t, const torch::Device& device, const char* what)
+{
+    TORCH_CHECK(t.layout() == torch::kStrided && t.device() == device, what, " must be a strided tensor on ", device);
+}
+
+// The elements one behind the other in memory, whatever the order of dimensions.
+bool dense(const torch::Tensor& t)
+{
+    return t.is_contiguous() || t.is_non_overlapping_and_dense();
+}
+
+int64_t whole_blocks(int64_t n)
+{
+    return (n + kBlock - 1) / kBlock * kBlock;
+}
+
+// The step's gradient of p in p's order of elements: p.grad() itself where that has the same strides.
+torch::Tensor gradient_like(const torch::Tensor& p, const torch::Tensor& grad)
+{
+    if (grad.strides() == p.strides() || (grad.is_contiguous() && p.is_contiguous())) return grad;
+    return torch::empty_like(p).copy_(grad);
+}
+
+std::vector<vetrast_moment_tensor> moment_list(const std::vector<torch::Tensor>& ms, const std::vector<torch::Tensor>& vs, const torch::Device& device)
+{
+    TORCH_CHECK(ms.size() == vs.size(), "as many first moments as second ones are needed, not ", ms.size(), " and ", vs.size());
+    std::vector<vetrast_moment_tensor> list(ms.size());
+    for (size_t k = 0; k < ms.size(); ++k)
+    {
+        check_on(ms[k], device, "moments");
+        check_on(vs[k], device, "moments");
+        TORCH_CHECK(ms[k].scalar_type() == torch::kFloat32 && vs[k].scalar_type() == torch::kFloat32 && dense(ms[k]) && dense(vs[k]),
+                    "moments must be dense float32 tensors");
+        TORCH_CHECK(ms[k].sizes() == vs[k].sizes() && (ms[k].strides() == vs[k].strides() || (ms[k].is_contiguous() && vs[k].is_contiguous())),
+                    "both moments of a tensor must have one shape and order");
+        std::memset(&list[k], 0, sizeof(list[k]));
+        list[k].exp_avg    = ms[k].data_ptr<float>();
+        list[k].exp_avg_sq = vs[k].data_ptr<float>();
+        list[k].n          = ms[k].numel();
+    }
+    return list;
+}
+
+void place_codes(std::vector<vetrast_moment_tensor>& list, const torch::Tensor& m, const torch::Tensor& v, const torch::Tensor& scale)
+{
+    int64_t at = 0;
+    for (auto& t : list)
+    {
+        t.exp_avg_code    = m.data_ptr<uint8_t>() + at;
+        t.exp_avg_sq_code = v.data_ptr<uint8_t>() + at;
+        t.block_scale     = scale.data_ptr<uint8_t>() + at / kBlock * 2;
+        at += whole_blocks(t.n);
+    }
+}
+}  // namespace
+
+AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
+{
+    TORCH_CHECK(options.moment_bits == 32 || options.moment_bits == 8, "AdamW: moment_bits is 32 or 8, not ", options.moment_bits);
+    TORCH_CHECK(options.beta1 >= 0 && options.beta1 < 1 && options.beta2 >= 0 && options.beta2 < 1, "AdamW: betas lie in [0, 1)");
+    TORCH_CHECK((float)options.eps > 0, "AdamW: eps must be above zero");
+    TORCH_CHECK(groups.size() <= VETRAST_ADAMW_MAX_GROUPS, "AdamW: at most ", VETRAST_ADAMW_MAX_GROUPS, " groups");
+    for (auto& g : groups)
+    {
+        for (auto& p : g.params)
+        {
+            TORCH_CHECK(p.defined() && p.is_cuda(), "AdamW: parameters must be tensors on the GPU");
+            if (slots_.empty()) device_ = p.device();
+            for (auto& s : slots_) TORCH_CHECK(!s.param.is_same(p), "AdamW: a parameter is in the list twice");
+            slots_.push_back({p, (int)lr_.size(), 0, -1, 0});
+        }
+        lr_.push_back(g.lr);
+        weight_decay_.push_back(g.weight_decay);
+    }
+    TORCH_CHECK(!slots_.empty(), "AdamW: no parameters");
+    c10::DeviceGuard guard(device_);
+    lay_out();
+    if (options_.capturable)
+    {
+        const int64_t bytes = (int64_t)vetrast_adamw_device_state_bytes((int32_t)lr_.size());
+        device_state_       = torch::zeros({bytes}, torch::TensorOptions(device_).dtype(torch::kUInt8));
+        device_step         = device_state_.narrow(0, 0, 8).view(torch::kInt64);
+        lr_factor           = device_state_.narrow(0, 8, 4).view(torch::kFloat32);
+        lr_factor.fill_(1.0);
+    }
+}
+
+void AdamW::fill_master(const Slot& s)
+{
+    // in the parameter's order of memory
+    master.narrow(0, s.first, s.n).copy_(s.param.detach().as_strided({s.n}, {1}));
+}
+
+// Room in the flat state for every parameter as it is now. What a parameter of unchanged size had moves along.
+void AdamW::lay_out()
+{
+    torch::NoGradGuard no_grad;
+    int64_t at = 0;
+    std::vector<int64_t> from(slots_.size(), -1);
+    for (size_t k = 0; k < slots_.size(); ++k)
+    {
+        Slot& s = slots_[k];
+        type_of(s.param, "AdamW: parameters");
+        check_on(s.param, device_, "AdamW: parameters");
+        TORCH_CHECK(dense(s.param), "AdamW: parameters must be dense, without gaps or overlaps");
+        if (s.n == s.param.numel()) from[k] = s.first;
+        else s.step = 0;
+        s.n     = s.param.numel();
+        s.first = at;
+        at += whole_blocks(s.n);
+    }
+    const auto bytes     = torch::TensorOptions(device_).dtype(torch::kUInt8);
+    const auto floats    = torch::TensorOptions(device_).dtype(torch::kFloat32);
+    const bool eight     = options_.moment_bits == 8;
+    const auto old_m     = exp_avg, old_v = exp_avg_sq, old_scale = block_scale, old_master = master;
+    exp_avg              = torch::zeros({at}, eight ? bytes : floats);
+    exp_avg_sq           = torch::zeros({at}, eight ? bytes : floats);
+    if (eight) block_scale = torch::zeros({at / kBlock, 2}, bytes);
+    if (options_.master_weights) master = torch::zeros({at}, floats);
+    for (size_t k = 0; k < slots_.size(); ++k)
+    {
+        const Slot& s   = slots_[k];
+        const int64_t n = whole_blocks(s.n);
+        if (from[k] >= 0 && n > 0)
+        {
+            exp_avg.narrow(0, s.first, n).copy_(old_m.narrow(0, from[k], n));
+            exp_avg_sq.narrow(0, s.first, n).copy_(old_v.narrow(0, from[k], n));
+            if (eight) block_scale.narrow(0, s.first / kBlock, n / kBlock).copy_(old_scale.narrow(0, from[k] / kBlock, n / kBlock));
+            if (master.defined()) master.narrow(0, s.first, n).copy_(old_master.narrow(0, from[k], n));
+        }
+        else if (master.defined()) fill_master(s);
+    }
+}
+
+void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
+{
+    torch::NoGradGuard no_grad;
+    c10::DeviceGuard guard(device_);
+    const bool capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    TORCH_CHECK(options_.capturable || !capturing, "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
+    bool moved = false;
+    for (auto& s : slots_) moved |= s.param.numel() != s.n;
+    if (moved)
+    {
+        TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
+        lay_out();
+    }
+    const bool eight          = options_.moment_bits == 8;
+    const int64_t moment_size = eight ? 1 : 4;
+    char* m                   = (char*)exp_avg.data_ptr();
+    char* v                   = (char*)exp_avg_sq.data_ptr();
+    uint8_t* scales           = eight ? block_scale.data_ptr<uint8_t>() : nullptr;
+    float* masters            = master.defined() ? master.data_ptr<float>() : nullptr;
+    tensors_.clear();
+    groups_.clear();
+    if (options_.capturable)
+        for (size_t g = 0; g < lr_.size(); ++g) groups_.push_back({lr_[g], weight_decay_[g], 0});
+    group_of_.assign(lr_.size(), -1);
+    std::vector<torch::Tensor> reordered;
+    for (auto& s : slots_)
+    {
+        const torch::Tensor& p    = s.param;
+        const torch::Tensor& grad = p.grad();
+        if (!grad.defined()) continue;
+        check_on(p, device_, "AdamW: parameters");
+        check_on(grad, device_, "AdamW: gradients");
+        const int32_t type = type_of(p, "AdamW: parameters");
+        TORCH_CHECK(grad.scalar_type() == p.scalar_type() && grad.sizes() == p.sizes(), "AdamW: a gradient must have its parameter's type and shape");
+        TORCH_CHECK(dense(p), "AdamW: parameters must be dense, without gaps or overlaps");
+        torch::Tensor g = gradient_like(p, grad);
+        if (!g.is_same(grad)) reordered.push_back(g);
+        int64_t& place   = group_of_[s.group];
+        const auto fits  = [&](int64_t k) { return groups_[k].lr == lr_[s.group] && groups_[k].weight_decay == weight_decay_[s.group] && groups_[k].step == s.step + 1; };
+        if (options_.capturable) place = s.group;
+        else if (place < 0 || !fits(place))
+        {
+            // parameters of a group that started later are a group of their own here
+            place = 0;
+            while (place < (int64_t)groups_.size() && !fits(place)) ++place;
+            if (place == (int64_t)groups_.size()) groups_.push_back({lr_[s.group], weight_decay_[s.group], s.step + 1});
+        }
+        vetrast_adamw_tensor t;
+        const bool with_master = masters && type != VETRAST_F32;
+        t.param                = with_master ? (void*)(masters + s.first) : p.data_ptr();
+        t.copy                 = with_master ? p.data_ptr() : nullptr;
+        t.grad                 = g.data_ptr();
+        t.exp_avg              = m + s.first * moment_size;
+        t.exp_avg_sq           = v + s.first * moment_size;
+        t.block_scale          = scales ? scales + s.first / kBlock * 2 : nullptr;
+        t.n                    = s.n;
+        t.first_number         = s.first;
+        t.param_type           = with_master ? (int32_t)VETRAST_F32 : type;
+        t.grad_type            = type;
+        t.copy_type            = with_master ? type : 0;
+        t.group                = (int32_t)place;
+        tensors_.push_back(t);
+    }
+    vetrast_adamw_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.tensors             = tensors_.data();
+    a.groups              = groups_.data();
+    a.num_tensors         = (int32_t)tensors_.size();
+    a.num_groups          = (int32_t)groups_.size();
+    a.beta1               = options_.beta1;
+    a.beta2               = options_.beta2;
+    a.eps                 = options_.eps;
+    a.moment_bits         = options_.moment_bits;
+    a.stochastic_rounding = options_.stochastic_rounding ? 1 : 0;
+    a.seed                = options_.seed;
+    a.zero_grad           = zero_grad ? 1 : 0;
+    a.device_state        = device_state_.defined() ? device_state_.data_ptr() : nullptr;
+    if (grad_scale.has_value() && grad_scale->defined())
+    {
+        const torch::Tensor& x = *grad_scale;
+        check_on(x, device_, "AdamW: grad_scale");
+        TORCH_CHECK(x.scalar_type() == torch::kFloat32 && x.is_contiguous() && (x.numel() == 1 || x.numel() == 2),
+                    "AdamW: grad_scale is one float32, or the two that grad_norm returns");
+        a.grad_scale = x.data_ptr<float>() + x.numel() - 1;
+    }
+    check(vetrast_adamw_step(context_on(device_), &a, stream_on(device_)), "adamw_step");
+    for (auto& s : slots_)
+    {
+        const torch::Tensor& grad = s.param.grad();
+        if (!grad.defined()) continue;
+        s.step += 1;
+        // the kernel wrote through raw pointers: tell everyone who keys on the version counters
+        s.param.unsafeGetTensorImpl()->bump_version();
+        if (zero_grad) grad.unsafeGetTensorImpl()->bump_version();
+    }
+    // the kernel cleared copies of these
+    if (zero_grad && !reordered.empty())
+        for (auto& s : slots_)
+        {
+            const torch::Tensor& grad = s.param.grad();
+            if (!grad.defined() || grad.strides() == s.param.strides()) continue;
+            if (dense(grad)) s.param.mutable_grad().zero_();
+            else s.param.mutable_grad() = torch::zeros_like(s.param);
+        }
+}
+
+void AdamW::zero_grad()
+{
+    torch::NoGradGuard no_grad;
+    for (auto& s : slots_)
+        if (s.param.grad().defined()) s.param.mutable_grad().zero_();
+}
+
+torch::Tensor AdamW::grad_norm(double max_norm, double scale)
+{
+    std::vector<torch::Tensor> grads;
+    grads.reserve(slots_.size());
+    for (auto& s : slots_)
+        if (s.param.grad().defined()) grads.push_back(s.param.grad());
+    return GradNorm(grads, max_norm, scale);
+}
+
+void AdamW::set_lr(int64_t group, double lr)
+{
+    TORCH_CHECK(group >= 0 && group < (int64_t)lr_.size(), "AdamW: no group ", group);
+    lr_[group] = lr;
+}
+
+std::vector<int64_t> AdamW::steps() const
+{
+    std::vector<int64_t> r;
+    const int64_t all = options_.capturable ? device_step.item<int64_t>() : 0;
+    for (auto& s : slots_) r.push_back(options_.capturable ? all : s.step);
+    return r;
+}
+
+void AdamW::set_step(int64_t step)
+{
+    TORCH_CHECK(step >= 0, "AdamW: steps are counted from 0");
+    for (auto& s : slots_) s.step = step;
+    if (options_.capturable) device_step.fill_(step);
+}
+
+std::vector<std::pair<int64_t, int64_t>> AdamW::layout() const
+{
+    std::vector<std::pair<int64_t, int64_t>> r;
+    for (auto& s : slots_) r.push_back({s.first, s.n});
+    return r;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> AdamW::moments() const
+{
+    if (options_.moment_bits == 32) return {exp_avg, exp_avg_sq};
+    return UnpackMoments(exp_avg, exp_avg_sq, block_scale);
+}
+
+void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, int64_t step)
+{
+    torch::NoGradGuard no_grad;
+    c10::DeviceGuard guard(device_);
+    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device_);
+    TORCH_CHECK(list.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", list.size());
+    for (size_t k = 0; k < list.size(); ++k)
+        TORCH_CHECK(list[k].n == slots_[k].n, "AdamW: parameter ", k, " has ", slots_[k].n, " elements, its moments have ", list[k].n);
+    set_step(step);
+    if (options_.moment_bits == 8)
+    {
+        place_codes(list, exp_avg, exp_avg_sq, block_scale);
+        check(vetrast_pack_moments(context_on(device_), list.data(), (int32_t)list.size(), stream_on(device_)), "pack_moments");
+        return;
+    }
+    for (size_t k = 0; k < list.size(); ++k)
+    {
+        exp_avg.narrow(0, slots_[k].first, slots_[k].n).copy_(exp_avgs[k].as_strided({slots_[k].n}, {1}));
+        exp_avg_sq.narrow(0, slots_[k].first, slots_[k].n).copy_(exp_avg_sqs[k].as_strided({slots_[k].n}, {1}));
+    }
+}
+
+void AdamW::reload_master()
+{
+    torch::NoGradGuard no_grad;
+    if (!master.defined()) return;
+    c10::DeviceGuard guard(device_);
+    for (auto& s : slots_)
+    {
+        TORCH_CHECK(s.param.numel() == s.n && dense(s.param), "AdamW: a parameter has changed its size; step() notices that by itself");
+        fill_master(s);
+    }
+}
+
+torch::Tensor GradNorm(const std::vector<torch::Tensor>& gradients, double max_norm, double scale)
+{
+    std::vector<vetrast_gradient> list;
+    std::vector<torch::Tensor> gathered;  // of gradients with gaps
+    list.reserve(gradients.size());
+    std::optional<torch::Device> device;
+    c10::OptionalDeviceGuard guard;
+    for (auto& g : gradients)
+    {
+        if (!g.defined()) continue;
+        if (!device)
+        {
+            TORCH_CHECK(g.is_cuda(), "grad_norm: gradients must be tensors on the GPU");
+            device = g.device();
+            guard.reset_device(*device);
+        }
+        check_on(g, *device, "grad_norm: gradients");
+        const int32_t type = type_of(g, "grad_norm: gradients");
+        const void* data   = g.data_ptr();
+        if (!dense(g))
+        {
+            gathered.push_back(g.contiguous());
+            data = gathered.back().data_ptr();
+        }
+        list.push_back({data, g.numel(), type, 0});
+    }
+    TORCH_CHECK(device, "grad_norm: no gradients");
+    vetrast_gradient_norm_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.gradients             = list.data();
+    a.num_gradients         = (int32_t)list.size();
+    a.max_norm              = max_norm;
+    a.scale                 = scale;
+    a.workspace_bytes       = vetrast_gradient_norm_workspace_bytes(list.data(), a.num_gradients);
+    torch::Tensor workspace = torch::empty({(int64_t)a.workspace_bytes}, torch::TensorOptions(*device).dtype(torch::kUInt8));
+    torch::Tensor out       = torch::empty({2}, torch::TensorOptions(*device).dtype(torch::kFloat32));
+    a.workspace             = workspace.data_ptr();
+    a.out                   = out.data_ptr<float>();
+    check(vetrast_gradient_norm(context_on(*device), &a, stream_on(*device)), "gradient_norm");
+    return out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs)
+{
+    TORCH_CHECK(!exp_avgs.empty() && exp_avgs[0].is_cuda(), "pack_moments: a list of tensors on the GPU is needed");
+    const torch::Device device = exp_avgs[0].device();
+    c10::DeviceGuard guard(device);
+    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device);
+    int64_t total                           = 0;
+    for (auto& t : list) total += whole_blocks(t.n);
+    const auto bytes    = torch::TensorOptions(device).dtype(torch::kUInt8);
+    torch::Tensor m     = torch::empty({total}, bytes), v = torch::empty({total}, bytes);
+    torch::Tensor scale = torch::empty({total / kBlock, 2}, bytes);
+    place_codes(list, m, v, scale);
+    check(vetrast_pack_moments(context_on(device), list.data(), (int32_t)list.size(), stream_on(device)), "pack_moments");
+    return {m, v, scale};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> UnpackMoments(const torch::Tensor& exp_avg, const torch::Tensor& exp_avg_sq, const torch::Tensor& block_scale)
+{
+    TORCH_CHECK(exp_avg.is_cuda(), "unpack_moments: tensors on the GPU are needed");
+    const torch::Device device = exp_avg.device();
+    c10::DeviceGuard guard(device);
+    for (const torch::Tensor* t : {&exp_avg, &exp_avg_sq, &block_scale})
+    {
+        check_on(*t, device, "unpack_moments: codes and scales");
+        TORCH_CHECK(t->scalar_type() == torch::kUInt8 && t->is_contiguous(), "unpack_moments: codes and scales are contiguous uint8 tensors");
+    }
+    const int64_t n = exp_avg.numel();
+    TORCH_CHECK(n % kBlock == 0 && exp_avg_sq.numel() == n && block_scale.numel() == n / kBlock * 2,
+                "unpack_moments: whole blocks of ", kBlock, " codes with two scales each are needed");
+    const auto floats = torch::TensorOptions(device).dtype(torch::kFloat32);
+    torch::Tensor m = torch::empty({n}, floats), v = torch::empty({n}, floats);
+    vetrast_moment_tensor t;
+    t.exp_avg         = m.data_ptr<float>();
+    t.exp_avg_sq      = v.data_ptr<float>();
+    t.exp_avg_code    = exp_avg.data_ptr<uint8_t>();
+    t.exp_avg_sq_code = exp_avg_sq.data_ptr<uint8_t>();
+    t.block_scale     = block_scale.data_ptr<uint8_t>();
+    t.n               = n;
+    check(vetrast_unpack_moments(context_on(device), &t, 1, stream_on(device)), "unpack_moments");
+    return {m, v};
+}
+}  // namespace vet_amd

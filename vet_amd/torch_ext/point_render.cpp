@@ -1,6 +1,7 @@
 // libtorch host side of the MI355X blending point rasterizer: autograd Function with the reference's argument order,
 // calling the C ABI of include/vetrast.h. See point_render.h for the reference lines each piece mirrors.
 #include "point_render.h"
+#include "adamw.h"
 #include "vet_adapter.h"
 
 #include <algorithm>
@@ -1249,6 +1250,38 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
              pybind11::arg("eps") = 1e-8, pybind11::arg("weight_decay") = 0.0)
         .def("step", &vet_amd::MyAdam::step, pybind11::arg("zero_grad") = false)
         .def("zero_grad", &vet_amd::MyAdam::zero_grad);
+    using vet_amd::AdamW;
+    pybind11::class_<AdamW>(m, "AdamW")
+        .def(pybind11::init([](std::vector<std::tuple<std::vector<torch::Tensor>, double, double>> groups, double beta1,
+                               double beta2, double eps, int moment_bits, bool master_weights, bool stochastic_rounding,
+                               uint64_t seed, bool capturable) {
+                 std::vector<AdamW::Group> gs;
+                 for (auto& g : groups) gs.push_back({std::get<0>(g), std::get<1>(g), std::get<2>(g)});
+                 AdamW::Options o{beta1, beta2, eps, moment_bits, master_weights, stochastic_rounding, seed, capturable};
+                 return std::make_unique<AdamW>(std::move(gs), o);
+             }),
+             pybind11::arg("groups"), pybind11::arg("beta1") = 0.9, pybind11::arg("beta2") = 0.999, pybind11::arg("eps") = 1e-8,
+             pybind11::arg("moment_bits") = 32, pybind11::arg("master_weights") = false,
+             pybind11::arg("stochastic_rounding") = false, pybind11::arg("seed") = 0, pybind11::arg("capturable") = false)
+        .def("step", &AdamW::step, pybind11::arg("zero_grad") = false, pybind11::arg("grad_scale") = pybind11::none())
+        .def("zero_grad", &AdamW::zero_grad)
+        .def("grad_norm", &AdamW::grad_norm, pybind11::arg("max_norm") = 0.0, pybind11::arg("scale") = 1.0)
+        .def("set_lr", &AdamW::set_lr, pybind11::arg("group"), pybind11::arg("lr"))
+        .def("steps", &AdamW::steps)
+        .def("set_step", &AdamW::set_step, pybind11::arg("step"))
+        .def("layout", &AdamW::layout)
+        .def("moments", &AdamW::moments)
+        .def("load_moments", &AdamW::load_moments, pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
+        .def("reload_master", &AdamW::reload_master)
+        .def_readonly("exp_avg", &AdamW::exp_avg)
+        .def_readonly("exp_avg_sq", &AdamW::exp_avg_sq)
+        .def_readonly("block_scale", &AdamW::block_scale)
+        .def_readonly("master", &AdamW::master)
+        .def_readonly("device_step", &AdamW::device_step)
+        .def_readonly("lr_factor", &AdamW::lr_factor);
+    m.def("grad_norm", &vet_amd::GradNorm, pybind11::arg("gradients"), pybind11::arg("max_norm") = 0.0, pybind11::arg("scale") = 1.0);
+    m.def("pack_moments", &vet_amd::PackMoments, pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"));
+    m.def("unpack_moments", &vet_amd::UnpackMoments, pybind11::arg("exp_avg"), pybind11::arg("exp_avg_sq"), pybind11::arg("block_scale"));
     m.def(
         "fill_scene_grid_with_loss",
         [](int batch, torch::Tensor bb_min, torch::Tensor bb_length, torch::Tensor value, torch::Tensor access_count,

@@ -56,6 +56,44 @@ def MyAdam(groups, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
     return load().MyAdam([(list(ts), float(lr)) for ts, lr in groups], beta1, beta2, eps, weight_decay)
 
 
+def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weights=False, stochastic_rounding=False, seed=0,
+          capturable=False):
+    """AdamW over everything a training step has gradients for, in one launch for up to 60 tensors (vetrast_adamw_step).
+
+    groups: list of (list of parameter tensors, learning rate, weight decay). Parameters are dense CUDA tensors of float32,
+    bfloat16 or float16 in any order of dimensions; gradients are found in .grad at every step.
+    moment_bits: 32, or 8 for moments of a byte each with two scale bytes for every 128 elements. master_weights: 16-bit
+    parameters have float32 masters with the optimiser. stochastic_rounding: bfloat16 parameters without masters are rounded
+    by random bits, a function of `seed`, step and element. capturable: the step count lies on the device, so that steps may
+    be captured in a graph; device_step and lr_factor (on every group's rate) may be written between replays.
+
+    step(zero_grad=False, grad_scale=None): grad_scale is one float32 on the GPU, or what grad_norm returned; where it is not
+    finite the step changes nothing (but clears gradients with zero_grad). zero_grad(), grad_norm(max_norm, scale),
+    set_lr(group, lr), steps(), set_step(n), layout() -> [(first element, elements)] in the flat state tensors exp_avg,
+    exp_avg_sq, block_scale and master; moments() -> both as flat float32; load_moments(exp_avgs, exp_avg_sqs, step),
+    reload_master()."""
+    return load().AdamW([(list(ts), float(lr), float(wd)) for ts, lr, wd in groups], beta1, beta2, eps, int(moment_bits),
+                        bool(master_weights), bool(stochastic_rounding), int(seed), bool(capturable))
+
+
+def grad_norm(gradients, max_norm=0.0, scale=1.0):
+    """The 2-norm of `scale` times all gradients together and the factor that brings it to at most max_norm (`scale` times
+    min(1, max_norm / norm); just `scale` with max_norm <= 0; NaN for a norm that is not finite), as float32 [2] on the GPU
+    (vetrast_gradient_norm). AdamW.step takes it as grad_scale without a wait on the host."""
+    return load().grad_norm(list(gradients), float(max_norm), float(scale))
+
+
+def pack_moments(exp_avgs, exp_avg_sqs):
+    """First and second moments of a list of float32 tensors rounded to codes of 8 bits (vetrast_pack_moments): flat uint8
+    codes of either, each tensor at a multiple of 128 elements, and their scales [blocks, 2]."""
+    return load().pack_moments(list(exp_avgs), list(exp_avg_sqs))
+
+
+def unpack_moments(exp_avg, exp_avg_sq, block_scale):
+    """What codes and scales as AdamW(moment_bits=8) and pack_moments hold them stand for: two flat float32 tensors."""
+    return load().unpack_moments(exp_avg, exp_avg_sq, block_scale)
+
+
 def fill_scene_grid_with_loss(batch, cell_bb_min, cell_bb_length, cell_value, cell_access_count, views, poses_se3,
                               intrinsics, loss_img):
     """PointRendererCache::FillSceneGridWithLoss of the reference (src/lib/rendering/RenderForward.cu:763-791): adds
