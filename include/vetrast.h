@@ -360,23 +360,25 @@ int vetrast_adam_step(vetrast_ctx* ctx, const vetrast_adam_args* args, void* str
 
 /* ---- AdamW over lists of tensors ----------------------------------------------------------------------------------
  * The optimiser of everything a training step has gradients for, descriptors and render network alike, in as few launches
- * as the list needs (one for up to 60 tensors). Per element, with t the group's step:
+ * as the list needs (one for up to 120 tensors). Per element, with t the group's step:
  *   g = grad * *grad_scale;  m = beta1 * m + (1 - beta1) * g;  v = beta2 * v + ((1 - beta2) * g) * g
  *   param = (1 - lr * weight_decay) * param - lr / (1 - beta1^t) * (m / (sqrt(v) * (1 / sqrt(1 - beta2^t)) + eps))
- * in 32 bits, every operation rounded on its own. The reference steps its network with torch's Adam, one tensor at a time;
- * with weight_decay 0 this is the same update.
+ * in 32 bits; the moments are rounded after every operation, in this order. The reference steps its network with torch's
+ * Adam, one tensor at a time; with weight_decay 0 this is the same update.
  *
- * Moments in 8 bits. A tensor's elements form blocks of VETRAST_MOMENT_BLOCK from its first element on. A block has two
- * scale bytes, D of the first and of the second moment, and a code c stands for
+ * State. The moments of all tensors lie in flat arrays that the caller owns, and so do float32 masters of 16-bit parameters
+ * where wanted. Tensor k has the elements from `first` on, a multiple of VETRAST_MOMENT_BLOCK, and the arrays hold whole
+ * blocks: VETRAST_MOMENT_BLOCK * ceil(n / VETRAST_MOMENT_BLOCK) elements a tensor, zero behind its last one (the step keeps
+ * them zero). Zeroed memory is the state before the first step.
+ *
+ * Moments in 8 bits. A block has two scale bytes, D of the first and of the second moment, and a code c stands for
  *   float(bits = (c << 20) + (D << 23)) - 2^(D - 127)
  * i.e. a float with three mantissa bits, moved so that zero is a code and the values next to it are evenly spaced. The first
  * moment's code is 7 such bits below a sign bit and spans 15 binades below the block's largest value, the second's is 8 bits
  * and spans 31. Codes are rounded up or down by random bits (unbiased), since beta2 = 0.999 moves the second moment by less
  * than half a step of 8 bits at a time: rounded to nearest it settles at a quarter of its value. A second moment above zero
- * stays above zero. A block that meets a value that is not finite, or above 3.19e38, has D = 255 and reads as NaN from then on, all
- * of it. Zeroed memory is a state of zeros.
- * Code arrays are whole blocks long: VETRAST_MOMENT_BLOCK * ceil(n / VETRAST_MOMENT_BLOCK) bytes, 8-byte aligned, zero behind
- * the last element; scale bytes: two for every block, 2-byte aligned. */
+ * stays above zero. A block that meets a value that is not finite, or above 3.19e38, has D = 255 and reads as NaN from then
+ * on, all of it. */
 #define VETRAST_MOMENT_BLOCK 128
 
 typedef enum vetrast_dtype
@@ -388,17 +390,13 @@ typedef enum vetrast_dtype
 
 typedef struct vetrast_adamw_tensor
 {
-    void* param;          /* device [n] of param_type, updated in place */
-    void* grad;           /* device [n] of grad_type; cleared with zero_grad */
-    void* copy;           /* optional, device [n] of copy_type: receives param rounded to nearest; needs a float32 param */
-    void* exp_avg;        /* device float [n], or uint8 codes with moment_bits = 8 */
-    void* exp_avg_sq;     /* the same */
-    uint8_t* block_scale; /* device [ceil(n / VETRAST_MOMENT_BLOCK)][2] with moment_bits = 8, else unused */
-    int64_t n;            /* >= 0; every array is contiguous, aligned to its element at least */
-    int64_t first_number; /* multiple of VETRAST_MOMENT_BLOCK: where the tensor's elements stand in the stream of random bits
-                             (modulo 2^33). Tensors of one optimiser should not overlap there. */
-    int32_t param_type, grad_type, copy_type; /* vetrast_dtype; copy_type: BF16 or F16 */
+    void* param;   /* device [n] of param_type, contiguous, aligned to its element; updated in place */
+    void* grad;    /* device [n] of grad_type, the same; cleared with zero_grad */
+    int64_t n;     /* >= 0 */
+    int64_t first; /* its place in the flat arrays and, modulo 2^33, in the stream of random bits */
+    int32_t param_type, grad_type; /* vetrast_dtype */
     int32_t group;
+    int32_t reserved;
 } vetrast_adamw_tensor;
 
 typedef struct vetrast_adamw_group
@@ -423,10 +421,14 @@ typedef struct vetrast_adamw_args
     const vetrast_adamw_tensor* tensors; /* host [num_tensors] */
     const vetrast_adamw_group* groups;   /* host [num_groups] */
     int32_t num_tensors, num_groups;     /* num_groups <= VETRAST_ADAMW_MAX_GROUPS */
-    double beta1, beta2, eps;
+    void* exp_avg;        /* device float [], or uint8 [] with moment_bits = 8; 16-byte aligned like all flat arrays */
+    void* exp_avg_sq;     /* the same */
+    uint8_t* block_scale; /* with moment_bits = 8: device [elements / VETRAST_MOMENT_BLOCK][2] */
+    float* master;        /* optional, device: 16-bit parameters are stepped here, and receive the result rounded to nearest */
+    double beta1, beta2, eps;    /* eps >= FLT_MIN: a second moment of zero divides by it */
     int32_t moment_bits;         /* 32 or 8 */
-    int32_t stochastic_rounding; /* BF16 parameters are rounded by random bits instead of to nearest */
-    uint64_t seed;               /* of the random bits; they are a function of seed, step and element */
+    int32_t stochastic_rounding; /* BF16 parameters without master are rounded by random bits instead of to nearest */
+    uint64_t seed;               /* of the random bits; they are a function of seed, step and place */
     int32_t zero_grad;           /* gradients are cleared in the same pass */
     int32_t reserved;
     const float* grad_scale; /* optional, device: gradients are multiplied by it. Where it is not finite the step is left
@@ -435,7 +437,7 @@ typedef struct vetrast_adamw_args
     void* device_state;      /* optional, device; see above */
 } vetrast_adamw_args;
 #define VETRAST_ADAMW_MAX_GROUPS 1024
-/* Tensors of a call must not overlap in memory. Enqueues kernels only; allocates nothing. */
+/* Tensors of a call must not overlap in memory or in the flat arrays. Enqueues kernels only; allocates nothing. */
 int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* args, void* stream);
 
 /* The 2-norm of all gradients together and the factor that clips it:
@@ -463,18 +465,25 @@ size_t vetrast_gradient_norm_workspace_bytes(const vetrast_gradient* gradients, 
 int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* args, void* stream);
 
 /* Moments to 8 bits, rounded to nearest (ties away from zero), and back: a run with moments in 32 bits is continued in 8 and
- * the other way round. Any alignment of the floats. */
+ * the other way round. Packing writes whole blocks, zeros behind a tensor's last element. */
 typedef struct vetrast_moment_tensor
 {
-    float* exp_avg;          /* device [n] */
-    float* exp_avg_sq;       /* device [n]; >= 0 */
-    uint8_t* exp_avg_code;   /* device, whole blocks, 8-byte aligned; as in vetrast_adamw_tensor */
-    uint8_t* exp_avg_sq_code;
-    uint8_t* block_scale;
+    float* exp_avg;    /* device [n], contiguous, aligned to 4 bytes */
+    float* exp_avg_sq; /* the same; its magnitudes are taken */
     int64_t n;
+    int64_t first;     /* place in the flat arrays, a multiple of VETRAST_MOMENT_BLOCK */
 } vetrast_moment_tensor;
-int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream);
-int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream);
+typedef struct vetrast_moments_args
+{
+    const vetrast_moment_tensor* tensors; /* host [num_tensors] */
+    int32_t num_tensors;
+    int32_t reserved;
+    uint8_t* exp_avg; /* the flat arrays of vetrast_adamw_args with moment_bits = 8 */
+    uint8_t* exp_avg_sq;
+    uint8_t* block_scale;
+} vetrast_moments_args;
+int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream);
+int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream);
 
 /* Error lifting: adds the per-pixel error of one rendered view to every cell of the scene grid whose projection covers
  * the pixel. Replaces PointRendererCache::FillSceneGridWithLoss and its kernel FillSceneGridWithLossRasterize

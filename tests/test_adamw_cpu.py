@@ -27,7 +27,8 @@ def ctx():
 def test_every_struct_field_sits_where_the_c_compiler_puts_it(tmp_path):
     pairs = [("vetrast_adamw_tensor", abi.AdamWTensor), ("vetrast_adamw_group", abi.AdamWGroup), ("vetrast_adamw_args", abi.AdamWArgs),
              ("vetrast_adamw_device_state", abi.AdamWDeviceState), ("vetrast_gradient", abi.Gradient),
-             ("vetrast_gradient_norm_args", abi.GradientNormArgs), ("vetrast_moment_tensor", abi.MomentTensor)]
+             ("vetrast_gradient_norm_args", abi.GradientNormArgs), ("vetrast_moment_tensor", abi.MomentTensor),
+             ("vetrast_moments_args", abi.MomentsArgs)]
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "vetrast.h"', 'int main(void) {']
     for name, mirror in pairs:
         lines.append(f'printf("{name} size %zu\\n", sizeof({name}));')
@@ -48,7 +49,7 @@ def test_every_struct_field_sits_where_the_c_compiler_puts_it(tmp_path):
 
 def step_args(bits=8, **changes):
     t, g, a = abi.AdamWTensor(), abi.AdamWGroup(), abi.AdamWArgs()
-    t.param = t.grad = t.exp_avg = t.exp_avg_sq = t.block_scale = AT
+    t.param = t.grad = a.exp_avg = a.exp_avg_sq = a.block_scale = AT
     t.n = 10
     g.lr, g.step = 1e-3, 1
     a.num_tensors = a.num_groups = 1
@@ -65,19 +66,18 @@ def step_args(bits=8, **changes):
     dict(a_num_tensors=-1), dict(a_num_groups=-1), dict(a_num_groups=abi.ADAMW_MAX_GROUPS + 1), dict(a_num_groups=0),
     dict(a_moment_bits=16), dict(a_moment_bits=0), dict(a_beta1=1.0), dict(a_beta1=-0.1), dict(a_beta1=float("nan")), dict(a_beta2=1.0),
     dict(a_beta2=float("nan")), dict(a_eps=0.0), dict(a_eps=-1e-8), dict(a_eps=float("nan")), dict(a_eps=float("inf")), dict(a_eps=1e-60),
-    dict(a_grad_scale=AT + 2), dict(a_device_state=AT + 8), dict(g_step=0), dict(g_step=-3), dict(g_lr=float("nan")),
+    dict(a_eps=1e-39), dict(a_grad_scale=AT + 2), dict(a_device_state=AT + 8), dict(g_step=0), dict(g_step=-3), dict(g_lr=float("nan")),
     dict(g_lr=float("inf")), dict(g_weight_decay=float("nan")), dict(t_n=-1), dict(t_group=1), dict(t_group=-1), dict(t_param_type=3),
-    dict(t_param_type=-1), dict(t_grad_type=3), dict(t_first_number=-128), dict(t_first_number=64), dict(t_param=None), dict(t_grad=None),
-    dict(t_exp_avg=None), dict(t_exp_avg_sq=None), dict(t_block_scale=None), dict(t_param=AT + 2), dict(t_grad=AT + 2),
-    dict(t_param=AT + 1, t_param_type=1), dict(t_grad=AT + 1, t_grad_type=2), dict(t_copy=AT), dict(t_copy=AT, t_copy_type=1, t_param_type=1),
-    dict(t_copy=AT, t_copy_type=3), dict(t_copy=AT + 1, t_copy_type=1), dict(t_exp_avg=AT + 4), dict(t_exp_avg_sq=AT + 4),
-    dict(t_block_scale=AT + 1)], ids=str)
+    dict(t_param_type=-1), dict(t_grad_type=3), dict(t_first=-128), dict(t_first=64), dict(t_first=1 << 38), dict(t_n=(1 << 38) + 1),
+    dict(t_param=None), dict(t_grad=None), dict(a_exp_avg=None), dict(a_exp_avg_sq=None), dict(a_block_scale=None), dict(t_param=AT + 2),
+    dict(t_grad=AT + 2), dict(t_param=AT + 1, t_param_type=1), dict(t_grad=AT + 1, t_grad_type=2), dict(a_exp_avg=AT + 8),
+    dict(a_exp_avg_sq=AT + 4), dict(a_block_scale=AT + 2), dict(a_master=AT + 4)], ids=str)
 def test_step_refuses(change, lib, ctx):
     assert lib.vetrast_adamw_step(ctx, C.byref(step_args(**change)), None) == abi.ERR_INVALID_ARG
 
 
 def test_step_refuses_in_32_bits_too(lib, ctx):
-    for change in (dict(t_exp_avg=AT + 2), dict(t_exp_avg_sq=AT + 1), dict(t_param=None)):
+    for change in (dict(a_exp_avg=AT + 8), dict(a_exp_avg_sq=AT + 1), dict(a_exp_avg=None), dict(t_param=None)):
         assert lib.vetrast_adamw_step(ctx, C.byref(step_args(bits=32, **change)), None) == abi.ERR_INVALID_ARG
     a = step_args()
     a.tensors = None
@@ -134,18 +134,20 @@ def test_norm_workspace(lib, ctx):
     assert lib.vetrast_gradient_norm(None, C.byref(norm_args()), None) == lib.vetrast_gradient_norm(ctx, None, None) == abi.ERR_INVALID_ARG
 
 
-@pytest.mark.parametrize("change", [dict(n=-1), dict(exp_avg=None), dict(exp_avg_sq=None), dict(exp_avg_code=None), dict(exp_avg_sq_code=None),
-                                    dict(block_scale=None), dict(exp_avg=AT + 2), dict(exp_avg_sq=AT + 1), dict(exp_avg_code=AT + 4),
-                                    dict(exp_avg_sq_code=AT + 4), dict(block_scale=AT + 1)], ids=str)
+@pytest.mark.parametrize("change", [
+    dict(t_n=-1), dict(t_exp_avg=None), dict(t_exp_avg_sq=None), dict(t_exp_avg=AT + 2), dict(t_exp_avg_sq=AT + 1), dict(t_first=-128),
+    dict(t_first=100), dict(t_first=1 << 38), dict(a_exp_avg=None), dict(a_exp_avg_sq=None), dict(a_block_scale=None), dict(a_exp_avg=AT + 8),
+    dict(a_exp_avg_sq=AT + 4), dict(a_block_scale=AT + 2), dict(a_num_tensors=-1), dict(a_tensors=None)], ids=str)
 def test_conversions_refuse(change, lib, ctx):
-    t = abi.MomentTensor()
-    t.exp_avg = t.exp_avg_sq = t.exp_avg_code = t.exp_avg_sq_code = t.block_scale = AT
-    t.n = 10
+    t, a = abi.MomentTensor(), abi.MomentsArgs()
+    t.exp_avg = t.exp_avg_sq = a.exp_avg = a.exp_avg_sq = a.block_scale = AT
+    t.n, a.num_tensors, a.tensors = 10, 1, C.pointer(t)
     for k, v in change.items():
-        setattr(t, k, v)
+        where, name = k.split("_", 1)
+        setattr({"t": t, "a": a}[where], name, v)
     for call in (lib.vetrast_pack_moments, lib.vetrast_unpack_moments):
-        assert call(ctx, C.byref(t), 1, None) == abi.ERR_INVALID_ARG
-        assert call(ctx, C.byref(t), -1, None) == call(ctx, None, 1, None) == call(None, C.byref(t), 1, None) == abi.ERR_INVALID_ARG
+        assert call(ctx, C.byref(a), None) == abi.ERR_INVALID_ARG
+        assert call(None, C.byref(a), None) == call(ctx, None, None) == abi.ERR_INVALID_ARG
 
 
 @pytest.mark.parametrize("size", [1e-44, 1e-38, 1e-20, 1.0, 1.9374999, 1.9375, 1.9999999, 1e30, 3.4e38])

@@ -125,10 +125,9 @@ ADAMW_MAX_GROUPS = 1024
 
 class AdamWTensor(C.Structure):
     _fields_ = [
-        ("param", C.c_void_p), ("grad", C.c_void_p), ("copy", C.c_void_p),
-        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("block_scale", C.c_void_p),
-        ("n", C.c_int64), ("first_number", C.c_int64),
-        ("param_type", C.c_int32), ("grad_type", C.c_int32), ("copy_type", C.c_int32), ("group", C.c_int32),
+        ("param", C.c_void_p), ("grad", C.c_void_p),
+        ("n", C.c_int64), ("first", C.c_int64),
+        ("param_type", C.c_int32), ("grad_type", C.c_int32), ("group", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -144,6 +143,7 @@ class AdamWArgs(C.Structure):
     _fields_ = [
         ("tensors", C.POINTER(AdamWTensor)), ("groups", C.POINTER(AdamWGroup)),
         ("num_tensors", C.c_int32), ("num_groups", C.c_int32),
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("block_scale", C.c_void_p), ("master", C.c_void_p),
         ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
         ("moment_bits", C.c_int32), ("stochastic_rounding", C.c_int32),
         ("seed", C.c_uint64),
@@ -165,10 +165,13 @@ class GradientNormArgs(C.Structure):
 
 
 class MomentTensor(C.Structure):
+    _fields_ = [("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("n", C.c_int64), ("first", C.c_int64)]
+
+
+class MomentsArgs(C.Structure):
     _fields_ = [
-        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
-        ("exp_avg_code", C.c_void_p), ("exp_avg_sq_code", C.c_void_p), ("block_scale", C.c_void_p),
-        ("n", C.c_int64),
+        ("tensors", C.POINTER(MomentTensor)), ("num_tensors", C.c_int32), ("reserved", C.c_int32),
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("block_scale", C.c_void_p),
     ]
 
 
@@ -262,8 +265,8 @@ SYMBOLS = {
     "vetrast_adamw_step": (C.c_int, [C.c_void_p, C.POINTER(AdamWArgs), C.c_void_p]),
     "vetrast_gradient_norm_workspace_bytes": (C.c_size_t, [C.POINTER(Gradient), C.c_int32]),
     "vetrast_gradient_norm": (C.c_int, [C.c_void_p, C.POINTER(GradientNormArgs), C.c_void_p]),
-    "vetrast_pack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentTensor), C.c_int32, C.c_void_p]),
-    "vetrast_unpack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentTensor), C.c_int32, C.c_void_p]),
+    "vetrast_pack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
+    "vetrast_unpack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
     "vetrast_lift_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "vetrast_lift_workspace_bytes_for_image": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     "vetrast_lift_error": (C.c_int, [C.c_void_p, C.POINTER(LiftArgs), C.c_void_p]),

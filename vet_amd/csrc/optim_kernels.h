@@ -1,61 +1,184 @@
 // Optimiser kernels over lists of tensors: AdamW with moments in 32 or 8 bits, the norm of all gradients, moments to 8 bits and back.
+//
+// A launch takes a table of tensors in its arguments (no copy to the device, nothing to keep, and what a graph captures is whole). It is
+// cut into chunks of kOptimChunk elements, 8 a thread, and every workgroup goes through chunks blockIdx.x, blockIdx.x + gridDim.x, ...
 #pragma once
 #include "common.h"
 
 namespace vetrast
 {
 constexpr uint32_t kOptimChunk   = 8 * kBlock;  // elements a workgroup takes at a time: 8 a thread
-constexpr int kAdamWEntries      = 60;          // tensors of one launch: what 4 KB of kernel arguments hold
-constexpr int kAdamWGroups       = 8;           // ... and of how many groups
-constexpr int kNormEntries       = 160;
-constexpr int kMomentEntries     = 80;
 constexpr int kMomentBlock       = VETRAST_MOMENT_BLOCK;
-constexpr uint32_t kMomentMargin = 0x100100;    // see code_base
+constexpr uint32_t kMomentMargin = 0x100100;  // see code_base
 static_assert(kOptimChunk % kMomentBlock == 0 && kMomentBlock == 16 * 8, "16 lanes of 8 elements hold a block");
 
-enum { kAligned = 1u << 6, kHasCopy = 1u << 7 };  // bits of AdamWEntry::types, above param | grad << 2 | copy << 4; group << 8
-
-struct AdamWEntry
+// Tables hold up to 64 * GROUPS entries: lane k of a wave knows which chunk of the launch is the first of entries k, k + 64, ...
+template <int GROUPS>
+struct ChunkFinder
 {
-    void* param;
-    void* grad;
-    void* copy;
-    void* m;
-    void* v;
-    uint8_t* scale;
-    uint32_t n;
-    uint32_t first;  // chunk of the launch that is this entry's first
-    uint32_t types;
-    uint32_t pair;   // number of the entry's first pair of elements in the stream of random bits
+    uint32_t begins[GROUPS];
+    template <class Launch>
+    __device__ __forceinline__ explicit ChunkFinder(const Launch& a)
+    {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q)
+        {
+            const uint32_t k = q * kWave + threadIdx.x % kWave;
+            begins[q]        = k < a.entries ? a.e[k].first_chunk : 0xFFFFFFFFu;
+        }
+    }
+    // The entry of a chunk; all lanes of the wave take part.
+    __device__ __forceinline__ uint32_t operator()(uint32_t chunk) const
+    {
+        uint32_t k = 0;
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) k += (uint32_t)__popcll(__ballot(begins[q] <= chunk));
+        return k - 1u;
+    }
+};
+constexpr int finder_groups(int entries) { return (entries + kWave - 1) / kWave; }
+
+// ---- eight elements of a tensor ----------------------------------------------------------------------------------------
+
+// As they lie in memory, 32 bytes or (16-bit types) 16. Loads of several arrays are under way before the first is looked at.
+struct RawEight
+{
+    uint4 a, b;
 };
 
-struct AdamWGroup
+// Elements i ... i + 7 of p, those from `count` on as zeros. whole: all eight are there and p + i is 16-byte aligned.
+__device__ __forceinline__ RawEight load_raw(const void* p, uint32_t type, uint32_t i, uint32_t count, bool whole)
 {
-    float step_size;     // lr / (1 - beta1^step)
-    float keep;          // 1 - lr * weight_decay
-    float inv_sqrt_bc2;  // 1 / sqrt(1 - beta2^step)
-    uint32_t key;        // of this step's random bits
-};
+    RawEight r;
+    r.a = r.b = make_uint4(0, 0, 0, 0);
+    if (type == VETRAST_F32)
+    {
+        const uint32_t* x = (const uint32_t*)p + i;
+        if (whole)
+        {
+            r.a = ((const uint4*)x)[0];
+            r.b = ((const uint4*)x)[1];
+        }
+        else if (count)
+        {
+            uint32_t w[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) w[j] = x[min(j, count - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) w[j] = j < count ? w[j] : 0u;
+            r.a = make_uint4(w[0], w[1], w[2], w[3]);
+            r.b = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    }
+    else
+    {
+        const uint16_t* x = (const uint16_t*)p + i;
+        if (whole) r.a = *(const uint4*)x;
+        else if (count)
+        {
+            uint32_t w[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) w[j] = x[min(j, count - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) w[j] = j < count ? w[j] : 0u;
+            r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        }
+    }
+    return r;
+}
 
-struct AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel leaves for the step's launches
+__device__ __forceinline__ void store_raw(void* p, uint32_t type, uint32_t i, uint32_t count, bool whole, const RawEight& r)
 {
-    vetrast_adamw_device_state state;
-    AdamWGroup group[1];
-};
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == VETRAST_F32)
+    {
+        uint32_t* x = (uint32_t*)p + i;
+        if (whole)
+        {
+            ((uint4*)x)[0] = r.a;
+            ((uint4*)x)[1] = r.b;
+        }
+        else
+        {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (j < count) x[j] = w[j];
+        }
+    }
+    else
+    {
+        uint16_t* x = (uint16_t*)p + i;
+        if (whole) *(uint4*)x = r.a;
+        else
+        {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (j < count) x[j] = (uint16_t)(w[j / 2] >> 16 * (j % 2));
+        }
+    }
+}
 
-struct AdamWLaunch
+__device__ __forceinline__ void to_floats(const RawEight& r, uint32_t type, float* x)
 {
-    AdamWEntry e[kAdamWEntries];
-    AdamWGroup g[kAdamWGroups];
-    const float* grad_scale;
-    const AdamWDevice* device;  // where set, g[].key are places in device->group
-    uint32_t entries, chunks;
-    float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
-    int zero_grad, stochastic;
-};
-static_assert(sizeof(AdamWLaunch) <= 4096, "kernel arguments");
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == VETRAST_F32)
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+    }
+    else if (type == VETRAST_BF16)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            x[2 * j]     = __uint_as_float(w[j] << 16);
+            x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+    }
+    else
+    {
+        typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            const Half2 h = __builtin_bit_cast(Half2, w[j]);
+            x[2 * j]      = (float)h[0];
+            x[2 * j + 1]  = (float)h[1];
+        }
+    }
+}
 
-// A step's key of the random bits: two rounds of a 64-bit mixing function (the finalizer of splitmix64) over seed and step.
+// Rounded to nearest.
+__device__ __forceinline__ RawEight from_floats(const float* x, uint32_t type)
+{
+    RawEight r;
+    r.b = make_uint4(0, 0, 0, 0);
+    if (type == VETRAST_F32)
+    {
+        r.a = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        r.b = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+        return r;
+    }
+    uint32_t w[4];
+    if (type == VETRAST_BF16)
+    {
+        typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, (Pair){(__bf16)x[2 * j], (__bf16)x[2 * j + 1]});
+    }
+    else
+    {
+        typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, (Pair){(_Float16)x[2 * j], (_Float16)x[2 * j + 1]});
+    }
+    r.a = make_uint4(w[0], w[1], w[2], w[3]);
+    return r;
+}
+
+// ---- random bits -------------------------------------------------------------------------------------------------------
+
+// A step's key: two rounds of a 64-bit mixing function (the finalizer of splitmix64) over seed and step.
 __host__ __device__ inline uint64_t mix64(uint64_t z)
 {
     z += 0x9E3779B97F4A7C15ull;
@@ -68,17 +191,31 @@ __host__ __device__ inline uint32_t step_key(uint64_t seed, int64_t step)
     return (uint32_t)mix64(mix64(seed) + (uint64_t)step);
 }
 
-// 32 random bits for a pair of elements. The lower 20 are the first element's, the upper 20 the second's.
-__device__ __forceinline__ uint32_t pair_bits(uint32_t pair, uint32_t key)
+// 20 random bits for each of 8 elements, the first of which is half of pair number `pair`: 32 bits of a hash serve two elements, the
+// lower 20 and the upper 20 of them (products of 32 bits take four times as long as other instructions, and the 8-bit step is
+// bound by instructions).
+__device__ __forceinline__ void random_eight(uint32_t pair, uint32_t key, uint32_t* r)
 {
-    uint32_t x = pair * 0x9E3779B1u;
-    x ^= x >> 15;
-    x ^= key;
-    x *= 0xBB67AE85u;
-    x ^= x >> 15;
-    x *= 0xA54FF53Bu;
-    return x ^ (x >> 15);
+    const uint32_t start = pair * 0x9E3779B1u;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+    {
+        uint32_t x = start + j * 0x9E3779B1u;
+        x          = x ^ (x >> 15) ^ key;
+        x *= 0xBB67AE85u;
+        x ^= x >> 15;
+        x *= 0xA54FF53Bu;
+        x ^= x >> 15;
+        r[2 * j]     = x & 0xFFFFFu;
+        r[2 * j + 1] = x >> 12;
+    }
 }
+
+// Odd factors make of an element's bits others that go with them without correlation to speak of (measured over 2^20 elements).
+__device__ __forceinline__ uint32_t second_bits(uint32_t r) { return __umul24(r, 0x5D3u) & 0xFFFFFu; }
+__device__ __forceinline__ uint32_t parameter_bits(uint32_t r) { return __umul24(r, 0xE2Bu) >> 4 & 0xFFFFu; }
+
+// ---- moments in 8 bits -------------------------------------------------------------------------------------------------
 
 // The largest of 16 lanes' values, in all of them (a row of a wave).
 __device__ __forceinline__ uint32_t row_max(uint32_t v)
@@ -99,132 +236,148 @@ __device__ __forceinline__ uint32_t code_base(uint32_t largest)
     return exponent >= 255 ? 255u : (uint32_t)max(exponent - BINADES, 1);
 }
 
-// Code of magnitude x, `r` in [0, 2^20): x + 2^(D-127) is a float whose bits less those of 2^(D-127) are the code, 20 bits below it
-// decide between it and the next. Evenly spaced values between two codes, so random r leaves the mean as it is.
-__device__ __forceinline__ uint32_t magnitude_code(float x, uint32_t base_bits, uint32_t r)
+// A code stands for float(bits = (code << 20) + base) - float(base). Magnitude x gets it from x + float(base), whose bits less those of
+// the base are the code, with 20 bits below it that decide between it and the next: values between two codes are evenly
+// spaced, so r in [0, 2^20) that is random leaves the mean as it is.
+__device__ __forceinline__ uint32_t offset_bits(float x, uint32_t base, uint32_t r)
 {
-    return (__float_as_uint(x + __uint_as_float(base_bits)) + r - base_bits) >> 20;
-}
-__device__ __forceinline__ float code_value(uint32_t code, uint32_t base_bits)
-{
-    return __uint_as_float((code << 20) + base_bits) - __uint_as_float(base_bits);
+    return __float_as_uint(fabsf(x) + __uint_as_float(base)) + r - base;
 }
 
-// Eight codes of both moments as two pairs of words, from the values and their random bits.
-__device__ __forceinline__ void encode_moments(const float* m, const float* v, const uint32_t* rm, const uint32_t* rv, uint2& mc, uint2& vc, uint32_t& scale)
+__device__ __forceinline__ float code_value(uint32_t code, uint32_t base)
 {
-    uint32_t top_m = 0, top_v = 0;
+    return __uint_as_float((code << 20) + base) - __uint_as_float(base);
+}
+
+// The middle one of three.
+__device__ __forceinline__ uint32_t middle(uint32_t a, uint32_t b, uint32_t c)
+{
+    return max(min(a, b), min(max(a, b), c));
+}
+
+struct Codes
+{
+    uint2 m, v;      // eight each
+    uint32_t scale;  // of the block: D of the first moment, of the second above it
+};
+
+// m, v: of this lane's eight elements, a block is a row of 16 lanes. rm, rv: their random bits. v >= 0.
+// Maxima of floats pass over NaN, and of integers do not. The second moment is looked at as integers; where the first is not finite
+// after a step, the second is not either, as it has its square, or the block was lost before. lost: the block's first moment is not
+// finite, whatever the second says.
+__device__ __forceinline__ Codes encode_moments(const float* m, const float* v, const uint32_t* rm, const uint32_t* rv, bool lost)
+{
+    float top_m    = 0.f;
+    uint32_t top_v = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
-        top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-        top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        top_m = fmaxf(top_m, fabsf(m[j]));
+        top_v = max(top_v, __float_as_uint(v[j]));
     }
-    const uint32_t dm = code_base<15>(row_max(top_m)), dv = code_base<31>(row_max(top_v));
+    const uint32_t dv = code_base<31>(row_max(top_v));
+    uint32_t dm       = code_base<15>(row_max(__float_as_uint(top_m)));
+    if (dv == 255u)
+    {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+        dm = code_base<15>(row_max(top));
+    }
+    if (lost) dm = 255u;
     const uint32_t bm = dm << 23, bv = dv << 23;
-    uint32_t a[2] = {0, 0}, b[2] = {0, 0};
+    uint32_t a[8], b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
-        const uint32_t bits = __float_as_uint(m[j]);
-        const uint32_t cm   = magnitude_code(fabsf(m[j]), bm, rm[j]) | ((bits >> 31) << 7);
-        const uint32_t cv   = max(magnitude_code(v[j], bv, rv[j]), min(__float_as_uint(v[j]), 1u));
-        a[j / 4] |= cm << (8 * (j % 4));
-        b[j / 4] |= cv << (8 * (j % 4));
+        // seven bits of code to the top, below the sign
+        a[j] = (offset_bits(m[j], bm, rm[j]) << 4 & 0x7FFFFFFFu) | (__float_as_uint(m[j]) & 0x80000000u);
+        // above zero is at least code 1: a code is never above a value's own bits, so the middle one says so
+        b[j] = middle(__float_as_uint(v[j]), 1u, offset_bits(v[j], bv, rv[j]) >> 20);
     }
-    mc    = dm == 255 ? make_uint2(0, 0) : make_uint2(a[0], a[1]);  // code 0 at D = 255: infinity less infinity
-    vc    = dv == 255 ? make_uint2(0, 0) : make_uint2(b[0], b[1]);
-    scale = dm | (dv << 8);
+    Codes c;
+    uint32_t w[2], x[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+    {
+        const uint32_t low  = __builtin_amdgcn_perm(a[4 * q + 1], a[4 * q], 0x0C0C0703);  // top bytes
+        const uint32_t high = __builtin_amdgcn_perm(a[4 * q + 3], a[4 * q + 2], 0x07030C0C);
+        w[q]                = low | high;
+        x[q]                = b[4 * q] | b[4 * q + 1] << 8 | b[4 * q + 2] << 16 | b[4 * q + 3] << 24;
+    }
+    c.m     = dm == 255u ? make_uint2(0, 0) : make_uint2(w[0], w[1]);  // code 0 at D = 255: infinity less infinity
+    c.v     = dv == 255u ? make_uint2(0, 0) : make_uint2(x[0], x[1]);
+    c.scale = dm | dv << 8;
+    return c;
 }
 
-__device__ __forceinline__ void decode_moments(uint2 mc, uint2 vc, uint32_t scale, float* m, float* v)
+__device__ __forceinline__ void decode_moments(const Codes& c, float* m, float* v)
 {
-    const uint32_t bm = (scale & 255u) << 23, bv = ((scale >> 8) & 255u) << 23;
+    const uint32_t bm = (c.scale & 255u) << 23, bv = c.scale >> 8 << 23;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
-        const uint32_t wm = j < 4 ? mc.x : mc.y, wv = j < 4 ? vc.x : vc.y;
-        const uint32_t cm = (wm >> (8 * (j % 4))) & 255u, cv = (wv >> (8 * (j % 4))) & 255u;
-        m[j] = copysignf(code_value(cm & 127u, bm), __uint_as_float(cm << 24));
-        v[j] = code_value(cv, bv);
+        const uint32_t wm = j < 4 ? c.m.x : c.m.y, wv = j < 4 ? c.v.x : c.v.y;
+        m[j] = copysignf(code_value(wm >> 8 * (j % 4) & 127u, bm), __uint_as_float(wm << (24 - 8 * (j % 4))));
+        v[j] = code_value(wv >> 8 * (j % 4) & 255u, bv);
     }
 }
 
-// Elements of the three types as floats and back, eight at a time or one.
-template <int T>
-struct Element;
-template <>
-struct Element<VETRAST_F32>
+// ---- AdamW -------------------------------------------------------------------------------------------------------------
+
+struct AdamWEntry
 {
-    using type = float;
-    static __device__ __forceinline__ float get(float x) { return x; }
-    static __device__ __forceinline__ float put(float x) { return x; }
+    void* param;
+    void* grad;
+    uint32_t n;
+    uint32_t first_chunk;  // of the launch
+    uint32_t block;        // place in the flat arrays
+    uint32_t flags;        // kAdamW..., slot of the group from bit 8 on
 };
-template <>
-struct Element<VETRAST_BF16>
+enum
 {
-    using type = __bf16;
-    static __device__ __forceinline__ float get(__bf16 x) { return (float)x; }
-    static __device__ __forceinline__ __bf16 put(float x) { return (__bf16)x; }
-};
-template <>
-struct Element<VETRAST_F16>
-{
-    using type = _Float16;
-    static __device__ __forceinline__ float get(_Float16 x) { return (float)x; }
-    static __device__ __forceinline__ _Float16 put(float x) { return (_Float16)x; }
+    kAdamWParam   = 3,       // type
+    kAdamWGrad    = 3 << 2,  // type
+    kAdamWAligned = 1 << 4,  // param and grad to 16 bytes
+    kAdamWMaster  = 1 << 5
 };
 
-// `count` of the 8 elements from p + i on (the others read as zero); `whole`: all eight, and 16-byte aligned.
-template <int T>
-__device__ __forceinline__ void load_eight(const void* p_, uint32_t i, uint32_t count, bool whole, float* x)
+struct AdamWGroup
 {
-    using E    = typename Element<T>::type;
-    const E* p = (const E*)p_ + i;
-    if (whole)
-    {
-        typedef E Vec __attribute__((ext_vector_type(16 / sizeof(E))));
-        constexpr int W = 16 / sizeof(E);
-#pragma unroll
-        for (int q = 0; q < 8 / W; ++q)
-        {
-            const Vec w = ((const Vec*)p)[q];
-#pragma unroll
-            for (int j = 0; j < W; ++j) x[q * W + j] = Element<T>::get(w[j]);
-        }
-    }
-    else
-    {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) x[j] = j < count ? Element<T>::get(p[j]) : 0.f;
-    }
-}
+    float step_size;     // lr / (1 - beta1^step)
+    float keep;          // 1 - lr * weight_decay
+    float inv_sqrt_bc2;  // 1 / sqrt(1 - beta2^step)
+    uint32_t key;        // of this step's random bits
+};
 
-template <int T>
-__device__ __forceinline__ void store_eight(void* p_, uint32_t i, uint32_t count, bool whole, const float* x)
+struct AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel leaves for the step's launches
 {
-    using E = typename Element<T>::type;
-    E* p    = (E*)p_ + i;
-    if (whole)
-    {
-        typedef E Vec __attribute__((ext_vector_type(16 / sizeof(E))));
-        constexpr int W = 16 / sizeof(E);
-#pragma unroll
-        for (int q = 0; q < 8 / W; ++q)
-        {
-            Vec w;
-#pragma unroll
-            for (int j = 0; j < W; ++j) w[j] = Element<T>::put(x[q * W + j]);
-            ((Vec*)p)[q] = w;
-        }
-    }
-    else
-    {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-            if (j < count) p[j] = Element<T>::put(x[j]);
-    }
-}
+    vetrast_adamw_device_state state;
+    AdamWGroup group[1];
+};
+
+constexpr int kAdamWEntries = 120;  // what 4 KB of kernel arguments hold
+constexpr int kAdamWFew     = 8;    // ... and a launch whose arguments are 400 bytes
+constexpr int kAdamWGroups  = 8;
+struct AdamWCommon
+{
+    AdamWGroup g[kAdamWGroups];
+    void* m;
+    void* v;
+    uint16_t* scale;
+    float* master;
+    const float* grad_scale;
+    const AdamWDevice* device;  // where set, g[].key are places in device->group
+    uint32_t entries, chunks;
+    float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
+    int zero_grad, stochastic, exact_root;
+};
+template <int ENTRIES>
+struct AdamWLaunch : AdamWCommon
+{
+    AdamWEntry e[ENTRIES];
+};
+static_assert(sizeof(AdamWLaunch<kAdamWEntries>) <= 4096, "kernel arguments");
 
 // Step count, learning rates and keys of a step whose count lies on the device; one thread a group.
 struct AdamWBeginGroup
@@ -242,9 +395,8 @@ struct AdamWBegin
     int first, groups, last;
 };
 
-// The groups' constants of step `state.step + 1`, or of the step before where gradients overflowed (nothing is read of them then). The
-// launch with the last groups writes the new count; each launch reads the old one, so it is a kernel of one workgroup that waits in
-// between.
+// The groups' constants of step `state.step + 1`. The launch with the last groups writes the new count, unless gradients overflowed: then
+// nothing is read of the constants.
 __global__ void __launch_bounds__(kBeginGroups) adamw_begin_kernel(const AdamWBegin a)
 {
     const bool counts  = !a.grad_scale || isfinite(*a.grad_scale);
@@ -266,167 +418,168 @@ __global__ void __launch_bounds__(kBeginGroups) adamw_begin_kernel(const AdamWBe
     if (a.last && counts && k == 0) a.device->state.step = step;
 }
 
-template <int BITS, int P, int G>
-__device__ __forceinline__ void adamw_eight(const AdamWLaunch& a, const AdamWEntry& e, const AdamWGroup& g, float grad_scale, bool leave, uint32_t i)
+template <int BITS, class Launch>
+__global__ void __launch_bounds__(kBlock) adamw_step_kernel(const Launch a)
 {
-    const uint32_t n     = e.n;
-    const uint32_t count = i < n ? min(n - i, 8u) : 0u;
-    const bool whole     = count == 8u && (e.types & kAligned);
-    const bool codes     = i < (n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
-    float gr[8], p[8], m[8], v[8];
-    if (leave)
+    const ChunkFinder<finder_groups(sizeof(a.e) / sizeof(a.e[0]))> find(a);
+    const float grad_scale = a.grad_scale ? *a.grad_scale : 1.f;
+    const bool leave       = !isfinite(grad_scale);
+    for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
     {
-        const float zero[8] = {};
-        if (a.zero_grad) store_eight<G>(e.grad, i, count, whole, zero);
-        return;
-    }
-    load_eight<G>(e.grad, i, count, whole, gr);
-    load_eight<P>(e.param, i, count, whole, p);
-    if constexpr (BITS == 32)
-    {
-        load_eight<VETRAST_F32>(e.m, i, count, whole, m);
-        load_eight<VETRAST_F32>(e.v, i, count, whole, v);
-    }
-    else
-    {
-        uint2 mc = make_uint2(0, 0), vc = make_uint2(0, 0);
-        uint32_t scale = 0;
-        if (codes)
+        const AdamWEntry& e  = a.e[find(chunk)];
+        const uint32_t flags = e.flags, n = e.n;
+        const uint32_t p_type = flags & kAdamWParam, g_type = (flags & kAdamWGrad) >> 2;
+        const uint32_t i      = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
+        const uint32_t count  = i < n ? min(n - i, 8u) : 0u;
+        const bool whole      = count == 8u && (flags & kAdamWAligned);
+        const uint32_t block  = e.block + i / kMomentBlock;
+        const size_t at       = (size_t)block * kMomentBlock + i % kMomentBlock;  // in the flat arrays
+        const bool inside     = i < (n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
+        const RawEight zero   = {};
+        if (leave)
         {
-            mc    = *(const uint2*)((const uint8_t*)e.m + i);
-            vc    = *(const uint2*)((const uint8_t*)e.v + i);
-            scale = ((const uint16_t*)e.scale)[i / kMomentBlock];
+            if (a.zero_grad) store_raw(e.grad, g_type, i, count, whole, zero);
+            continue;
         }
-        decode_moments(mc, vc, scale, m, v);
-    }
-    uint32_t rm[8];
-    if (BITS == 8 || (P == VETRAST_BF16 && a.stochastic))
-    {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
+        const bool master = flags & kAdamWMaster;
+        RawEight rg, rp = zero, r1 = zero, r2 = zero;
+        Codes codes     = {};
+        rg              = load_raw(e.grad, g_type, i, count, whole);
+        if (!master) rp = load_raw(e.param, p_type, i, count, whole);
+        if (inside)
         {
-            const uint32_t r = pair_bits(e.pair + i / 2 + j, g.key);
-            rm[2 * j]        = r & 0xFFFFFu;
-            rm[2 * j + 1]    = r >> 12;
+            if (master) rp = {((const uint4*)(a.master + at))[0], ((const uint4*)(a.master + at))[1]};
+            if constexpr (BITS == 32)
+            {
+                r1 = {((const uint4*)((float*)a.m + at))[0], ((const uint4*)((float*)a.m + at))[1]};
+                r2 = {((const uint4*)((float*)a.v + at))[0], ((const uint4*)((float*)a.v + at))[1]};
+            }
+            else
+            {
+                codes.m     = *(const uint2*)((const uint8_t*)a.m + at);
+                codes.v     = *(const uint2*)((const uint8_t*)a.v + at);
+                codes.scale = a.scale[block];
+            }
         }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-    {
-        const float x = gr[j] * grad_scale;
-        m[j]          = m[j] * a.beta1 + x * a.one_minus_beta1;
-        v[j]          = v[j] * a.beta2 + (x * a.one_minus_beta2) * x;
-        const float d = sqrtf(v[j]) * g.inv_sqrt_bc2 + a.eps;
-        p[j]          = p[j] * g.keep - g.step_size * (m[j] / d);
-    }
-    if (e.types & kHasCopy)
-    {
-        if ((e.types >> 4 & 3) == VETRAST_BF16) store_eight<VETRAST_BF16>(e.copy, i, count, whole, p);
-        else store_eight<VETRAST_F16>(e.copy, i, count, whole, p);
-    }
-    if (P == VETRAST_BF16 && a.stochastic)
-    {
+        AdamWGroup g = a.g[flags >> 8];
+        if (a.device) g = a.device->group[g.key];
+        const bool random = a.stochastic && p_type == VETRAST_BF16 && !master;
+        uint32_t r[8];
+        if (BITS == 8 || random) random_eight((uint32_t)(at / 2), g.key, r);
+
+        float x[8], p[8], m[8], v[8];
+        to_floats(rg, g_type, x);
+        to_floats(rp, master ? VETRAST_F32 : p_type, p);
+        if constexpr (BITS == 32)
+        {
+            to_floats(r1, VETRAST_F32, m);
+            to_floats(r2, VETRAST_F32, v);
+        }
+        else decode_moments(codes, m, v);
+        // Rounded after every operation: both kinds of state, and whoever steps them elsewhere, get the same bits.
 #pragma unroll
         for (int j = 0; j < 8; ++j)
         {
-            const uint32_t bits = __float_as_uint(p[j]);
-            const uint32_t r    = (rm[j] * 0xE2Bu) >> 4 & 0xFFFFu;
-            if ((bits & 0x7F800000u) != 0x7F800000u) p[j] = __uint_as_float((bits + r) & 0xFFFF0000u);
+            x[j] *= grad_scale;
+            m[j] = m[j] * a.beta1 + x[j] * a.one_minus_beta1;
+            v[j] = v[j] * a.beta2 + (x[j] * a.one_minus_beta2) * x[j];
         }
-    }
-    store_eight<P>(e.param, i, count, whole, p);
-    if constexpr (BITS == 32)
-    {
-        store_eight<VETRAST_F32>(e.m, i, count, whole, m);
-        store_eight<VETRAST_F32>(e.v, i, count, whole, v);
-    }
-    else
-    {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-            if (j >= count) m[j] = v[j] = 0.f;
-        uint32_t rv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rv[j] = rm[j] * 0x5D3u & 0xFFFFFu;
-        uint2 mc, vc;
-        uint32_t scale;
-        encode_moments(m, v, rm, rv, mc, vc, scale);
-        if (codes)
+        // With 8-bit moments root and quotient are the instructions for them, good to 1.54 half steps of float32 each, as the step is
+        // bound by instructions; with 32-bit ones it waits for memory and they are rounded to nearest. The root instruction takes
+        // values below 2^-126 for zero: eps makes up for that unless it is tiny itself.
+        if (BITS == 32 || a.exact_root)
         {
-            *(uint2*)((uint8_t*)e.m + i) = mc;
-            *(uint2*)((uint8_t*)e.v + i) = vc;
-            if (i % kMomentBlock == 0) ((uint16_t*)e.scale)[i / kMomentBlock] = (uint16_t)scale;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = sqrtf(v[j]);
         }
-    }
-    if (a.zero_grad)
-    {
-        const float zero[8] = {};
-        store_eight<G>(e.grad, i, count, whole, zero);
-    }
-}
-
-// The entry a chunk belongs to: lane k holds where entry k begins.
-__device__ __forceinline__ uint32_t entry_of(uint32_t begins, uint32_t chunk)
-{
-    return (uint32_t)__popcll(__ballot(begins <= chunk)) - 1u;
-}
-
-template <int BITS>
-__global__ void __launch_bounds__(kBlock) adamw_step_kernel(const AdamWLaunch a)
-{
-    const uint32_t lane   = threadIdx.x % kWave;
-    const uint32_t begins = lane < a.entries ? a.e[lane].first : 0xFFFFFFFFu;
-    const float scale     = a.grad_scale ? *a.grad_scale : 1.f;
-    const bool leave      = !isfinite(scale);
-    for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
-    {
-        const uint32_t k    = entry_of(begins, chunk);
-        const AdamWEntry& e = a.e[k];
-        const uint32_t slot = e.types >> 8;
-        AdamWGroup g        = a.g[slot];
-        if (a.device) g = a.device->group[g.key];
-        const uint32_t i = (chunk - e.first) * kOptimChunk + threadIdx.x * 8u;
-        switch (e.types & 15u)
+        else
         {
-#define VET_ADAMW(P, G) \
-    case P | G << 2: adamw_eight<BITS, P, G>(a, e, g, scale, leave, i); break;
-            VET_ADAMW(VETRAST_F32, VETRAST_F32)
-            VET_ADAMW(VETRAST_F32, VETRAST_BF16)
-            VET_ADAMW(VETRAST_F32, VETRAST_F16)
-            VET_ADAMW(VETRAST_BF16, VETRAST_F32)
-            VET_ADAMW(VETRAST_BF16, VETRAST_BF16)
-            VET_ADAMW(VETRAST_BF16, VETRAST_F16)
-            VET_ADAMW(VETRAST_F16, VETRAST_F32)
-            VET_ADAMW(VETRAST_F16, VETRAST_BF16)
-            VET_ADAMW(VETRAST_F16, VETRAST_F16)
-#undef VET_ADAMW
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_sqrtf(v[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+        {
+            const float d = fmaf(x[j], g.inv_sqrt_bc2, a.eps);
+            const float q = BITS == 32 ? m[j] / d : m[j] * __builtin_amdgcn_rcpf(d);
+            p[j]          = fmaf(-g.step_size, q, p[j] * g.keep);
+        }
+
+        if (master)
+        {
+            const RawEight out = from_floats(p, VETRAST_F32);
+            if (inside)
+            {
+                ((uint4*)(a.master + at))[0] = out.a;
+                ((uint4*)(a.master + at))[1] = out.b;
+            }
+        }
+        RawEight out;
+        if (random)
+        {
+            out.b = make_uint4(0, 0, 0, 0);
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+            {
+                const bool finite = __builtin_isfinite(p[j]);
+                w[j]              = __float_as_uint(p[j]) + (finite ? parameter_bits(r[j]) : 0u);
+            }
+            out.a = make_uint4(__builtin_amdgcn_perm(w[1], w[0], 0x07060302), __builtin_amdgcn_perm(w[3], w[2], 0x07060302),
+                               __builtin_amdgcn_perm(w[5], w[4], 0x07060302), __builtin_amdgcn_perm(w[7], w[6], 0x07060302));
+        }
+        else out = from_floats(p, p_type);
+        store_raw(e.param, p_type, i, count, whole, out);
+        if constexpr (BITS == 32)
+        {
+            const RawEight o1 = from_floats(m, VETRAST_F32), o2 = from_floats(v, VETRAST_F32);
+            if (inside)
+            {
+                ((uint4*)((float*)a.m + at))[0] = o1.a;
+                ((uint4*)((float*)a.m + at))[1] = o1.b;
+                ((uint4*)((float*)a.v + at))[0] = o2.a;
+                ((uint4*)((float*)a.v + at))[1] = o2.b;
+            }
+        }
+        else
+        {
+            uint32_t rv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rv[j] = second_bits(r[j]);
+            const Codes c = encode_moments(m, v, r, rv, (codes.scale & 255u) == 255u);
+            if (inside)
+            {
+                *(uint2*)((uint8_t*)a.m + at) = c.m;
+                *(uint2*)((uint8_t*)a.v + at) = c.v;
+                if (i % kMomentBlock == 0) a.scale[block] = (uint16_t)c.scale;
+            }
+        }
+        if (a.zero_grad) store_raw(e.grad, g_type, i, count, whole, zero);
     }
 }
 
+// ---- norms -------------------------------------------------------------------------------------------------------------
+
+constexpr int kNormEntries = 250;
 struct NormEntry
 {
     const void* grad;
-    uint32_t n, first, type, aligned;
+    uint32_t n_type;  // n << 2 | type
+    uint32_t first_chunk;
 };
 struct NormLaunch
 {
-    NormEntry e[kNormEntries];
     double* partial;  // of this launch, one a workgroup
     uint32_t entries, chunks;
+    NormEntry e[kNormEntries];
 };
 static_assert(sizeof(NormLaunch) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ double wave_sum(double x)
-{
-    for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_down(x, d);
-    return x;
-}
-// Sum over a workgroup of kBlock threads, in thread 0.
+// Sum over a workgroup of kBlock threads, in all of them.
 __device__ __forceinline__ double block_sum(double x)
 {
     __shared__ double part[kBlock / kWave];
-    x = wave_sum(x);
+    for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_down(x, d);
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
     __syncthreads();
     x = 0;
@@ -434,30 +587,21 @@ __device__ __forceinline__ double block_sum(double x)
     return x;
 }
 
-template <int T>
-__device__ __forceinline__ double squares_of_eight(const NormEntry& e, uint32_t i)
-{
-    const uint32_t count = i < e.n ? min(e.n - i, 8u) : 0u;
-    float x[8];
-    load_eight<T>(e.grad, i, count, count == 8u && e.aligned, x);
-    double s = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += (double)x[j] * (double)x[j];
-    return s;
-}
-
+// In 64 bits throughout: no square overflows or vanishes, and a sum of any length is good to the last bit of a float.
 __global__ void __launch_bounds__(kBlock) gradient_squares_kernel(const NormLaunch a)
 {
+    const ChunkFinder<finder_groups(kNormEntries)> find(a);
     double sum = 0;
-    uint32_t k = 0;
     for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
     {
-        while (k + 1 < a.entries && a.e[k + 1].first <= chunk) ++k;
-        const NormEntry& e = a.e[k];
-        const uint32_t i   = (chunk - e.first) * kOptimChunk + threadIdx.x * 8u;
-        if (e.type == VETRAST_F32) sum += squares_of_eight<VETRAST_F32>(e, i);
-        else if (e.type == VETRAST_BF16) sum += squares_of_eight<VETRAST_BF16>(e, i);
-        else sum += squares_of_eight<VETRAST_F16>(e, i);
+        const NormEntry& e   = a.e[find(chunk)];
+        const uint32_t n     = e.n_type >> 2, type = e.n_type & 3u;
+        const uint32_t i     = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
+        const uint32_t count = i < n ? min(n - i, 8u) : 0u;
+        float x[8];
+        to_floats(load_raw(e.grad, type, i, count, count == 8u && (uintptr_t)e.grad % 16 == 0), type, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fma((double)x[j], (double)x[j], sum);
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
@@ -478,64 +622,70 @@ __global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const double* __r
     }
 }
 
+// ---- moments to 8 bits and back ----------------------------------------------------------------------------------------
+
+constexpr int kMomentEntries = 120;
 struct MomentEntry
 {
     float *m, *v;
-    uint8_t *mc, *vc, *scale;
-    uint32_t n, first;
+    uint32_t n, first_chunk, block, reserved;
 };
 struct MomentLaunch
 {
-    MomentEntry e[kMomentEntries];
+    uint8_t *m, *v;
+    uint16_t* scale;
     uint32_t entries, chunks;
+    MomentEntry e[kMomentEntries];
 };
 static_assert(sizeof(MomentLaunch) <= 4096, "kernel arguments");
 
 template <bool PACK>
 __global__ void __launch_bounds__(kBlock) convert_moments_kernel(const MomentLaunch a)
 {
-    uint32_t k = 0;
+    const ChunkFinder<finder_groups(kMomentEntries)> find(a);
     for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
     {
-        while (k + 1 < a.entries && a.e[k + 1].first <= chunk) ++k;
-        const MomentEntry& e = a.e[k];
-        const uint32_t i     = (chunk - e.first) * kOptimChunk + threadIdx.x * 8u;
+        const MomentEntry& e = a.e[find(chunk)];
+        const uint32_t i     = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
         const uint32_t count = i < e.n ? min(e.n - i, 8u) : 0u;
         const bool whole     = count == 8u && (((uintptr_t)e.m | (uintptr_t)e.v) & 15) == 0;
-        const bool codes     = i < (e.n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
+        const uint32_t block = e.block + i / kMomentBlock;
+        const size_t at      = (size_t)block * kMomentBlock + i % kMomentBlock;
+        const bool inside    = i < (e.n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
         float m[8], v[8];
-        uint2 mc = make_uint2(0, 0), vc = make_uint2(0, 0);
-        uint32_t scale = 0;
         if constexpr (PACK)
         {
-            load_eight<VETRAST_F32>(e.m, i, count, whole, m);
-            load_eight<VETRAST_F32>(e.v, i, count, whole, v);
-            uint32_t half[8];
+            const RawEight r1 = load_raw(e.m, VETRAST_F32, i, count, whole), r2 = load_raw(e.v, VETRAST_F32, i, count, whole);
+            to_floats(r1, VETRAST_F32, m);
+            to_floats(r2, VETRAST_F32, v);
+            uint32_t half[8], lost = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
             {
                 v[j]    = fabsf(v[j]);
                 half[j] = 1u << 19;
+                lost |= __builtin_isfinite(m[j]) ? 0u : 1u;
             }
-            encode_moments(m, v, half, half, mc, vc, scale);
-            if (codes)
+            const Codes c = encode_moments(m, v, half, half, row_max(lost) != 0);
+            if (inside)
             {
-                *(uint2*)(e.mc + i) = mc;
-                *(uint2*)(e.vc + i) = vc;
-                if (i % kMomentBlock == 0) ((uint16_t*)e.scale)[i / kMomentBlock] = (uint16_t)scale;
+                *(uint2*)(a.m + at) = c.m;
+                *(uint2*)(a.v + at) = c.v;
+                if (i % kMomentBlock == 0) a.scale[block] = (uint16_t)c.scale;
             }
         }
         else
         {
-            if (codes)
+            Codes c = {};
+            if (inside)
             {
-                mc    = *(const uint2*)(e.mc + i);
-                vc    = *(const uint2*)(e.vc + i);
-                scale = ((const uint16_t*)e.scale)[i / kMomentBlock];
+                c.m     = *(const uint2*)(a.m + at);
+                c.v     = *(const uint2*)(a.v + at);
+                c.scale = a.scale[block];
             }
-            decode_moments(mc, vc, scale, m, v);
-            store_eight<VETRAST_F32>(e.m, i, count, whole, m);
-            store_eight<VETRAST_F32>(e.v, i, count, whole, v);
+            decode_moments(c, m, v);
+            store_raw(e.m, VETRAST_F32, i, count, whole, from_floats(m, VETRAST_F32));
+            store_raw(e.v, VETRAST_F32, i, count, whole, from_floats(v, VETRAST_F32));
         }
     }
 }

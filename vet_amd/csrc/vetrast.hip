@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 #include <type_traits>
 #include <mutex>
 #include <new>
@@ -478,10 +479,71 @@ void launch_lift(const vetrast_lift_args* a, char* ws, size_t num_sums, hipStrea
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
-constexpr int64_t kOptimEntryElements = 1 << 30;  // a longer tensor is several entries of a launch: places inside one are 32 bits
+constexpr int64_t kOptimEntryElements = 1 << 29;  // a longer tensor is several entries of a launch: places inside one are 32 bits
 constexpr uint32_t kOptimGrid         = 2048;     // workgroups of a launch at most, each goes through its share of chunks
 constexpr uint32_t kNormGrid          = 1024;
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
+inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays, whose blocks have numbers of 32 bits
+{
+    return first >= 0 && first % kMomentBlock == 0 && first < ((int64_t)1 << 38) && n <= ((int64_t)1 << 38);
+}
+
+// The launches of a list of tensors; `l` has what they share.
+template <int ENTRIES>
+void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStream_t stream)
+{
+    int slot_group[kAdamWGroups], slots = 0;
+    l.entries = l.chunks = 0;
+    const auto launch = [&] {
+        if (l.entries == 0) return;
+        const dim3 grid(std::min(l.chunks, kOptimGrid));
+        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        else hipLaunchKernelGGL((adamw_step_kernel<8, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        l.entries = l.chunks = 0;
+        slots                = 0;
+    };
+    for (int k = 0; k < a->num_tensors; ++k)
+    {
+        const vetrast_adamw_tensor& t = a->tensors[k];
+        for (int64_t from = 0; from < t.n; from += kOptimEntryElements)
+        {
+            int slot = 0;
+            while (slot < slots && slot_group[slot] != t.group) ++slot;
+            if (l.entries == (uint32_t)ENTRIES || slot == kAdamWGroups)
+            {
+                launch();
+                slot = 0;
+            }
+            if (slot == slots)
+            {
+                const vetrast_adamw_group& g = a->groups[t.group];
+                AdamWGroup& c                = l.g[slot];
+                slot_group[slots++]          = t.group;
+                if (l.device) c = {0.f, 0.f, 0.f, (uint32_t)t.group};
+                else
+                {
+                    // bias corrections in double, handed to the kernel rounded once
+                    c.step_size    = (float)(g.lr / (1.0 - std::pow(a->beta1, (double)g.step)));
+                    c.keep         = (float)(1.0 - g.lr * g.weight_decay);
+                    c.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)g.step)));
+                    c.key          = step_key(a->seed, g.step);
+                }
+            }
+            AdamWEntry& e      = l.e[l.entries++];
+            e.param            = static_cast<char*>(t.param) + from * (int64_t)dtype_bytes(t.param_type);
+            e.grad             = static_cast<char*>(t.grad) + from * (int64_t)dtype_bytes(t.grad_type);
+            e.n                = (uint32_t)std::min(t.n - from, kOptimEntryElements);
+            e.first_chunk      = l.chunks;
+            e.block            = (uint32_t)((t.first + from) / kMomentBlock);
+            e.flags            = (uint32_t)t.param_type | (uint32_t)t.grad_type << 2 | (uint32_t)slot << 8;
+            if (aligned_to(e.param, 16) && aligned_to(e.grad, 16)) e.flags |= kAdamWAligned;
+            if (a->master && t.param_type != VETRAST_F32) e.flags |= kAdamWMaster;
+            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+        }
+    }
+    launch();
+}
+
 
 }  // namespace
 
@@ -1338,31 +1400,30 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
     if (a->num_tensors < 0 || a->num_groups < 0 || a->num_groups > VETRAST_ADAMW_MAX_GROUPS) return VETRAST_ERR_INVALID_ARG;
     if (a->moment_bits != 32 && a->moment_bits != 8) return VETRAST_ERR_INVALID_ARG;
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0)) return VETRAST_ERR_INVALID_ARG;
-    if (!((float)a->eps > 0.f) || !std::isfinite((float)a->eps)) return VETRAST_ERR_INVALID_ARG;  // a second moment of zero divides by it
+    if (!((float)a->eps >= std::numeric_limits<float>::min()) || !std::isfinite((float)a->eps)) return VETRAST_ERR_INVALID_ARG;
     if ((a->num_tensors > 0 && !a->tensors) || (a->num_groups > 0 && !a->groups)) return VETRAST_ERR_INVALID_ARG;
     if (!aligned_to(a->grad_scale, 4) || !aligned_to(a->device_state, 16)) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->exp_avg, 16) || !aligned_to(a->exp_avg_sq, 16) || !aligned_to(a->block_scale, 16) || !aligned_to(a->master, 16))
+        return VETRAST_ERR_INVALID_ARG;
     for (int k = 0; k < a->num_groups; ++k)
     {
         const vetrast_adamw_group& g = a->groups[k];
         if (!std::isfinite(g.lr) || !std::isfinite(g.weight_decay)) return VETRAST_ERR_INVALID_ARG;
         if (!a->device_state && g.step < 1) return VETRAST_ERR_INVALID_ARG;
     }
+    int64_t entries = 0;
     for (int k = 0; k < a->num_tensors; ++k)
     {
         const vetrast_adamw_tensor& t = a->tensors[k];
         if (t.n < 0 || t.group < 0 || t.group >= a->num_groups) return VETRAST_ERR_INVALID_ARG;
         if (!is_dtype(t.param_type) || !is_dtype(t.grad_type)) return VETRAST_ERR_INVALID_ARG;
-        if (t.first_number < 0 || t.first_number % kMomentBlock != 0) return VETRAST_ERR_INVALID_ARG;
+        if (!is_place(t.first, t.n)) return VETRAST_ERR_INVALID_ARG;
         if (t.n == 0) continue;
-        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return VETRAST_ERR_INVALID_ARG;
+        if (!t.param || !t.grad || !a->exp_avg || !a->exp_avg_sq || (a->moment_bits == 8 && !a->block_scale)) return VETRAST_ERR_INVALID_ARG;
         if (!aligned_to(t.param, dtype_bytes(t.param_type)) || !aligned_to(t.grad, dtype_bytes(t.grad_type))) return VETRAST_ERR_INVALID_ARG;
-        if (t.copy && (t.param_type != VETRAST_F32 || (t.copy_type != VETRAST_BF16 && t.copy_type != VETRAST_F16) || !aligned_to(t.copy, 2)))
-            return VETRAST_ERR_INVALID_ARG;
-        const size_t moment_alignment = a->moment_bits == 8 ? 8 : 4;
-        if (!aligned_to(t.exp_avg, moment_alignment) || !aligned_to(t.exp_avg_sq, moment_alignment)) return VETRAST_ERR_INVALID_ARG;
-        if (a->moment_bits == 8 && (!t.block_scale || !aligned_to(t.block_scale, 2))) return VETRAST_ERR_INVALID_ARG;
+        entries += (t.n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
-    hipStream_t stream = (hipStream_t)stream_;
+    hipStream_t stream  = (hipStream_t)stream_;
     AdamWDevice* device = static_cast<AdamWDevice*>(a->device_state);
     if (device)
     {
@@ -1380,72 +1441,35 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
             hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(kBeginGroups), 0, stream, b);
         }
     }
-    AdamWLaunch l;
-    l.grad_scale      = a->grad_scale;
-    l.device          = device;
-    l.beta1           = (float)a->beta1;
-    l.one_minus_beta1 = (float)(1.0 - a->beta1);
-    l.beta2           = (float)a->beta2;
-    l.one_minus_beta2 = (float)(1.0 - a->beta2);
-    l.eps             = (float)a->eps;
-    l.zero_grad       = a->zero_grad;
-    l.stochastic      = a->stochastic_rounding;
-    l.entries = l.chunks = 0;
-    int slot_group[kAdamWGroups], slots = 0;
-    const auto launch = [&] {
-        if (l.entries == 0) return;
-        const dim3 grid(std::min(l.chunks, kOptimGrid));
-        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32>), grid, dim3(kBlock), 0, stream, l);
-        else hipLaunchKernelGGL((adamw_step_kernel<8>), grid, dim3(kBlock), 0, stream, l);
-        l.entries = l.chunks = 0;
-        slots                = 0;
+    const auto share = [&](AdamWCommon& l) {
+        l.m               = a->exp_avg;
+        l.v               = a->exp_avg_sq;
+        l.scale           = reinterpret_cast<uint16_t*>(a->block_scale);
+        l.master          = a->master;
+        l.grad_scale      = a->grad_scale;
+        l.device          = device;
+        l.beta1           = (float)a->beta1;
+        l.one_minus_beta1 = (float)(1.0 - a->beta1);
+        l.beta2           = (float)a->beta2;
+        l.one_minus_beta2 = (float)(1.0 - a->beta2);
+        l.eps             = (float)a->eps;
+        l.zero_grad       = a->zero_grad;
+        l.stochastic      = a->stochastic_rounding;
+        // the root instruction's zero for values below 2^-126 is up to 2^-63 off, times at most 1 / sqrt(1 - beta2): half a step of eps
+        l.exact_root = std::ldexp(1.0, -63) / std::sqrt(1.0 - a->beta2) > std::ldexp(a->eps, -24);
     };
-    for (int k = 0; k < a->num_tensors; ++k)
+    if (entries <= kAdamWFew)
     {
-        const vetrast_adamw_tensor& t = a->tensors[k];
-        for (int64_t from = 0; from < t.n; from += kOptimEntryElements)
-        {
-            int slot = 0;
-            while (slot < slots && slot_group[slot] != t.group) ++slot;
-            if (l.entries == (uint32_t)kAdamWEntries || slot == kAdamWGroups)
-            {
-                launch();
-                slot = 0;
-            }
-            if (slot == slots)
-            {
-                const vetrast_adamw_group& g = a->groups[t.group];
-                AdamWGroup& c                = l.g[slot];
-                slot_group[slots++]          = t.group;
-                if (device) c = {0.f, 0.f, 0.f, (uint32_t)t.group};
-                else
-                {
-                    // bias corrections in double, handed to the kernel rounded once
-                    c.step_size    = (float)(g.lr / (1.0 - std::pow(a->beta1, (double)g.step)));
-                    c.keep         = (float)(1.0 - g.lr * g.weight_decay);
-                    c.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)g.step)));
-                    c.key          = step_key(a->seed, g.step);
-                }
-            }
-            AdamWEntry& e = l.e[l.entries++];
-            const int64_t moment_bytes = a->moment_bits / 8;
-            e.param = static_cast<char*>(t.param) + from * (int64_t)dtype_bytes(t.param_type);
-            e.grad  = static_cast<char*>(t.grad) + from * (int64_t)dtype_bytes(t.grad_type);
-            e.copy  = t.copy ? static_cast<char*>(t.copy) + from * 2 : nullptr;
-            e.m     = static_cast<char*>(t.exp_avg) + from * moment_bytes;
-            e.v     = static_cast<char*>(t.exp_avg_sq) + from * moment_bytes;
-            e.scale = a->moment_bits == 8 ? t.block_scale + from / kMomentBlock * 2 : nullptr;
-            e.n     = (uint32_t)std::min(t.n - from, kOptimEntryElements);
-            e.first = l.chunks;
-            e.pair  = (uint32_t)((uint64_t)(t.first_number + from) / 2);
-            bool whole = aligned_to(e.param, 16) && aligned_to(e.grad, 16) && aligned_to(e.copy, 16);
-            if (a->moment_bits == 32) whole = whole && aligned_to(e.m, 16) && aligned_to(e.v, 16);
-            e.types = (uint32_t)t.param_type | (uint32_t)t.grad_type << 2 | (t.copy ? (uint32_t)t.copy_type << 4 | kHasCopy : 0u) |
-                      (whole ? kAligned : 0u) | (uint32_t)slot << 8;
-            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
-        }
+        AdamWLaunch<kAdamWFew> l;
+        share(l);
+        launch_adamw(a, l, stream);
     }
-    launch();
+    else
+    {
+        AdamWLaunch<kAdamWEntries> l;
+        share(l);
+        launch_adamw(a, l, stream);
+    }
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
 }
@@ -1494,13 +1518,12 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
         for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
         {
             if (l.entries == (uint32_t)kNormEntries) launch();
-            NormEntry& e = l.e[l.entries++];
-            e.grad       = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
-            e.n          = (uint32_t)std::min(g.n - from, kOptimEntryElements);
-            e.first      = l.chunks;
-            e.type       = (uint32_t)g.type;
-            e.aligned    = aligned_to(e.grad, 16) ? 1u : 0u;
-            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+            NormEntry& e     = l.e[l.entries++];
+            e.grad           = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
+            const uint32_t n = (uint32_t)std::min(g.n - from, kOptimEntryElements);
+            e.n_type         = n << 2 | (uint32_t)g.type;
+            e.first_chunk    = l.chunks;
+            l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
         }
     }
     launch();
@@ -1509,20 +1532,22 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
     return VETRAST_OK;
 }
 
-static int convert_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, hipStream_t stream, bool pack)
+static int convert_moments(vetrast_ctx* ctx, const vetrast_moments_args* a, hipStream_t stream, bool pack)
 {
-    if (!ctx || num_tensors < 0 || (num_tensors > 0 && !tensors)) return VETRAST_ERR_INVALID_ARG;
-    for (int k = 0; k < num_tensors; ++k)
+    if (!ctx || !a || a->num_tensors < 0 || (a->num_tensors > 0 && !a->tensors)) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->exp_avg, 16) || !aligned_to(a->exp_avg_sq, 16) || !aligned_to(a->block_scale, 16)) return VETRAST_ERR_INVALID_ARG;
+    for (int k = 0; k < a->num_tensors; ++k)
     {
-        const vetrast_moment_tensor& t = tensors[k];
-        if (t.n < 0) return VETRAST_ERR_INVALID_ARG;
+        const vetrast_moment_tensor& t = a->tensors[k];
+        if (t.n < 0 || !is_place(t.first, t.n)) return VETRAST_ERR_INVALID_ARG;
         if (t.n == 0) continue;
-        if (!t.exp_avg || !t.exp_avg_sq || !t.exp_avg_code || !t.exp_avg_sq_code || !t.block_scale) return VETRAST_ERR_INVALID_ARG;
-        if (!aligned_to(t.exp_avg, 4) || !aligned_to(t.exp_avg_sq, 4) || !aligned_to(t.exp_avg_code, 8) ||
-            !aligned_to(t.exp_avg_sq_code, 8) || !aligned_to(t.block_scale, 2))
-            return VETRAST_ERR_INVALID_ARG;
+        if (!t.exp_avg || !t.exp_avg_sq || !a->exp_avg || !a->exp_avg_sq || !a->block_scale) return VETRAST_ERR_INVALID_ARG;
+        if (!aligned_to(t.exp_avg, 4) || !aligned_to(t.exp_avg_sq, 4)) return VETRAST_ERR_INVALID_ARG;
     }
     MomentLaunch l;
+    l.m       = a->exp_avg;
+    l.v       = a->exp_avg_sq;
+    l.scale   = reinterpret_cast<uint16_t*>(a->block_scale);
     l.entries = l.chunks = 0;
     const auto launch = [&] {
         if (l.entries == 0) return;
@@ -1531,20 +1556,18 @@ static int convert_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensor
         else hipLaunchKernelGGL((convert_moments_kernel<false>), grid, dim3(kBlock), 0, stream, l);
         l.entries = l.chunks = 0;
     };
-    for (int k = 0; k < num_tensors; ++k)
+    for (int k = 0; k < a->num_tensors; ++k)
     {
-        const vetrast_moment_tensor& t = tensors[k];
+        const vetrast_moment_tensor& t = a->tensors[k];
         for (int64_t from = 0; from < t.n; from += kOptimEntryElements)
         {
             if (l.entries == (uint32_t)kMomentEntries) launch();
             MomentEntry& e = l.e[l.entries++];
             e.m            = t.exp_avg + from;
             e.v            = t.exp_avg_sq + from;
-            e.mc           = t.exp_avg_code + from;
-            e.vc           = t.exp_avg_sq_code + from;
-            e.scale        = t.block_scale + from / kMomentBlock * 2;
             e.n            = (uint32_t)std::min(t.n - from, kOptimEntryElements);
-            e.first        = l.chunks;
+            e.first_chunk  = l.chunks;
+            e.block        = (uint32_t)((t.first + from) / kMomentBlock);
             l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
         }
     }
@@ -1553,14 +1576,14 @@ static int convert_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensor
     return VETRAST_OK;
 }
 
-int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream)
+int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream)
 {
-    return convert_moments(ctx, tensors, num_tensors, (hipStream_t)stream, true);
+    return convert_moments(ctx, args, (hipStream_t)stream, true);
 }
 
-int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moment_tensor* tensors, int32_t num_tensors, void* stream)
+int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream)
 {
-    return convert_moments(ctx, tensors, num_tensors, (hipStream_t)stream, false);
+    return convert_moments(ctx, args, (hipStream_t)stream, false);
 }
 
 size_t vetrast_lift_workspace_bytes(int64_t num_cells)

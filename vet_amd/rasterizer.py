@@ -342,32 +342,27 @@ class Rasterizer:
         a.lr, a.beta1, a.beta2, a.eps, a.weight_decay, a.zero_grad = lr, beta1, beta2, eps, weight_decay, int(zero_grad)
         abi.check(self.lib.vetrast_adam_step(self.ctx, C.byref(a), self._stream()), "adam_step")
 
-    def adamw_step(self, tensors, groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, stochastic_rounding=False, seed=0,
-                   zero_grad=False, grad_scale=None, device_state=None):
-        """One AdamW step in place on a list of tensors (vetrast_adamw_step). tensors: dicts of contiguous CUDA tensors param, grad,
-        exp_avg, exp_avg_sq and, as wanted, block_scale and copy, with first_number and group (0 where left out). groups:
-        (lr, weight_decay, step). device_state: a uint8 tensor of vetrast_adamw_device_state_bytes(len(groups)) bytes."""
+    def adamw_step(self, tensors, groups, exp_avg, exp_avg_sq, block_scale=None, master=None, beta1=0.9, beta2=0.999, eps=1e-8,
+                   moment_bits=32, stochastic_rounding=False, seed=0, zero_grad=False, grad_scale=None, device_state=None):
+        """One AdamW step in place on a list of tensors (vetrast_adamw_step). tensors: (param, grad, first, group) with contiguous
+        CUDA tensors; groups: (lr, weight_decay, step); exp_avg ... master: the flat arrays, in which a tensor has the elements from
+        `first` on. device_state: a uint8 tensor of vetrast_adamw_device_state_bytes(len(groups)) bytes."""
         ts, gs, a = (abi.AdamWTensor * max(len(tensors), 1))(), (abi.AdamWGroup * max(len(groups), 1))(), abi.AdamWArgs()
-        for t, d in zip(ts, tensors):
-            n = d["param"].numel()
-            for name in ("param", "grad", "exp_avg", "exp_avg_sq", "block_scale", "copy"):
-                x = d.get(name)
-                if x is not None:
-                    assert x.is_cuda and x.is_contiguous()
-                    setattr(t, name, x.data_ptr())
-            blocks = -(-n // abi.MOMENT_BLOCK)
-            state = n if moment_bits == 32 else blocks * abi.MOMENT_BLOCK
-            assert d["grad"].numel() == n and d["exp_avg"].numel() >= state and d["exp_avg_sq"].numel() >= state
-            assert all(d[k].dtype == (torch.float32 if moment_bits == 32 else torch.uint8) for k in ("exp_avg", "exp_avg_sq"))
-            assert moment_bits == 32 or (d["block_scale"].dtype == torch.uint8 and d["block_scale"].numel() >= 2 * blocks)
-            t.n, t.first_number, t.group = n, d.get("first_number", 0), d.get("group", 0)
-            t.param_type, t.grad_type = _DTYPES[d["param"].dtype], _DTYPES[d["grad"].dtype]
-            if d.get("copy") is not None:
-                assert d["copy"].numel() == n
-                t.copy_type = _DTYPES[d["copy"].dtype]
+        end = 0
+        for t, (param, grad, first, group) in zip(ts, tensors):
+            assert param.is_cuda and param.is_contiguous() and grad.is_cuda and grad.is_contiguous() and grad.numel() == param.numel()
+            t.param, t.grad, t.n, t.first, t.group = param.data_ptr(), grad.data_ptr(), param.numel(), first, group
+            t.param_type, t.grad_type = _DTYPES[param.dtype], _DTYPES[grad.dtype]
+            end = max(end, first + -(-t.n // abi.MOMENT_BLOCK) * abi.MOMENT_BLOCK)
         for g, (lr, weight_decay, step) in zip(gs, groups):
             g.lr, g.weight_decay, g.step = lr, weight_decay, step
         a.tensors, a.groups, a.num_tensors, a.num_groups = ts, gs, len(tensors), len(groups)
+        moments = torch.float32 if moment_bits == 32 else torch.uint8
+        for name, x, dtype, need in (("exp_avg", exp_avg, moments, end), ("exp_avg_sq", exp_avg_sq, moments, end),
+                                     ("block_scale", block_scale, torch.uint8, end // abi.MOMENT_BLOCK * 2), ("master", master, torch.float32, end)):
+            if x is not None:
+                assert x.is_cuda and x.is_contiguous() and x.dtype == dtype and x.numel() >= need
+                setattr(a, name, x.data_ptr())
         a.beta1, a.beta2, a.eps, a.moment_bits, a.seed = beta1, beta2, eps, moment_bits, seed
         a.stochastic_rounding, a.zero_grad = int(stochastic_rounding), int(zero_grad)
         if grad_scale is not None:
@@ -392,18 +387,21 @@ class Rasterizer:
         abi.check(self.lib.vetrast_gradient_norm(self.ctx, C.byref(a), self._stream()), "gradient_norm")
         return out
 
-    def convert_moments(self, tensors, pack):
-        """float32 moments to 8 bits or back (vetrast_pack_moments, vetrast_unpack_moments): a list of (exp_avg, exp_avg_sq, code,
-        code_sq, block_scale), the first two float32 of the same number of elements."""
-        ts = (abi.MomentTensor * max(len(tensors), 1))()
-        for t, (m, v, mc, vc, scale) in zip(ts, tensors):
-            n, blocks = m.numel(), -(-m.numel() // abi.MOMENT_BLOCK)
-            assert all(x.is_cuda and x.is_contiguous() for x in (m, v, mc, vc, scale)) and m.dtype == v.dtype == torch.float32
-            assert v.numel() == n and min(mc.numel(), vc.numel()) >= blocks * abi.MOMENT_BLOCK and scale.numel() >= 2 * blocks
-            t.exp_avg, t.exp_avg_sq, t.n = m.data_ptr(), v.data_ptr(), n
-            t.exp_avg_code, t.exp_avg_sq_code, t.block_scale = mc.data_ptr(), vc.data_ptr(), scale.data_ptr()
+    def convert_moments(self, tensors, exp_avg, exp_avg_sq, block_scale, pack):
+        """float32 moments to 8 bits or back (vetrast_pack_moments, vetrast_unpack_moments). tensors: (exp_avg, exp_avg_sq, first),
+        float32; the others are the flat arrays."""
+        ts, a = (abi.MomentTensor * max(len(tensors), 1))(), abi.MomentsArgs()
+        end = 0
+        for t, (m, v, first) in zip(ts, tensors):
+            assert all(x.is_cuda and x.is_contiguous() and x.dtype == torch.float32 and x.numel() == m.numel() for x in (m, v))
+            t.exp_avg, t.exp_avg_sq, t.n, t.first = m.data_ptr(), v.data_ptr(), m.numel(), first
+            end = max(end, first + -(-t.n // abi.MOMENT_BLOCK) * abi.MOMENT_BLOCK)
+        for x, need in ((exp_avg, end), (exp_avg_sq, end), (block_scale, end // abi.MOMENT_BLOCK * 2)):
+            assert x.is_cuda and x.is_contiguous() and x.dtype == torch.uint8 and x.numel() >= need
+        a.tensors, a.num_tensors = ts, len(tensors)
+        a.exp_avg, a.exp_avg_sq, a.block_scale = exp_avg.data_ptr(), exp_avg_sq.data_ptr(), block_scale.data_ptr()
         call = self.lib.vetrast_pack_moments if pack else self.lib.vetrast_unpack_moments
-        abi.check(call(self.ctx, ts, len(tensors), self._stream()), "convert_moments")
+        abi.check(call(self.ctx, C.byref(a), self._stream()), "convert_moments")
 
     def lift_error(self, cell_bb_min, cell_bb_length, cell_value, cell_access_count, view, poses_se3, intrinsics,
                    loss_image, border_pixels=abi.LIFT_BORDER_PIXELS, workspace=None, static_scratch=False):

@@ -68,43 +68,34 @@ int64_t whole_blocks(int64_t n)
     return (n + kBlock - 1) / kBlock * kBlock;
 }
 
-// The step's gradient of p in p's order of elements: p.grad() itself where that has the same strides.
-torch::Tensor gradient_like(const torch::Tensor& p, const torch::Tensor& grad)
+bool same_order(const torch::Tensor& a, const torch::Tensor& b)
 {
-    if (grad.strides() == p.strides() || (grad.is_contiguous() && p.is_contiguous())) return grad;
-    return torch::empty_like(p).copy_(grad);
+    return (a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides();
 }
 
-std::vector<vetrast_moment_tensor> moment_list(const std::vector<torch::Tensor>& ms, const std::vector<torch::Tensor>& vs, const torch::Device& device)
+// Moments of a list of tensors, placed one behind the other in flat arrays; `total`: elements of these.
+std::vector<vetrast_moment_tensor> moment_list(const std::vector<torch::Tensor>& ms, const std::vector<torch::Tensor>& vs, const torch::Device& device,
+                                               int64_t& total)
 {
     TORCH_CHECK(ms.size() == vs.size(), "as many first moments as second ones are needed, not ", ms.size(), " and ", vs.size());
     std::vector<vetrast_moment_tensor> list(ms.size());
+    total = 0;
     for (size_t k = 0; k < ms.size(); ++k)
     {
         check_on(ms[k], device, "moments");
         check_on(vs[k], device, "moments");
         TORCH_CHECK(ms[k].scalar_type() == torch::kFloat32 && vs[k].scalar_type() == torch::kFloat32 && dense(ms[k]) && dense(vs[k]),
                     "moments must be dense float32 tensors");
-        TORCH_CHECK(ms[k].sizes() == vs[k].sizes() && (ms[k].strides() == vs[k].strides() || (ms[k].is_contiguous() && vs[k].is_contiguous())),
-                    "both moments of a tensor must have one shape and order");
-        std::memset(&list[k], 0, sizeof(list[k]));
-        list[k].exp_avg    = ms[k].data_ptr<float>();
-        list[k].exp_avg_sq = vs[k].data_ptr<float>();
-        list[k].n          = ms[k].numel();
+        TORCH_CHECK(ms[k].sizes() == vs[k].sizes() && same_order(ms[k], vs[k]), "both moments of a tensor must have one shape and order");
+        list[k] = {ms[k].data_ptr<float>(), vs[k].data_ptr<float>(), ms[k].numel(), total};
+        total += whole_blocks(list[k].n);
     }
     return list;
 }
 
-void place_codes(std::vector<vetrast_moment_tensor>& list, const torch::Tensor& m, const torch::Tensor& v, const torch::Tensor& scale)
+vetrast_moments_args moments_args(const std::vector<vetrast_moment_tensor>& list, const torch::Tensor& m, const torch::Tensor& v, const torch::Tensor& scale)
 {
-    int64_t at = 0;
-    for (auto& t : list)
-    {
-        t.exp_avg_code    = m.data_ptr<uint8_t>() + at;
-        t.exp_avg_sq_code = v.data_ptr<uint8_t>() + at;
-        t.block_scale     = scale.data_ptr<uint8_t>() + at / kBlock * 2;
-        at += whole_blocks(t.n);
-    }
+    return {list.data(), (int32_t)list.size(), 0, m.data_ptr<uint8_t>(), v.data_ptr<uint8_t>(), scale.data_ptr<uint8_t>()};
 }
 }  // namespace
 
@@ -199,18 +190,13 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
         lay_out();
     }
-    const bool eight          = options_.moment_bits == 8;
-    const int64_t moment_size = eight ? 1 : 4;
-    char* m                   = (char*)exp_avg.data_ptr();
-    char* v                   = (char*)exp_avg_sq.data_ptr();
-    uint8_t* scales           = eight ? block_scale.data_ptr<uint8_t>() : nullptr;
-    float* masters            = master.defined() ? master.data_ptr<float>() : nullptr;
+    const bool eight = options_.moment_bits == 8;
     tensors_.clear();
     groups_.clear();
     if (options_.capturable)
         for (size_t g = 0; g < lr_.size(); ++g) groups_.push_back({lr_[g], weight_decay_[g], 0});
     group_of_.assign(lr_.size(), -1);
-    std::vector<torch::Tensor> reordered;
+    std::vector<torch::Tensor> reordered;  // gradients that were copied into their parameter's order
     for (auto& s : slots_)
     {
         const torch::Tensor& p    = s.param;
@@ -221,10 +207,15 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         const int32_t type = type_of(p, "AdamW: parameters");
         TORCH_CHECK(grad.scalar_type() == p.scalar_type() && grad.sizes() == p.sizes(), "AdamW: a gradient must have its parameter's type and shape");
         TORCH_CHECK(dense(p), "AdamW: parameters must be dense, without gaps or overlaps");
-        torch::Tensor g = gradient_like(p, grad);
-        if (!g.is_same(grad)) reordered.push_back(g);
-        int64_t& place   = group_of_[s.group];
-        const auto fits  = [&](int64_t k) { return groups_[k].lr == lr_[s.group] && groups_[k].weight_decay == weight_decay_[s.group] && groups_[k].step == s.step + 1; };
+        void* gradient = nullptr;
+        if (same_order(p, grad)) gradient = grad.data_ptr();
+        else
+        {
+            reordered.push_back(torch::empty_like(p).copy_(grad));
+            gradient = reordered.back().data_ptr();
+        }
+        int64_t& place  = group_of_[s.group];
+        const auto fits = [&](int64_t k) { return groups_[k].lr == lr_[s.group] && groups_[k].weight_decay == weight_decay_[s.group] && groups_[k].step == s.step + 1; };
         if (options_.capturable) place = s.group;
         else if (place < 0 || !fits(place))
         {
@@ -233,21 +224,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
             while (place < (int64_t)groups_.size() && !fits(place)) ++place;
             if (place == (int64_t)groups_.size()) groups_.push_back({lr_[s.group], weight_decay_[s.group], s.step + 1});
         }
-        vetrast_adamw_tensor t;
-        const bool with_master = masters && type != VETRAST_F32;
-        t.param                = with_master ? (void*)(masters + s.first) : p.data_ptr();
-        t.copy                 = with_master ? p.data_ptr() : nullptr;
-        t.grad                 = g.data_ptr();
-        t.exp_avg              = m + s.first * moment_size;
-        t.exp_avg_sq           = v + s.first * moment_size;
-        t.block_scale          = scales ? scales + s.first / kBlock * 2 : nullptr;
-        t.n                    = s.n;
-        t.first_number         = s.first;
-        t.param_type           = with_master ? (int32_t)VETRAST_F32 : type;
-        t.grad_type            = type;
-        t.copy_type            = with_master ? type : 0;
-        t.group                = (int32_t)place;
-        tensors_.push_back(t);
+        tensors_.push_back({p.data_ptr(), gradient, s.n, s.first, type, type, (int32_t)place, 0});
     }
     vetrast_adamw_args a;
     std::memset(&a, 0, sizeof(a));
@@ -255,6 +232,10 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
     a.groups              = groups_.data();
     a.num_tensors         = (int32_t)tensors_.size();
     a.num_groups          = (int32_t)groups_.size();
+    a.exp_avg             = exp_avg.data_ptr();
+    a.exp_avg_sq          = exp_avg_sq.data_ptr();
+    a.block_scale         = eight ? block_scale.data_ptr<uint8_t>() : nullptr;
+    a.master              = master.defined() ? master.data_ptr<float>() : nullptr;
     a.beta1               = options_.beta1;
     a.beta2               = options_.beta2;
     a.eps                 = options_.eps;
@@ -279,17 +260,11 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         s.step += 1;
         // the kernel wrote through raw pointers: tell everyone who keys on the version counters
         s.param.unsafeGetTensorImpl()->bump_version();
-        if (zero_grad) grad.unsafeGetTensorImpl()->bump_version();
+        if (!zero_grad) continue;
+        if (same_order(s.param, grad)) grad.unsafeGetTensorImpl()->bump_version();
+        else if (dense(grad)) s.param.mutable_grad().zero_();  // the kernel cleared its copy
+        else s.param.mutable_grad() = torch::zeros_like(s.param);
     }
-    // the kernel cleared copies of these
-    if (zero_grad && !reordered.empty())
-        for (auto& s : slots_)
-        {
-            const torch::Tensor& grad = s.param.grad();
-            if (!grad.defined() || grad.strides() == s.param.strides()) continue;
-            if (dense(grad)) s.param.mutable_grad().zero_();
-            else s.param.mutable_grad() = torch::zeros_like(s.param);
-        }
 }
 
 void AdamW::zero_grad()
@@ -346,15 +321,16 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
 {
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
-    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device_);
+    int64_t total = 0;
+    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device_, total);
     TORCH_CHECK(list.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", list.size());
     for (size_t k = 0; k < list.size(); ++k)
         TORCH_CHECK(list[k].n == slots_[k].n, "AdamW: parameter ", k, " has ", slots_[k].n, " elements, its moments have ", list[k].n);
     set_step(step);
     if (options_.moment_bits == 8)
     {
-        place_codes(list, exp_avg, exp_avg_sq, block_scale);
-        check(vetrast_pack_moments(context_on(device_), list.data(), (int32_t)list.size(), stream_on(device_)), "pack_moments");
+        const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);
+        check(vetrast_pack_moments(context_on(device_), &a, stream_on(device_)), "pack_moments");
         return;
     }
     for (size_t k = 0; k < list.size(); ++k)
@@ -423,14 +399,13 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const std::v
     TORCH_CHECK(!exp_avgs.empty() && exp_avgs[0].is_cuda(), "pack_moments: a list of tensors on the GPU is needed");
     const torch::Device device = exp_avgs[0].device();
     c10::DeviceGuard guard(device);
-    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device);
-    int64_t total                           = 0;
-    for (auto& t : list) total += whole_blocks(t.n);
+    int64_t total = 0;
+    const std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device, total);
     const auto bytes    = torch::TensorOptions(device).dtype(torch::kUInt8);
     torch::Tensor m     = torch::empty({total}, bytes), v = torch::empty({total}, bytes);
     torch::Tensor scale = torch::empty({total / kBlock, 2}, bytes);
-    place_codes(list, m, v, scale);
-    check(vetrast_pack_moments(context_on(device), list.data(), (int32_t)list.size(), stream_on(device)), "pack_moments");
+    const vetrast_moments_args a = moments_args(list, m, v, scale);
+    check(vetrast_pack_moments(context_on(device), &a, stream_on(device)), "pack_moments");
     return {m, v, scale};
 }
 
@@ -449,14 +424,9 @@ std::tuple<torch::Tensor, torch::Tensor> UnpackMoments(const torch::Tensor& exp_
                 "unpack_moments: whole blocks of ", kBlock, " codes with two scales each are needed");
     const auto floats = torch::TensorOptions(device).dtype(torch::kFloat32);
     torch::Tensor m = torch::empty({n}, floats), v = torch::empty({n}, floats);
-    vetrast_moment_tensor t;
-    t.exp_avg         = m.data_ptr<float>();
-    t.exp_avg_sq      = v.data_ptr<float>();
-    t.exp_avg_code    = exp_avg.data_ptr<uint8_t>();
-    t.exp_avg_sq_code = exp_avg_sq.data_ptr<uint8_t>();
-    t.block_scale     = block_scale.data_ptr<uint8_t>();
-    t.n               = n;
-    check(vetrast_unpack_moments(context_on(device), &t, 1, stream_on(device)), "unpack_moments");
+    const std::vector<vetrast_moment_tensor> list{{m.data_ptr<float>(), v.data_ptr<float>(), n, 0}};
+    const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);
+    check(vetrast_unpack_moments(context_on(device), &a, stream_on(device)), "unpack_moments");
     return {m, v};
 }
 }  // namespace vet_amd

@@ -12,7 +12,7 @@
 namespace vet_amd
 {
 // The reference steps its texture with MyAdam (src/lib/models/my_adam.cpp) and its network with torch::optim::Adam, a dozen
-// elementwise launches a tensor; this class takes both kinds of tensors, in one launch for up to 60 of them.
+// elementwise launches a tensor; this class takes both kinds of tensors, in one launch for up to 120 of them.
 class AdamW
 {
    public:

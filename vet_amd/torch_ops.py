@@ -58,7 +58,7 @@ def MyAdam(groups, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
 
 def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weights=False, stochastic_rounding=False, seed=0,
           capturable=False):
-    """AdamW over everything a training step has gradients for, in one launch for up to 60 tensors (vetrast_adamw_step).
+    """AdamW over everything a training step has gradients for, in one launch for up to 120 tensors (vetrast_adamw_step).
 
     groups: list of (list of parameter tensors, learning rate, weight decay). Parameters are dense CUDA tensors of float32,
     bfloat16 or float16 in any order of dimensions; gradients are found in .grad at every step.
