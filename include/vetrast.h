@@ -458,7 +458,8 @@ typedef struct vetrast_gradient_norm_args
     int32_t reserved;
     double max_norm, scale;
     float* out;      /* device [2] */
-    void* workspace; /* device, 8-byte aligned; not shared by calls that may overlap */
+    void* workspace; /* device, 16-byte aligned. Zeroed before the first call that uses it, and left alone between calls.
+                        Not shared by calls that may overlap, replays of graphs among them */
     size_t workspace_bytes;
 } vetrast_gradient_norm_args;
 size_t vetrast_gradient_norm_workspace_bytes(const vetrast_gradient* gradients, int32_t num_gradients);

@@ -108,7 +108,7 @@ def norm_args(**changes):
 
 
 @pytest.mark.parametrize("change", [
-    dict(a_num_gradients=-1), dict(a_out=None), dict(a_out=AT + 2), dict(a_workspace=None), dict(a_workspace=AT + 4),
+    dict(a_num_gradients=-1), dict(a_out=None), dict(a_out=AT + 2), dict(a_workspace=None), dict(a_workspace=AT + 8),
     dict(a_scale=float("nan")), dict(a_scale=float("inf")), dict(a_max_norm=float("nan")), dict(t_n=-1), dict(t_type=3), dict(t_type=-1),
     dict(t_grad=None), dict(t_grad=AT + 2), dict(t_grad=AT + 1, t_type=1)], ids=str)
 def test_norm_refuses(change, lib, ctx):
@@ -126,7 +126,7 @@ def test_norm_workspace(lib, ctx):
     many = (abi.Gradient * 1000)()
     for g in many:
         g.n = 1 << 33
-    assert lib.vetrast_gradient_norm_workspace_bytes(many, 1000) >= 8 * 1000 * need // 200
+    assert lib.vetrast_gradient_norm_workspace_bytes(many, 1000) > 60 * (need - 4096)  # 16 entries each, 240 a launch
     a = norm_args(a_workspace_bytes=need - 1)
     assert lib.vetrast_gradient_norm(ctx, C.byref(a), None) == abi.ERR_WORKSPACE_SMALL
     a.gradients = None

@@ -1,13 +1,14 @@
 // Optimiser kernels over lists of tensors: AdamW with moments in 32 or 8 bits, the norm of all gradients, moments to 8 bits and back.
 //
-// A launch takes a table of tensors in its arguments (no copy to the device, nothing to keep, and what a graph captures is whole). It is
-// cut into chunks of kOptimChunk elements, 8 a thread, and every workgroup goes through chunks blockIdx.x, blockIdx.x + gridDim.x, ...
+// A launch takes a table of tensors in its arguments (no copy to the device, nothing to keep, and what a graph captures is whole). The
+// tensors are cut into chunks of kOptimChunk elements, 8 a thread, one for each workgroup (27.5 M float32 elements: 142 us; workgroups of a
+// grid of 2048 that go on to further chunks 154 us), but for norms, where a workgroup leaves a sum.
 #pragma once
 #include "common.h"
 
 namespace vetrast
 {
-constexpr uint32_t kOptimChunk   = 8 * kBlock;  // elements a workgroup takes at a time: 8 a thread
+constexpr uint32_t kOptimChunk   = 8 * kBlock;  // elements
 constexpr int kMomentBlock       = VETRAST_MOMENT_BLOCK;
 constexpr uint32_t kMomentMargin = 0x100100;  // see code_base
 static_assert(kOptimChunk % kMomentBlock == 0 && kMomentBlock == 16 * 8, "16 lanes of 8 elements hold a block");
@@ -46,76 +47,131 @@ struct RawEight
     uint4 a, b;
 };
 
-// Elements i ... i + 7 of p, those from `count` on as zeros. whole: all eight are there and p + i is 16-byte aligned.
-__device__ __forceinline__ RawEight load_raw(const void* p, uint32_t type, uint32_t i, uint32_t count, bool whole)
+// A thread's eight elements of a chunk that begins at element `start` of a tensor: the eight from 8 * threadIdx.x on, or (halves) the four
+// from 4 * threadIdx.x on and the four kOptimChunk / 2 behind these, with which a wave's access to float32 has no gaps. Writes gain by
+// that, in what the last-level cache holds: 10 M first and second moments written 24.9 us, in halves 18.8; a step of 4 M elements with
+// masters 20.3 us, in halves 18.5. Beyond it a step does not (27.5 M float32: 142 us either way).
+// Addresses are one scalar for the workgroup and 32 bits for the thread. Registers that a load does not fill are left alone: to clear
+// them would wait for what is under way.
+template <int BYTES, bool HALVES = false>
+__device__ __forceinline__ RawEight load_eight(const void* p, uint32_t start)
 {
+    const char* base = (const char*)p + (size_t)start * BYTES;
     RawEight r;
-    r.a = r.b = make_uint4(0, 0, 0, 0);
-    if (type == VETRAST_F32)
+    if constexpr (HALVES)
     {
-        const uint32_t* x = (const uint32_t*)p + i;
-        if (whole)
+        constexpr uint32_t half = kOptimChunk / 2 * BYTES;
+        const uint32_t here     = threadIdx.x * 4u * BYTES;
+        if constexpr (BYTES == 4)
         {
-            r.a = ((const uint4*)x)[0];
-            r.b = ((const uint4*)x)[1];
+            r.a = *(const uint4*)(base + here);
+            r.b = *(const uint4*)(base + here + half);
         }
-        else if (count)
+        else
         {
-            uint32_t w[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) w[j] = x[min(j, count - 1)];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) w[j] = j < count ? w[j] : 0u;
-            r.a = make_uint4(w[0], w[1], w[2], w[3]);
-            r.b = make_uint4(w[4], w[5], w[6], w[7]);
+            const uint2 x = *(const uint2*)(base + here), y = *(const uint2*)(base + here + half);
+            r.a = make_uint4(x.x, x.y, y.x, y.y);
         }
     }
     else
     {
-        const uint16_t* x = (const uint16_t*)p + i;
-        if (whole) r.a = *(const uint4*)x;
-        else if (count)
-        {
-            uint32_t w[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) w[j] = x[min(j, count - 1)];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) w[j] = j < count ? w[j] : 0u;
-            r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-        }
+        const uint32_t here = threadIdx.x * 8u * BYTES;
+        r.a                 = *(const uint4*)(base + here);
+        if constexpr (BYTES == 4) r.b = *(const uint4*)(base + here + 16);
     }
     return r;
 }
-
-__device__ __forceinline__ void store_raw(void* p, uint32_t type, uint32_t i, uint32_t count, bool whole, const RawEight& r)
+template <int BYTES, bool HALVES = false>
+__device__ __forceinline__ void store_eight(void* p, uint32_t start, const RawEight& r)
 {
-    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-    if (type == VETRAST_F32)
+    char* base = (char*)p + (size_t)start * BYTES;
+    if constexpr (HALVES)
     {
-        uint32_t* x = (uint32_t*)p + i;
-        if (whole)
+        constexpr uint32_t half = kOptimChunk / 2 * BYTES;
+        const uint32_t here     = threadIdx.x * 4u * BYTES;
+        if constexpr (BYTES == 4)
         {
-            ((uint4*)x)[0] = r.a;
-            ((uint4*)x)[1] = r.b;
+            *(uint4*)(base + here)        = r.a;
+            *(uint4*)(base + here + half) = r.b;
         }
         else
         {
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (j < count) x[j] = w[j];
+            *(uint2*)(base + here)        = make_uint2(r.a.x, r.a.y);
+            *(uint2*)(base + here + half) = make_uint2(r.a.z, r.a.w);
         }
     }
     else
     {
-        uint16_t* x = (uint16_t*)p + i;
-        if (whole) *(uint4*)x = r.a;
-        else
-        {
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (j < count) x[j] = (uint16_t)(w[j / 2] >> 16 * (j % 2));
-        }
+        const uint32_t here    = threadIdx.x * 8u * BYTES;
+        *(uint4*)(base + here) = r.a;
+        if constexpr (BYTES == 4) *(uint4*)(base + here + 16) = r.b;
     }
+}
+
+// The first `count` of them, at any address; the others read as zeros and are not written.
+template <int BYTES>
+__device__ __forceinline__ RawEight load_some(const void* p, uint32_t start, uint32_t count)
+{
+    RawEight r;
+    r.a = r.b = make_uint4(0, 0, 0, 0);
+    if (count)
+    {
+        const char* base    = (const char*)p + (size_t)start * BYTES;
+        const uint32_t here = threadIdx.x * 8u * BYTES;
+        uint32_t w[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+        {
+            const char* x = base + here + min(j, count - 1) * BYTES;
+            if constexpr (BYTES == 4) w[j] = *(const uint32_t*)x;
+            else w[j] = *(const uint16_t*)x;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) w[j] = j < count ? w[j] : 0u;
+        if constexpr (BYTES == 4)
+        {
+            r.a = make_uint4(w[0], w[1], w[2], w[3]);
+            r.b = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        else r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+    return r;
+}
+template <int BYTES>
+__device__ __forceinline__ void store_some(void* p, uint32_t start, uint32_t count, const RawEight& r)
+{
+    char* base          = (char*)p + (size_t)start * BYTES;
+    const uint32_t here = threadIdx.x * 8u * BYTES;
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+        if (j < count)
+        {
+            if constexpr (BYTES == 4) *(uint32_t*)(base + here + j * 4) = w[j];
+            else *(uint16_t*)(base + here + j * 2) = (uint16_t)(w[j / 2] >> 16 * (j % 2));
+        }
+}
+
+// Of a type known at run time, `whole` where all threads have their eight at 16-byte addresses.
+__device__ __forceinline__ RawEight load_any(const void* p, uint32_t type, uint32_t start, uint32_t count, bool whole)
+{
+    if (type == VETRAST_F32) return whole ? load_eight<4>(p, start) : load_some<4>(p, start, count);
+    return whole ? load_eight<2>(p, start) : load_some<2>(p, start, count);
+}
+__device__ __forceinline__ void store_any(void* p, uint32_t type, uint32_t start, uint32_t count, bool whole, const RawEight& r)
+{
+    if (type == VETRAST_F32)
+    {
+        if (whole) store_eight<4>(p, start, r);
+        else store_some<4>(p, start, count, r);
+    }
+    else if (whole) store_eight<2>(p, start, r);
+    else store_some<2>(p, start, count, r);
+}
+__device__ __forceinline__ uint32_t count_of(uint32_t start, uint32_t n)
+{
+    const uint32_t i = start + threadIdx.x * 8u;
+    return i < n ? min(n - i, 8u) : 0u;
 }
 
 __device__ __forceinline__ void to_floats(const RawEight& r, uint32_t type, float* x)
@@ -152,7 +208,6 @@ __device__ __forceinline__ void to_floats(const RawEight& r, uint32_t type, floa
 __device__ __forceinline__ RawEight from_floats(const float* x, uint32_t type)
 {
     RawEight r;
-    r.b = make_uint4(0, 0, 0, 0);
     if (type == VETRAST_F32)
     {
         r.a = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -191,17 +246,27 @@ __host__ __device__ inline uint32_t step_key(uint64_t seed, int64_t step)
     return (uint32_t)mix64(mix64(seed) + (uint64_t)step);
 }
 
-// 20 random bits for each of 8 elements, the first of which is half of pair number `pair`: 32 bits of a hash serve two elements, the
+__device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_t c)
+{
+    uint32_t x;
+    asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x96" : "=v"(x) : "v"(a), "v"(b), "v"(c));
+    return x;
+}
+
+// 20 random bits for each of a thread's eight elements; `pair`: number of the chunk's first pair of elements. 32 bits of a hash serve two
+// elements, the
 // lower 20 and the upper 20 of them (products of 32 bits take four times as long as other instructions, and the 8-bit step is
 // bound by instructions).
+template <bool HALVES>
 __device__ __forceinline__ void random_eight(uint32_t pair, uint32_t key, uint32_t* r)
 {
-    const uint32_t start = pair * 0x9E3779B1u;
+    const uint32_t start = pair * 0x9E3779B1u + threadIdx.x * ((HALVES ? 2u : 4u) * 0x9E3779B1u);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
     {
-        uint32_t x = start + j * 0x9E3779B1u;
-        x          = x ^ (x >> 15) ^ key;
+        const uint32_t k = HALVES && j >= 2 ? kOptimChunk / 4 + j - 2 : j;
+        uint32_t x       = start + k * 0x9E3779B1u;
+        x                = exclusive_or(x, x >> 15, key);
         x *= 0xBB67AE85u;
         x ^= x >> 15;
         x *= 0xA54FF53Bu;
@@ -211,9 +276,17 @@ __device__ __forceinline__ void random_eight(uint32_t pair, uint32_t key, uint32
     }
 }
 
-// Odd factors make of an element's bits others that go with them without correlation to speak of (measured over 2^20 elements).
-__device__ __forceinline__ uint32_t second_bits(uint32_t r) { return __umul24(r, 0x5D3u) & 0xFFFFFu; }
-__device__ __forceinline__ uint32_t parameter_bits(uint32_t r) { return __umul24(r, 0xE2Bu) >> 4 & 0xFFFFu; }
+// Odd factors make of an element's bits others that go with them without correlation to speak of (measured over 2^20 elements). The
+// instruction is named: for products of which only the lower bits are used the compiler takes the one of 32 bits, four times as long.
+template <uint32_t FACTOR>
+__device__ __forceinline__ uint32_t times(uint32_t r)
+{
+    uint32_t x;
+    asm("v_mul_u32_u24 %0, %1, %2" : "=v"(x) : "s"(FACTOR), "v"(r));
+    return x;
+}
+__device__ __forceinline__ uint32_t second_bits(uint32_t r) { return times<0x5D3>(r) & 0xFFFFFu; }
+__device__ __forceinline__ uint32_t parameter_bits(uint32_t r) { return times<0xE2B>(r) >> 4 & 0xFFFFu; }
 
 // ---- moments in 8 bits -------------------------------------------------------------------------------------------------
 
@@ -239,20 +312,33 @@ __device__ __forceinline__ uint32_t code_base(uint32_t largest)
 // A code stands for float(bits = (code << 20) + base) - float(base). Magnitude x gets it from x + float(base), whose bits less those of
 // the base are the code, with 20 bits below it that decide between it and the next: values between two codes are evenly
 // spaced, so r in [0, 2^20) that is random leaves the mean as it is.
-__device__ __forceinline__ uint32_t offset_bits(float x, uint32_t base, uint32_t r)
+__device__ __forceinline__ uint32_t offset_bits(float x, float base, uint32_t minus_base, uint32_t r)
 {
-    return __float_as_uint(fabsf(x) + __uint_as_float(base)) + r - base;
+    uint32_t d;  // a sum of three, which the compiler makes two of
+    asm("v_add3_u32 %0, %1, %2, %3" : "=v"(d) : "v"(__float_as_uint(fabsf(x) + base)), "v"(r), "v"(minus_base));
+    return d;
 }
 
+// `BITS` bits of w from bit AT on, as a number that the compiler does not take apart: with the shift and sum behind it two
+// instructions, and not three.
+template <int AT, int BITS>
+__device__ __forceinline__ uint32_t field(uint32_t w)
+{
+    uint32_t x;
+    asm("v_bfe_u32 %0, %1, %2, %3" : "=v"(x) : "v"(w), "i"(AT), "i"(BITS));
+    return x;
+}
 __device__ __forceinline__ float code_value(uint32_t code, uint32_t base)
 {
     return __uint_as_float((code << 20) + base) - __uint_as_float(base);
 }
 
-// The middle one of three.
+// The middle one of three: one instruction, which the compiler does not find for unsigned variables.
 __device__ __forceinline__ uint32_t middle(uint32_t a, uint32_t b, uint32_t c)
 {
-    return max(min(a, b), min(max(a, b), c));
+    uint32_t x;
+    asm("v_med3_u32 %0, %1, %2, %3" : "=v"(x) : "v"(a), "v"(b), "v"(c));
+    return x;
 }
 
 struct Codes
@@ -285,15 +371,16 @@ __device__ __forceinline__ Codes encode_moments(const float* m, const float* v, 
         dm = code_base<15>(row_max(top));
     }
     if (lost) dm = 255u;
-    const uint32_t bm = dm << 23, bv = dv << 23;
+    const float bm = __uint_as_float(dm << 23), bv = __uint_as_float(dv << 23);
+    const uint32_t minus_m = 0u - (dm << 23), minus_v = 0u - (dv << 23);
     uint32_t a[8], b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
         // seven bits of code to the top, below the sign
-        a[j] = (offset_bits(m[j], bm, rm[j]) << 4 & 0x7FFFFFFFu) | (__float_as_uint(m[j]) & 0x80000000u);
+        a[j] = __float_as_uint(copysignf(__uint_as_float(offset_bits(m[j], bm, minus_m, rm[j]) << 4), m[j]));
         // above zero is at least code 1: a code is never above a value's own bits, so the middle one says so
-        b[j] = middle(__float_as_uint(v[j]), 1u, offset_bits(v[j], bv, rv[j]) >> 20);
+        b[j] = middle(__float_as_uint(v[j]), 1u, offset_bits(v[j], bv, minus_v, rv[j]) >> 20);
     }
     Codes c;
     uint32_t w[2], x[2];
@@ -311,16 +398,19 @@ __device__ __forceinline__ Codes encode_moments(const float* m, const float* v, 
     return c;
 }
 
-__device__ __forceinline__ void decode_moments(const Codes& c, float* m, float* v)
+template <int AT>
+__device__ __forceinline__ void decode_one(uint32_t wm, uint32_t wv, uint32_t bm, uint32_t bv, float& m, float& v)
 {
-    const uint32_t bm = (c.scale & 255u) << 23, bv = c.scale >> 8 << 23;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-    {
-        const uint32_t wm = j < 4 ? c.m.x : c.m.y, wv = j < 4 ? c.v.x : c.v.y;
-        m[j] = copysignf(code_value(wm >> 8 * (j % 4) & 127u, bm), __uint_as_float(wm << (24 - 8 * (j % 4))));
-        v[j] = code_value(wv >> 8 * (j % 4) & 255u, bv);
-    }
+    m = copysignf(code_value(field<AT, 7>(wm), bm), __uint_as_float(wm << (24 - AT)));
+    v = code_value(field<AT, 8>(wv), bv);
+}
+__device__ __forceinline__ void decode_four(uint32_t wm, uint32_t wv, uint32_t scale, float* m, float* v)
+{
+    const uint32_t bm = (scale & 255u) << 23, bv = scale >> 8 << 23;
+    decode_one<0>(wm, wv, bm, bv, m[0], v[0]);
+    decode_one<8>(wm, wv, bm, bv, m[1], v[1]);
+    decode_one<16>(wm, wv, bm, bv, m[2], v[2]);
+    decode_one<24>(wm, wv, bm, bv, m[3], v[3]);
 }
 
 // ---- AdamW -------------------------------------------------------------------------------------------------------------
@@ -344,11 +434,24 @@ enum
 
 struct AdamWGroup
 {
-    float step_size;     // lr / (1 - beta1^step)
-    float keep;          // 1 - lr * weight_decay
-    float inv_sqrt_bc2;  // 1 / sqrt(1 - beta2^step)
-    uint32_t key;        // of this step's random bits
+    float root;    // with s = lr / (1 - beta1^step): the parameter changes by m / (root * sqrt(v) + floor), root is
+    float floor;   // 1 / (s sqrt(1 - beta2^step)) and floor eps / s
+    float keep;    // 1 - lr * weight_decay
+    uint32_t key;  // of this step's random bits
 };
+
+__host__ __device__ inline AdamWGroup adamw_group(double lr, double weight_decay, double eps, double bc1, double bc2, uint32_t key)
+{
+    const double s = lr / bc1;
+    AdamWGroup g;
+    g.root  = (float)(1.0 / (s * sqrt(bc2)));
+    g.floor = (float)(eps / s);
+    if (!(fabsf(g.root) <= 3e38f) || !(fabsf(g.floor) <= 3e38f)) g.root = 0.f, g.floor = __builtin_inff();  // no step to speak of
+    if (fabsf(g.floor) < 1.17549435e-38f) g.floor = copysignf(1.17549435e-38f, g.floor);  // a reciprocal's smallest argument
+    g.keep = (float)(1.0 - lr * weight_decay);
+    g.key  = key;
+    return g;
+}
 
 struct AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel leaves for the step's launches
 {
@@ -369,7 +472,7 @@ struct AdamWCommon
     const float* grad_scale;
     const AdamWDevice* device;  // where set, g[].key are places in device->group
     uint32_t entries, chunks;
-    float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
+    float beta1, one_minus_beta1, beta2, one_minus_beta2;
     int zero_grad, stochastic, exact_root;
 };
 template <int ENTRIES>
@@ -390,7 +493,7 @@ struct AdamWBegin
     AdamWBeginGroup g[kBeginGroups];
     AdamWDevice* device;
     const float* grad_scale;
-    double beta1, beta2;
+    double beta1, beta2, eps;
     uint64_t seed;
     int first, groups, last;
 };
@@ -406,171 +509,211 @@ __global__ void __launch_bounds__(kBeginGroups) adamw_begin_kernel(const AdamWBe
     const int k = (int)threadIdx.x;
     if (k < a.groups)
     {
-        const double lr  = a.g[k].lr * (double)factor;
-        const double bc1 = 1.0 - pow(a.beta1, (double)step), bc2 = 1.0 - pow(a.beta2, (double)step);
-        AdamWGroup g;
-        g.step_size    = (float)(lr / bc1);
-        g.keep         = (float)(1.0 - lr * a.g[k].weight_decay);
-        g.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2));
-        g.key          = step_key(a.seed, step);
-        a.device->group[a.first + k] = g;
+        a.device->group[a.first + k] = adamw_group(a.g[k].lr * (double)factor, a.g[k].weight_decay, a.eps, 1.0 - pow(a.beta1, (double)step),
+                                                   1.0 - pow(a.beta2, (double)step), step_key(a.seed, step));
     }
     if (a.last && counts && k == 0) a.device->state.step = step;
+}
+
+// Chunks of four kinds. In whole ones every thread has its eight elements at addresses that are multiples of 16, parameter and gradient
+// of one width: their loads are straight code, all of them under way at once. `kAnyChunk` does for everything else.
+enum ChunkKind
+{
+    kFloatChunk,   // float32
+    kShortChunk,   // 16 bits
+    kMasterChunk,  // 16 bits, with masters
+    kAnyChunk
+};
+
+template <int BITS, ChunkKind KIND>
+__device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEntry& e, uint32_t start, float grad_scale)
+{
+    constexpr bool ANY    = KIND == kAnyChunk;
+    constexpr bool HALVES = BITS == 32 && !ANY;  // blocks of 8-bit moments are eight elements of 16 neighbouring lanes
+    constexpr int BYTES   = KIND == kFloatChunk ? 4 : 2;
+    const uint32_t flags  = e.flags;
+    const uint32_t p_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : flags & kAdamWParam;
+    const uint32_t g_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : (flags & kAdamWGrad) >> 2;
+    const bool master     = ANY ? flags & kAdamWMaster : KIND == kMasterChunk;
+    const uint32_t count  = ANY ? count_of(start, e.n) : 8u;
+    const bool whole      = e.n - start >= kOptimChunk && (flags & kAdamWAligned);
+    const auto clear      = [&] {
+        const RawEight zero = {};
+        if constexpr (ANY) store_any(e.grad, g_type, start, count, whole, zero);
+        else store_eight<BYTES, HALVES>(e.grad, start, zero);
+    };
+    if (!isfinite(grad_scale))
+    {
+        if (a.zero_grad) clear();
+        return;
+    }
+    // places of the chunk in the flat arrays, and whether this thread's eight belong to a block of the tensor
+    const uint32_t block = e.block + start / kMomentBlock;
+    const size_t at      = (size_t)block * kMomentBlock;
+    const uint32_t mine  = threadIdx.x * 8u;
+    const bool inside    = !ANY || start + mine < (e.n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
+    uint8_t *mcs = (uint8_t*)a.m + at, *vcs = (uint8_t*)a.v + at;
+    uint16_t* scales = a.scale + block;
+
+    RawEight rg, rp, r1, r2;
+    Codes codes;
+    if constexpr (ANY) rg = load_any(e.grad, g_type, start, count, whole);
+    else rg = load_eight<BYTES, HALVES>(e.grad, start);
+    if constexpr (ANY)
+    {
+        rp = r1 = r2 = RawEight{};
+        codes        = Codes{};
+        if (!master) rp = load_any(e.param, p_type, start, count, whole);
+    }
+    if (inside)
+    {
+        if (master) rp = load_eight<4, HALVES>(a.master + at, 0);
+        else if constexpr (!ANY) rp = load_eight<BYTES, HALVES>(e.param, start);
+        if constexpr (BITS == 32)
+        {
+            r1 = load_eight<4, HALVES>((float*)a.m + at, 0);
+            r2 = load_eight<4, HALVES>((float*)a.v + at, 0);
+        }
+        else
+        {
+            codes.m     = *(const uint2*)(mcs + mine);
+            codes.v     = *(const uint2*)(vcs + mine);
+            codes.scale = scales[mine / kMomentBlock];
+        }
+    }
+    AdamWGroup g = a.g[flags >> 8];
+    if (a.device) g = a.device->group[g.key];
+    const bool random = KIND != kFloatChunk && !master && a.stochastic && p_type == VETRAST_BF16;
+    uint32_t r[8];
+    if (BITS == 8 || random) random_eight<HALVES>((uint32_t)(at / 2), g.key, r);
+
+    float x[8], p[8], m[8], v[8];
+    to_floats(rg, g_type, x);
+    to_floats(rp, master ? VETRAST_F32 : p_type, p);
+    if constexpr (BITS == 32)
+    {
+        to_floats(r1, VETRAST_F32, m);
+        to_floats(r2, VETRAST_F32, v);
+    }
+    else
+    {
+        decode_four(codes.m.x, codes.v.x, codes.scale, m, v);
+        decode_four(codes.m.y, codes.v.y, codes.scale, m + 4, v + 4);
+    }
+    // Rounded after every operation: both kinds of state, and whoever steps them elsewhere, get the same bits.
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+    {
+        x[j] *= grad_scale;
+        m[j] = m[j] * a.beta1 + x[j] * a.one_minus_beta1;
+        v[j] = v[j] * a.beta2 + (x[j] * a.one_minus_beta2) * x[j];
+    }
+    // With 8-bit moments root and quotient are the instructions for them, good to 1.54 half steps of float32 each, as the step is
+    // bound by instructions; with 32-bit ones it waits for memory and they are rounded to nearest. The root instruction takes
+    // values below 2^-126 for zero: eps makes up for that unless it is tiny itself.
+    if (BITS == 32 || a.exact_root)
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = sqrtf(v[j]);
+    }
+    else
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_sqrtf(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+    {
+        const float d = fmaf(x[j], g.root, g.floor);
+        p[j]          = BITS == 32 ? p[j] * g.keep - m[j] / d : fmaf(-m[j], __builtin_amdgcn_rcpf(d), p[j] * g.keep);
+    }
+
+    bool lost = true;  // whether one of these eight may not be finite
+    if constexpr (BITS == 32)
+    {
+        if (inside)
+        {
+            store_eight<4, HALVES>((float*)a.m + at, 0, from_floats(m, VETRAST_F32));
+            store_eight<4, HALVES>((float*)a.v + at, 0, from_floats(v, VETRAST_F32));
+        }
+    }
+    else
+    {
+        uint32_t rv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rv[j] = second_bits(r[j]);
+        const Codes c = encode_moments(m, v, r, rv, (codes.scale & 255u) == 255u);
+        if (inside)
+        {
+            *(uint2*)(mcs + mine) = c.m;
+            *(uint2*)(vcs + mine) = c.v;
+            if (mine % kMomentBlock == 0) scales[mine / kMomentBlock] = (uint16_t)c.scale;
+        }
+        lost = c.scale >> 8 == 255u;  // a gradient that is not finite shows there; of parameters and first moments that are not,
+                                      // the lower bits are zeros
+    }
+    RawEight out;
+    if (random)
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = parameter_bits(r[j]);
+        if (lost)
+        {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = __builtin_isfinite(p[j]) ? r[j] : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] += __float_as_uint(p[j]);
+        out.a = make_uint4(__builtin_amdgcn_perm(r[1], r[0], 0x07060302), __builtin_amdgcn_perm(r[3], r[2], 0x07060302),
+                           __builtin_amdgcn_perm(r[5], r[4], 0x07060302), __builtin_amdgcn_perm(r[7], r[6], 0x07060302));
+    }
+    else out = from_floats(p, p_type);
+    if constexpr (ANY) store_any(e.param, p_type, start, count, whole, out);
+    else store_eight<BYTES, HALVES>(e.param, start, out);
+    if (master && inside) store_eight<4, HALVES>(a.master + at, 0, from_floats(p, VETRAST_F32));
+    if (a.zero_grad) clear();
 }
 
 template <int BITS, class Launch>
 __global__ void __launch_bounds__(kBlock) adamw_step_kernel(const Launch a)
 {
     const ChunkFinder<finder_groups(sizeof(a.e) / sizeof(a.e[0]))> find(a);
+    const AdamWEntry& e    = a.e[find(blockIdx.x)];
+    const uint32_t start   = (blockIdx.x - e.first_chunk) * kOptimChunk;
     const float grad_scale = a.grad_scale ? *a.grad_scale : 1.f;
-    const bool leave       = !isfinite(grad_scale);
-    for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
-    {
-        const AdamWEntry& e  = a.e[find(chunk)];
-        const uint32_t flags = e.flags, n = e.n;
-        const uint32_t p_type = flags & kAdamWParam, g_type = (flags & kAdamWGrad) >> 2;
-        const uint32_t i      = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
-        const uint32_t count  = i < n ? min(n - i, 8u) : 0u;
-        const bool whole      = count == 8u && (flags & kAdamWAligned);
-        const uint32_t block  = e.block + i / kMomentBlock;
-        const size_t at       = (size_t)block * kMomentBlock + i % kMomentBlock;  // in the flat arrays
-        const bool inside     = i < (n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
-        const RawEight zero   = {};
-        if (leave)
-        {
-            if (a.zero_grad) store_raw(e.grad, g_type, i, count, whole, zero);
-            continue;
-        }
-        const bool master = flags & kAdamWMaster;
-        RawEight rg, rp = zero, r1 = zero, r2 = zero;
-        Codes codes     = {};
-        rg              = load_raw(e.grad, g_type, i, count, whole);
-        if (!master) rp = load_raw(e.param, p_type, i, count, whole);
-        if (inside)
-        {
-            if (master) rp = {((const uint4*)(a.master + at))[0], ((const uint4*)(a.master + at))[1]};
-            if constexpr (BITS == 32)
-            {
-                r1 = {((const uint4*)((float*)a.m + at))[0], ((const uint4*)((float*)a.m + at))[1]};
-                r2 = {((const uint4*)((float*)a.v + at))[0], ((const uint4*)((float*)a.v + at))[1]};
-            }
-            else
-            {
-                codes.m     = *(const uint2*)((const uint8_t*)a.m + at);
-                codes.v     = *(const uint2*)((const uint8_t*)a.v + at);
-                codes.scale = a.scale[block];
-            }
-        }
-        AdamWGroup g = a.g[flags >> 8];
-        if (a.device) g = a.device->group[g.key];
-        const bool random = a.stochastic && p_type == VETRAST_BF16 && !master;
-        uint32_t r[8];
-        if (BITS == 8 || random) random_eight((uint32_t)(at / 2), g.key, r);
-
-        float x[8], p[8], m[8], v[8];
-        to_floats(rg, g_type, x);
-        to_floats(rp, master ? VETRAST_F32 : p_type, p);
-        if constexpr (BITS == 32)
-        {
-            to_floats(r1, VETRAST_F32, m);
-            to_floats(r2, VETRAST_F32, v);
-        }
-        else decode_moments(codes, m, v);
-        // Rounded after every operation: both kinds of state, and whoever steps them elsewhere, get the same bits.
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-        {
-            x[j] *= grad_scale;
-            m[j] = m[j] * a.beta1 + x[j] * a.one_minus_beta1;
-            v[j] = v[j] * a.beta2 + (x[j] * a.one_minus_beta2) * x[j];
-        }
-        // With 8-bit moments root and quotient are the instructions for them, good to 1.54 half steps of float32 each, as the step is
-        // bound by instructions; with 32-bit ones it waits for memory and they are rounded to nearest. The root instruction takes
-        // values below 2^-126 for zero: eps makes up for that unless it is tiny itself.
-        if (BITS == 32 || a.exact_root)
-        {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = sqrtf(v[j]);
-        }
-        else
-        {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_sqrtf(v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-        {
-            const float d = fmaf(x[j], g.inv_sqrt_bc2, a.eps);
-            const float q = BITS == 32 ? m[j] / d : m[j] * __builtin_amdgcn_rcpf(d);
-            p[j]          = fmaf(-g.step_size, q, p[j] * g.keep);
-        }
-
-        if (master)
-        {
-            const RawEight out = from_floats(p, VETRAST_F32);
-            if (inside)
-            {
-                ((uint4*)(a.master + at))[0] = out.a;
-                ((uint4*)(a.master + at))[1] = out.b;
-            }
-        }
-        RawEight out;
-        if (random)
-        {
-            out.b = make_uint4(0, 0, 0, 0);
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-            {
-                const bool finite = __builtin_isfinite(p[j]);
-                w[j]              = __float_as_uint(p[j]) + (finite ? parameter_bits(r[j]) : 0u);
-            }
-            out.a = make_uint4(__builtin_amdgcn_perm(w[1], w[0], 0x07060302), __builtin_amdgcn_perm(w[3], w[2], 0x07060302),
-                               __builtin_amdgcn_perm(w[5], w[4], 0x07060302), __builtin_amdgcn_perm(w[7], w[6], 0x07060302));
-        }
-        else out = from_floats(p, p_type);
-        store_raw(e.param, p_type, i, count, whole, out);
-        if constexpr (BITS == 32)
-        {
-            const RawEight o1 = from_floats(m, VETRAST_F32), o2 = from_floats(v, VETRAST_F32);
-            if (inside)
-            {
-                ((uint4*)((float*)a.m + at))[0] = o1.a;
-                ((uint4*)((float*)a.m + at))[1] = o1.b;
-                ((uint4*)((float*)a.v + at))[0] = o2.a;
-                ((uint4*)((float*)a.v + at))[1] = o2.b;
-            }
-        }
-        else
-        {
-            uint32_t rv[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) rv[j] = second_bits(r[j]);
-            const Codes c = encode_moments(m, v, r, rv, (codes.scale & 255u) == 255u);
-            if (inside)
-            {
-                *(uint2*)((uint8_t*)a.m + at) = c.m;
-                *(uint2*)((uint8_t*)a.v + at) = c.v;
-                if (i % kMomentBlock == 0) a.scale[block] = (uint16_t)c.scale;
-            }
-        }
-        if (a.zero_grad) store_raw(e.grad, g_type, i, count, whole, zero);
-    }
+    const uint32_t p_type = e.flags & kAdamWParam, g_type = (e.flags & kAdamWGrad) >> 2;
+    if (e.n - start < kOptimChunk || !(e.flags & kAdamWAligned) || (p_type == VETRAST_F32) != (g_type == VETRAST_F32))
+        adamw_chunk<BITS, kAnyChunk>(a, e, start, grad_scale);
+    else if (p_type == VETRAST_F32) adamw_chunk<BITS, kFloatChunk>(a, e, start, grad_scale);
+    else if (e.flags & kAdamWMaster) adamw_chunk<BITS, kMasterChunk>(a, e, start, grad_scale);
+    else adamw_chunk<BITS, kShortChunk>(a, e, start, grad_scale);
 }
 
 // ---- norms -------------------------------------------------------------------------------------------------------------
 
-constexpr int kNormEntries = 250;
+constexpr int kNormEntries = 240;
 struct NormEntry
 {
     const void* grad;
     uint32_t n_type;  // n << 2 | type
     uint32_t first_chunk;
 };
+constexpr uint32_t kNormSlots = 32;
+struct NormWorkspace
+{
+    // Workgroups that have left their sum, by slot, and slots that are complete; zero between calls. A line each: an addition to one place
+    // takes 12 ns, and a call has up to a thousand workgroups.
+    uint32_t done[kNormSlots + 1][16];
+    uint32_t unused[16];
+    double partial[1];
+};
 struct NormLaunch
 {
-    double* partial;  // of this launch, one a workgroup
+    NormWorkspace* workspace;
+    float* out;
+    double max_norm, scale;
     uint32_t entries, chunks;
+    uint32_t first, total;  // this launch's first workgroup among those of the call, and their number
     NormEntry e[kNormEntries];
 };
 static_assert(sizeof(NormLaunch) <= 4096, "kernel arguments");
@@ -580,6 +723,7 @@ __device__ __forceinline__ double block_sum(double x)
 {
     __shared__ double part[kBlock / kWave];
     for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_down(x, d);
+    __syncthreads();
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
     __syncthreads();
     x = 0;
@@ -587,8 +731,27 @@ __device__ __forceinline__ double block_sum(double x)
     return x;
 }
 
-// In 64 bits throughout: no square overflows or vanishes, and a sum of any length is good to the last bit of a float.
-__global__ void __launch_bounds__(kBlock) gradient_squares_kernel(const NormLaunch a)
+// Leaves a workgroup's sum, and says whether it was the last of the call to do so; one thread of each. The sum goes past the caches of this
+// XCD (an atomic store of agent scope) and has arrived when the wait ends, so whoever finds all counts complete may read all sums. A
+// release would write back the whole L2 for it: 1024 workgroups 54 us instead of 31, in one slot.
+__device__ __forceinline__ bool leave_sum(NormWorkspace* w, uint32_t number, uint32_t total, double sum)
+{
+    const auto add = [](uint32_t* p) { return __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u; };
+    __hip_atomic_store(&w->partial[number], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint32_t slots = total <= 2 * kNormSlots ? 1u : kNormSlots;  // a second count takes 1 us
+    const uint32_t slot  = number % slots;
+    if (add(&w->done[slot][0]) != (total - slot + slots - 1) / slots) return false;
+    __hip_atomic_store(&w->done[slot][0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (slots == 1) return true;
+    if (add(&w->done[kNormSlots][0]) != slots) return false;
+    __hip_atomic_store(&w->done[kNormSlots][0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
+// In 64 bits throughout: no square overflows or vanishes, and a sum of any length is good to the last bit of a float. The workgroup that is
+// the last of the call to leave its sum adds all of them, in the order of their numbers: one launch instead of two, 4 us of a host's time.
+__global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const NormLaunch a)
 {
     const ChunkFinder<finder_groups(kNormEntries)> find(a);
     double sum = 0;
@@ -596,29 +759,34 @@ __global__ void __launch_bounds__(kBlock) gradient_squares_kernel(const NormLaun
     {
         const NormEntry& e   = a.e[find(chunk)];
         const uint32_t n     = e.n_type >> 2, type = e.n_type & 3u;
-        const uint32_t i     = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
-        const uint32_t count = i < n ? min(n - i, 8u) : 0u;
+        const uint32_t start = (chunk - e.first_chunk) * kOptimChunk;
+        RawEight r;
+        if (n - start >= kOptimChunk && (uintptr_t)e.grad % 16 == 0)
+        {
+            if (type == VETRAST_F32) r = load_eight<4, true>(e.grad, start);
+            else r = load_eight<2>(e.grad, start);
+        }
+        else r = load_any(e.grad, type, start, count_of(start, n), false);
         float x[8];
-        to_floats(load_raw(e.grad, type, i, count, count == 8u && (uintptr_t)e.grad % 16 == 0), type, x);
+        to_floats(r, type, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fma((double)x[j], (double)x[j], sum);
     }
     sum = block_sum(sum);
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
-}
-
-// Norm and factor from the workgroups' sums, added in an order of their own number.
-__global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const double* __restrict__ partial, uint32_t count, double max_norm, double scale, float* __restrict__ out)
-{
-    double sum = 0;
-    for (uint32_t k = threadIdx.x; k < count; k += kBlock) sum += partial[k];
+    __shared__ bool last;
+    if (threadIdx.x == 0) last = leave_sum(a.workspace, a.first + blockIdx.x, a.total, sum);
+    __syncthreads();
+    if (!last) return;
+    sum = 0;
+    for (uint32_t k = threadIdx.x; k < a.total; k += kBlock)
+        sum += __hip_atomic_load(&a.workspace->partial[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sum = block_sum(sum);
     if (threadIdx.x == 0)
     {
-        const double norm = fabs(scale) * sqrt(sum);
+        const double norm = fabs(a.scale) * sqrt(sum);
         const float told  = (float)norm;
-        out[0]            = told;
-        out[1]            = !isfinite(told) ? __builtin_nanf("") : (float)(max_norm > 0 && norm > max_norm ? scale * (max_norm / norm) : scale);
+        a.out[0]          = told;
+        a.out[1]          = !isfinite(told) ? __builtin_nanf("") : (float)(a.max_norm > 0 && norm > a.max_norm ? a.scale * (a.max_norm / norm) : a.scale);
     }
 }
 
@@ -639,54 +807,83 @@ struct MomentLaunch
 };
 static_assert(sizeof(MomentLaunch) <= 4096, "kernel arguments");
 
+__device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
+{
+    const uint32_t block = e.block + start / kMomentBlock;
+    const size_t at      = (size_t)block * kMomentBlock;
+    const uint32_t mine  = threadIdx.x * 8u, count = count_of(start, e.n);
+    const RawEight r1 = load_any(e.m, VETRAST_F32, start, count, whole), r2 = load_any(e.v, VETRAST_F32, start, count, whole);
+    float m[8], v[8];
+    to_floats(r1, VETRAST_F32, m);
+    to_floats(r2, VETRAST_F32, v);
+    uint32_t half[8], lost = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+    {
+        v[j]    = fabsf(v[j]);
+        half[j] = 1u << 19;
+        lost |= __builtin_isfinite(m[j]) ? 0u : 1u;
+    }
+    const Codes c = encode_moments(m, v, half, half, row_max(lost) != 0);
+    if (start + mine < (e.n + kMomentBlock - 1) / kMomentBlock * kMomentBlock)
+    {
+        *(uint2*)(a.m + at + mine) = c.m;
+        *(uint2*)(a.v + at + mine) = c.v;
+        if (mine % kMomentBlock == 0) a.scale[block + mine / kMomentBlock] = (uint16_t)c.scale;
+    }
+}
+
+// Four elements' codes at a time, so that a wave's writes have no gaps. `whole`: all of them are there, at 16-byte addresses.
+__device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
+{
+    const uint32_t block = e.block + start / kMomentBlock;
+    const size_t at      = (size_t)block * kMomentBlock;
+    uint32_t wm[2], wv[2], scale[2];
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q)
+    {
+        const uint32_t i = q * (kOptimChunk / 2) + threadIdx.x * 4u;
+        wm[q] = wv[q] = scale[q] = 0;
+        if (whole || start + i < e.n)
+        {
+            wm[q]    = *(const uint32_t*)(a.m + at + i);
+            wv[q]    = *(const uint32_t*)(a.v + at + i);
+            scale[q] = a.scale[block + i / kMomentBlock];
+        }
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q)
+    {
+        const uint32_t i = q * (kOptimChunk / 2) + threadIdx.x * 4u;
+        float m[4], v[4];
+        decode_four(wm[q], wv[q], scale[q], m, v);
+        float *pm = e.m + start, *pv = e.v + start;
+        if (whole)
+        {
+            *(float4*)(pm + i) = make_float4(m[0], m[1], m[2], m[3]);
+            *(float4*)(pv + i) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        else
+        {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (start + i + j < e.n)
+                {
+                    pm[i + j] = m[j];
+                    pv[i + j] = v[j];
+                }
+        }
+    }
+}
+
 template <bool PACK>
 __global__ void __launch_bounds__(kBlock) convert_moments_kernel(const MomentLaunch a)
 {
     const ChunkFinder<finder_groups(kMomentEntries)> find(a);
-    for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x)
-    {
-        const MomentEntry& e = a.e[find(chunk)];
-        const uint32_t i     = (chunk - e.first_chunk) * kOptimChunk + threadIdx.x * 8u;
-        const uint32_t count = i < e.n ? min(e.n - i, 8u) : 0u;
-        const bool whole     = count == 8u && (((uintptr_t)e.m | (uintptr_t)e.v) & 15) == 0;
-        const uint32_t block = e.block + i / kMomentBlock;
-        const size_t at      = (size_t)block * kMomentBlock + i % kMomentBlock;
-        const bool inside    = i < (e.n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
-        float m[8], v[8];
-        if constexpr (PACK)
-        {
-            const RawEight r1 = load_raw(e.m, VETRAST_F32, i, count, whole), r2 = load_raw(e.v, VETRAST_F32, i, count, whole);
-            to_floats(r1, VETRAST_F32, m);
-            to_floats(r2, VETRAST_F32, v);
-            uint32_t half[8], lost = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-            {
-                v[j]    = fabsf(v[j]);
-                half[j] = 1u << 19;
-                lost |= __builtin_isfinite(m[j]) ? 0u : 1u;
-            }
-            const Codes c = encode_moments(m, v, half, half, row_max(lost) != 0);
-            if (inside)
-            {
-                *(uint2*)(a.m + at) = c.m;
-                *(uint2*)(a.v + at) = c.v;
-                if (i % kMomentBlock == 0) a.scale[block] = (uint16_t)c.scale;
-            }
-        }
-        else
-        {
-            Codes c = {};
-            if (inside)
-            {
-                c.m     = *(const uint2*)(a.m + at);
-                c.v     = *(const uint2*)(a.v + at);
-                c.scale = a.scale[block];
-            }
-            decode_moments(c, m, v);
-            store_raw(e.m, VETRAST_F32, i, count, whole, from_floats(m, VETRAST_F32));
-            store_raw(e.v, VETRAST_F32, i, count, whole, from_floats(v, VETRAST_F32));
-        }
-    }
+    const MomentEntry& e = a.e[find(blockIdx.x)];
+    const uint32_t start = (blockIdx.x - e.first_chunk) * kOptimChunk;
+    const bool whole     = e.n - start >= kOptimChunk && (((uintptr_t)e.m | (uintptr_t)e.v) & 15) == 0;
+    if constexpr (PACK) pack_chunk(a, e, start, whole);
+    else unpack_chunk(a, e, start, whole);
 }
 }  // namespace vetrast

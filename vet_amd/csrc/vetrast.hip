@@ -480,8 +480,7 @@ inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<ui
 inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
 constexpr int64_t kOptimEntryElements = 1 << 29;  // a longer tensor is several entries of a launch: places inside one are 32 bits
-constexpr uint32_t kOptimGrid         = 2048;     // workgroups of a launch at most, each goes through its share of chunks
-constexpr uint32_t kNormGrid          = 1024;
+constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays, whose blocks have numbers of 32 bits
 {
@@ -496,7 +495,7 @@ void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStrea
     l.entries = l.chunks = 0;
     const auto launch = [&] {
         if (l.entries == 0) return;
-        const dim3 grid(std::min(l.chunks, kOptimGrid));
+        const dim3 grid(l.chunks);
         if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
         else hipLaunchKernelGGL((adamw_step_kernel<8, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
         l.entries = l.chunks = 0;
@@ -520,14 +519,9 @@ void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStrea
                 AdamWGroup& c                = l.g[slot];
                 slot_group[slots++]          = t.group;
                 if (l.device) c = {0.f, 0.f, 0.f, (uint32_t)t.group};
-                else
-                {
-                    // bias corrections in double, handed to the kernel rounded once
-                    c.step_size    = (float)(g.lr / (1.0 - std::pow(a->beta1, (double)g.step)));
-                    c.keep         = (float)(1.0 - g.lr * g.weight_decay);
-                    c.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)g.step)));
-                    c.key          = step_key(a->seed, g.step);
-                }
+                else  // bias corrections in double, handed to the kernel rounded once
+                    c = adamw_group(g.lr, g.weight_decay, a->eps, 1.0 - std::pow(a->beta1, (double)g.step), 1.0 - std::pow(a->beta2, (double)g.step),
+                                    step_key(a->seed, g.step));
             }
             AdamWEntry& e      = l.e[l.entries++];
             e.param            = static_cast<char*>(t.param) + from * (int64_t)dtype_bytes(t.param_type);
@@ -1432,6 +1426,7 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         b.grad_scale = a->grad_scale;
         b.beta1      = a->beta1;
         b.beta2      = a->beta2;
+        b.eps        = a->eps;
         b.seed       = a->seed;
         for (b.first = 0, b.last = 0; !b.last; b.first += kBeginGroups)
         {
@@ -1452,7 +1447,6 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         l.one_minus_beta1 = (float)(1.0 - a->beta1);
         l.beta2           = (float)a->beta2;
         l.one_minus_beta2 = (float)(1.0 - a->beta2);
-        l.eps             = (float)a->eps;
         l.zero_grad       = a->zero_grad;
         l.stochastic      = a->stochastic_rounding;
         // the root instruction's zero for values below 2^-126 is up to 2^-63 off, times at most 1 / sqrt(1 - beta2): half a step of eps
@@ -1483,7 +1477,7 @@ size_t vetrast_gradient_norm_workspace_bytes(const vetrast_gradient* gradients, 
         if (gradients[k].n < 0) return 0;
         entries += (gradients[k].n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
-    return (size_t)std::max<int64_t>((entries + kNormEntries - 1) / kNormEntries, 1) * kNormGrid * sizeof(double);
+    return sizeof(NormWorkspace) + (size_t)std::max<int64_t>((entries + kNormEntries - 1) / kNormEntries, 1) * kNormGrid * sizeof(double);
 }
 
 int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a, void* stream_)
@@ -1491,7 +1485,7 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
     if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
     if (a->num_gradients < 0 || (a->num_gradients > 0 && !a->gradients) || !a->out || !a->workspace) return VETRAST_ERR_INVALID_ARG;
     if (!std::isfinite(a->scale) || std::isnan(a->max_norm)) return VETRAST_ERR_INVALID_ARG;
-    if (!aligned_to(a->out, 4) || !aligned_to(a->workspace, 8)) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->out, 4) || !aligned_to(a->workspace, 16)) return VETRAST_ERR_INVALID_ARG;
     for (int k = 0; k < a->num_gradients; ++k)
     {
         const vetrast_gradient& g = a->gradients[k];
@@ -1500,34 +1494,41 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
     }
     if (a->workspace_bytes < vetrast_gradient_norm_workspace_bytes(a->gradients, a->num_gradients)) return VETRAST_ERR_WORKSPACE_SMALL;
     hipStream_t stream = (hipStream_t)stream_;
-    double* partial    = static_cast<double*>(a->workspace);
-    uint32_t partials  = 0;
     NormLaunch l;
-    l.entries = l.chunks = 0;
-    const auto launch = [&] {
-        if (l.entries == 0) return;
-        const uint32_t grid = std::min(l.chunks, kNormGrid);
-        l.partial           = partial + partials;
-        hipLaunchKernelGGL(gradient_squares_kernel, dim3(grid), dim3(kBlock), 0, stream, l);
-        partials += grid;
+    l.workspace = static_cast<NormWorkspace*>(a->workspace);
+    l.out       = a->out;
+    l.max_norm  = a->max_norm;
+    l.scale     = a->scale;
+    // twice through the list: the launches have to know how many workgroups the call has
+    const auto each = [&](auto&& launch) {
         l.entries = l.chunks = 0;
-    };
-    for (int k = 0; k < a->num_gradients; ++k)
-    {
-        const vetrast_gradient& g = a->gradients[k];
-        for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
+        uint32_t first = 0;
+        const auto close = [&] {
+            const uint32_t grid = std::max(std::min(l.chunks, kNormGrid), 1u);
+            l.first             = first;
+            launch(grid);
+            first += grid;
+            l.entries = l.chunks = 0;
+        };
+        for (int k = 0; k < a->num_gradients; ++k)
         {
-            if (l.entries == (uint32_t)kNormEntries) launch();
-            NormEntry& e     = l.e[l.entries++];
-            e.grad           = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
-            const uint32_t n = (uint32_t)std::min(g.n - from, kOptimEntryElements);
-            e.n_type         = n << 2 | (uint32_t)g.type;
-            e.first_chunk    = l.chunks;
-            l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
+            const vetrast_gradient& g = a->gradients[k];
+            for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
+            {
+                if (l.entries == (uint32_t)kNormEntries) close();
+                NormEntry& e     = l.e[l.entries++];
+                e.grad           = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
+                const uint32_t n = (uint32_t)std::min(g.n - from, kOptimEntryElements);
+                e.n_type         = n << 2 | (uint32_t)g.type;
+                e.first_chunk    = l.chunks;
+                l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
+            }
         }
-    }
-    launch();
-    hipLaunchKernelGGL(gradient_norm_kernel, dim3(1), dim3(kBlock), 0, stream, partial, partials, a->max_norm, a->scale, a->out);
+        if (l.entries > 0 || first == 0) close();
+        return first;
+    };
+    l.total = each([](uint32_t) {});
+    each([&](uint32_t grid) { hipLaunchKernelGGL(gradient_norm_kernel, dim3(grid), dim3(kBlock), 0, stream, l); });
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
 }
@@ -1551,7 +1552,7 @@ static int convert_moments(vetrast_ctx* ctx, const vetrast_moments_args* a, hipS
     l.entries = l.chunks = 0;
     const auto launch = [&] {
         if (l.entries == 0) return;
-        const dim3 grid(std::min(l.chunks, kOptimGrid));
+        const dim3 grid(l.chunks);
         if (pack) hipLaunchKernelGGL((convert_moments_kernel<true>), grid, dim3(kBlock), 0, stream, l);
         else hipLaunchKernelGGL((convert_moments_kernel<false>), grid, dim3(kBlock), 0, stream, l);
         l.entries = l.chunks = 0;

@@ -374,14 +374,15 @@ class Rasterizer:
         abi.check(self.lib.vetrast_adamw_step(self.ctx, C.byref(a), self._stream()), "adamw_step")
 
     def gradient_norm(self, gradients, max_norm=0.0, scale=1.0, out=None, workspace=None):
-        """Norm of all gradients and the factor that clips it, float32 [2] (vetrast_gradient_norm)."""
+        """Norm of all gradients and the factor that clips it, float32 [2] (vetrast_gradient_norm). workspace: zeroed before its first
+        use."""
         gs, a = (abi.Gradient * max(len(gradients), 1))(), abi.GradientNormArgs()
         for g, x in zip(gs, gradients):
             assert x.is_cuda and x.is_contiguous()
             g.grad, g.n, g.type = x.data_ptr(), x.numel(), _DTYPES[x.dtype]
         need = self.lib.vetrast_gradient_norm_workspace_bytes(gs, len(gradients))
         out = torch.empty(2, device="cuda") if out is None else out
-        workspace = torch.empty(need, dtype=torch.uint8, device="cuda") if workspace is None else workspace
+        workspace = torch.zeros(need, dtype=torch.uint8, device="cuda") if workspace is None else workspace
         a.gradients, a.num_gradients, a.max_norm, a.scale = gs, len(gradients), max_norm, scale
         a.out, a.workspace, a.workspace_bytes = out.data_ptr(), workspace.data_ptr(), workspace.numel()
         abi.check(self.lib.vetrast_gradient_norm(self.ctx, C.byref(a), self._stream()), "gradient_norm")

@@ -19,26 +19,48 @@ void check(int st, const char* where)
     TORCH_CHECK(st == VETRAST_OK, "vetrast ", where, " failed: ", st, " (", vetrast_status_string(st), ")");
 }
 
-// A context serves one host thread at a time and belongs to a device. The caller has made `device` the current one.
+void* stream_on(const torch::Device& device)
+{
+    return (void*)c10::hip::getCurrentHIPStream(device.index()).stream();
+}
+
+bool capturing()
+{
+    return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
+// What a host thread keeps. A context serves one host thread at a time and belongs to a device, a norm's workspace serves one stream.
+struct Kept
+{
+    std::map<int, vetrast_ctx*> contexts;
+    std::map<std::pair<int, void*>, torch::Tensor> workspaces;
+    ~Kept()
+    {
+        for (auto& c : contexts) vetrast_destroy(c.second);
+    }
+};
+Kept& kept()
+{
+    thread_local Kept k;
+    return k;
+}
+
+// The caller has made `device` the current one.
 vetrast_ctx* context_on(const torch::Device& device)
 {
-    struct Contexts
-    {
-        std::map<int, vetrast_ctx*> of;
-        ~Contexts()
-        {
-            for (auto& c : of) vetrast_destroy(c.second);
-        }
-    };
-    thread_local Contexts contexts;
-    vetrast_ctx*& ctx = contexts.of[device.index()];
+    vetrast_ctx*& ctx = kept().contexts[device.index()];
     if (!ctx) check(vetrast_create(&ctx), "create");
     return ctx;
 }
 
-void* stream_on(const torch::Device& device)
+// Zeroed memory for vetrast_gradient_norm, which leaves it zeroed where that counts. A captured call has its own, cleared in the graph.
+torch::Tensor norm_workspace(const torch::Device& device, size_t bytes)
 {
-    return (void*)c10::hip::getCurrentHIPStream(device.index()).stream();
+    const auto options = torch::TensorOptions(device).dtype(torch::kUInt8);
+    if (capturing()) return torch::zeros({(int64_t)bytes}, options);
+    torch::Tensor& w = kept().workspaces[{device.index(), stream_on(device)}];
+    if (!w.defined() || w.numel() < (int64_t)bytes) w = torch::zeros({(int64_t)bytes}, options);
+    return w;
 }
 
 int32_t type_of(const torch::Tensor& t, const char* what)
@@ -181,8 +203,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
 {
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
-    const bool capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
-    TORCH_CHECK(options_.capturable || !capturing, "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
+    TORCH_CHECK(options_.capturable || !capturing(), "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
     bool moved = false;
     for (auto& s : slots_) moved |= s.param.numel() != s.n;
     if (moved)
@@ -386,7 +407,7 @@ torch::Tensor GradNorm(const std::vector<torch::Tensor>& gradients, double max_n
     a.max_norm              = max_norm;
     a.scale                 = scale;
     a.workspace_bytes       = vetrast_gradient_norm_workspace_bytes(list.data(), a.num_gradients);
-    torch::Tensor workspace = torch::empty({(int64_t)a.workspace_bytes}, torch::TensorOptions(*device).dtype(torch::kUInt8));
+    torch::Tensor workspace = norm_workspace(*device, a.workspace_bytes);
     torch::Tensor out       = torch::empty({2}, torch::TensorOptions(*device).dtype(torch::kFloat32));
     a.workspace             = workspace.data_ptr();
     a.out                   = out.data_ptr<float>();
