@@ -360,7 +360,7 @@ int vetrast_adam_step(vetrast_ctx* ctx, const vetrast_adam_args* args, void* str
 
 /* ---- AdamW over lists of tensors ----------------------------------------------------------------------------------
  * The optimiser of everything a training step has gradients for, descriptors and render network alike, in as few launches
- * as the list needs (one for up to 120 tensors). Per element, with t the group's step:
+ * as the list needs (one for up to 160 tensors). Per element, with t the group's step:
  *   g = grad * *grad_scale;  m = beta1 * m + (1 - beta1) * g;  v = beta2 * v + ((1 - beta2) * g) * g
  *   param = (1 - lr * weight_decay) * param - lr / (1 - beta1^t) * (m / (sqrt(v) * (1 / sqrt(1 - beta2^t)) + eps))
  * in 32 bits; the moments are rounded after every operation, in this order. The reference steps its network with torch's

@@ -300,7 +300,7 @@ def test_a_step_whose_factor_is_not_finite_is_left_out(bits, value, rasterizer):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [8, 9, 64, 65, 120, 121, 531])
+@pytest.mark.parametrize("count", [8, 9, 64, 65, 160, 161, 531])
 def test_long_lists_many_groups_and_mixed_types(bits, count, rasterizer):
     """Up to and beyond what a launch takes, in tensors and in groups, every combination of types, empty tensors among them."""
     rng = np.random.default_rng(10)
@@ -350,7 +350,7 @@ def test_a_tensor_of_several_entries(rasterizer):
     p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
     flat = fresh(-(-n // 128) * 128)
     rasterizer.adamw_step([(p, g, 0, 0)], [(1e-3, 0.0, 1)], *flat, moment_bits=8, stochastic_rounding=True, seed=9)
-    for first, end in ((0, 5120), ((1 << 29) - 1280, (1 << 29) + 2560), ((1 << 30) - 1280, (1 << 30) + 2560), ((n // 128 - 9) * 128, n)):
+    for first, end in ((0, 5120), ((1 << 28) - 1280, (1 << 28) + 2560), ((1 << 30) - 1280, (1 << 30) + 2560), ((n // 128 - 9) * 128, n)):
         part, own = torch.zeros(end - first, dtype=torch.bfloat16, device="cuda"), fresh(-(-end // 128) * 128)
         rasterizer.adamw_step([(part, g[first:end].clone(), first, 0)], [(1e-3, 0.0, 1)], *own, moment_bits=8, stochastic_rounding=True, seed=9)
         assert torch.equal(part, p[first:end]) and part.any()

@@ -25,7 +25,7 @@ struct ChunkFinder
         for (int q = 0; q < GROUPS; ++q)
         {
             const uint32_t k = q * kWave + threadIdx.x % kWave;
-            begins[q]        = k < a.entries ? a.e[k].first_chunk : 0xFFFFFFFFu;
+            begins[q]        = k < a.entries ? a.e[k].begins() : 0xFFFFFFFFu;
         }
     }
     // The entry of a chunk; all lanes of the wave take part.
@@ -415,21 +415,17 @@ __device__ __forceinline__ void decode_four(uint32_t wm, uint32_t wv, uint32_t s
 
 // ---- AdamW -------------------------------------------------------------------------------------------------------------
 
+// 24 bytes, so that a launch takes 160 of them: a further launch costs a list 4 us.
 struct AdamWEntry
 {
-    void* param;
-    void* grad;
-    uint32_t n;
-    uint32_t first_chunk;  // of the launch
-    uint32_t block;        // place in the flat arrays
-    uint32_t flags;        // kAdamW..., slot of the group from bit 8 on
-};
-enum
-{
-    kAdamWParam   = 3,       // type
-    kAdamWGrad    = 3 << 2,  // type
-    kAdamWAligned = 1 << 4,  // param and grad to 16 bytes
-    kAdamWMaster  = 1 << 5
+    uint32_t param_low, grad_low;
+    uint16_t param_high, grad_high;  // of addresses of 48 bits
+    uint32_t n_slot;                 // n << 3 | slot of the group
+    uint32_t block;                  // place in the flat arrays
+    uint32_t chunk_types;            // first chunk of the launch << 4 | type of the gradient << 2 | type of the parameter
+    __device__ __forceinline__ uint32_t begins() const { return chunk_types >> 4; }
+    __device__ __forceinline__ void* param() const { return (void*)((uint64_t)param_high << 32 | param_low); }
+    __device__ __forceinline__ void* grad() const { return (void*)((uint64_t)grad_high << 32 | grad_low); }
 };
 
 struct AdamWGroup
@@ -459,7 +455,7 @@ struct AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel le
     AdamWGroup group[1];
 };
 
-constexpr int kAdamWEntries = 120;  // what 4 KB of kernel arguments hold
+constexpr int kAdamWEntries = 160;  // what 4 KB of kernel arguments hold
 constexpr int kAdamWFew     = 8;    // ... and a launch whose arguments are 400 bytes
 constexpr int kAdamWGroups  = 8;
 struct AdamWCommon
@@ -473,7 +469,7 @@ struct AdamWCommon
     const AdamWDevice* device;  // where set, g[].key are places in device->group
     uint32_t entries, chunks;
     float beta1, one_minus_beta1, beta2, one_minus_beta2;
-    int zero_grad, stochastic, exact_root;
+    int zero_grad, stochastic;
 };
 template <int ENTRIES>
 struct AdamWLaunch : AdamWCommon
@@ -515,6 +511,15 @@ __global__ void __launch_bounds__(kBeginGroups) adamw_begin_kernel(const AdamWBe
     if (a.last && counts && k == 0) a.device->state.step = step;
 }
 
+struct AdamWChunk
+{
+    void *param, *grad;
+    uint32_t n, slot, p_type, g_type;
+    uint32_t start;  // the chunk's first element
+    uint32_t block;  // of the tensor, in the flat arrays
+    bool whole;      // all its elements are there, at 16-byte addresses
+};
+
 // Chunks of four kinds. In whole ones every thread has its eight elements at addresses that are multiples of 16, parameter and gradient
 // of one width: their loads are straight code, all of them under way at once. `kAnyChunk` does for everything else.
 enum ChunkKind
@@ -525,21 +530,19 @@ enum ChunkKind
     kAnyChunk
 };
 
-template <int BITS, ChunkKind KIND>
-__device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEntry& e, uint32_t start, float grad_scale)
+template <int BITS, bool EXACT, ChunkKind KIND>
+__device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChunk& e, float grad_scale)
 {
     constexpr bool ANY    = KIND == kAnyChunk;
     constexpr bool HALVES = BITS == 32 && !ANY;  // blocks of 8-bit moments are eight elements of 16 neighbouring lanes
     constexpr int BYTES   = KIND == kFloatChunk ? 4 : 2;
-    const uint32_t flags  = e.flags;
-    const uint32_t p_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : flags & kAdamWParam;
-    const uint32_t g_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : (flags & kAdamWGrad) >> 2;
-    const bool master     = ANY ? flags & kAdamWMaster : KIND == kMasterChunk;
-    const uint32_t count  = ANY ? count_of(start, e.n) : 8u;
-    const bool whole      = e.n - start >= kOptimChunk && (flags & kAdamWAligned);
+    const uint32_t p_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : e.p_type;
+    const uint32_t g_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : e.g_type;
+    const bool master     = ANY ? a.master && p_type != VETRAST_F32 : KIND == kMasterChunk;
+    const uint32_t start = e.start, count = ANY ? count_of(start, e.n) : 8u;
     const auto clear      = [&] {
         const RawEight zero = {};
-        if constexpr (ANY) store_any(e.grad, g_type, start, count, whole, zero);
+        if constexpr (ANY) store_any(e.grad, g_type, start, count, e.whole, zero);
         else store_eight<BYTES, HALVES>(e.grad, start, zero);
     };
     if (!isfinite(grad_scale))
@@ -557,13 +560,13 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEnt
 
     RawEight rg, rp, r1, r2;
     Codes codes;
-    if constexpr (ANY) rg = load_any(e.grad, g_type, start, count, whole);
+    if constexpr (ANY) rg = load_any(e.grad, g_type, start, count, e.whole);
     else rg = load_eight<BYTES, HALVES>(e.grad, start);
     if constexpr (ANY)
     {
         rp = r1 = r2 = RawEight{};
         codes        = Codes{};
-        if (!master) rp = load_any(e.param, p_type, start, count, whole);
+        if (!master) rp = load_any(e.param, p_type, start, count, e.whole);
     }
     if (inside)
     {
@@ -581,7 +584,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEnt
             codes.scale = scales[mine / kMomentBlock];
         }
     }
-    AdamWGroup g = a.g[flags >> 8];
+    AdamWGroup g = a.g[e.slot];
     if (a.device) g = a.device->group[g.key];
     const bool random = KIND != kFloatChunk && !master && a.stochastic && p_type == VETRAST_BF16;
     uint32_t r[8];
@@ -611,7 +614,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEnt
     // With 8-bit moments root and quotient are the instructions for them, good to 1.54 half steps of float32 each, as the step is
     // bound by instructions; with 32-bit ones it waits for memory and they are rounded to nearest. The root instruction takes
     // values below 2^-126 for zero: eps makes up for that unless it is tiny itself.
-    if (BITS == 32 || a.exact_root)
+    if constexpr (BITS == 32 || EXACT)
     {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = sqrtf(v[j]);
@@ -668,25 +671,33 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWEnt
                            __builtin_amdgcn_perm(r[5], r[4], 0x07060302), __builtin_amdgcn_perm(r[7], r[6], 0x07060302));
     }
     else out = from_floats(p, p_type);
-    if constexpr (ANY) store_any(e.param, p_type, start, count, whole, out);
+    if constexpr (ANY) store_any(e.param, p_type, start, count, e.whole, out);
     else store_eight<BYTES, HALVES>(e.param, start, out);
     if (master && inside) store_eight<4, HALVES>(a.master + at, 0, from_floats(p, VETRAST_F32));
     if (a.zero_grad) clear();
 }
 
-template <int BITS, class Launch>
+// EXACT: eps is so small that roots of values below 2^-126 count.
+template <int BITS, bool EXACT, class Launch>
 __global__ void __launch_bounds__(kBlock) adamw_step_kernel(const Launch a)
 {
     const ChunkFinder<finder_groups(sizeof(a.e) / sizeof(a.e[0]))> find(a);
-    const AdamWEntry& e    = a.e[find(blockIdx.x)];
-    const uint32_t start   = (blockIdx.x - e.first_chunk) * kOptimChunk;
-    const float grad_scale = a.grad_scale ? *a.grad_scale : 1.f;
-    const uint32_t p_type = e.flags & kAdamWParam, g_type = (e.flags & kAdamWGrad) >> 2;
-    if (e.n - start < kOptimChunk || !(e.flags & kAdamWAligned) || (p_type == VETRAST_F32) != (g_type == VETRAST_F32))
-        adamw_chunk<BITS, kAnyChunk>(a, e, start, grad_scale);
-    else if (p_type == VETRAST_F32) adamw_chunk<BITS, kFloatChunk>(a, e, start, grad_scale);
-    else if (e.flags & kAdamWMaster) adamw_chunk<BITS, kMasterChunk>(a, e, start, grad_scale);
-    else adamw_chunk<BITS, kShortChunk>(a, e, start, grad_scale);
+    const AdamWEntry& entry = a.e[find(blockIdx.x)];
+    const float grad_scale  = a.grad_scale ? *a.grad_scale : 1.f;
+    AdamWChunk e;
+    e.param  = entry.param();
+    e.grad   = entry.grad();
+    e.n      = entry.n_slot >> 3;
+    e.slot   = entry.n_slot & 7u;
+    e.p_type = entry.chunk_types & 3u;
+    e.g_type = entry.chunk_types >> 2 & 3u;
+    e.start  = (blockIdx.x - entry.begins()) * kOptimChunk;
+    e.block  = entry.block;
+    e.whole  = e.n - e.start >= kOptimChunk && (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
+    if (!e.whole || (e.p_type == VETRAST_F32) != (e.g_type == VETRAST_F32)) adamw_chunk<BITS, EXACT, kAnyChunk>(a, e, grad_scale);
+    else if (e.p_type == VETRAST_F32) adamw_chunk<BITS, EXACT, kFloatChunk>(a, e, grad_scale);
+    else if (a.master) adamw_chunk<BITS, EXACT, kMasterChunk>(a, e, grad_scale);
+    else adamw_chunk<BITS, EXACT, kShortChunk>(a, e, grad_scale);
 }
 
 // ---- norms -------------------------------------------------------------------------------------------------------------
@@ -697,6 +708,7 @@ struct NormEntry
     const void* grad;
     uint32_t n_type;  // n << 2 | type
     uint32_t first_chunk;
+    __device__ __forceinline__ uint32_t begins() const { return first_chunk; }
 };
 constexpr uint32_t kNormSlots = 32;
 struct NormWorkspace
@@ -797,6 +809,7 @@ struct MomentEntry
 {
     float *m, *v;
     uint32_t n, first_chunk, block, reserved;
+    __device__ __forceinline__ uint32_t begins() const { return first_chunk; }
 };
 struct MomentLaunch
 {

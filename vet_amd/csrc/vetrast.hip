@@ -479,7 +479,7 @@ void launch_lift(const vetrast_lift_args* a, char* ws, size_t num_sums, hipStrea
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
-constexpr int64_t kOptimEntryElements = 1 << 29;  // a longer tensor is several entries of a launch: places inside one are 32 bits
+constexpr int64_t kOptimEntryElements = 1 << 28;  // a longer tensor is several entries of a launch: places inside one are 32 bits
 constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays, whose blocks have numbers of 32 bits
@@ -491,13 +491,16 @@ inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat array
 template <int ENTRIES>
 void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStream_t stream)
 {
+    // the root instruction's zero for values below 2^-126 is up to 2^-63 off, times at most 1 / sqrt(1 - beta2): half a step of eps
+    const bool exact = std::ldexp(1.0, -63) / std::sqrt(1.0 - a->beta2) > std::ldexp(a->eps, -24);
     int slot_group[kAdamWGroups], slots = 0;
     l.entries = l.chunks = 0;
     const auto launch = [&] {
         if (l.entries == 0) return;
         const dim3 grid(l.chunks);
-        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
-        else hipLaunchKernelGGL((adamw_step_kernel<8, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, true, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        else if (exact) hipLaunchKernelGGL((adamw_step_kernel<8, true, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        else hipLaunchKernelGGL((adamw_step_kernel<8, false, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
         l.entries = l.chunks = 0;
         slots                = 0;
     };
@@ -523,16 +526,18 @@ void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStrea
                     c = adamw_group(g.lr, g.weight_decay, a->eps, 1.0 - std::pow(a->beta1, (double)g.step), 1.0 - std::pow(a->beta2, (double)g.step),
                                     step_key(a->seed, g.step));
             }
-            AdamWEntry& e      = l.e[l.entries++];
-            e.param            = static_cast<char*>(t.param) + from * (int64_t)dtype_bytes(t.param_type);
-            e.grad             = static_cast<char*>(t.grad) + from * (int64_t)dtype_bytes(t.grad_type);
-            e.n                = (uint32_t)std::min(t.n - from, kOptimEntryElements);
-            e.first_chunk      = l.chunks;
-            e.block            = (uint32_t)((t.first + from) / kMomentBlock);
-            e.flags            = (uint32_t)t.param_type | (uint32_t)t.grad_type << 2 | (uint32_t)slot << 8;
-            if (aligned_to(e.param, 16) && aligned_to(e.grad, 16)) e.flags |= kAdamWAligned;
-            if (a->master && t.param_type != VETRAST_F32) e.flags |= kAdamWMaster;
-            l.chunks += (e.n + kOptimChunk - 1) / kOptimChunk;
+            const uint64_t param = reinterpret_cast<uintptr_t>(t.param) + (uint64_t)from * dtype_bytes(t.param_type);
+            const uint64_t grad  = reinterpret_cast<uintptr_t>(t.grad) + (uint64_t)from * dtype_bytes(t.grad_type);
+            const uint32_t n     = (uint32_t)std::min(t.n - from, kOptimEntryElements);
+            AdamWEntry& e        = l.e[l.entries++];
+            e.param_low          = (uint32_t)param;
+            e.grad_low           = (uint32_t)grad;
+            e.param_high         = (uint16_t)(param >> 32);
+            e.grad_high          = (uint16_t)(grad >> 32);
+            e.n_slot             = n << 3 | (uint32_t)slot;
+            e.block              = (uint32_t)((t.first + from) / kMomentBlock);
+            e.chunk_types        = l.chunks << 4 | (uint32_t)t.grad_type << 2 | (uint32_t)t.param_type;
+            l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
         }
     }
     launch();
@@ -1415,6 +1420,7 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         if (t.n == 0) continue;
         if (!t.param || !t.grad || !a->exp_avg || !a->exp_avg_sq || (a->moment_bits == 8 && !a->block_scale)) return VETRAST_ERR_INVALID_ARG;
         if (!aligned_to(t.param, dtype_bytes(t.param_type)) || !aligned_to(t.grad, dtype_bytes(t.grad_type))) return VETRAST_ERR_INVALID_ARG;
+        if ((reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad)) >> 48) return VETRAST_ERR_INVALID_ARG;
         entries += (t.n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
     hipStream_t stream  = (hipStream_t)stream_;
@@ -1449,8 +1455,6 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         l.one_minus_beta2 = (float)(1.0 - a->beta2);
         l.zero_grad       = a->zero_grad;
         l.stochastic      = a->stochastic_rounding;
-        // the root instruction's zero for values below 2^-126 is up to 2^-63 off, times at most 1 / sqrt(1 - beta2): half a step of eps
-        l.exact_root = std::ldexp(1.0, -63) / std::sqrt(1.0 - a->beta2) > std::ldexp(a->eps, -24);
     };
     if (entries <= kAdamWFew)
     {

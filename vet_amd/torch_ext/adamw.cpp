@@ -96,23 +96,29 @@ bool same_order(const torch::Tensor& a, const torch::Tensor& b)
 }
 
 // Moments of a list of tensors, placed one behind the other in flat arrays; `total`: elements of these.
-std::vector<vetrast_moment_tensor> moment_list(const std::vector<torch::Tensor>& ms, const std::vector<torch::Tensor>& vs, const torch::Device& device,
-                                               int64_t& total)
+std::vector<vetrast_moment_tensor> moment_list(const TensorPointers& ms, const TensorPointers& vs, const torch::Device& device, int64_t& total)
 {
     TORCH_CHECK(ms.size() == vs.size(), "as many first moments as second ones are needed, not ", ms.size(), " and ", vs.size());
     std::vector<vetrast_moment_tensor> list(ms.size());
     total = 0;
     for (size_t k = 0; k < ms.size(); ++k)
     {
-        check_on(ms[k], device, "moments");
-        check_on(vs[k], device, "moments");
-        TORCH_CHECK(ms[k].scalar_type() == torch::kFloat32 && vs[k].scalar_type() == torch::kFloat32 && dense(ms[k]) && dense(vs[k]),
-                    "moments must be dense float32 tensors");
-        TORCH_CHECK(ms[k].sizes() == vs[k].sizes() && same_order(ms[k], vs[k]), "both moments of a tensor must have one shape and order");
-        list[k] = {ms[k].data_ptr<float>(), vs[k].data_ptr<float>(), ms[k].numel(), total};
+        const torch::Tensor &m = *ms[k], &v = *vs[k];
+        check_on(m, device, "moments");
+        check_on(v, device, "moments");
+        TORCH_CHECK(m.scalar_type() == torch::kFloat32 && v.scalar_type() == torch::kFloat32 && dense(m) && dense(v), "moments must be dense float32 tensors");
+        TORCH_CHECK(m.sizes() == v.sizes() && same_order(m, v), "both moments of a tensor must have one shape and order");
+        list[k] = {m.data_ptr<float>(), v.data_ptr<float>(), m.numel(), total};
         total += whole_blocks(list[k].n);
     }
     return list;
+}
+
+TensorPointers pointers(const std::vector<torch::Tensor>& list)
+{
+    TensorPointers r;
+    for (auto& t : list) r.push_back(&t);
+    return r;
 }
 
 vetrast_moments_args moments_args(const std::vector<vetrast_moment_tensor>& list, const torch::Tensor& m, const torch::Tensor& v, const torch::Tensor& scale)
@@ -297,10 +303,9 @@ void AdamW::zero_grad()
 
 torch::Tensor AdamW::grad_norm(double max_norm, double scale)
 {
-    std::vector<torch::Tensor> grads;
+    TensorPointers grads;
     grads.reserve(slots_.size());
-    for (auto& s : slots_)
-        if (s.param.grad().defined()) grads.push_back(s.param.grad());
+    for (auto& s : slots_) grads.push_back(&s.param.grad());
     return GradNorm(grads, max_norm, scale);
 }
 
@@ -343,7 +348,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     int64_t total = 0;
-    std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device_, total);
+    std::vector<vetrast_moment_tensor> list = moment_list(pointers(exp_avgs), pointers(exp_avg_sqs), device_, total);
     TORCH_CHECK(list.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", list.size());
     for (size_t k = 0; k < list.size(); ++k)
         TORCH_CHECK(list[k].n == slots_[k].n, "AdamW: parameter ", k, " has ", slots_[k].n, " elements, its moments have ", list[k].n);
@@ -373,15 +378,16 @@ void AdamW::reload_master()
     }
 }
 
-torch::Tensor GradNorm(const std::vector<torch::Tensor>& gradients, double max_norm, double scale)
+torch::Tensor GradNorm(const TensorPointers& gradients, double max_norm, double scale)
 {
     std::vector<vetrast_gradient> list;
     std::vector<torch::Tensor> gathered;  // of gradients with gaps
     list.reserve(gradients.size());
     std::optional<torch::Device> device;
     c10::OptionalDeviceGuard guard;
-    for (auto& g : gradients)
+    for (const torch::Tensor* gradient : gradients)
     {
+        const torch::Tensor& g = *gradient;
         if (!g.defined()) continue;
         if (!device)
         {
@@ -415,10 +421,10 @@ torch::Tensor GradNorm(const std::vector<torch::Tensor>& gradients, double max_n
     return out;
 }
 
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const TensorPointers& exp_avgs, const TensorPointers& exp_avg_sqs)
 {
-    TORCH_CHECK(!exp_avgs.empty() && exp_avgs[0].is_cuda(), "pack_moments: a list of tensors on the GPU is needed");
-    const torch::Device device = exp_avgs[0].device();
+    TORCH_CHECK(!exp_avgs.empty() && exp_avgs[0]->is_cuda(), "pack_moments: a list of tensors on the GPU is needed");
+    const torch::Device device = exp_avgs[0]->device();
     c10::DeviceGuard guard(device);
     int64_t total = 0;
     const std::vector<vetrast_moment_tensor> list = moment_list(exp_avgs, exp_avg_sqs, device, total);

@@ -12,7 +12,7 @@
 namespace vet_amd
 {
 // The reference steps its texture with MyAdam (src/lib/models/my_adam.cpp) and its network with torch::optim::Adam, a dozen
-// elementwise launches a tensor; this class takes both kinds of tensors, in one launch for up to 120 of them.
+// elementwise launches a tensor; this class takes both kinds of tensors, in one launch for up to 160 of them.
 class AdamW
 {
    public:
@@ -81,11 +81,14 @@ class AdamW
     std::vector<int64_t> group_of_;
 };
 
+// Lists of tensors that somebody else holds (a Python list of a hundred is half of a call's time when it is copied).
+using TensorPointers = std::vector<const torch::Tensor*>;
+
 // vetrast_gradient_norm over tensors on one GPU (undefined ones are left out): float32 [2], the norm of `scale` times the gradients and
 // the factor that brings it to at most max_norm (<= 0: `scale`).
-torch::Tensor GradNorm(const std::vector<torch::Tensor>& gradients, double max_norm = 0.0, double scale = 1.0);
+torch::Tensor GradNorm(const TensorPointers& gradients, double max_norm = 0.0, double scale = 1.0);
 
 // Moments of a list of tensors as codes and scales, in flat tensors laid out as AdamW keeps them, and such flat tensors back as float32.
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> PackMoments(const TensorPointers& exp_avgs, const TensorPointers& exp_avg_sqs);
 std::tuple<torch::Tensor, torch::Tensor> UnpackMoments(const torch::Tensor& exp_avg, const torch::Tensor& exp_avg_sq, const torch::Tensor& block_scale);
 }  // namespace vet_amd

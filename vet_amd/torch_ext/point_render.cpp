@@ -1237,6 +1237,20 @@ std::vector<torch::Tensor> adapter_selftest(torch::Tensor texture, torch::Tensor
     return vet_amd::BlendPointCloudOf(&info, g_cache.get(), &bundle);
 }
 
+// The tensors of a list, which holds them; None is left out.
+vet_amd::TensorPointers tensors_of(const pybind11::list& list)
+{
+    vet_amd::TensorPointers r;
+    r.reserve(list.size());
+    for (pybind11::handle h : list)
+    {
+        if (h.is_none()) continue;
+        TORCH_CHECK(THPVariable_Check(h.ptr()), "a list of tensors is needed");
+        r.push_back(&THPVariable_Unpack(h.ptr()));
+    }
+    return r;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     pybind11::class_<vet_amd::MyAdam>(m, "MyAdam")
@@ -1279,8 +1293,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def_readonly("master", &AdamW::master)
         .def_readonly("device_step", &AdamW::device_step)
         .def_readonly("lr_factor", &AdamW::lr_factor);
-    m.def("grad_norm", &vet_amd::GradNorm, pybind11::arg("gradients"), pybind11::arg("max_norm") = 0.0, pybind11::arg("scale") = 1.0);
-    m.def("pack_moments", &vet_amd::PackMoments, pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"));
+    m.def(
+        "grad_norm",
+        [](const pybind11::list& gradients, double max_norm, double scale) {
+            return vet_amd::GradNorm(tensors_of(gradients), max_norm, scale);
+        },
+        pybind11::arg("gradients"), pybind11::arg("max_norm") = 0.0, pybind11::arg("scale") = 1.0);
+    m.def(
+        "pack_moments",
+        [](const pybind11::list& exp_avgs, const pybind11::list& exp_avg_sqs) {
+            return vet_amd::PackMoments(tensors_of(exp_avgs), tensors_of(exp_avg_sqs));
+        },
+        pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"));
     m.def("unpack_moments", &vet_amd::UnpackMoments, pybind11::arg("exp_avg"), pybind11::arg("exp_avg_sq"), pybind11::arg("block_scale"));
     m.def(
         "fill_scene_grid_with_loss",

@@ -58,7 +58,7 @@ def MyAdam(groups, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
 
 def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weights=False, stochastic_rounding=False, seed=0,
           capturable=False):
-    """AdamW over everything a training step has gradients for, in one launch for up to 120 tensors (vetrast_adamw_step).
+    """AdamW over everything a training step has gradients for, in one launch for up to 160 tensors (vetrast_adamw_step).
 
     groups: list of (list of parameter tensors, learning rate, weight decay). Parameters are dense CUDA tensors of float32,
     bfloat16 or float16 in any order of dimensions; gradients are found in .grad at every step.
@@ -80,7 +80,7 @@ def grad_norm(gradients, max_norm=0.0, scale=1.0):
     """The 2-norm of `scale` times all gradients together and the factor that brings it to at most max_norm (`scale` times
     min(1, max_norm / norm); just `scale` with max_norm <= 0; NaN for a norm that is not finite), as float32 [2] on the GPU
     (vetrast_gradient_norm). AdamW.step takes it as grad_scale without a wait on the host."""
-    return load().grad_norm(list(gradients), float(max_norm), float(scale))
+    return load().grad_norm(list(gradients), max_norm, scale)
 
 
 def pack_moments(exp_avgs, exp_avg_sqs):
