@@ -157,6 +157,18 @@ def test_step_against_64_bits(bits, master, param, grad, rasterizer):
     batch.check()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("param,grad", [(F, F), (B, B), (F, B), (H, H), (B, F)], ids=lambda t: str(t).replace("torch.", ""))
+def test_step_of_many_elements(bits, master, param, grad, rasterizer):
+    """Calls that are large enough for workgroups of four waves."""
+    sizes = [1_400_003, 0, 2048 * 40, 2048 * 3 + 5, 7, 130_000]
+    groups = [(0.01, 0.1, 3), (0.002, 0.0, 40)]
+    batch = Batch(np.random.default_rng(17), [(n, param, grad, k % 2) for k, n in enumerate(sizes)], bits, master)
+    batch.step(rasterizer, groups, seed=12, stochastic_rounding=True, grad_scale=torch.tensor([3.0], device="cuda"))
+    batch.compare(groups, 12, stochastic=True, scale=3.0)
+
+
 @pytest.mark.parametrize("eps", [1e-6, 1e-15, 1e-30])
 def test_tiny_eps_and_tiny_gradients(eps, rasterizer):
     """Second moments below the smallest normal number count where eps is small enough to let them."""

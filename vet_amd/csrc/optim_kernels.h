@@ -1,7 +1,7 @@
 // Optimiser kernels over lists of tensors: AdamW with moments in 32 or 8 bits, the norm of all gradients, moments to 8 bits and back.
 //
 // A launch takes a table of tensors in its arguments (no copy to the device, nothing to keep, and what a graph captures is whole). The
-// tensors are cut into chunks of kOptimChunk elements, 8 a thread, one for each workgroup (27.5 M float32 elements: 142 us; workgroups of a
+// tensors are cut into chunks of 8 elements a thread, one for each workgroup (27.5 M float32 elements: 142 us; workgroups of a
 // grid of 2048 that go on to further chunks 154 us), but for norms, where a workgroup leaves a sum.
 #pragma once
 #include "common.h"
@@ -9,9 +9,10 @@
 namespace vetrast
 {
 constexpr uint32_t kOptimChunk   = 8 * kBlock;  // elements
+constexpr uint32_t kWaveChunk    = 8 * kWave;   // ... of a workgroup of one wave
 constexpr int kMomentBlock       = VETRAST_MOMENT_BLOCK;
 constexpr uint32_t kMomentMargin = 0x100100;  // see code_base
-static_assert(kOptimChunk % kMomentBlock == 0 && kMomentBlock == 16 * 8, "16 lanes of 8 elements hold a block");
+static_assert(kWaveChunk % kMomentBlock == 0 && kMomentBlock == 16 * 8, "16 lanes of 8 elements hold a block");
 
 // Tables hold up to 64 * GROUPS entries: lane k of a wave knows which chunk of the launch is the first of entries k, k + 64, ...
 template <int GROUPS>
@@ -48,19 +49,19 @@ struct RawEight
 };
 
 // A thread's eight elements of a chunk that begins at element `start` of a tensor: the eight from 8 * threadIdx.x on, or (halves) the four
-// from 4 * threadIdx.x on and the four kOptimChunk / 2 behind these, with which a wave's access to float32 has no gaps. Writes gain by
+// from 4 * threadIdx.x on and the four HALF elements behind these, with which a wave's access to float32 has no gaps. Writes gain by
 // that, in what the last-level cache holds: 10 M first and second moments written 24.9 us, in halves 18.8; a step of 4 M elements with
 // masters 20.3 us, in halves 18.5. Beyond it a step does not (27.5 M float32: 142 us either way).
 // Addresses are one scalar for the workgroup and 32 bits for the thread. Registers that a load does not fill are left alone: to clear
 // them would wait for what is under way.
-template <int BYTES, bool HALVES = false>
+template <int BYTES, uint32_t HALF = 0>
 __device__ __forceinline__ RawEight load_eight(const void* p, uint32_t start)
 {
     const char* base = (const char*)p + (size_t)start * BYTES;
     RawEight r;
-    if constexpr (HALVES)
+    if constexpr (HALF != 0)
     {
-        constexpr uint32_t half = kOptimChunk / 2 * BYTES;
+        constexpr uint32_t half = HALF * BYTES;
         const uint32_t here     = threadIdx.x * 4u * BYTES;
         if constexpr (BYTES == 4)
         {
@@ -81,13 +82,13 @@ __device__ __forceinline__ RawEight load_eight(const void* p, uint32_t start)
     }
     return r;
 }
-template <int BYTES, bool HALVES = false>
+template <int BYTES, uint32_t HALF = 0>
 __device__ __forceinline__ void store_eight(void* p, uint32_t start, const RawEight& r)
 {
     char* base = (char*)p + (size_t)start * BYTES;
-    if constexpr (HALVES)
+    if constexpr (HALF != 0)
     {
-        constexpr uint32_t half = kOptimChunk / 2 * BYTES;
+        constexpr uint32_t half = HALF * BYTES;
         const uint32_t here     = threadIdx.x * 4u * BYTES;
         if constexpr (BYTES == 4)
         {
@@ -257,14 +258,14 @@ __device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_
 // elements, the
 // lower 20 and the upper 20 of them (products of 32 bits take four times as long as other instructions, and the 8-bit step is
 // bound by instructions).
-template <bool HALVES>
+template <uint32_t HALF>
 __device__ __forceinline__ void random_eight(uint32_t pair, uint32_t key, uint32_t* r)
 {
-    const uint32_t start = pair * 0x9E3779B1u + threadIdx.x * ((HALVES ? 2u : 4u) * 0x9E3779B1u);
+    const uint32_t start = pair * 0x9E3779B1u + threadIdx.x * ((HALF != 0 ? 2u : 4u) * 0x9E3779B1u);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
     {
-        const uint32_t k = HALVES && j >= 2 ? kOptimChunk / 4 + j - 2 : j;
+        const uint32_t k = HALF != 0 && j >= 2 ? HALF / 2 + j - 2 : j;
         uint32_t x       = start + k * 0x9E3779B1u;
         x                = exclusive_or(x, x >> 15, key);
         x *= 0xBB67AE85u;
@@ -530,11 +531,11 @@ enum ChunkKind
     kAnyChunk
 };
 
-template <int BITS, bool EXACT, ChunkKind KIND>
+template <int BITS, bool EXACT, uint32_t CHUNK, ChunkKind KIND>
 __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChunk& e, float grad_scale)
 {
     constexpr bool ANY    = KIND == kAnyChunk;
-    constexpr bool HALVES = BITS == 32 && !ANY;  // blocks of 8-bit moments are eight elements of 16 neighbouring lanes
+    constexpr uint32_t HALF = BITS == 32 && !ANY ? CHUNK / 2 : 0;  // blocks of 8-bit moments are eight elements of 16 neighbouring lanes
     constexpr int BYTES   = KIND == kFloatChunk ? 4 : 2;
     const uint32_t p_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : e.p_type;
     const uint32_t g_type = KIND == kFloatChunk ? (uint32_t)VETRAST_F32 : e.g_type;
@@ -543,7 +544,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     const auto clear      = [&] {
         const RawEight zero = {};
         if constexpr (ANY) store_any(e.grad, g_type, start, count, e.whole, zero);
-        else store_eight<BYTES, HALVES>(e.grad, start, zero);
+        else store_eight<BYTES, HALF>(e.grad, start, zero);
     };
     if (!isfinite(grad_scale))
     {
@@ -561,7 +562,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     RawEight rg, rp, r1, r2;
     Codes codes;
     if constexpr (ANY) rg = load_any(e.grad, g_type, start, count, e.whole);
-    else rg = load_eight<BYTES, HALVES>(e.grad, start);
+    else rg = load_eight<BYTES, HALF>(e.grad, start);
     if constexpr (ANY)
     {
         rp = r1 = r2 = RawEight{};
@@ -570,12 +571,12 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     }
     if (inside)
     {
-        if (master) rp = load_eight<4, HALVES>(a.master + at, 0);
-        else if constexpr (!ANY) rp = load_eight<BYTES, HALVES>(e.param, start);
+        if (master) rp = load_eight<4, HALF>(a.master + at, 0);
+        else if constexpr (!ANY) rp = load_eight<BYTES, HALF>(e.param, start);
         if constexpr (BITS == 32)
         {
-            r1 = load_eight<4, HALVES>((float*)a.m + at, 0);
-            r2 = load_eight<4, HALVES>((float*)a.v + at, 0);
+            r1 = load_eight<4, HALF>((float*)a.m + at, 0);
+            r2 = load_eight<4, HALF>((float*)a.v + at, 0);
         }
         else
         {
@@ -588,7 +589,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     if (a.device) g = a.device->group[g.key];
     const bool random = KIND != kFloatChunk && !master && a.stochastic && p_type == VETRAST_BF16;
     uint32_t r[8];
-    if (BITS == 8 || random) random_eight<HALVES>((uint32_t)(at / 2), g.key, r);
+    if (BITS == 8 || random) random_eight<HALF>((uint32_t)(at / 2), g.key, r);
 
     float x[8], p[8], m[8], v[8];
     to_floats(rg, g_type, x);
@@ -636,8 +637,8 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     {
         if (inside)
         {
-            store_eight<4, HALVES>((float*)a.m + at, 0, from_floats(m, VETRAST_F32));
-            store_eight<4, HALVES>((float*)a.v + at, 0, from_floats(v, VETRAST_F32));
+            store_eight<4, HALF>((float*)a.m + at, 0, from_floats(m, VETRAST_F32));
+            store_eight<4, HALF>((float*)a.v + at, 0, from_floats(v, VETRAST_F32));
         }
     }
     else
@@ -672,15 +673,19 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     }
     else out = from_floats(p, p_type);
     if constexpr (ANY) store_any(e.param, p_type, start, count, e.whole, out);
-    else store_eight<BYTES, HALVES>(e.param, start, out);
-    if (master && inside) store_eight<4, HALVES>(a.master + at, 0, from_floats(p, VETRAST_F32));
+    else store_eight<BYTES, HALF>(e.param, start, out);
+    if (master && inside) store_eight<4, HALF>(a.master + at, 0, from_floats(p, VETRAST_F32));
     if (a.zero_grad) clear();
 }
 
 // EXACT: eps is so small that roots of values below 2^-126 count.
-template <int BITS, bool EXACT, class Launch>
-__global__ void __launch_bounds__(kBlock) adamw_step_kernel(const Launch a)
+// THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.1 us,
+// with four waves 4.1; 1 M 4.8 and 6.4 with 8-bit moments; 4 M 18.8 and 18.1), and with 8-bit moments of 16-bit parameters, where
+// compute units that are never idle count (16 M: 31.6 us and 32.5). Else it is four, whose accesses lie closer together.
+template <int BITS, bool EXACT, int THREADS, class Launch>
+__global__ void __launch_bounds__(THREADS) adamw_step_kernel(const Launch a)
 {
+    constexpr uint32_t CHUNK = 8 * THREADS;
     const ChunkFinder<finder_groups(sizeof(a.e) / sizeof(a.e[0]))> find(a);
     const AdamWEntry& entry = a.e[find(blockIdx.x)];
     const float grad_scale  = a.grad_scale ? *a.grad_scale : 1.f;
@@ -691,13 +696,13 @@ __global__ void __launch_bounds__(kBlock) adamw_step_kernel(const Launch a)
     e.slot   = entry.n_slot & 7u;
     e.p_type = entry.chunk_types & 3u;
     e.g_type = entry.chunk_types >> 2 & 3u;
-    e.start  = (blockIdx.x - entry.begins()) * kOptimChunk;
+    e.start  = (blockIdx.x - entry.begins()) * CHUNK;
     e.block  = entry.block;
-    e.whole  = e.n - e.start >= kOptimChunk && (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
-    if (!e.whole || (e.p_type == VETRAST_F32) != (e.g_type == VETRAST_F32)) adamw_chunk<BITS, EXACT, kAnyChunk>(a, e, grad_scale);
-    else if (e.p_type == VETRAST_F32) adamw_chunk<BITS, EXACT, kFloatChunk>(a, e, grad_scale);
-    else if (a.master) adamw_chunk<BITS, EXACT, kMasterChunk>(a, e, grad_scale);
-    else adamw_chunk<BITS, EXACT, kShortChunk>(a, e, grad_scale);
+    e.whole  = e.n - e.start >= CHUNK && (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
+    if (!e.whole || (e.p_type == VETRAST_F32) != (e.g_type == VETRAST_F32)) adamw_chunk<BITS, EXACT, CHUNK, kAnyChunk>(a, e, grad_scale);
+    else if (e.p_type == VETRAST_F32) adamw_chunk<BITS, EXACT, CHUNK, kFloatChunk>(a, e, grad_scale);
+    else if (a.master) adamw_chunk<BITS, EXACT, CHUNK, kMasterChunk>(a, e, grad_scale);
+    else adamw_chunk<BITS, EXACT, CHUNK, kShortChunk>(a, e, grad_scale);
 }
 
 // ---- norms -------------------------------------------------------------------------------------------------------------
@@ -775,7 +780,7 @@ __global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const NormLaunch 
         RawEight r;
         if (n - start >= kOptimChunk && (uintptr_t)e.grad % 16 == 0)
         {
-            if (type == VETRAST_F32) r = load_eight<4, true>(e.grad, start);
+            if (type == VETRAST_F32) r = load_eight<4, kOptimChunk / 2>(e.grad, start);
             else r = load_eight<2>(e.grad, start);
         }
         else r = load_any(e.grad, type, start, count_of(start, n), false);

@@ -480,6 +480,7 @@ inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<ui
 inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
 constexpr int64_t kOptimEntryElements = 1 << 28;  // a longer tensor is several entries of a launch: places inside one are 32 bits
+constexpr int64_t kOptimSmall         = 1500000;  // elements up to which workgroups of one wave are faster
 constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays, whose blocks have numbers of 32 bits
@@ -488,7 +489,7 @@ inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat array
 }
 
 // The launches of a list of tensors; `l` has what they share.
-template <int ENTRIES>
+template <int THREADS, int ENTRIES>
 void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStream_t stream)
 {
     // the root instruction's zero for values below 2^-126 is up to 2^-63 off, times at most 1 / sqrt(1 - beta2): half a step of eps
@@ -497,10 +498,10 @@ void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStrea
     l.entries = l.chunks = 0;
     const auto launch = [&] {
         if (l.entries == 0) return;
-        const dim3 grid(l.chunks);
-        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, true, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
-        else if (exact) hipLaunchKernelGGL((adamw_step_kernel<8, true, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
-        else hipLaunchKernelGGL((adamw_step_kernel<8, false, AdamWLaunch<ENTRIES>>), grid, dim3(kBlock), 0, stream, l);
+        const dim3 grid(l.chunks), block(THREADS);
+        if (a->moment_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, true, THREADS, AdamWLaunch<ENTRIES>>), grid, block, 0, stream, l);
+        else if (exact) hipLaunchKernelGGL((adamw_step_kernel<8, true, THREADS, AdamWLaunch<ENTRIES>>), grid, block, 0, stream, l);
+        else hipLaunchKernelGGL((adamw_step_kernel<8, false, THREADS, AdamWLaunch<ENTRIES>>), grid, block, 0, stream, l);
         l.entries = l.chunks = 0;
         slots                = 0;
     };
@@ -537,7 +538,7 @@ void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStrea
             e.n_slot             = n << 3 | (uint32_t)slot;
             e.block              = (uint32_t)((t.first + from) / kMomentBlock);
             e.chunk_types        = l.chunks << 4 | (uint32_t)t.grad_type << 2 | (uint32_t)t.param_type;
-            l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
+            l.chunks += (n + 8 * THREADS - 1) / (8 * THREADS);
         }
     }
     launch();
@@ -1410,7 +1411,8 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         if (!std::isfinite(g.lr) || !std::isfinite(g.weight_decay)) return VETRAST_ERR_INVALID_ARG;
         if (!a->device_state && g.step < 1) return VETRAST_ERR_INVALID_ARG;
     }
-    int64_t entries = 0;
+    int64_t entries = 0, elements = 0;
+    bool floats = false;  // float32 parameters or masters
     for (int k = 0; k < a->num_tensors; ++k)
     {
         const vetrast_adamw_tensor& t = a->tensors[k];
@@ -1422,6 +1424,8 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         if (!aligned_to(t.param, dtype_bytes(t.param_type)) || !aligned_to(t.grad, dtype_bytes(t.grad_type))) return VETRAST_ERR_INVALID_ARG;
         if ((reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad)) >> 48) return VETRAST_ERR_INVALID_ARG;
         entries += (t.n + kOptimEntryElements - 1) / kOptimEntryElements;
+        elements += t.n;
+        floats = floats || t.param_type == VETRAST_F32 || a->master;
     }
     hipStream_t stream  = (hipStream_t)stream_;
     AdamWDevice* device = static_cast<AdamWDevice*>(a->device_state);
@@ -1456,17 +1460,21 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* a, void* stre
         l.zero_grad       = a->zero_grad;
         l.stochastic      = a->stochastic_rounding;
     };
+    const bool waves = elements <= kOptimSmall || (a->moment_bits == 8 && !floats);  // see adamw_step_kernel
+    const auto step  = [&](auto& l) {
+        share(l);
+        if (waves) launch_adamw<kWave>(a, l, stream);
+        else launch_adamw<kBlock>(a, l, stream);
+    };
     if (entries <= kAdamWFew)
     {
         AdamWLaunch<kAdamWFew> l;
-        share(l);
-        launch_adamw(a, l, stream);
+        step(l);
     }
     else
     {
         AdamWLaunch<kAdamWEntries> l;
-        share(l);
-        launch_adamw(a, l, stream);
+        step(l);
     }
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
