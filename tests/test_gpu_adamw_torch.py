@@ -167,6 +167,35 @@ def test_moments_move_between_widths():
     assert all(t.numel() == 0 for t in torch_ops.unpack_moments(*torch_ops.pack_moments([torch.zeros(0, device="cuda")], [torch.zeros(0, device="cuda")])))
 
 
+def test_moments_follow_the_parameters_order():
+    """Loaded in any order of dimensions, they mean the same elements; flat ones are in the order of memory."""
+    base = torch.randn(4, 3, 5, 6, generator=torch.Generator().manual_seed(3)).cuda()
+    p = base.clone(memory_format=torch.channels_last).requires_grad_(True)
+    p.grad = torch.zeros_like(p)
+    m, v = torch.randn_like(base).contiguous(), torch.rand_like(base).contiguous()
+    for bits in (32, 8):
+        forms = []
+        for x, y in ((m, v), (m.clone(memory_format=torch.channels_last), v), (m.transpose(0, 3).contiguous().transpose(0, 3), v),
+                     (m.permute(0, 2, 3, 1).reshape(-1), v.permute(0, 2, 3, 1).reshape(-1))):
+            opt = torch_ops.AdamW([([p], 0.01)], moment_bits=bits)
+            opt.load_moments([x], [y], 5)
+            forms.append(opt.moments())
+        assert all(torch.equal(a[0], forms[0][0]) and torch.equal(a[1], forms[0][1]) for a in forms)
+        if bits == 32:
+            assert torch.equal(forms[0][0][:360].view(4, 5, 6, 3).permute(0, 3, 1, 2), m)
+
+
+def test_zeros_stay_behind_the_last_element():
+    """Also in masters of a block that is lost."""
+    p = parameter((130,), torch.bfloat16, 50)
+    opt = torch_ops.AdamW([([p], 0.01)], moment_bits=8, master_weights=True)
+    p.grad[129] = float("nan")
+    for _ in range(2):
+        opt.step()
+    assert torch.isnan(p[128:]).all() and torch.isfinite(p[:128]).all()
+    assert not opt.master[130:].any() and not opt.exp_avg[130:].any() and not opt.exp_avg_sq[130:].any()
+
+
 def test_refusals():
     p = parameter((8, 8))
     make = lambda ps=None, **kw: torch_ops.AdamW([([p] if ps is None else ps, 0.01, 0.0)], **kw)  # noqa: E731
@@ -200,6 +229,13 @@ def test_refusals():
                  lambda: torch_ops.unpack_moments(*[torch.zeros(128, device="cuda")] * 3)):
         with pytest.raises(RuntimeError):
             call()
+    q = parameter((8,))
+    turned = torch_ops.AdamW([([q], 0.01)])
+    q.data = q.data.bfloat16()
+    q.grad = None
+    q.grad = torch.zeros_like(q)
+    with pytest.raises(RuntimeError, match="type"):
+        turned.step()
     fixed = make(capturable=True)
     fixed.step()
     p.data = torch.zeros(3, 3, device="cuda")

@@ -674,7 +674,15 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     else out = from_floats(p, p_type);
     if constexpr (ANY) store_any(e.param, p_type, start, count, e.whole, out);
     else store_eight<BYTES, HALF>(e.param, start, out);
-    if (master && inside) store_eight<4, HALF>(a.master + at, 0, from_floats(p, VETRAST_F32));
+    if (master && inside)
+    {
+        if constexpr (ANY)  // zeros behind the last element, whatever a lost block makes of them
+        {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) p[j] = j < count ? p[j] : 0.f;
+        }
+        store_eight<4, HALF>(a.master + at, 0, from_floats(p, VETRAST_F32));
+    }
     if (a.zero_grad) clear();
 }
 
@@ -851,7 +859,8 @@ __device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEn
     }
 }
 
-// Four elements' codes at a time, so that a wave's writes have no gaps. `whole`: all of them are there, at 16-byte addresses.
+// Four elements' codes at a time, so that a wave's writes have no gaps, and past the L2, which holds none of what they write for long: 10 M
+// elements 24.9 us with eight a lane, 18.9 with four, 16.1 past the L2. `whole`: all of them are there, at 16-byte addresses.
 __device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
 {
     const uint32_t block = e.block + start / kMomentBlock;
@@ -878,8 +887,9 @@ __device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const Moment
         float *pm = e.m + start, *pv = e.v + start;
         if (whole)
         {
-            *(float4*)(pm + i) = make_float4(m[0], m[1], m[2], m[3]);
-            *(float4*)(pv + i) = make_float4(v[0], v[1], v[2], v[3]);
+            typedef float Four __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store((Four){m[0], m[1], m[2], m[3]}, (Four*)(pm + i));
+            __builtin_nontemporal_store((Four){v[0], v[1], v[2], v[3]}, (Four*)(pv + i));
         }
         else
         {

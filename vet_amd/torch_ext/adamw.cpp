@@ -140,13 +140,14 @@ AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
             TORCH_CHECK(p.defined() && p.is_cuda(), "AdamW: parameters must be tensors on the GPU");
             if (slots_.empty()) device_ = p.device();
             for (auto& s : slots_) TORCH_CHECK(!s.param.is_same(p), "AdamW: a parameter is in the list twice");
-            slots_.push_back({p, (int)lr_.size(), 0, -1, 0});
+            slots_.push_back({p, (int)lr_.size(), type_of(p, "AdamW: parameters"), 0, -1, 0});
         }
         lr_.push_back(g.lr);
         weight_decay_.push_back(g.weight_decay);
     }
     TORCH_CHECK(!slots_.empty(), "AdamW: no parameters");
     c10::DeviceGuard guard(device_);
+    context_on(device_);  // here and not in a step that may be captured
     lay_out();
     if (options_.capturable)
     {
@@ -173,7 +174,6 @@ void AdamW::lay_out()
     for (size_t k = 0; k < slots_.size(); ++k)
     {
         Slot& s = slots_[k];
-        type_of(s.param, "AdamW: parameters");
         check_on(s.param, device_, "AdamW: parameters");
         TORCH_CHECK(dense(s.param), "AdamW: parameters must be dense, without gaps or overlaps");
         if (s.n == s.param.numel()) from[k] = s.first;
@@ -232,6 +232,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         check_on(p, device_, "AdamW: parameters");
         check_on(grad, device_, "AdamW: gradients");
         const int32_t type = type_of(p, "AdamW: parameters");
+        TORCH_CHECK(type == s.type, "AdamW: a parameter has changed its type");
         TORCH_CHECK(grad.scalar_type() == p.scalar_type() && grad.sizes() == p.sizes(), "AdamW: a gradient must have its parameter's type and shape");
         TORCH_CHECK(dense(p), "AdamW: parameters must be dense, without gaps or overlaps");
         void* gradient = nullptr;
@@ -347,11 +348,21 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
 {
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
-    int64_t total = 0;
-    std::vector<vetrast_moment_tensor> list = moment_list(pointers(exp_avgs), pointers(exp_avg_sqs), device_, total);
-    TORCH_CHECK(list.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", list.size());
-    for (size_t k = 0; k < list.size(); ++k)
-        TORCH_CHECK(list[k].n == slots_[k].n, "AdamW: parameter ", k, " has ", slots_[k].n, " elements, its moments have ", list[k].n);
+    TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
+    std::vector<torch::Tensor> kept[2];
+    for (size_t k = 0; k < slots_.size(); ++k)
+        for (int which = 0; which < 2; ++which)
+        {
+            TORCH_CHECK(k < exp_avg_sqs.size(), "AdamW: as many second moments as first ones are needed");
+            const torch::Tensor &p = slots_[k].param, &x = which ? exp_avg_sqs[k] : exp_avgs[k];
+            check_on(x, device_, "AdamW: moments");
+            TORCH_CHECK(x.scalar_type() == torch::kFloat32, "AdamW: moments must be float32 tensors");
+            TORCH_CHECK(x.sizes() == p.sizes() || (x.dim() == 1 && x.numel() == slots_[k].n), "AdamW: parameter ", k, " and its moments differ in shape");
+            if (x.sizes() == p.sizes() && !same_order(x, p)) kept[which].push_back(torch::empty_like(p, x.options()).copy_(x));
+            else kept[which].push_back(dense(x) ? x : x.contiguous());
+        }
+    int64_t total                           = 0;
+    std::vector<vetrast_moment_tensor> list = moment_list(pointers(kept[0]), pointers(kept[1]), device_, total);
     set_step(step);
     if (options_.moment_bits == 8)
     {
@@ -361,8 +372,8 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     }
     for (size_t k = 0; k < list.size(); ++k)
     {
-        exp_avg.narrow(0, slots_[k].first, slots_[k].n).copy_(exp_avgs[k].as_strided({slots_[k].n}, {1}));
-        exp_avg_sq.narrow(0, slots_[k].first, slots_[k].n).copy_(exp_avg_sqs[k].as_strided({slots_[k].n}, {1}));
+        exp_avg.narrow(0, slots_[k].first, slots_[k].n).copy_(kept[0][k].as_strided({slots_[k].n}, {1}));
+        exp_avg_sq.narrow(0, slots_[k].first, slots_[k].n).copy_(kept[1][k].as_strided({slots_[k].n}, {1}));
     }
 }
 

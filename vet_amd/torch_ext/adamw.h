@@ -13,6 +13,7 @@ namespace vet_amd
 {
 // The reference steps its texture with MyAdam (src/lib/models/my_adam.cpp) and its network with torch::optim::Adam, a dozen
 // elementwise launches a tensor; this class takes both kinds of tensors, in one launch for up to 160 of them.
+// An object serves one host thread and one stream at a time.
 class AdamW
 {
    public:
@@ -51,7 +52,8 @@ class AdamW
     std::vector<std::pair<int64_t, int64_t>> layout() const;
     // Both moments as flat float32 tensors laid out like the state (the state itself where it is float32).
     std::tuple<torch::Tensor, torch::Tensor> moments() const;
-    // Takes over float32 moments, two tensors a parameter in the order of its memory, from a run with either kind of state.
+    // Takes over float32 moments, two tensors a parameter, from a run with either kind of state: of the parameter's shape, or flat in
+    // the order of its memory.
     void load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, int64_t step);
     // Masters are read from the parameters again (after a checkpoint was loaded into these).
     void reload_master();
@@ -67,6 +69,7 @@ class AdamW
     {
         torch::Tensor param;
         int group     = 0;
+        int32_t type  = 0;
         int64_t first = 0, n = 0, step = 0;
     };
     void lay_out();

@@ -60,7 +60,7 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
           capturable=False):
     """AdamW over everything a training step has gradients for, in one launch for up to 160 tensors (vetrast_adamw_step).
 
-    groups: list of (list of parameter tensors, learning rate, weight decay). Parameters are dense CUDA tensors of float32,
+    groups: list of (list of parameter tensors, learning rate[, weight decay]). Parameters are dense CUDA tensors of float32,
     bfloat16 or float16 in any order of dimensions; gradients are found in .grad at every step.
     moment_bits: 32, or 8 for moments of a byte each with two scale bytes for every 128 elements. master_weights: 16-bit
     parameters have float32 masters with the optimiser. stochastic_rounding: bfloat16 parameters without masters are rounded
@@ -72,8 +72,8 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
     set_lr(group, lr), steps(), set_step(n), layout() -> [(first element, elements)] in the flat state tensors exp_avg,
     exp_avg_sq, block_scale and master; moments() -> both as flat float32; load_moments(exp_avgs, exp_avg_sqs, step),
     reload_master()."""
-    return load().AdamW([(list(ts), float(lr), float(wd)) for ts, lr, wd in groups], beta1, beta2, eps, int(moment_bits),
-                        bool(master_weights), bool(stochastic_rounding), int(seed), bool(capturable))
+    return load().AdamW([(list(g[0]), float(g[1]), float(g[2]) if len(g) > 2 else 0.0) for g in groups], beta1, beta2, eps,
+                        int(moment_bits), bool(master_weights), bool(stochastic_rounding), int(seed), bool(capturable))
 
 
 def grad_norm(gradients, max_norm=0.0, scale=1.0):
