@@ -169,6 +169,12 @@ def test_step_of_many_elements(bits, master, param, grad, rasterizer):
     batch.compare(groups, 12, stochastic=True, scale=3.0)
 
 
+def test_tiny_eps_and_many_elements(rasterizer):
+    batch = Batch(np.random.default_rng(18), [(1_600_001, F, F, 0), (300, B, B, 0)], 8)
+    batch.step(rasterizer, [(0.01, 0.0, 2)], eps=1e-15, seed=1)
+    batch.compare([(0.01, 0.0, 2)], 1, eps=1e-15)
+
+
 @pytest.mark.parametrize("eps", [1e-6, 1e-15, 1e-30])
 def test_tiny_eps_and_tiny_gradients(eps, rasterizer):
     """Second moments below the smallest normal number count where eps is small enough to let them."""

@@ -245,6 +245,15 @@ def test_refusals():
         fixed.step()
 
 
+def test_parameters_made_in_inference_mode():
+    with torch.inference_mode():
+        p = torch.zeros(100, device="cuda")
+        p.grad = torch.ones(100, device="cuda")
+    opt = torch_ops.AdamW([([p], 0.5)])
+    opt.step(zero_grad=True)
+    assert opt.steps() == [1] and torch.allclose(p, torch.full_like(p, -0.5)) and not p.grad.any()
+
+
 def test_no_gradient_anywhere_changes_nothing():
     p = parameter((40,), gradient=False)
     was = p.detach().clone()

@@ -247,7 +247,7 @@ __host__ __device__ inline uint32_t step_key(uint64_t seed, int64_t step)
     return (uint32_t)mix64(mix64(seed) + (uint64_t)step);
 }
 
-__device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_t c)
+__device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_t c)  // of three, in one instruction
 {
     uint32_t x;
     asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x96" : "=v"(x) : "v"(a), "v"(b), "v"(c));
@@ -255,9 +255,8 @@ __device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_
 }
 
 // 20 random bits for each of a thread's eight elements; `pair`: number of the chunk's first pair of elements. 32 bits of a hash serve two
-// elements, the
-// lower 20 and the upper 20 of them (products of 32 bits take four times as long as other instructions, and the 8-bit step is
-// bound by instructions).
+// elements, the lower 20 and the upper 20 of them: products of 32 bits take four times as long as other instructions, and the 8-bit
+// step is bound by instructions.
 template <uint32_t HALF>
 __device__ __forceinline__ void random_eight(uint32_t pair, uint32_t key, uint32_t* r)
 {
@@ -686,6 +685,11 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
     if (a.zero_grad) clear();
 }
 
+// One pass over parameter, gradient and state, each read and written once.
+//   32 bits: bound by memory. 27.5 M float32 elements, 28 bytes each: 142 us, 5.4 TB/s.
+//   8 bits:  10 M float32 elements, 16 bytes each: 28.6 us, 5.6 TB/s, bound by memory. 40 M bf16 elements, 10 bytes each: 76 us, 5.3 TB/s; the
+//            same loads and stores with nothing in between 74 us, and the vector units are at 87 %: 424 instructions for a wave's 512
+//            elements (549 before bits were taken out of words, medians and products by the instructions for them).
 // EXACT: eps is so small that roots of values below 2^-126 count.
 // THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.1 us,
 // with four waves 4.1; 1 M 4.8 and 6.4 with 8-bit moments; 4 M 18.8 and 18.1), and with 8-bit moments of 16-bit parameters, where
@@ -776,6 +780,7 @@ __device__ __forceinline__ bool leave_sum(NormWorkspace* w, uint32_t number, uin
 
 // In 64 bits throughout: no square overflows or vanishes, and a sum of any length is good to the last bit of a float. The workgroup that is
 // the last of the call to leave its sum adds all of them, in the order of their numbers: one launch instead of two, 4 us of a host's time.
+// 27.5 M float32: 21.7 us, 5.1 TB/s. 100 k: 4.2 us, what a launch, a sum's way to memory, the count and the sums' way back take.
 __global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const NormLaunch a)
 {
     const ChunkFinder<finder_groups(kNormEntries)> find(a);
@@ -833,6 +838,7 @@ struct MomentLaunch
 };
 static_assert(sizeof(MomentLaunch) <= 4096, "kernel arguments");
 
+// 10 M elements: 17.0 us, 5.9 TB/s, bound by memory.
 __device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
 {
     const uint32_t block = e.block + start / kMomentBlock;

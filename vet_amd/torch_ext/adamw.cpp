@@ -287,9 +287,12 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         if (!grad.defined()) continue;
         s.step += 1;
         // the kernel wrote through raw pointers: tell everyone who keys on the version counters
-        s.param.unsafeGetTensorImpl()->bump_version();
+        if (!s.param.is_inference()) s.param.unsafeGetTensorImpl()->bump_version();
         if (!zero_grad) continue;
-        if (same_order(s.param, grad)) grad.unsafeGetTensorImpl()->bump_version();
+        if (same_order(s.param, grad))
+        {
+            if (!grad.is_inference()) grad.unsafeGetTensorImpl()->bump_version();
+        }
         else if (dense(grad)) s.param.mutable_grad().zero_();  // the kernel cleared its copy
         else s.param.mutable_grad() = torch::zeros_like(s.param);
     }

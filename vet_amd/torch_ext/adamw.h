@@ -37,7 +37,8 @@ class AdamW
     AdamW(std::vector<Group> groups, Options options);
 
     // One step on every parameter that has a gradient. grad_scale: float32 on the GPU, one element or the two that GradNorm
-    // returns (the last counts); where it is not finite, parameters, moments and the device's step count stay as they are.
+    // returns (the last counts); where it is not finite, parameters, moments and the device's step count stay as they are (a count
+    // on the host goes up all the same: it does not see the device).
     // A parameter whose number of elements has changed starts anew, as MyAdam does.
     void step(bool zero_grad = false, const std::optional<torch::Tensor>& grad_scale = std::nullopt);
     void zero_grad();
@@ -59,7 +60,8 @@ class AdamW
     void reload_master();
 
     // The state, flat: every parameter starts at a multiple of VETRAST_MOMENT_BLOCK elements. exp_avg and exp_avg_sq are float32,
-    // or uint8 codes with block_scale uint8 [blocks, 2]; master is float32 or undefined.
+    // or uint8 codes with block_scale uint8 [blocks, 2]; master is float32 or undefined. They are other tensors after a step that
+    // found a parameter of another size.
     torch::Tensor exp_avg, exp_avg_sq, block_scale, master;
     // With capturable: steps done (int64 [1]) and a factor on every group's learning rate (float32 [1]); both may be written.
     torch::Tensor device_step, lr_factor;
