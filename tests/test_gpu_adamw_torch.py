@@ -143,6 +143,28 @@ def test_a_parameter_that_changes_its_size_starts_anew(bits):
             assert torch.equal(ps[k], twins[k])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_load_for_parameters_that_changed_their_size(bits):
+    """Before any step has seen the new size: the state is laid out for it."""
+    ps = [parameter((4, 100), torch.bfloat16, 60), parameter((30,), torch.bfloat16, 61)]
+    opt = torch_ops.AdamW([(ps, 0.01)], moment_bits=bits, master_weights=True)
+    opt.step()
+    kept = opt.master[512:542].clone()
+    ps[0].data = torch.randn(4, 1500, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    ms = [torch.full((4, 1500), 0.25, device="cuda"), torch.full((30,), -1.0, device="cuda")]
+    opt.load_moments(ms, [m * m for m in ms], 7)
+    assert opt.layout() == [(0, 6000), (6016, 30)] and opt.steps() == [7, 7]
+    assert torch.equal(opt.master[:6000], ps[0].detach().float().reshape(-1)) and torch.equal(opt.master[6016:6046], kept)
+    m, v = opt.moments()
+    for (f, n), x in zip(opt.layout(), ms):  # a power of two is within half a code of itself, and the offset another 2^-15 of it
+        assert (abs(m[f:f + n] - x.reshape(-1)) <= abs(x.reshape(-1)) / 16).all() and (abs(v[f:f + n] - x.reshape(-1) ** 2) <= x.reshape(-1) ** 2 / 16).all()
+    fixed = torch_ops.AdamW([(ps, 0.01)], moment_bits=bits, capturable=True)
+    ps[1].data = torch.zeros(31, dtype=torch.bfloat16, device="cuda")
+    ms[1] = torch.zeros(31, device="cuda")
+    with pytest.raises(RuntimeError, match="change their size"):
+        fixed.load_moments(ms, ms, 1)
+
+
 def test_moments_move_between_widths():
     ps = [parameter((4, 777), seed=13), parameter((777,), seed=14)]
     full = torch_ops.AdamW([(ps, 0.01, 0.0)])
@@ -316,6 +338,21 @@ def test_a_captured_step_needs_its_count_on_the_device():
     opt.step()
     torch.cuda.synchronize()
     assert opt.steps() == [2] and not torch.equal(p, was)
+
+
+def test_a_captured_step_does_not_replace_gradients():
+    """One that its elements share cannot be cleared in place."""
+    p = parameter((40,), gradient=False)
+    opt = torch_ops.AdamW([([p], 0.01, 0.0)], capturable=True)
+    p.grad = torch.ones(1, device="cuda").expand(40)
+    was, graph = p.detach().clone(), torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cleared"):
+        with torch.cuda.graph(graph):
+            opt.step(zero_grad=True)
+    torch.cuda.synchronize()
+    assert opt.steps() == [0] and torch.equal(p, was)
+    opt.step(zero_grad=True)
+    assert opt.steps() == [1] and not p.grad.any() and p.grad.is_contiguous() and not torch.equal(p, was)
 
 
 def test_two_graphs_of_norms_side_by_side():

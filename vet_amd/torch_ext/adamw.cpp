@@ -205,18 +205,22 @@ void AdamW::lay_out()
     }
 }
 
+// A new layout if a parameter has changed its size.
+void AdamW::follow_sizes()
+{
+    bool moved = false;
+    for (auto& s : slots_) moved |= s.param.numel() != s.n;
+    if (!moved) return;
+    TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
+    lay_out();
+}
+
 void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
 {
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(options_.capturable || !capturing(), "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
-    bool moved = false;
-    for (auto& s : slots_) moved |= s.param.numel() != s.n;
-    if (moved)
-    {
-        TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
-        lay_out();
-    }
+    follow_sizes();
     const bool eight = options_.moment_bits == 8;
     tensors_.clear();
     groups_.clear();
@@ -239,6 +243,8 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         if (same_order(p, grad)) gradient = grad.data_ptr();
         else
         {
+            // what clears it below is another tensor, which a replay would not read
+            TORCH_CHECK(!zero_grad || dense(grad) || !capturing(), "AdamW: a gradient with gaps or overlaps cannot be cleared in a captured step");
             reordered.push_back(torch::empty_like(p).copy_(grad));
             gradient = reordered.back().data_ptr();
         }
@@ -352,6 +358,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
+    follow_sizes();
     std::vector<torch::Tensor> kept[2];
     for (size_t k = 0; k < slots_.size(); ++k)
         for (int which = 0; which < 2; ++which)

@@ -32,8 +32,8 @@ class AdamW
         uint64_t seed            = 0;      // of the random bits, also those that round 8-bit moments
         bool capturable          = false;  // the step count lies on the device, steps may be captured in a graph
     };
-    // Parameters: dense tensors on one GPU (any order of dimensions), float32, bfloat16 or float16; their gradients are found in
-    // .grad() at every step. Masters are read from the parameters here, moments are zero.
+    // Parameters: dense tensors on one GPU (any order of dimensions), float32, bfloat16 or float16, no two of which share memory;
+    // their gradients are found in .grad() at every step (these may share memory only while steps do not clear them). Masters are read from the parameters here, moments are zero.
     AdamW(std::vector<Group> groups, Options options);
 
     // One step on every parameter that has a gradient. grad_scale: float32 on the GPU, one element or the two that GradNorm
@@ -60,8 +60,8 @@ class AdamW
     void reload_master();
 
     // The state, flat: every parameter starts at a multiple of VETRAST_MOMENT_BLOCK elements. exp_avg and exp_avg_sq are float32,
-    // or uint8 codes with block_scale uint8 [blocks, 2]; master is float32 or undefined. They are other tensors after a step that
-    // found a parameter of another size.
+    // or uint8 codes with block_scale uint8 [blocks, 2]; master is float32 or undefined. They are other tensors after a step or
+    // load_moments that found a parameter of another size.
     torch::Tensor exp_avg, exp_avg_sq, block_scale, master;
     // With capturable: steps done (int64 [1]) and a factor on every group's learning rate (float32 [1]); both may be written.
     torch::Tensor device_step, lr_factor;
@@ -75,6 +75,7 @@ class AdamW
         int64_t first = 0, n = 0, step = 0;
     };
     void lay_out();
+    void follow_sizes();
     void fill_master(const Slot& s);
     std::vector<Slot> slots_;
     std::vector<double> lr_, weight_decay_;

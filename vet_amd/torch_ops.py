@@ -61,7 +61,8 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
     """AdamW over everything a training step has gradients for, in one launch for up to 160 tensors (vetrast_adamw_step).
 
     groups: list of (list of parameter tensors, learning rate[, weight decay]). Parameters are dense CUDA tensors of float32,
-    bfloat16 or float16 in any order of dimensions; gradients are found in .grad at every step.
+    bfloat16 or float16 in any order of dimensions, no two of which share memory; gradients are found in .grad at every step, and
+    may share memory only while steps do not clear them.
     moment_bits: 32, or 8 for moments of a byte each with two scale bytes for every 128 elements. master_weights: 16-bit
     parameters have float32 masters with the optimiser. stochastic_rounding: bfloat16 parameters without masters are rounded
     by random bits, a function of `seed`, step and element. capturable: the step count lies on the device, so that steps may
