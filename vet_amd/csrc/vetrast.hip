@@ -489,6 +489,47 @@ inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat array
     return first >= 0 && first % kMomentBlock == 0 && first < ((int64_t)1 << 38) && n <= ((int64_t)1 << 38);
 }
 
+// The launches of a norm.
+template <int ENTRIES>
+void launch_norm(const vetrast_gradient_norm_args* a, hipStream_t stream)
+{
+    NormLaunch<ENTRIES> l;
+    l.workspace = static_cast<NormWorkspace*>(a->workspace);
+    l.out       = a->out;
+    l.max_norm  = a->max_norm;
+    l.scale     = a->scale;
+    // twice through the list: the launches have to know how many workgroups the call has
+    const auto each = [&](auto&& launch) {
+        l.entries = l.chunks = 0;
+        uint32_t first = 0;
+        const auto close = [&] {
+            const uint32_t grid = std::max(std::min(l.chunks, kNormGrid), 1u);
+            l.first             = first;
+            launch(grid);
+            first += grid;
+            l.entries = l.chunks = 0;
+        };
+        for (int k = 0; k < a->num_gradients; ++k)
+        {
+            const vetrast_gradient& g = a->gradients[k];
+            for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
+            {
+                if (l.entries == (uint32_t)ENTRIES) close();
+                NormEntry& e     = l.e[l.entries++];
+                e.grad           = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
+                const uint32_t n = (uint32_t)std::min(g.n - from, kOptimEntryElements);
+                e.n_type         = n << 2 | (uint32_t)g.type;
+                e.first_chunk    = l.chunks;
+                l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
+            }
+        }
+        if (l.entries > 0 || first == 0) close();
+        return first;
+    };
+    l.total = each([](uint32_t) {});
+    each([&](uint32_t grid) { hipLaunchKernelGGL((gradient_norm_kernel<ENTRIES>), dim3(grid), dim3(kBlock), 0, stream, l); });
+}
+
 // The launches of a list of tensors; `l` has what they share.
 template <int THREADS, int ENTRIES>
 void launch_adamw(const vetrast_adamw_args* a, AdamWLaunch<ENTRIES>& l, hipStream_t stream)
@@ -1499,49 +1540,18 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
     if (a->num_gradients < 0 || (a->num_gradients > 0 && !a->gradients) || !a->out || !a->workspace) return VETRAST_ERR_INVALID_ARG;
     if (!std::isfinite(a->scale) || std::isnan(a->max_norm)) return VETRAST_ERR_INVALID_ARG;
     if (!aligned_to(a->out, 4) || !aligned_to(a->workspace, 16)) return VETRAST_ERR_INVALID_ARG;
+    int64_t entries = 0;
     for (int k = 0; k < a->num_gradients; ++k)
     {
         const vetrast_gradient& g = a->gradients[k];
         if (g.n < 0 || !is_dtype(g.type)) return VETRAST_ERR_INVALID_ARG;
         if (g.n > 0 && (!g.grad || !aligned_to(g.grad, dtype_bytes(g.type)))) return VETRAST_ERR_INVALID_ARG;
+        entries += (g.n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
     if (a->workspace_bytes < vetrast_gradient_norm_workspace_bytes(a->gradients, a->num_gradients)) return VETRAST_ERR_WORKSPACE_SMALL;
     hipStream_t stream = (hipStream_t)stream_;
-    NormLaunch l;
-    l.workspace = static_cast<NormWorkspace*>(a->workspace);
-    l.out       = a->out;
-    l.max_norm  = a->max_norm;
-    l.scale     = a->scale;
-    // twice through the list: the launches have to know how many workgroups the call has
-    const auto each = [&](auto&& launch) {
-        l.entries = l.chunks = 0;
-        uint32_t first = 0;
-        const auto close = [&] {
-            const uint32_t grid = std::max(std::min(l.chunks, kNormGrid), 1u);
-            l.first             = first;
-            launch(grid);
-            first += grid;
-            l.entries = l.chunks = 0;
-        };
-        for (int k = 0; k < a->num_gradients; ++k)
-        {
-            const vetrast_gradient& g = a->gradients[k];
-            for (int64_t from = 0; from < g.n; from += kOptimEntryElements)
-            {
-                if (l.entries == (uint32_t)kNormEntries) close();
-                NormEntry& e     = l.e[l.entries++];
-                e.grad           = static_cast<const char*>(g.grad) + from * (int64_t)dtype_bytes(g.type);
-                const uint32_t n = (uint32_t)std::min(g.n - from, kOptimEntryElements);
-                e.n_type         = n << 2 | (uint32_t)g.type;
-                e.first_chunk    = l.chunks;
-                l.chunks += (n + kOptimChunk - 1) / kOptimChunk;
-            }
-        }
-        if (l.entries > 0 || first == 0) close();
-        return first;
-    };
-    l.total = each([](uint32_t) {});
-    each([&](uint32_t grid) { hipLaunchKernelGGL(gradient_norm_kernel, dim3(grid), dim3(kBlock), 0, stream, l); });
+    if (entries <= kNormFew) launch_norm<kNormFew>(a, stream);
+    else launch_norm<kNormEntries>(a, stream);
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
 }
