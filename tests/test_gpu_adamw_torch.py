@@ -1,5 +1,7 @@
 """The optimiser for libtorch callers (torch_ops.AdamW, grad_norm, pack_moments, unpack_moments): what it does with parameters as
 programs have them, its refusals, captured steps, and a run of everything together behind the rasterizer."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -387,6 +389,32 @@ def test_steps_on_another_stream():
         b.step(grad_scale=b.grad_norm(1.0))
     torch.cuda.synchronize()
     assert torch.equal(p, q) and torch.equal(a.exp_avg, b.exp_avg)
+
+
+def test_host_threads_side_by_side():
+    """Each with parameters and a stream of its own: they end where they end one after the other."""
+    def train(seed, ends):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ps = [parameter((n,), seed=seed + n, gradient=False) for n in (1000, 5, 300000)]
+            opt = torch_ops.AdamW([(ps, 0.01, 0.1)], moment_bits=8, seed=seed)
+            for k in range(60):
+                for p in ps:
+                    p.grad = p.detach() * 0.1 + k * 1e-3
+                norm = opt.grad_norm(1.0)
+                opt.step(True, norm)
+            ends[seed] = [t.clone() for t in (*ps, *states(opt), norm)]
+            torch.cuda.current_stream().synchronize()
+
+    alone, together = {}, {}
+    for seed in range(4):
+        train(seed, alone)
+    threads = [threading.Thread(target=train, args=(seed, together)) for seed in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed], strict=True)), seed
 
 
 @pytest.mark.parametrize("bits", [32, 8])
