@@ -48,6 +48,23 @@ struct RawEight
     uint4 a, b;
 };
 
+// Loads and stores of many bytes at addresses that are multiples of an element's size only: the same instructions as at multiples of 16,
+// a little slower where they straddle lines.
+typedef uint32_t LooseFour __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t LooseTwo __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ uint4 load_four(const char* p)
+{
+    const LooseFour x = *(const LooseFour*)p;
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint2 load_two(const char* p)
+{
+    const LooseTwo x = *(const LooseTwo*)p;
+    return make_uint2(x[0], x[1]);
+}
+__device__ __forceinline__ void store_four(char* p, const uint4& x) { *(LooseFour*)p = (LooseFour){x.x, x.y, x.z, x.w}; }
+__device__ __forceinline__ void store_two(char* p, uint32_t x, uint32_t y) { *(LooseTwo*)p = (LooseTwo){x, y}; }
+
 // A thread's eight elements of a chunk that begins at element `start` of a tensor: the eight from 8 * threadIdx.x on, or (halves) the four
 // from 4 * threadIdx.x on and the four HALF elements behind these, with which a wave's access to float32 has no gaps. Writes gain by
 // that, in what the last-level cache holds: 10 M first and second moments written 24.9 us, in halves 18.8; a step of 4 M elements with
@@ -65,20 +82,20 @@ __device__ __forceinline__ RawEight load_eight(const void* p, uint32_t start)
         const uint32_t here     = threadIdx.x * 4u * BYTES;
         if constexpr (BYTES == 4)
         {
-            r.a = *(const uint4*)(base + here);
-            r.b = *(const uint4*)(base + here + half);
+            r.a = load_four(base + here);
+            r.b = load_four(base + here + half);
         }
         else
         {
-            const uint2 x = *(const uint2*)(base + here), y = *(const uint2*)(base + here + half);
+            const uint2 x = load_two(base + here), y = load_two(base + here + half);
             r.a = make_uint4(x.x, x.y, y.x, y.y);
         }
     }
     else
     {
         const uint32_t here = threadIdx.x * 8u * BYTES;
-        r.a                 = *(const uint4*)(base + here);
-        if constexpr (BYTES == 4) r.b = *(const uint4*)(base + here + 16);
+        r.a                 = load_four(base + here);
+        if constexpr (BYTES == 4) r.b = load_four(base + here + 16);
     }
     return r;
 }
@@ -92,24 +109,24 @@ __device__ __forceinline__ void store_eight(void* p, uint32_t start, const RawEi
         const uint32_t here     = threadIdx.x * 4u * BYTES;
         if constexpr (BYTES == 4)
         {
-            *(uint4*)(base + here)        = r.a;
-            *(uint4*)(base + here + half) = r.b;
+            store_four(base + here, r.a);
+            store_four(base + here + half, r.b);
         }
         else
         {
-            *(uint2*)(base + here)        = make_uint2(r.a.x, r.a.y);
-            *(uint2*)(base + here + half) = make_uint2(r.a.z, r.a.w);
+            store_two(base + here, r.a.x, r.a.y);
+            store_two(base + here + half, r.a.z, r.a.w);
         }
     }
     else
     {
-        const uint32_t here    = threadIdx.x * 8u * BYTES;
-        *(uint4*)(base + here) = r.a;
-        if constexpr (BYTES == 4) *(uint4*)(base + here + 16) = r.b;
+        const uint32_t here = threadIdx.x * 8u * BYTES;
+        store_four(base + here, r.a);
+        if constexpr (BYTES == 4) store_four(base + here + 16, r.b);
     }
 }
 
-// The first `count` of them, at any address; the others read as zeros and are not written.
+// The first `count` of them; the others read as zeros and are not written.
 template <int BYTES>
 __device__ __forceinline__ RawEight load_some(const void* p, uint32_t start, uint32_t count)
 {
@@ -153,7 +170,7 @@ __device__ __forceinline__ void store_some(void* p, uint32_t start, uint32_t cou
         }
 }
 
-// Of a type known at run time, `whole` where all threads have their eight at 16-byte addresses.
+// Of a type known at run time, `whole` where all threads have their eight.
 __device__ __forceinline__ RawEight load_any(const void* p, uint32_t type, uint32_t start, uint32_t count, bool whole)
 {
     if (type == VETRAST_F32) return whole ? load_eight<4>(p, start) : load_some<4>(p, start, count);
@@ -424,8 +441,10 @@ struct AdamWEntry
     uint32_t block;                  // place in the flat arrays
     uint32_t chunk_types;            // first chunk of the launch << 4 | type of the gradient << 2 | type of the parameter
     __device__ __forceinline__ uint32_t begins() const { return chunk_types >> 4; }
-    __device__ __forceinline__ void* param() const { return (void*)((uint64_t)param_high << 32 | param_low); }
-    __device__ __forceinline__ void* grad() const { return (void*)((uint64_t)grad_high << 32 | grad_low); }
+    // Known to lie in global memory: else the compiler takes flat instructions, which wait for each other and for scalar loads.
+    typedef __attribute__((address_space(1))) void Global;
+    __device__ __forceinline__ void* param() const { return (void*)(Global*)((uint64_t)param_high << 32 | param_low); }
+    __device__ __forceinline__ void* grad() const { return (void*)(Global*)((uint64_t)grad_high << 32 | grad_low); }
 };
 
 struct AdamWGroup
@@ -449,7 +468,7 @@ __host__ __device__ inline AdamWGroup adamw_group(double lr, double weight_decay
     return g;
 }
 
-struct AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel leaves for the step's launches
+struct alignas(16) AdamWDevice  // vetrast_adamw_device_state and what adamw_begin_kernel leaves for the step's launches
 {
     vetrast_adamw_device_state state;
     AdamWGroup group[1];
@@ -511,17 +530,30 @@ __global__ void __launch_bounds__(kBeginGroups) adamw_begin_kernel(const AdamWBe
     if (a.last && counts && k == 0) a.device->state.step = step;
 }
 
+// Both by scalar loads (the device's were written by an earlier launch); left alone the compiler makes one of the two, a flat one, which waits
+// for all loads under way before the random bits.
+__device__ __forceinline__ AdamWGroup group_of(const AdamWCommon& a, uint32_t slot)
+{
+    AdamWGroup g = a.g[slot];
+    asm("" : "+s"(g.root), "+s"(g.floor), "+s"(g.keep));
+    if (a.device)
+    {
+        typedef uint32_t Four __attribute__((ext_vector_type(4)));
+        g = __builtin_bit_cast(AdamWGroup, *(const __attribute__((address_space(4))) Four*)(uintptr_t)&a.device->group[g.key]);
+    }
+    return g;
+}
+
 struct AdamWChunk
 {
     void *param, *grad;
     uint32_t n, slot, p_type, g_type;
     uint32_t start;  // the chunk's first element
     uint32_t block;  // of the tensor, in the flat arrays
-    bool whole;      // all its elements are there, at 16-byte addresses
+    bool whole;      // all its elements are there
 };
 
-// Chunks of four kinds. In whole ones every thread has its eight elements at addresses that are multiples of 16, parameter and gradient
-// of one width: their loads are straight code, all of them under way at once. `kAnyChunk` does for everything else.
+// Chunks of four kinds. In whole ones every thread has its eight elements, parameter and gradient of one width: their loads are straight code, all of them under way at once. `kAnyChunk` does for everything else.
 enum ChunkKind
 {
     kFloatChunk,   // float32
@@ -584,8 +616,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
             codes.scale = scales[mine / kMomentBlock];
         }
     }
-    AdamWGroup g = a.g[e.slot];
-    if (a.device) g = a.device->group[g.key];
+    const AdamWGroup g = group_of(a, e.slot);
     const bool random = KIND != kFloatChunk && !master && a.stochastic && p_type == VETRAST_BF16;
     uint32_t r[8];
     if (BITS == 8 || random) random_eight<HALF>((uint32_t)(at / 2), g.key, r);
@@ -710,7 +741,7 @@ __global__ void __launch_bounds__(THREADS) adamw_step_kernel(const Launch a)
     e.g_type = entry.chunk_types >> 2 & 3u;
     e.start  = (blockIdx.x - entry.begins()) * CHUNK;
     e.block  = entry.block;
-    e.whole  = e.n - e.start >= CHUNK && (((uintptr_t)e.param | (uintptr_t)e.grad) & 15) == 0;
+    e.whole  = e.n - e.start >= CHUNK;
     if (!e.whole || (e.p_type == VETRAST_F32) != (e.g_type == VETRAST_F32)) adamw_chunk<BITS, EXACT, CHUNK, kAnyChunk>(a, e, grad_scale);
     else if (e.p_type == VETRAST_F32) adamw_chunk<BITS, EXACT, CHUNK, kFloatChunk>(a, e, grad_scale);
     else if (a.master) adamw_chunk<BITS, EXACT, CHUNK, kMasterChunk>(a, e, grad_scale);
@@ -794,7 +825,7 @@ __global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const NormLaunch<
         const uint32_t n     = e.n_type >> 2, type = e.n_type & 3u;
         const uint32_t start = (chunk - e.first_chunk) * kOptimChunk;
         RawEight r;
-        if (n - start >= kOptimChunk && (uintptr_t)e.grad % 16 == 0)
+        if (n - start >= kOptimChunk)
         {
             if (type == VETRAST_F32) r = load_eight<4, kOptimChunk / 2>(e.grad, start);
             else r = load_eight<2>(e.grad, start);
@@ -869,7 +900,7 @@ __device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEn
 }
 
 // Four elements' codes at a time, so that a wave's writes have no gaps, and past the L2, which holds none of what they write for long: 10 M
-// elements 24.9 us with eight a lane, 18.9 with four, 16.1 past the L2. `whole`: all of them are there, at 16-byte addresses.
+// elements 24.9 us with eight a lane, 18.9 with four, 16.1 past the L2. `whole`: all of them are there.
 __device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
 {
     const uint32_t block = e.block + start / kMomentBlock;
@@ -896,7 +927,7 @@ __device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const Moment
         float *pm = e.m + start, *pv = e.v + start;
         if (whole)
         {
-            typedef float Four __attribute__((ext_vector_type(4)));
+            typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
             __builtin_nontemporal_store((Four){m[0], m[1], m[2], m[3]}, (Four*)(pm + i));
             __builtin_nontemporal_store((Four){v[0], v[1], v[2], v[3]}, (Four*)(pv + i));
         }
@@ -919,7 +950,7 @@ __global__ void __launch_bounds__(kBlock) convert_moments_kernel(const MomentLau
     const ChunkFinder<finder_groups(kMomentEntries)> find(a);
     const MomentEntry& e = a.e[find(blockIdx.x)];
     const uint32_t start = (blockIdx.x - e.first_chunk) * kOptimChunk;
-    const bool whole     = e.n - start >= kOptimChunk && (((uintptr_t)e.m | (uintptr_t)e.v) & 15) == 0;
+    const bool whole     = e.n - start >= kOptimChunk;
     if constexpr (PACK) pack_chunk(a, e, start, whole);
     else unpack_chunk(a, e, start, whole);
 }
