@@ -718,13 +718,14 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
 
 // One pass over parameter, gradient and state, each read and written once.
 //   32 bits: bound by memory. 27.5 M float32 elements, 28 bytes each: 142 us, 5.4 TB/s.
-//   8 bits:  10 M float32 elements, 16 bytes each: 28.6 us, 5.6 TB/s, bound by memory. 40 M bf16 elements, 10 bytes each: 76 us, 5.3 TB/s; the
-//            same loads and stores with nothing in between 74 us, and the vector units are at 87 %: 424 instructions for a wave's 512
-//            elements (549 before bits were taken out of words, medians and products by the instructions for them).
+//   8 bits:  10 M float32 elements, 16 bytes each: 28.3 us, 5.7 TB/s, bound by memory. 40 M bf16 elements, 10 bytes each: 75 us, 5.4 TB/s; the
+//            same loads and stores with nothing in between 74 us, and the vector units are at work for 87 to 92 % of the time: 434
+//            instructions for a wave's 512 elements (549 before bits were taken out of words, medians and products by the
+//            instructions for them), of which roots, quotients and 32-bit products take four times as long as the others.
 // EXACT: eps is so small that roots of values below 2^-126 count.
-// THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.1 us,
-// with four waves 4.1; 1 M 4.8 and 6.4 with 8-bit moments; 4 M 18.8 and 18.1), and with 8-bit moments of 16-bit parameters, where
-// compute units that are never idle count (16 M: 31.6 us and 32.5). Else it is four, whose accesses lie closer together.
+// THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.5 us,
+// with four waves 5.1; 600 k 5.3 and 6.6; 1.5 M 9.4 and 8.8), and with 8-bit moments of 16-bit parameters, where compute units that are
+// never idle count (16 M: 30.8 us and 32.6; 40 M 74.8 and 76.9). Else it is four, whose accesses lie closer together.
 template <int BITS, bool EXACT, int THREADS, class Launch>
 __global__ void __launch_bounds__(THREADS) adamw_step_kernel(const Launch a)
 {

@@ -480,7 +480,7 @@ inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<ui
 inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
 constexpr int64_t kOptimEntryElements = 1 << 27;  // a longer tensor is several entries of a launch: places inside one are 32 bits
-constexpr int64_t kOptimSmall         = 1500000;  // elements up to which workgroups of one wave are faster
+constexpr int64_t kOptimSmall         = 800000;   // elements up to which workgroups of one wave are faster
 constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 static_assert(std::max(kAdamWEntries, kMomentEntries) * (kOptimEntryElements / 8) < (int64_t)1 << 32, "threads of a launch are counted in 32 bits");
