@@ -3,6 +3,7 @@
 
 #include <cstring>
 #include <map>
+#include <utility>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -159,21 +160,24 @@ AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
     }
 }
 
-void AdamW::fill_master(const Slot& s)
+void AdamW::fill_master(const Slot& s, torch::Tensor& to)
 {
     // in the parameter's order of memory
-    master.narrow(0, s.first, s.n).copy_(s.param.detach().as_strided({s.n}, {1}));
+    to.narrow(0, s.first, s.n).copy_(s.param.detach().as_strided({s.n}, {1}));
 }
 
-// Room in the flat state for every parameter as it is now. What a parameter of unchanged size had moves along.
+// Room in the flat state for every parameter as it is now. What a parameter of unchanged size had moves along. Nothing of the object
+// changes before everything that may throw is done (a parameter that is refused, memory that runs out while both states are there):
+// places and lengths are what the kernels go by, and always those of the arrays that are there.
 void AdamW::lay_out()
 {
     torch::NoGradGuard no_grad;
+    std::vector<Slot> slots = slots_;
+    std::vector<int64_t> from(slots.size(), -1);
     int64_t at = 0;
-    std::vector<int64_t> from(slots_.size(), -1);
-    for (size_t k = 0; k < slots_.size(); ++k)
+    for (size_t k = 0; k < slots.size(); ++k)
     {
-        Slot& s = slots_[k];
+        Slot& s = slots[k];
         check_on(s.param, device_, "AdamW: parameters");
         TORCH_CHECK(dense(s.param), "AdamW: parameters must be dense, without gaps or overlaps");
         if (s.n == s.param.numel()) from[k] = s.first;
@@ -182,27 +186,46 @@ void AdamW::lay_out()
         s.first = at;
         at += whole_blocks(s.n);
     }
-    const auto bytes     = torch::TensorOptions(device_).dtype(torch::kUInt8);
-    const auto floats    = torch::TensorOptions(device_).dtype(torch::kFloat32);
-    const bool eight     = options_.moment_bits == 8;
-    const auto old_m     = exp_avg, old_v = exp_avg_sq, old_scale = block_scale, old_master = master;
-    exp_avg              = torch::zeros({at}, eight ? bytes : floats);
-    exp_avg_sq           = torch::zeros({at}, eight ? bytes : floats);
-    if (eight) block_scale = torch::zeros({at / kBlock, 2}, bytes);
-    if (options_.master_weights) master = torch::zeros({at}, floats);
-    for (size_t k = 0; k < slots_.size(); ++k)
+    const auto bytes  = torch::TensorOptions(device_).dtype(torch::kUInt8);
+    const auto floats = torch::TensorOptions(device_).dtype(torch::kFloat32);
+    const bool eight  = options_.moment_bits == 8;
+    torch::Tensor m   = torch::zeros({at}, eight ? bytes : floats);
+    torch::Tensor v   = torch::zeros({at}, eight ? bytes : floats);
+    torch::Tensor scales, masters;
+    if (eight) scales = torch::zeros({at / kBlock, 2}, bytes);
+    if (options_.master_weights) masters = torch::zeros({at}, floats);
+    for (size_t k = 0; k < slots.size(); ++k)
     {
-        const Slot& s   = slots_[k];
+        const Slot& s   = slots[k];
         const int64_t n = whole_blocks(s.n);
         if (from[k] >= 0 && n > 0)
         {
-            exp_avg.narrow(0, s.first, n).copy_(old_m.narrow(0, from[k], n));
-            exp_avg_sq.narrow(0, s.first, n).copy_(old_v.narrow(0, from[k], n));
-            if (eight) block_scale.narrow(0, s.first / kBlock, n / kBlock).copy_(old_scale.narrow(0, from[k] / kBlock, n / kBlock));
-            if (master.defined()) master.narrow(0, s.first, n).copy_(old_master.narrow(0, from[k], n));
+            m.narrow(0, s.first, n).copy_(exp_avg.narrow(0, from[k], n));
+            v.narrow(0, s.first, n).copy_(exp_avg_sq.narrow(0, from[k], n));
+            if (eight) scales.narrow(0, s.first / kBlock, n / kBlock).copy_(block_scale.narrow(0, from[k] / kBlock, n / kBlock));
+            if (masters.defined()) masters.narrow(0, s.first, n).copy_(master.narrow(0, from[k], n));
         }
-        else if (master.defined()) fill_master(s);
+        else if (masters.defined()) fill_master(s, masters);
     }
+    slots_.swap(slots);
+    exp_avg     = std::move(m);
+    exp_avg_sq  = std::move(v);
+    block_scale = std::move(scales);
+    master      = std::move(masters);
+    elements_   = at;
+}
+
+// The kernels go by the layout, not by the arrays' lengths, and the arrays are open to the caller.
+void AdamW::check_state() const
+{
+    const auto fits = [&](const torch::Tensor& t, bool there, torch::ScalarType type, int64_t n) {
+        return there ? t.defined() && t.device() == device_ && t.scalar_type() == type && t.is_contiguous() && t.numel() == n : !t.defined();
+    };
+    const bool eight = options_.moment_bits == 8;
+    const auto type  = eight ? torch::kUInt8 : torch::kFloat32;
+    TORCH_CHECK(fits(exp_avg, true, type, elements_) && fits(exp_avg_sq, true, type, elements_) && fits(block_scale, eight, torch::kUInt8, elements_ / kBlock * 2) &&
+                    fits(master, options_.master_weights, torch::kFloat32, elements_),
+                "AdamW: a state tensor is not the one that was laid out: copy into it, and leave its size and type as they are");
 }
 
 // A new layout if a parameter has changed its size.
@@ -220,6 +243,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(options_.capturable || !capturing(), "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
+    check_state();
     follow_sizes();
     const bool eight = options_.moment_bits == 8;
     tensors_.clear();
@@ -358,6 +382,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
+    check_state();
     follow_sizes();
     std::vector<torch::Tensor> kept[2];
     for (size_t k = 0; k < slots_.size(); ++k)
@@ -390,12 +415,13 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
 void AdamW::reload_master()
 {
     torch::NoGradGuard no_grad;
-    if (!master.defined()) return;
+    if (!options_.master_weights) return;
     c10::DeviceGuard guard(device_);
+    check_state();
     for (auto& s : slots_)
     {
         TORCH_CHECK(s.param.numel() == s.n && dense(s.param), "AdamW: a parameter has changed its size; step() notices that by itself");
-        fill_master(s);
+        fill_master(s, master);
     }
 }
 

@@ -76,12 +76,14 @@ class AdamW
     };
     void lay_out();
     void follow_sizes();
-    void fill_master(const Slot& s);
+    void check_state() const;
+    static void fill_master(const Slot& s, torch::Tensor& to);
     std::vector<Slot> slots_;
     std::vector<double> lr_, weight_decay_;
     Options options_;
     torch::Device device_ = torch::kCPU;
     torch::Tensor device_state_;
+    int64_t elements_ = 0;  // of the flat state
     std::vector<vetrast_adamw_tensor> tensors_;  // of the call under way
     std::vector<vetrast_adamw_group> groups_;
     std::vector<int64_t> group_of_;
