@@ -95,3 +95,158 @@ def test_state_tensors_of_another_size_are_refused(bits):
         t.resize_(n)
     opt.step()
     assert opt.steps() == [1]
+
+
+# ---- parameters whose order in memory changes --------------------------------------------------------------------------
+
+def channels_last(t):
+    return t.contiguous(memory_format=torch.channels_last)
+
+
+def turned(t):
+    return t.transpose(0, 3).contiguous().transpose(0, 3)
+
+
+def turn(p, order):
+    """What net.to(memory_format=...) does: the same tensor object, with its elements and its gradient's in another order."""
+    p.data = order(p.data)
+    g, p.grad = p.grad, None
+    p.grad = order(g)
+
+
+def by_index(flat, p):
+    """Elements in the order of p's memory, in the order of p's indices."""
+    return flat.as_strided(p.shape, p.stride()).contiguous().reshape(-1)
+
+
+@pytest.mark.parametrize("dtype,masters", [(torch.float32, False), (torch.bfloat16, True), (torch.bfloat16, False)], ids=["f32", "bf16 masters", "bf16"])
+def test_state_follows_another_order_in_memory(dtype, masters):
+    """A twin that keeps its order takes the same steps, before and after, there and back and over an order of its own; also where another
+    parameter changes its size at the same time."""
+    shapes = [(9,), (6, 5, 3, 4), (2, 3, 1, 5)]
+    ps, qs = ([parameter(s, dtype, 90 + k) for k, s in enumerate(shapes)] for _ in range(2))
+    a, b = (torch_ops.AdamW([(x, 0.01, 0.1)], master_weights=masters) for x in (ps, qs))
+    for k, order in enumerate((torch.clone, channels_last, turned, channels_last, torch.Tensor.contiguous)):
+        for p in ps[1:]:
+            turn(p, order)
+        if k == 2:
+            for x in (ps, qs):
+                grow(x[0], (1000,), 4)
+        arrays = [t.data_ptr() for t in states(a)]
+        for _ in range(2):
+            a.step(zero_grad=False)
+            b.step(zero_grad=False)
+        assert k == 2 or arrays == [t.data_ptr() for t in states(a)]
+        assert a.layout() == b.layout() and a.steps() == b.steps()
+        for p, q, (f, n) in zip(ps, qs, a.layout()):
+            assert torch.equal(p, q)
+            for x, y in zip(states(a), states(b)):
+                assert torch.equal(by_index(x[f:f + n], p), by_index(y[f:f + n], q)) and x[f:f + n].any()
+            p.grad.mul_(-0.7)
+            q.grad.mul_(-0.7)
+
+
+@pytest.mark.parametrize("masters", [False, True])
+def test_codes_follow_another_order_in_memory(masters):
+    """Their blocks get other elements: moments are within half a code of what they were, and the step is the definition's from there."""
+    dtype = torch.bfloat16 if masters else torch.float32
+    p = parameter((16, 5, 3, 4), dtype, 95)
+    opt = torch_ops.AdamW([([p], 0.01, 0.1)], moment_bits=8, master_weights=masters, seed=2)
+    for _ in range(2):
+        opt.step()
+    was = [by_index(t, p) for t in opt.moments()]
+    turn(p, channels_last)
+    m, v = opt.moments()
+    unit = np.exp2(numbers(opt.block_scale) - 127.0)
+    for k, (x, y) in enumerate(zip((m, v), was)):
+        want = numbers(torch.empty_like(p, dtype=torch.float32).copy_(y.view(p.shape)).permute(0, 2, 3, 1).reshape(-1))
+        u = np.repeat(unit[:, k], 128)[:960]
+        assert (np.abs(numbers(x)[:960] - want) <= (np.abs(want) + u) / 16 * 1.0001 + (u / 8 if k else 0)).all() and not x[960:].any()
+    memory = lambda t: t.detach().permute(0, 2, 3, 1).reshape(-1)  # noqa: E731
+    held_p = (opt.master[:960] if masters else memory(p)).clone()
+    want, *_, tol, _, _ = om.step64(numbers(held_p), numbers(memory(p.grad)), numbers(m)[:960], numbers(v)[:960], 3, 0.01, 0.1)
+    opt.step()
+    held_p = opt.master[:960] if masters else memory(p)
+    assert (np.abs(numbers(held_p) - want) <= tol).all()
+    assert not masters or torch.equal(memory(p), held_p.to(dtype))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_orders_that_are_one_move_nothing(bits):
+    """Strides of dimensions of one element, and shapes of contiguous parameters."""
+    p = parameter((40, 7, 1, 1), seed=96)
+    opt = torch_ops.AdamW([([p], 0.01)], moment_bits=bits)
+    opt.step()
+    was = [t.clone() for t in states(opt)]
+    for data in (channels_last(p.data), p.data.as_strided(p.shape, (7, 1, 5, 9)), p.data.reshape(7, 40), p.data.reshape(-1), p.data.reshape(4, 7, 2, 5)):
+        p.data = data
+        opt.moments()
+        assert all(torch.equal(x, y) for x, y in zip(was, states(opt)))
+    p.grad = None
+    p.grad = torch.ones_like(p)
+    turn(p, channels_last)
+    opt.step()
+    assert opt.steps() == [2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_another_shape_in_another_order_is_refused(bits):
+    p = parameter((5, 3), seed=97)
+    opt = torch_ops.AdamW([([p], 0.01)], moment_bits=bits)
+    opt.step()
+    before, data, grad = held(opt), p.data, p.grad
+    p.grad = None
+    p.data = data.t()
+    p.grad = grad.t()
+    was = p.detach().clone()
+    for call in (opt.step, opt.moments, lambda: opt.load_moments([grad], [grad], 1)):
+        with pytest.raises(RuntimeError, match="shape and the order"):
+            call()
+    assert torch.equal(p, was) and same(before, held(opt))
+    p.grad = None
+    p.data = data
+    p.grad = grad
+    opt.step()
+    assert opt.steps() == [2]
+
+
+def test_masters_and_moments_are_taken_over_in_the_present_order():
+    p = parameter((6, 5, 3, 4), torch.bfloat16, 98)
+    opt = torch_ops.AdamW([([p], 0.01)], master_weights=True)
+    opt.step()
+    turn(p, channels_last)
+    opt.reload_master()
+    memory = p.detach().permute(0, 2, 3, 1).reshape(-1)
+    assert torch.equal(opt.master[:360], memory.float())
+    m, v = torch.rand(6, 5, 3, 4, device="cuda"), torch.rand(6, 5, 3, 4, device="cuda")
+    turn(p, torch.Tensor.contiguous)
+    opt.load_moments([m], [v], 4)
+    assert torch.equal(opt.exp_avg[:360], m.reshape(-1)) and torch.equal(opt.exp_avg_sq[:360], v.reshape(-1))
+    assert torch.equal(opt.master[:360], p.detach().float().reshape(-1))
+
+
+def test_a_captured_step_needs_the_order_that_it_found():
+    """With the count on the device the state follows in place, but not inside a graph, which would turn it again with every replay."""
+    p, q = (parameter((6, 5, 3, 4), seed=99) for _ in range(2))
+    a, b = (torch_ops.AdamW([([x], 0.01)], capturable=True) for x in (p, q))
+    a.step()
+    b.step()
+    turn(p, channels_last)
+    before, was = held(a), p.detach().clone()
+    with pytest.raises(RuntimeError, match="order in memory"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            a.step()
+    torch.cuda.synchronize()
+    assert same(before, held(a)) and torch.equal(p, was)
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for _ in range(4):
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
+        _ = torch.ones(1000, device="cuda").sum().item()
+    assert a.steps() == b.steps() == [6]

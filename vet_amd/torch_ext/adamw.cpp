@@ -96,6 +96,14 @@ bool same_order(const torch::Tensor& a, const torch::Tensor& b)
     return (a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides();
 }
 
+// Whether two orders of memory are one: strides of dimensions of one element say nothing.
+bool same_memory(at::IntArrayRef sizes, at::IntArrayRef a, at::IntArrayRef b)
+{
+    for (size_t d = 0; d < sizes.size(); ++d)
+        if (sizes[d] != 1 && a[d] != b[d]) return false;
+    return true;
+}
+
 // Moments of a list of tensors, placed one behind the other in flat arrays; `total`: elements of these.
 std::vector<vetrast_moment_tensor> moment_list(const TensorPointers& ms, const TensorPointers& vs, const torch::Device& device, int64_t& total)
 {
@@ -141,7 +149,11 @@ AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
             TORCH_CHECK(p.defined() && p.is_cuda(), "AdamW: parameters must be tensors on the GPU");
             if (slots_.empty()) device_ = p.device();
             for (auto& s : slots_) TORCH_CHECK(!s.param.is_same(p), "AdamW: a parameter is in the list twice");
-            slots_.push_back({p, (int)lr_.size(), type_of(p, "AdamW: parameters"), 0, -1, 0});
+            Slot s;
+            s.param = p;
+            s.group = (int)lr_.size();
+            s.type  = type_of(p, "AdamW: parameters");
+            slots_.push_back(std::move(s));
         }
         lr_.push_back(g.lr);
         weight_decay_.push_back(g.weight_decay);
@@ -181,7 +193,11 @@ void AdamW::lay_out()
         check_on(s.param, device_, "AdamW: parameters");
         TORCH_CHECK(dense(s.param), "AdamW: parameters must be dense, without gaps or overlaps");
         if (s.n == s.param.numel()) from[k] = s.first;
-        else s.step = 0;
+        else
+        {
+            s.step = 0;
+            take_order(s);
+        }
         s.n     = s.param.numel();
         s.first = at;
         at += whole_blocks(s.n);
@@ -228,14 +244,76 @@ void AdamW::check_state() const
                 "AdamW: a state tensor is not the one that was laid out: copy into it, and leave its size and type as they are");
 }
 
-// A new layout if a parameter has changed its size.
-void AdamW::follow_sizes()
+void AdamW::take_order(Slot& s)
+{
+    s.sizes   = s.param.sizes().vec();
+    s.strides = s.param.strides().vec();
+    s.rows    = s.param.is_contiguous();
+}
+
+// What the state of a parameter has in the order of memory that the parameter had, in the order that it has now (a network that was
+// turned to channels last, say). An element keeps its index. All is made aside first, as copies in place need no memory.
+void AdamW::reorder(Slot& s)
+{
+    const auto turned = [&](const torch::Tensor& flat) {
+        torch::Tensor to = torch::empty_strided(s.sizes, s.param.strides(), flat.options());
+        return to.copy_(flat.as_strided(s.sizes, s.strides)).as_strided({s.n}, {1});
+    };
+    const auto place     = [&](const torch::Tensor& array) { return array.narrow(0, s.first, s.n); };
+    torch::Tensor masters = master.defined() ? turned(place(master)) : master;
+    if (options_.moment_bits == 32)
+    {
+        const torch::Tensor m = turned(place(exp_avg)), v = turned(place(exp_avg_sq));
+        place(exp_avg).copy_(m);
+        place(exp_avg_sq).copy_(v);
+    }
+    else
+    {
+        // blocks get other elements, so codes are made anew, rounded to nearest; a lost block's elements lose the blocks that they come to
+        const auto floats = torch::TensorOptions(device_).dtype(torch::kFloat32);
+        torch::Tensor m = torch::empty({s.n}, floats), v = torch::empty({s.n}, floats);
+        const auto convert = [&](decltype(vetrast_pack_moments)& call, const char* where) {
+            const std::vector<vetrast_moment_tensor> list{{m.data_ptr<float>(), v.data_ptr<float>(), s.n, s.first}};
+            const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);
+            check(call(context_on(device_), &a, stream_on(device_)), where);
+        };
+        convert(vetrast_unpack_moments, "unpack_moments");
+        m = turned(m);
+        v = turned(v);
+        convert(vetrast_pack_moments, "pack_moments");
+    }
+    if (masters.defined()) place(master).copy_(masters);
+}
+
+// The state follows a parameter of unchanged size to another order in memory.
+void AdamW::follow_orders()
+{
+    for (auto& s : slots_)
+    {
+        const torch::Tensor& p = s.param;
+        if (p.sizes() == s.sizes && p.strides() == s.strides) continue;
+        if (p.numel() != s.n || !dense(p)) continue;  // laid out anew or refused where it is stepped
+        if (!(p.is_contiguous() && s.rows) && !(p.sizes() == s.sizes && same_memory(s.sizes, p.strides(), s.strides)))
+        {
+            TORCH_CHECK(p.sizes() == s.sizes, "AdamW: a parameter has changed its shape and the order of its elements in memory, it needs an optimiser of its own");
+            TORCH_CHECK(!capturing(), "AdamW: a parameter has changed its order in memory, take a step before the one that is captured");
+            reorder(s);
+        }
+        take_order(s);
+    }
+}
+
+// A new layout if a parameter has changed its size, and what it holds in the parameters' order.
+void AdamW::follow_parameters()
 {
     bool moved = false;
     for (auto& s : slots_) moved |= s.param.numel() != s.n;
-    if (!moved) return;
-    TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
-    lay_out();
+    if (moved)
+    {
+        TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
+        lay_out();
+    }
+    follow_orders();
 }
 
 void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
@@ -244,7 +322,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(options_.capturable || !capturing(), "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
     check_state();
-    follow_sizes();
+    follow_parameters();
     const bool eight = options_.moment_bits == 8;
     tensors_.clear();
     groups_.clear();
@@ -371,8 +449,12 @@ std::vector<std::pair<int64_t, int64_t>> AdamW::layout() const
     return r;
 }
 
-std::tuple<torch::Tensor, torch::Tensor> AdamW::moments() const
+std::tuple<torch::Tensor, torch::Tensor> AdamW::moments()
 {
+    torch::NoGradGuard no_grad;
+    c10::DeviceGuard guard(device_);
+    check_state();
+    follow_orders();
     if (options_.moment_bits == 32) return {exp_avg, exp_avg_sq};
     return UnpackMoments(exp_avg, exp_avg_sq, block_scale);
 }
@@ -383,7 +465,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
     check_state();
-    follow_sizes();
+    follow_parameters();
     std::vector<torch::Tensor> kept[2];
     for (size_t k = 0; k < slots_.size(); ++k)
         for (int which = 0; which < 2; ++which)
@@ -419,10 +501,9 @@ void AdamW::reload_master()
     c10::DeviceGuard guard(device_);
     check_state();
     for (auto& s : slots_)
-    {
         TORCH_CHECK(s.param.numel() == s.n && dense(s.param), "AdamW: a parameter has changed its size; step() notices that by itself");
-        fill_master(s, master);
-    }
+    follow_orders();
+    for (auto& s : slots_) fill_master(s, master);
 }
 
 torch::Tensor GradNorm(const TensorPointers& gradients, double max_norm, double scale)

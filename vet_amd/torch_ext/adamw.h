@@ -39,7 +39,8 @@ class AdamW
     // One step on every parameter that has a gradient. grad_scale: float32 on the GPU, one element or the two that GradNorm
     // returns (the last counts); where it is not finite, parameters, moments and the device's step count stay as they are (a count
     // on the host goes up all the same: it does not see the device).
-    // A parameter whose number of elements has changed starts anew, as MyAdam does.
+    // A parameter whose number of elements has changed starts anew, as MyAdam does. The state of one that has changed its order in memory
+    // follows it: an element keeps its index. 8-bit moments are rounded to nearest once more by that.
     void step(bool zero_grad = false, const std::optional<torch::Tensor>& grad_scale = std::nullopt);
     void zero_grad();
     // GradNorm of the parameters' gradients.
@@ -51,15 +52,17 @@ class AdamW
     void set_step(int64_t step);
     // First element and number of elements of every parameter in the flat state tensors.
     std::vector<std::pair<int64_t, int64_t>> layout() const;
-    // Both moments as flat float32 tensors laid out like the state (the state itself where it is float32).
-    std::tuple<torch::Tensor, torch::Tensor> moments() const;
+    // Both moments as flat float32 tensors laid out like the state (the state itself where it is float32), in the order of memory that
+    // the parameters have now.
+    std::tuple<torch::Tensor, torch::Tensor> moments();
     // Takes over float32 moments, two tensors a parameter, from a run with either kind of state: of the parameter's shape, or flat in
     // the order of its memory.
     void load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, int64_t step);
     // Masters are read from the parameters again (after a checkpoint was loaded into these).
     void reload_master();
 
-    // The state, flat: every parameter starts at a multiple of VETRAST_MOMENT_BLOCK elements. exp_avg and exp_avg_sq are float32,
+    // The state, flat: every parameter starts at a multiple of VETRAST_MOMENT_BLOCK elements, and has its own in the order of memory that
+    // it had at the last call of step, moments, load_moments or reload_master. exp_avg and exp_avg_sq are float32,
     // or uint8 codes with block_scale uint8 [blocks, 2]; master is float32 or undefined. They are other tensors after a step or
     // load_moments that found a parameter of another size.
     torch::Tensor exp_avg, exp_avg_sq, block_scale, master;
@@ -72,10 +75,15 @@ class AdamW
         torch::Tensor param;
         int group     = 0;
         int32_t type  = 0;
-        int64_t first = 0, n = 0, step = 0;
+        int64_t first = 0, n = -1, step = 0;
+        std::vector<int64_t> sizes, strides;  // of the parameter when its state was put in order
+        bool rows = true;                     // it was contiguous
     };
     void lay_out();
-    void follow_sizes();
+    static void take_order(Slot& s);
+    void reorder(Slot& s);
+    void follow_orders();
+    void follow_parameters();
     void check_state() const;
     static void fill_master(const Slot& s, torch::Tensor& to);
     std::vector<Slot> slots_;
