@@ -316,7 +316,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v)
     return max(v, dpp_move<0x121>(v));
 }
 
-// Scale byte D of a block whose largest magnitude has the float bits `largest`: its exponent less the binades that codes span, one
+// Scale byte D of a block whose largest magnitude has the float bits `largest`, without a sign: its exponent less the binades that codes span, one
 // more where rounding may carry (bits + 2^20 - 1 from rounding, and 2^8 from the offset 2^(D-127) at 15 binades). 255: not finite, or
 // so large that a code next to it would be infinite.
 template <int BINADES>
@@ -378,7 +378,7 @@ __device__ __forceinline__ Codes encode_moments(const float* m, const float* v, 
         top_m = fmaxf(top_m, fabsf(m[j]));
         top_v = max(top_v, __float_as_uint(v[j]));
     }
-    const uint32_t dv = code_base<31>(row_max(top_v));
+    const uint32_t dv = code_base<31>(row_max(top_v) & 0x7FFFFFFFu);  // a NaN may have the sign set, which is above all, and wraps there
     uint32_t dm       = code_base<15>(row_max(__float_as_uint(top_m)));
     if (dv == 255u)
     {
