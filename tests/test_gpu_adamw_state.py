@@ -250,3 +250,66 @@ def test_a_captured_step_needs_the_order_that_it_found():
         assert torch.equal(p, q)
         _ = torch.ones(1000, device="cuda").sum().item()
     assert a.steps() == b.steps() == [6]
+
+
+# ---- counts ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("by_moments", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_run_is_taken_up_with_every_parameters_count(bits, by_moments):
+    """After points were added one parameter is younger than the others, and one had no gradient at first: a run that is taken up from what
+    was saved goes on as the one that was never stopped."""
+    bits_of_copy = 32 if by_moments else bits  # float32 moments of an 8-bit run continue in 32 bits
+    ps = [parameter((4, 300), seed=110), parameter((77,), seed=111), parameter((6, 5), seed=112, gradient=False)]
+    opt = torch_ops.AdamW([(ps[:1], 0.01), (ps[1:], 0.02, 0.1)], moment_bits=bits, seed=6)
+    for _ in range(5):
+        opt.step()
+    grow(ps[0], (4, 450), 5)
+    ps[2].grad = torch.ones_like(ps[2])
+    opt.step()
+    opt.step()
+    saved = opt.steps()
+    assert saved == [2, 7, 2]
+    qs = [p.detach().clone().requires_grad_(True) for p in ps]
+    for p, q in zip(ps, qs):
+        q.grad = p.grad.clone()
+    copy = torch_ops.AdamW([(qs[:1], 0.01), (qs[1:], 0.02, 0.1)], moment_bits=bits_of_copy, seed=6)
+    if by_moments:
+        ms = [t.clone() for t in opt.moments()]
+        copy.load_moments(*([t[f:f + n] for f, n in opt.layout()] for t in ms), saved)
+    else:
+        for x, y in zip(states(copy), states(opt), strict=True):
+            x.copy_(y)
+        copy.set_step(saved)
+    assert copy.steps() == saved
+    before = [numbers(p).reshape(-1) for p in ps]
+    m, v = (numbers(t) for t in opt.moments())
+    lay = opt.layout()
+    opt.step()
+    copy.step()
+    assert opt.steps() == copy.steps() == [3, 8, 3]
+    for k, (p, q, (f, n)) in enumerate(zip(ps, qs, lay)):
+        rates = (0.01, 0.0) if k == 0 else (0.02, 0.1)
+        want, *_, tol, _, _ = om.step64(before[k], numbers(p.grad).reshape(-1), m[f:f + n], v[f:f + n], saved[k] + 1, *rates)
+        for x in (p, q):
+            assert (np.abs(numbers(x).reshape(-1) - want) <= tol).all()
+        assert bits != bits_of_copy or torch.equal(p, q)
+    assert bits != bits_of_copy or all(torch.equal(x, y) for x, y in zip(states(opt), states(copy)))
+
+
+def test_counts_are_checked():
+    ps = [parameter((30,), seed=113), parameter((5,), seed=114)]
+    ms = [torch.rand(30, device="cuda"), torch.rand(5, device="cuda")]
+    opt, fixed = (torch_ops.AdamW([(ps, 0.01)], capturable=c) for c in (False, True))
+    for o, bad in ((opt, [3]), (opt, []), (opt, [1, 2, 3]), (opt, [1, -1]), (fixed, [1, 2]), (fixed, [3]), (fixed, [-1, -1])):
+        for call in (lambda: o.set_step(bad), lambda: o.load_moments(ms, ms, bad)):
+            with pytest.raises(RuntimeError, match="count"):
+                call()
+        assert o.steps() == [0, 0] and not o.exp_avg.any() and not o.exp_avg_sq.any()
+    fixed.set_step([4, 4])
+    assert fixed.steps() == [4, 4] and fixed.device_step.item() == 4
+    fixed.load_moments(ms, ms, [6, 6])
+    opt.load_moments(ms, ms, [6, 0])
+    assert fixed.steps() == [6, 6] and opt.steps() == [6, 0] and torch.equal(opt.exp_avg, fixed.exp_avg) and opt.exp_avg.any()
+    opt.set_step(2)
+    assert opt.steps() == [2, 2]

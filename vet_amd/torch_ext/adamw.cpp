@@ -437,9 +437,24 @@ std::vector<int64_t> AdamW::steps() const
 
 void AdamW::set_step(int64_t step)
 {
-    TORCH_CHECK(step >= 0, "AdamW: steps are counted from 0");
-    for (auto& s : slots_) s.step = step;
-    if (options_.capturable) device_step.fill_(step);
+    set_step(std::vector<int64_t>(slots_.size(), step));
+}
+
+void AdamW::check_counts(const std::vector<int64_t>& steps) const
+{
+    TORCH_CHECK(steps.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but counts of ", steps.size());
+    for (int64_t n : steps)
+    {
+        TORCH_CHECK(n >= 0, "AdamW: steps are counted from 0");
+        TORCH_CHECK(!options_.capturable || n == steps[0], "AdamW: with capturable all parameters have one count");
+    }
+}
+
+void AdamW::set_step(const std::vector<int64_t>& steps)
+{
+    check_counts(steps);
+    if (options_.capturable) device_step.fill_(steps[0]);
+    for (size_t k = 0; k < slots_.size(); ++k) slots_[k].step = steps[k];
 }
 
 std::vector<std::pair<int64_t, int64_t>> AdamW::layout() const
@@ -461,9 +476,15 @@ std::tuple<torch::Tensor, torch::Tensor> AdamW::moments()
 
 void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, int64_t step)
 {
+    load_moments(exp_avgs, exp_avg_sqs, std::vector<int64_t>(slots_.size(), step));
+}
+
+void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, const std::vector<int64_t>& steps)
+{
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
+    check_counts(steps);
     check_state();
     follow_parameters();
     std::vector<torch::Tensor> kept[2];
@@ -480,7 +501,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
         }
     int64_t total                           = 0;
     std::vector<vetrast_moment_tensor> list = moment_list(pointers(kept[0]), pointers(kept[1]), device_, total);
-    set_step(step);
+    set_step(steps);
     if (options_.moment_bits == 8)
     {
         const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);

@@ -49,15 +49,18 @@ class AdamW
     void set_lr(int64_t group, double lr);
     // Steps done by every parameter; with capturable, all have the device's count (this waits for the device).
     std::vector<int64_t> steps() const;
+    // One count for all, or one a parameter as steps() gives them: those that began later have smaller ones.
     void set_step(int64_t step);
+    void set_step(const std::vector<int64_t>& steps);
     // First element and number of elements of every parameter in the flat state tensors.
     std::vector<std::pair<int64_t, int64_t>> layout() const;
     // Both moments as flat float32 tensors laid out like the state (the state itself where it is float32), in the order of memory that
     // the parameters have now.
     std::tuple<torch::Tensor, torch::Tensor> moments();
     // Takes over float32 moments, two tensors a parameter, from a run with either kind of state: of the parameter's shape, or flat in
-    // the order of its memory.
+    // the order of its memory. Counts as for set_step.
     void load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, int64_t step);
+    void load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::vector<torch::Tensor>& exp_avg_sqs, const std::vector<int64_t>& steps);
     // Masters are read from the parameters again (after a checkpoint was loaded into these).
     void reload_master();
 
@@ -85,6 +88,7 @@ class AdamW
     void follow_orders();
     void follow_parameters();
     void check_state() const;
+    void check_counts(const std::vector<int64_t>& steps) const;
     static void fill_master(const Slot& s, torch::Tensor& to);
     std::vector<Slot> slots_;
     std::vector<double> lr_, weight_decay_;

@@ -1265,6 +1265,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def("step", &vet_amd::MyAdam::step, pybind11::arg("zero_grad") = false)
         .def("zero_grad", &vet_amd::MyAdam::zero_grad);
     using vet_amd::AdamW;
+    using Tensors = std::vector<torch::Tensor>;
     pybind11::class_<AdamW>(m, "AdamW")
         .def(pybind11::init([](std::vector<std::tuple<std::vector<torch::Tensor>, double, double>> groups, double beta1,
                                double beta2, double eps, int moment_bits, bool master_weights, bool stochastic_rounding,
@@ -1282,10 +1283,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def("grad_norm", &AdamW::grad_norm, pybind11::arg("max_norm") = 0.0, pybind11::arg("scale") = 1.0)
         .def("set_lr", &AdamW::set_lr, pybind11::arg("group"), pybind11::arg("lr"))
         .def("steps", &AdamW::steps)
-        .def("set_step", &AdamW::set_step, pybind11::arg("step"))
+        .def("set_step", pybind11::overload_cast<int64_t>(&AdamW::set_step), pybind11::arg("step"))
+        .def("set_step", pybind11::overload_cast<const std::vector<int64_t>&>(&AdamW::set_step), pybind11::arg("step"))
         .def("layout", &AdamW::layout)
         .def("moments", &AdamW::moments)
-        .def("load_moments", &AdamW::load_moments, pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
+        .def("load_moments", pybind11::overload_cast<const Tensors&, const Tensors&, int64_t>(&AdamW::load_moments), pybind11::arg("exp_avgs"),
+             pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
+        .def("load_moments", pybind11::overload_cast<const Tensors&, const Tensors&, const std::vector<int64_t>&>(&AdamW::load_moments),
+             pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
         .def("reload_master", &AdamW::reload_master)
         .def_readonly("exp_avg", &AdamW::exp_avg)
         .def_readonly("exp_avg_sq", &AdamW::exp_avg_sq)

@@ -69,10 +69,10 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
     be captured in a graph; device_step and lr_factor (on every group's rate) may be written between replays.
 
     step(zero_grad=False, grad_scale=None): grad_scale is one float32 on the GPU, or what grad_norm returned; where it is not
-    finite the step changes nothing (but clears gradients with zero_grad; a count on the host goes up). zero_grad(), grad_norm(max_norm, scale),
-    set_lr(group, lr), steps(), set_step(n), layout() -> [(first element, elements)] in the flat state tensors exp_avg,
-    exp_avg_sq, block_scale and master; moments() -> both as flat float32; load_moments(exp_avgs, exp_avg_sqs, step),
-    reload_master()."""
+    finite the step changes nothing (but clears gradients with zero_grad; a count on the host goes up). zero_grad(),
+    grad_norm(max_norm, scale), set_lr(group, lr), steps() -> a count for each parameter, set_step(n or such a list),
+    layout() -> [(first element, elements)] in the flat state tensors exp_avg, exp_avg_sq, block_scale and master; moments() ->
+    both as flat float32; load_moments(exp_avgs, exp_avg_sqs, n or a list of counts), reload_master()."""
     return load().AdamW([(list(g[0]), float(g[1]), float(g[2]) if len(g) > 2 else 0.0) for g in groups], beta1, beta2, eps,
                         int(moment_bits), bool(master_weights), bool(stochastic_rounding), int(seed), bool(capturable))
 
