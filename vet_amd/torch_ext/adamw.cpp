@@ -2,6 +2,7 @@
 #include "adamw.h"
 
 #include <cstring>
+#include <limits>
 #include <map>
 #include <utility>
 
@@ -140,7 +141,9 @@ AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
 {
     TORCH_CHECK(options.moment_bits == 32 || options.moment_bits == 8, "AdamW: moment_bits is 32 or 8, not ", options.moment_bits);
     TORCH_CHECK(options.beta1 >= 0 && options.beta1 < 1 && options.beta2 >= 0 && options.beta2 < 1, "AdamW: betas lie in [0, 1)");
-    TORCH_CHECK((float)options.eps > 0, "AdamW: eps must be above zero");
+    // as vetrast_adamw_step has it
+    TORCH_CHECK((float)options.eps >= std::numeric_limits<float>::min() && (float)options.eps <= std::numeric_limits<float>::max(),
+                "AdamW: eps must be a finite float32 of at least 2^-126, not ", options.eps);
     TORCH_CHECK(groups.size() <= VETRAST_ADAMW_MAX_GROUPS, "AdamW: at most ", VETRAST_ADAMW_MAX_GROUPS, " groups");
     for (auto& g : groups)
     {
