@@ -313,3 +313,18 @@ def test_counts_are_checked():
     assert fixed.steps() == [6, 6] and opt.steps() == [6, 0] and torch.equal(opt.exp_avg, fixed.exp_avg) and opt.exp_avg.any()
     opt.set_step(2)
     assert opt.steps() == [2, 2]
+
+
+def test_more_counts_than_groups_are_refused():
+    """Parameters of one group with counts of their own."""
+    ps = [torch.zeros(1, device="cuda", requires_grad=True) for _ in range(1025)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = torch_ops.AdamW([(ps, 0.5)])
+    opt.set_step(list(range(1025)))
+    with pytest.raises(RuntimeError, match="1025 groups"):
+        opt.step()
+    assert opt.steps() == list(range(1025)) and not any(p.any() for p in ps) and not opt.exp_avg.any()
+    opt.set_step([0, 0] + list(range(2, 1025)))
+    opt.step()
+    assert opt.steps() == [1, 1] + list(range(3, 1026)) and ps[0].item() == ps[1].item() == pytest.approx(-0.5)

@@ -365,6 +365,8 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         }
         tensors_.push_back({p.data_ptr(), gradient, s.n, s.first, type, type, (int32_t)place, 0});
     }
+    TORCH_CHECK(groups_.size() <= VETRAST_ADAMW_MAX_GROUPS, "AdamW: ", groups_.size(), " groups, as parameters of one count, rate and decay each are one, and at most ",
+                VETRAST_ADAMW_MAX_GROUPS, " are possible");
     vetrast_adamw_args a;
     std::memset(&a, 0, sizeof(a));
     a.tensors             = tensors_.data();

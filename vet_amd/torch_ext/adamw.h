@@ -41,6 +41,7 @@ class AdamW
     // on the host goes up all the same: it does not see the device).
     // A parameter whose number of elements has changed starts anew, as MyAdam does. The state of one that has changed its order in memory
     // follows it: an element keeps its index. 8-bit moments are rounded to nearest once more by that.
+    // Parameters of one group that have different counts are several groups to the kernels: VETRAST_ADAMW_MAX_GROUPS in all.
     void step(bool zero_grad = false, const std::optional<torch::Tensor>& grad_scale = std::nullopt);
     void zero_grad();
     // GradNorm of the parameters' gradients.
