@@ -328,3 +328,22 @@ def test_more_counts_than_groups_are_refused():
     opt.set_step([0, 0] + list(range(2, 1025)))
     opt.step()
     assert opt.steps() == [1, 1] + list(range(3, 1026)) and ps[0].item() == ps[1].item() == pytest.approx(-0.5)
+
+
+# ---- parts of the state ------------------------------------------------------------------------------------------------
+
+def test_one_parameters_moments_are_read():
+    """Its codes and scales, which lie anywhere in the flat arrays."""
+    ms, vs = ([torch.rand(n, device="cuda") for n in (100, 300, 0, 1000, 1)] for _ in range(2))
+    codes = torch_ops.pack_moments(ms, vs)
+    whole, first = torch_ops.unpack_moments(*codes), 0
+    for x in ms:
+        end = first + -(-x.numel() // 128) * 128
+        part = torch_ops.unpack_moments(codes[0][first:end], codes[1][first:end], codes[2][first // 128:end // 128])
+        for a, b in zip(part, whole):
+            assert torch.equal(a, b[first:end])
+        first = end
+    moved = []  # at addresses of any byte
+    for t in codes:
+        moved.append(torch.zeros(t.numel() + 7, dtype=torch.uint8, device="cuda")[7:].view(t.shape).copy_(t))
+    assert all(torch.equal(a, b) for a, b in zip(torch_ops.unpack_moments(*moved), whole))

@@ -605,8 +605,12 @@ std::tuple<torch::Tensor, torch::Tensor> UnpackMoments(const torch::Tensor& exp_
                 "unpack_moments: whole blocks of ", kBlock, " codes with two scales each are needed");
     const auto floats = torch::TensorOptions(device).dtype(torch::kFloat32);
     torch::Tensor m = torch::empty({n}, floats), v = torch::empty({n}, floats);
+    if (n == 0) return {m, v};
     const std::vector<vetrast_moment_tensor> list{{m.data_ptr<float>(), v.data_ptr<float>(), n, 0}};
-    const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);
+    // flat arrays begin at multiples of 16 bytes; a part of one, such as the scales of one parameter, may not
+    const auto placed = [](const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); };
+    const torch::Tensor mc = placed(exp_avg), vc = placed(exp_avg_sq), scale = placed(block_scale);
+    const vetrast_moments_args a = moments_args(list, mc, vc, scale);
     check(vetrast_unpack_moments(context_on(device), &a, stream_on(device)), "unpack_moments");
     return {m, v};
 }

@@ -91,7 +91,8 @@ def pack_moments(exp_avgs, exp_avg_sqs):
 
 
 def unpack_moments(exp_avg, exp_avg_sq, block_scale):
-    """What codes and scales as AdamW(moment_bits=8) and pack_moments hold them stand for: two flat float32 tensors."""
+    """What codes and scales as AdamW(moment_bits=8) and pack_moments hold them stand for: two flat float32 tensors. Whole blocks of 128
+    codes, of one tensor as well as of all."""
     return load().unpack_moments(exp_avg, exp_avg_sq, block_scale)
 
 
