@@ -347,3 +347,22 @@ def test_one_parameters_moments_are_read():
     for t in codes:
         moved.append(torch.zeros(t.numel() + 7, dtype=torch.uint8, device="cuda")[7:].view(t.shape).copy_(t))
     assert all(torch.equal(a, b) for a, b in zip(torch_ops.unpack_moments(*moved), whole))
+
+
+# ---- streams -----------------------------------------------------------------------------------------------------------
+
+def test_norms_on_a_foreign_stream_keep_nothing():
+    """The handle of a stream that somebody else made may come back as another stream's: nothing is kept by it."""
+    gs = [torch.randn(300_001, device="cuda"), torch.ones(77, device="cuda")]
+    want = torch_ops.grad_norm(gs, 1.0)
+    for pooled in [torch.cuda.Stream() for _ in range(3)]:  # kept alive; foreign to torch in the second form
+        stream = torch.cuda.ExternalStream(pooled.cuda_stream)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        for _ in range(3):
+            with torch.cuda.stream(stream):
+                got = torch_ops.grad_norm(gs, 1.0)
+            stream.synchronize()
+            assert torch.equal(got, want)
+        del got
+        assert torch.cuda.memory_allocated() == before

@@ -31,7 +31,7 @@ bool capturing()
     return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
-// What a host thread keeps. A context serves one host thread at a time and belongs to a device, a norm's workspace serves one stream.
+// What a host thread keeps. A context serves one host thread at a time and belongs to a device, a norm's workspace serves one stream of torch's.
 struct Kept
 {
     std::map<int, vetrast_ctx*> contexts;
@@ -55,12 +55,17 @@ vetrast_ctx* context_on(const torch::Device& device)
     return ctx;
 }
 
-// Zeroed memory for vetrast_gradient_norm, which leaves it zeroed where that counts. A captured call has its own, cleared in the graph.
+// Zeroed memory for vetrast_gradient_norm, which leaves it zeroed where that counts. A captured call has its own, cleared in the graph, and
+// so has one on a stream that is not of torch's pool (its id is its handle): such a stream may be destroyed while its norm still runs,
+// and another that gets its handle would count in the same memory.
 torch::Tensor norm_workspace(const torch::Device& device, size_t bytes)
 {
     const auto options = torch::TensorOptions(device).dtype(torch::kUInt8);
-    if (capturing()) return torch::zeros({(int64_t)bytes}, options);
-    torch::Tensor& w = kept().workspaces[{device.index(), stream_on(device)}];
+    const auto stream  = c10::hip::getCurrentHIPStream(device.index());
+    void* handle       = (void*)stream.stream();
+    const bool foreign = handle != nullptr && (intptr_t)stream.id() == reinterpret_cast<intptr_t>(handle);
+    if (foreign || capturing()) return torch::zeros({(int64_t)bytes}, options);
+    torch::Tensor& w = kept().workspaces[{device.index(), handle}];
     if (!w.defined() || w.numel() < (int64_t)bytes) w = torch::zeros({(int64_t)bytes}, options);
     return w;
 }
