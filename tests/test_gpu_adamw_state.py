@@ -366,3 +366,54 @@ def test_norms_on_a_foreign_stream_keep_nothing():
             assert torch.equal(got, want)
         del got
         assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["freed with the object", "left for larger ones"])
+def test_state_that_another_stream_uses_is_not_given_out(bits, how):
+    """The optimiser was made on one stream and steps on another, which has not come to the step yet when the state is freed: its memory
+    is not handed out on the first stream meanwhile."""
+    p = parameter((3_000_001,), torch.bfloat16, 120)
+    opt = torch_ops.AdamW([([p], 0.01)], moment_bits=bits, master_weights=True, capturable=how == "freed with the object")
+    sizes = [(t.shape, t.dtype, t.data_ptr()) for t in states(opt)]
+    larger = torch.ones(5_000_000, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        if how == "freed with the object":
+            opt.step()
+            del opt
+        else:
+            p.data = larger
+            p.grad = None
+            p.grad = larger
+            opt.step()
+    busy = not side.query()
+    made = [torch.empty(shape, dtype=dtype, device="cuda") for shape, dtype, _ in sizes]
+    busy = busy and not side.query()
+    torch.cuda.synchronize()
+    assert busy and not {t.data_ptr() for t in made} & {address for *_, address in sizes}
+
+
+def test_an_optimiser_goes_from_stream_to_stream():
+    """With a wait in between, it steps as on one, captured or not."""
+    p, q = (parameter((100_000,), seed=121) for _ in range(2))
+    a, b = (torch_ops.AdamW([([x], 0.01)], moment_bits=8, capturable=True) for x in (p, q))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for k in range(9):
+        now, last = streams[k % 3], streams[(k - 1) % 3] if k else torch.cuda.current_stream()
+        now.wait_stream(last)
+        with torch.cuda.stream(now):
+            a.step()
+    torch.cuda.current_stream().wait_stream(streams[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    for _ in range(12):
+        b.step()
+    assert a.steps() == b.steps() == [12]
+    assert torch.equal(p, q) and all(torch.equal(x, y) for x, y in zip(states(a), states(b)))

@@ -6,6 +6,7 @@
 #include <map>
 #include <utility>
 
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -239,6 +240,18 @@ void AdamW::lay_out()
     elements_   = at;
 }
 
+// The arrays were allocated on one stream, and a caller may go on with another, after a wait for the first. When they are freed, here or
+// with the object, their memory must not be given out before what that other stream does with it has ended.
+void AdamW::use_on_stream()
+{
+    if (capturing()) return;  // a graph's memory is its owner's to keep
+    const c10::Stream stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device_.index()).unwrap();
+    if (stream_ == stream) return;
+    for (torch::Tensor* t : {&exp_avg, &exp_avg_sq, &block_scale, &master, &device_state_})
+        if (t->defined() && t->numel() > 0) t->record_stream(stream);
+    stream_ = stream;
+}
+
 // The kernels go by the layout, not by the arrays' lengths, and the arrays are open to the caller.
 void AdamW::check_state() const
 {
@@ -330,6 +343,7 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(options_.capturable || !capturing(), "AdamW: a step that is captured in a graph needs capturable, which keeps the step count on the device");
     check_state();
+    use_on_stream();
     follow_parameters();
     const bool eight = options_.moment_bits == 8;
     tensors_.clear();
@@ -463,7 +477,12 @@ void AdamW::check_counts(const std::vector<int64_t>& steps) const
 void AdamW::set_step(const std::vector<int64_t>& steps)
 {
     check_counts(steps);
-    if (options_.capturable) device_step.fill_(steps[0]);
+    if (options_.capturable)
+    {
+        c10::DeviceGuard guard(device_);
+        use_on_stream();
+        device_step.fill_(steps[0]);
+    }
     for (size_t k = 0; k < slots_.size(); ++k) slots_[k].step = steps[k];
 }
 
@@ -479,6 +498,7 @@ std::tuple<torch::Tensor, torch::Tensor> AdamW::moments()
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     check_state();
+    use_on_stream();
     follow_orders();
     if (options_.moment_bits == 32) return {exp_avg, exp_avg_sq};
     return UnpackMoments(exp_avg, exp_avg_sq, block_scale);
@@ -496,6 +516,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
     check_counts(steps);
     check_state();
+    use_on_stream();
     follow_parameters();
     std::vector<torch::Tensor> kept[2];
     for (size_t k = 0; k < slots_.size(); ++k)
@@ -531,6 +552,7 @@ void AdamW::reload_master()
     if (!options_.master_weights) return;
     c10::DeviceGuard guard(device_);
     check_state();
+    use_on_stream();
     for (auto& s : slots_)
         TORCH_CHECK(s.param.numel() == s.n && dense(s.param), "AdamW: a parameter has changed its size; step() notices that by itself");
     follow_orders();

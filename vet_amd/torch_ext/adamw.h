@@ -88,6 +88,7 @@ class AdamW
     void reorder(Slot& s);
     void follow_orders();
     void follow_parameters();
+    void use_on_stream();
     void check_state() const;
     void check_counts(const std::vector<int64_t>& steps) const;
     static void fill_master(const Slot& s, torch::Tensor& to);
@@ -96,6 +97,7 @@ class AdamW
     Options options_;
     torch::Device device_ = torch::kCPU;
     torch::Tensor device_state_;
+    std::optional<c10::Stream> stream_;  // that the arrays are known to be used on
     int64_t elements_ = 0;  // of the flat state
     std::vector<vetrast_adamw_tensor> tensors_;  // of the call under way
     std::vector<vetrast_adamw_group> groups_;
