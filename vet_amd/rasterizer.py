@@ -366,10 +366,11 @@ class Rasterizer:
         a.beta1, a.beta2, a.eps, a.moment_bits, a.seed = beta1, beta2, eps, moment_bits, seed
         a.stochastic_rounding, a.zero_grad = int(stochastic_rounding), int(zero_grad)
         if grad_scale is not None:
-            assert grad_scale.is_cuda and grad_scale.dtype == torch.float32
+            assert grad_scale.is_cuda and grad_scale.dtype == torch.float32 and grad_scale.numel() == 1
             a.grad_scale = grad_scale.data_ptr()
         if device_state is not None:
-            assert device_state.is_cuda and device_state.numel() >= self.lib.vetrast_adamw_device_state_bytes(len(groups))
+            assert device_state.is_cuda and device_state.is_contiguous() and device_state.dtype == torch.uint8
+            assert device_state.numel() >= self.lib.vetrast_adamw_device_state_bytes(len(groups))
             a.device_state = device_state.data_ptr()
         abi.check(self.lib.vetrast_adamw_step(self.ctx, C.byref(a), self._stream()), "adamw_step")
 
@@ -383,6 +384,8 @@ class Rasterizer:
         need = self.lib.vetrast_gradient_norm_workspace_bytes(gs, len(gradients))
         out = torch.empty(2, device="cuda") if out is None else out
         workspace = torch.zeros(need, dtype=torch.uint8, device="cuda") if workspace is None else workspace
+        assert out.is_cuda and out.is_contiguous() and out.dtype == torch.float32 and out.numel() >= 2
+        assert workspace.is_cuda and workspace.is_contiguous() and workspace.dtype == torch.uint8
         a.gradients, a.num_gradients, a.max_norm, a.scale = gs, len(gradients), max_norm, scale
         a.out, a.workspace, a.workspace_bytes = out.data_ptr(), workspace.data_ptr(), workspace.numel()
         abi.check(self.lib.vetrast_gradient_norm(self.ctx, C.byref(a), self._stream()), "gradient_norm")
