@@ -392,8 +392,8 @@ typedef struct vetrast_adamw_tensor
 {
     void* param;   /* device [n] of param_type, contiguous, aligned to its element; updated in place */
     void* grad;    /* device [n] of grad_type, the same; cleared with zero_grad */
-    int64_t n;     /* >= 0 */
-    int64_t first; /* its place in the flat arrays and, modulo 2^33, in the stream of random bits */
+    int64_t n;     /* >= 0, at most 2^38 */
+    int64_t first; /* below 2^38: its place in the flat arrays and, modulo 2^33, in the stream of random bits */
     int32_t param_type, grad_type; /* vetrast_dtype */
     int32_t group;
     int32_t reserved;
@@ -447,7 +447,7 @@ int vetrast_adamw_step(vetrast_ctx* ctx, const vetrast_adamw_args* args, void* s
 typedef struct vetrast_gradient
 {
     const void* grad; /* device [n], contiguous, aligned to its element */
-    int64_t n;
+    int64_t n;        /* >= 0, at most 2^38 */
     int32_t type; /* vetrast_dtype */
     int32_t reserved;
 } vetrast_gradient;
@@ -471,8 +471,8 @@ typedef struct vetrast_moment_tensor
 {
     float* exp_avg;    /* device [n], contiguous, aligned to 4 bytes */
     float* exp_avg_sq; /* the same; its magnitudes are taken */
-    int64_t n;
-    int64_t first;     /* place in the flat arrays, a multiple of VETRAST_MOMENT_BLOCK */
+    int64_t n;         /* >= 0, at most 2^38 */
+    int64_t first;     /* below 2^38: place in the flat arrays, a multiple of VETRAST_MOMENT_BLOCK */
 } vetrast_moment_tensor;
 typedef struct vetrast_moments_args
 {

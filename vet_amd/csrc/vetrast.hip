@@ -484,9 +484,10 @@ constexpr int64_t kOptimSmall         = 800000;   // elements up to which workgr
 constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 static_assert(std::max(kAdamWEntries, kMomentEntries) * (kOptimEntryElements / 8) < (int64_t)1 << 32, "threads of a launch are counted in 32 bits");
-inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays, whose blocks have numbers of 32 bits
+constexpr int64_t kOptimMaxElements   = (int64_t)1 << 38;  // of a tensor, and of the places in flat arrays, whose blocks have numbers of 32 bits
+inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays
 {
-    return first >= 0 && first % kMomentBlock == 0 && first < ((int64_t)1 << 38) && n <= ((int64_t)1 << 38);
+    return first >= 0 && first % kMomentBlock == 0 && first < kOptimMaxElements && n <= kOptimMaxElements;
 }
 
 // The launches of a norm.
@@ -1528,7 +1529,7 @@ size_t vetrast_gradient_norm_workspace_bytes(const vetrast_gradient* gradients, 
     int64_t entries = 0;
     for (int k = 0; k < num_gradients; ++k)
     {
-        if (gradients[k].n < 0) return 0;
+        if (gradients[k].n < 0 || gradients[k].n > kOptimMaxElements) return 0;
         entries += (gradients[k].n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
     return sizeof(NormWorkspace) + (size_t)std::max<int64_t>((entries + kNormEntries - 1) / kNormEntries, 1) * kNormGrid * sizeof(double);
@@ -1544,7 +1545,7 @@ int vetrast_gradient_norm(vetrast_ctx* ctx, const vetrast_gradient_norm_args* a,
     for (int k = 0; k < a->num_gradients; ++k)
     {
         const vetrast_gradient& g = a->gradients[k];
-        if (g.n < 0 || !is_dtype(g.type)) return VETRAST_ERR_INVALID_ARG;
+        if (g.n < 0 || g.n > kOptimMaxElements || !is_dtype(g.type)) return VETRAST_ERR_INVALID_ARG;
         if (g.n > 0 && (!g.grad || !aligned_to(g.grad, dtype_bytes(g.type)))) return VETRAST_ERR_INVALID_ARG;
         entries += (g.n + kOptimEntryElements - 1) / kOptimEntryElements;
     }
