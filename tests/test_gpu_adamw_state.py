@@ -417,3 +417,13 @@ def test_an_optimiser_goes_from_stream_to_stream():
         b.step()
     assert a.steps() == b.steps() == [12]
     assert torch.equal(p, q) and all(torch.equal(x, y) for x, y in zip(states(a), states(b)))
+
+
+def test_moments_come_in_pairs():
+    p = parameter((30,), seed=130)
+    opt = torch_ops.AdamW([([p], 0.01)])
+    ms = [torch.rand(30, device="cuda") for _ in range(2)]
+    for first, second in ((ms[:1], ms), (ms, ms[:1]), (ms[:1], [])):
+        with pytest.raises(RuntimeError, match="moments"):
+            opt.load_moments(first, second, 1)
+        assert opt.steps() == [0] and not opt.exp_avg.any()

@@ -514,6 +514,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(exp_avgs.size() == slots_.size(), "AdamW: ", slots_.size(), " parameters, but moments of ", exp_avgs.size());
+    TORCH_CHECK(exp_avg_sqs.size() == slots_.size(), "AdamW: as many second moments as first ones are needed, not ", exp_avg_sqs.size());
     check_counts(steps);
     check_state();
     use_on_stream();
@@ -522,7 +523,6 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
     for (size_t k = 0; k < slots_.size(); ++k)
         for (int which = 0; which < 2; ++which)
         {
-            TORCH_CHECK(k < exp_avg_sqs.size(), "AdamW: as many second moments as first ones are needed");
             const torch::Tensor &p = slots_[k].param, &x = which ? exp_avg_sqs[k] : exp_avgs[k];
             check_on(x, device_, "AdamW: moments");
             TORCH_CHECK(x.scalar_type() == torch::kFloat32, "AdamW: moments must be float32 tensors");
