@@ -427,3 +427,19 @@ def test_moments_come_in_pairs():
         with pytest.raises(RuntimeError, match="moments"):
             opt.load_moments(first, second, 1)
         assert opt.steps() == [0] and not opt.exp_avg.any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_of_a_parameter_with_gaps_are_refused(bits):
+    """It has no order in memory that they could be taken over in."""
+    p = parameter((6, 5, 3, 4), seed=131)
+    opt = torch_ops.AdamW([([p], 0.01)], moment_bits=bits)
+    was, before = p.data, held(opt)
+    p.data = torch.zeros(6, 5, 3, 8, device="cuda")[..., ::2]
+    for x in (torch.rand(6, 5, 3, 4, device="cuda"), torch.rand(360, device="cuda")):
+        with pytest.raises(RuntimeError, match="dense"):
+            opt.load_moments([x], [x], 1)
+        assert same(before, held(opt))
+    p.data = was
+    opt.load_moments([torch.rand(6, 5, 3, 4, device="cuda")], [torch.rand(360, device="cuda").view(6, 5, 3, 4)], 1)
+    assert opt.steps() == [1]

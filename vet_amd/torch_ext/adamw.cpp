@@ -524,6 +524,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
         for (int which = 0; which < 2; ++which)
         {
             const torch::Tensor &p = slots_[k].param, &x = which ? exp_avg_sqs[k] : exp_avgs[k];
+            TORCH_CHECK(dense(p), "AdamW: parameters must be dense, without gaps or overlaps");
             check_on(x, device_, "AdamW: moments");
             TORCH_CHECK(x.scalar_type() == torch::kFloat32, "AdamW: moments must be float32 tensors");
             TORCH_CHECK(x.sizes() == p.sizes() || (x.dim() == 1 && x.numel() == slots_[k].n), "AdamW: parameter ", k, " and its moments differ in shape");
