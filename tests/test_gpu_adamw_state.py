@@ -443,3 +443,19 @@ def test_moments_of_a_parameter_with_gaps_are_refused(bits):
     p.data = was
     opt.load_moments([torch.rand(6, 5, 3, 4, device="cuda")], [torch.rand(360, device="cuda").view(6, 5, 3, 4)], 1)
     assert opt.steps() == [1]
+
+
+def test_state_is_not_laid_out_in_a_captured_call():
+    """It would lie in the graph's memory, and be filled by replays only."""
+    p = parameter((30,), seed=132)
+    opt = torch_ops.AdamW([([p], 0.01)])
+    opt.step()
+    grow(p, (50,), 6)
+    before, ms = held(opt), [torch.rand(50, device="cuda")]
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.load_moments(ms, ms, 3)
+    torch.cuda.synchronize()
+    assert same(before, held(opt))
+    opt.load_moments(ms, ms, 3)
+    assert opt.steps() == [3] and opt.layout() == [(0, 50)] and torch.equal(opt.exp_avg[:50], ms[0])

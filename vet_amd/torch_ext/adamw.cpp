@@ -332,6 +332,7 @@ void AdamW::follow_parameters()
     if (moved)
     {
         TORCH_CHECK(!options_.capturable, "AdamW: parameters cannot change their size with capturable");
+        TORCH_CHECK(!capturing(), "AdamW: a parameter has changed its size, its state cannot be laid out in a captured call");  // in the graph's own memory
         lay_out();
     }
     follow_orders();
