@@ -49,7 +49,8 @@ struct RawEight
 };
 
 // Loads and stores of many bytes at addresses that are multiples of an element's size only: the same instructions as at multiples of 16,
-// a little slower where they straddle lines.
+// a little slower where they straddle lines (parameter and gradient one element on: 10 M float32 53.4 us and 53.6, with 8-bit moments 27.7
+// and 28.3; 16 M bf16 66.9 and 66.8, with 8-bit moments 27.9 and 32.2).
 typedef uint32_t LooseFour __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t LooseTwo __attribute__((ext_vector_type(2), aligned(2)));
 __device__ __forceinline__ uint4 load_four(const char* p)
@@ -553,7 +554,9 @@ struct AdamWChunk
     bool whole;      // all its elements are there
 };
 
-// Chunks of four kinds. In whole ones every thread has its eight elements, parameter and gradient of one width: their loads are straight code, all of them under way at once. `kAnyChunk` does for everything else.
+// Chunks of four kinds. In whole ones every thread has its eight elements, parameter and gradient of one width: their loads are straight code, all
+// of them under way at once. `kAnyChunk` does for everything else: tails, and gradients of another width, which move their bytes as
+// fast (16 M bf16 with float32 gradients 72.5 us, 5.3 TB/s, with 8-bit moments 34.1, 5.7; with bf16 gradients 66.9, 5.3, and 28.0, 5.7).
 enum ChunkKind
 {
     kFloatChunk,   // float32
@@ -718,14 +721,16 @@ __device__ __forceinline__ void adamw_chunk(const AdamWCommon& a, const AdamWChu
 
 // One pass over parameter, gradient and state, each read and written once.
 //   32 bits: bound by memory. 27.5 M float32 elements, 28 bytes each: 142 us, 5.4 TB/s.
-//   8 bits:  10 M float32 elements, 16 bytes each: 28.3 us, 5.7 TB/s, bound by memory. 40 M bf16 elements, 10 bytes each: 75 us, 5.4 TB/s; the
-//            same loads and stores with nothing in between 74 us, and the vector units are at work for 87 to 92 % of the time: 434
-//            instructions for a wave's 512 elements (549 before bits were taken out of words, medians and products by the
-//            instructions for them), of which roots, quotients and 32-bit products take four times as long as the others.
+//   8 bits:  10 M float32 elements, 16 bytes each: 28.0 us, 5.7 TB/s, bound by memory. 40 M bf16 elements, 10 bytes each: one tensor 73 to 76 us,
+//            5.3 to 5.5 TB/s, 291 tensors in two launches 49.6 and 34.9; the same loads and stores with nothing in between 74, 48.0 and 33.2.
+//            The vector units are at work for 82 to 92 % of the time: 435 instructions for a wave's 512 elements (549 before bits were
+//            taken out of words, medians and products by the instructions for them), of which roots, quotients and 32-bit
+//            products take four times as long as the others.
 // EXACT: eps is so small that roots of values below 2^-126 count.
-// THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.5 us,
-// with four waves 5.1; 600 k 5.3 and 6.6; 1.5 M 9.4 and 8.8), and with 8-bit moments of 16-bit parameters, where compute units that are
-// never idle count (16 M: 30.8 us and 32.6; 40 M 74.8 and 76.9). Else it is four, whose accesses lie closer together.
+// THREADS: a workgroup is one wave where the call is small, for then its waves spread over more compute units (100 k float32 elements: 3.8 us,
+// with four waves 5.2; 600 k 5.5 and 6.3; 800 k 6.0 and 6.5; 1 M 7.1 and 6.8; 1.5 M 8.9 and 8.6), and with 8-bit moments of 16-bit
+// parameters, where compute units that are never idle count (16 M: 29.1 us and 31.0; 40 M 72.7 and 75.4). Else it is four, whose accesses
+// lie closer together.
 template <int BITS, bool EXACT, int THREADS, class Launch>
 __global__ void __launch_bounds__(THREADS) adamw_step_kernel(const Launch a)
 {
@@ -814,7 +819,7 @@ __device__ __forceinline__ bool leave_sum(NormWorkspace* w, uint32_t number, uin
 
 // In 64 bits throughout: no square overflows or vanishes, and a sum of any length is good to the last bit of a float. The workgroup that is
 // the last of the call to leave its sum adds all of them, in the order of their numbers: one launch instead of two, 4 us of a host's time.
-// 27.5 M float32: 21.7 us, 5.1 TB/s. 100 k: 4.2 us, what a launch, a sum's way to memory, the count and the sums' way back take.
+// 27.5 M float32: 20.8 us, 5.3 TB/s. 100 k: 4.1 us, what a launch, a sum's way to memory, the count and the sums' way back take.
 template <int ENTRIES>
 __global__ void __launch_bounds__(kBlock) gradient_norm_kernel(const NormLaunch<ENTRIES> a)
 {
@@ -873,7 +878,7 @@ struct MomentLaunch
 };
 static_assert(sizeof(MomentLaunch) <= 4096, "kernel arguments");
 
-// 10 M elements: 17.0 us, 5.9 TB/s, bound by memory.
+// 10 M elements: 16.1 us, 6.2 TB/s, bound by memory.
 __device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
 {
     const uint32_t block = e.block + start / kMomentBlock;
@@ -901,7 +906,7 @@ __device__ __forceinline__ void pack_chunk(const MomentLaunch& a, const MomentEn
 }
 
 // Four elements' codes at a time, so that a wave's writes have no gaps, and past the L2, which holds none of what they write for long: 10 M
-// elements 24.9 us with eight a lane, 18.9 with four, 16.1 past the L2. `whole`: all of them are there.
+// elements 24.9 us with eight a lane, 18.9 with four, 15.8 past the L2. `whole`: all of them are there.
 __device__ __forceinline__ void unpack_chunk(const MomentLaunch& a, const MomentEntry& e, uint32_t start, bool whole)
 {
     const uint32_t block = e.block + start / kMomentBlock;

@@ -67,6 +67,7 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
     parameters have float32 masters with the optimiser. stochastic_rounding: bfloat16 parameters without masters are rounded
     by random bits, a function of `seed`, step and element. capturable: the step count lies on the device, so that steps may
     be captured in a graph; device_step and lr_factor (on every group's rate) may be written between replays.
+    A parameter that has changed its size starts anew, one that has changed its order in memory keeps its state.
 
     step(zero_grad=False, grad_scale=None): grad_scale is one float32 on the GPU, or what grad_norm returned; where it is not
     finite the step changes nothing (but clears gradients with zero_grad; a count on the host goes up). zero_grad(),
