@@ -459,3 +459,23 @@ def test_state_is_not_laid_out_in_a_captured_call():
     assert same(before, held(opt))
     opt.load_moments(ms, ms, 3)
     assert opt.steps() == [3] and opt.layout() == [(0, 50)] and torch.equal(opt.exp_avg[:50], ms[0])
+
+
+def test_a_parameter_without_a_gradient_may_change_shape_and_order():
+    """It stops no step of the others, and is refused once it is to be stepped."""
+    p, frozen = parameter((5, 3), seed=133), parameter((7, 4), seed=134, gradient=False)
+    opt = torch_ops.AdamW([([p, frozen], 0.01)])
+    opt.step()
+    frozen.data = frozen.data.t()
+    opt.step()
+    opt.moments()
+    assert opt.steps() == [2, 0]
+    frozen.grad = torch.ones_like(frozen)
+    with pytest.raises(RuntimeError, match="shape and the order"):
+        opt.step()
+    assert opt.steps() == [2, 0]
+    frozen.grad = None
+    frozen.data = frozen.data.t()
+    frozen.grad = torch.ones_like(frozen)
+    opt.step()
+    assert opt.steps() == [3, 1]

@@ -316,6 +316,7 @@ void AdamW::follow_orders()
         if (p.numel() != s.n || !dense(p)) continue;  // laid out anew or refused where it is stepped
         if (!(p.is_contiguous() && s.rows) && !(p.sizes() == s.sizes && same_memory(s.sizes, p.strides(), s.strides)))
         {
+            if (p.sizes() != s.sizes && !p.grad().defined()) continue;  // nothing is stepped, and with a gradient it is refused
             TORCH_CHECK(p.sizes() == s.sizes, "AdamW: a parameter has changed its shape and the order of its elements in memory, it needs an optimiser of its own");
             TORCH_CHECK(!capturing(), "AdamW: a parameter has changed its order in memory, take a step before the one that is captured");
             reorder(s);
