@@ -486,6 +486,29 @@ typedef struct vetrast_moments_args
 int vetrast_pack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream);
 int vetrast_unpack_moments(vetrast_ctx* ctx, const vetrast_moments_args* args, void* stream);
 
+/* ---- Dropout without a stored mask ---------------------------------------------------------------------------------
+ *   y[i] = (left out(i) ? 0 : x[i] * 65536 / (65536 - t)) + residual[i],   t = floor(65536 p + 1/2)
+ * in 32 bits, rounded once. Element i is left out where its 16 random bits are below t. They are those of Philox4x32 with
+ * seven rounds (Salmon et al., 2011) at the counter (i / 8, step), 64 bits each, under the key `seed`: of the four words that
+ * gives, word (i % 8) / 2, its lower half for even i. The backward pass is the same call on the upstream gradient, without a
+ * residual: nothing is kept between the two. p below 2^-17 leaves out nothing, from 1 - 2^-17 on everything is left out; what is left out is
+ * not looked at (a NaN there becomes 0). The same element of two calls with the same seed and step has the same bits: give
+ * every layer of a network a seed of its own and count steps. */
+typedef struct vetrast_dropout_args
+{
+    const void* x;        /* device [n], contiguous, aligned to its element */
+    const void* residual; /* the same, or NULL */
+    void* y;              /* the same; may be x or residual itself, and must not overlap them otherwise */
+    int64_t n;            /* >= 0, at most 2^38 */
+    int32_t type;         /* vetrast_dtype of all three */
+    int32_t reserved;
+    double p;             /* 0 .. 1 */
+    uint64_t seed, step;
+    const int64_t* device_step; /* optional, device: added to the step. For calls that are captured in a graph, whose replays
+                                   then differ as the caller counts on (vetrast_adamw_device_state.step does by itself) */
+} vetrast_dropout_args;
+int vetrast_dropout(vetrast_ctx* ctx, const vetrast_dropout_args* args, void* stream);
+
 /* Error lifting: adds the per-pixel error of one rendered view to every cell of the scene grid whose projection covers
  * the pixel. Replaces PointRendererCache::FillSceneGridWithLoss and its kernel FillSceneGridWithLossRasterize
  * (src/lib/rendering/RenderForward.cu:605-632,639-791; called once per view of a batch in the epoch before points are

@@ -175,6 +175,14 @@ class MomentsArgs(C.Structure):
     ]
 
 
+class DropoutArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+        ("n", C.c_int64), ("type", C.c_int32), ("reserved", C.c_int32),
+        ("p", C.c_double), ("seed", C.c_uint64), ("step", C.c_uint64), ("device_step", C.c_void_p),
+    ]
+
+
 class PackArgs(C.Structure):
     _fields_ = [
         ("num_points", C.c_int32),
@@ -267,6 +275,7 @@ SYMBOLS = {
     "vetrast_gradient_norm": (C.c_int, [C.c_void_p, C.POINTER(GradientNormArgs), C.c_void_p]),
     "vetrast_pack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
     "vetrast_unpack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
+    "vetrast_dropout": (C.c_int, [C.c_void_p, C.POINTER(DropoutArgs), C.c_void_p]),
     "vetrast_lift_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "vetrast_lift_workspace_bytes_for_image": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     "vetrast_lift_error": (C.c_int, [C.c_void_p, C.POINTER(LiftArgs), C.c_void_p]),

@@ -5,6 +5,7 @@ Run as `python -m vet_amd.build`. hipcc cross-compiles, so no GPU is needed.
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -18,7 +19,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-ffp-contract=off",
     "-munsafe-fp-atomics",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -27,13 +27,28 @@ HIPCC_FLAGS = [
 ]
 
 
+SOURCES = ["vetrast.hip", "entries.hip"]
+
+
 def build_library(verbose=True):
+    """The sources side by side, then one library of them."""
     os.makedirs(LIB_DIR, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc] + HIPCC_FLAGS + [os.path.join(CSRC, "vetrast.hip"), "-o", LIB_PATH]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    with tempfile.TemporaryDirectory() as objects:
+        running, names = [], []
+        for source in SOURCES:
+            names.append(os.path.join(objects, source + ".o"))
+            cmd = [hipcc] + HIPCC_FLAGS + ["-c", os.path.join(CSRC, source), "-o", names[-1]]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            running.append((cmd, subprocess.Popen(cmd)))
+        failed = [(cmd, status) for cmd, status in [(cmd, p.wait()) for cmd, p in running] if status != 0]
+        if failed:
+            raise subprocess.CalledProcessError(failed[0][1], failed[0][0])
+        cmd = [hipcc, "--offload-arch=gfx950", "-fPIC", "-shared"] + names + ["-o", LIB_PATH]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
     return LIB_PATH
 
 
@@ -56,7 +71,7 @@ def build_torch_extension(verbose=True):
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for i in inc + ["/opt/rocm/include", sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", i]
-    cmd += [os.path.join(HERE, "torch_ext", "point_render.cpp"), os.path.join(HERE, "torch_ext", "adamw.cpp"), "-o", TORCH_EXT_PATH,
+    cmd += [os.path.join(HERE, "torch_ext", name) for name in ("point_render.cpp", "adamw.cpp", "entries.cpp")] + ["-o", TORCH_EXT_PATH,
             f"-L{torch_lib}", f"-L{LIB_DIR}", "-lvetrast", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
             "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     if verbose:

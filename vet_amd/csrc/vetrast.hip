@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "common.h"
+#include "context.h"
 #include "forward_kernels.h"
 #include "sort_kernels.h"
 #include "build_kernels.h"
@@ -23,23 +24,6 @@
 #include "region_rule.h"
 
 using namespace vetrast;
-
-struct vetrast_ctx
-{
-    int device         = 0;
-    int profiling      = 0;
-    int last_hip_error = 0;
-    struct Span
-    {
-        int scope;
-        hipEvent_t start, stop;
-    };
-    std::vector<Span> spans;             // recorded since the last reset
-    std::vector<hipEvent_t> free_events;  // recycled events
-    float acc_ms[VETRAST_SCOPE_COUNT_]      = {};
-    int32_t acc_launches[VETRAST_SCOPE_COUNT_] = {};
-    char* lift_scratch = nullptr;  // this device's copy of the file-scope scratch array (vetrast_lift_error_static)
-};
 
 namespace
 {
@@ -66,53 +50,6 @@ inline size_t lift_sums_for(int64_t width, int64_t height)
     const size_t rows = (size_t)((height + kLiftRows - 1) / kLiftRows * kLiftRows);
     return std::min(kLiftSums, rows * ((size_t)width + 1));
 }
-
-#define VET_HIP(ctx, expr)                               \
-    do                                                   \
-    {                                                    \
-        hipError_t e_ = (expr);                          \
-        if (e_ != hipSuccess)                            \
-        {                                                \
-            if (ctx) (ctx)->last_hip_error = (int)e_;    \
-            return VETRAST_ERR_HIP;                      \
-        }                                                \
-    } while (0)
-
-// Brackets the launches of one scope with events when profiling is on.
-struct ScopeTimer
-{
-    vetrast_ctx* ctx;
-    hipStream_t stream;
-    int scope;
-    hipEvent_t start = nullptr, stop = nullptr;
-    bool on          = false;
-    ScopeTimer(vetrast_ctx* c, hipStream_t s, int sc) : ctx(c), stream(s), scope(sc)
-    {
-        if (!ctx->profiling) return;
-        start = take();
-        stop  = take();
-        if (!start || !stop) return;
-        on = hipEventRecord(start, stream) == hipSuccess;
-    }
-    ~ScopeTimer()
-    {
-        if (!on) return;
-        (void)hipEventRecord(stop, stream);
-        ctx->spans.push_back({scope, start, stop});
-    }
-    hipEvent_t take()
-    {
-        if (!ctx->free_events.empty())
-        {
-            hipEvent_t e = ctx->free_events.back();
-            ctx->free_events.pop_back();
-            return e;
-        }
-        hipEvent_t e = nullptr;
-        if (hipEventCreate(&e) != hipSuccess) return nullptr;
-        return e;
-    }
-};
 
 inline int grid_for(size_t n, int block = kBlock)
 {
@@ -476,15 +413,11 @@ void launch_lift(const vetrast_lift_args* a, char* ws, size_t num_sums, hipStrea
 }
 
 // Lists of tensors (optim_kernels.h)
-inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-inline bool is_dtype(int32_t t) { return t == VETRAST_F32 || t == VETRAST_BF16 || t == VETRAST_F16; }
-inline size_t dtype_bytes(int32_t t) { return t == VETRAST_F32 ? 4 : 2; }
 constexpr int64_t kOptimEntryElements = 1 << 27;  // a longer tensor is several entries of a launch: places inside one are 32 bits
 constexpr int64_t kOptimSmall         = 800000;   // elements up to which workgroups of one wave are faster
 constexpr uint32_t kNormGrid          = 768;      // workgroups of a launch at most, each goes through its share of chunks
 static_assert(kOptimEntryElements % kOptimChunk == 0, "whole chunks and blocks");
 static_assert(std::max(kAdamWEntries, kMomentEntries) * (kOptimEntryElements / 8) < (int64_t)1 << 32, "threads of a launch are counted in 32 bits");
-constexpr int64_t kOptimMaxElements   = (int64_t)1 << 38;  // of a tensor, and of the places in flat arrays, whose blocks have numbers of 32 bits
 inline bool is_place(int64_t first, int64_t n)  // of a tensor in the flat arrays
 {
     return first >= 0 && first % kMomentBlock == 0 && first < kOptimMaxElements && n <= kOptimMaxElements;

@@ -407,6 +407,22 @@ class Rasterizer:
         call = self.lib.vetrast_pack_moments if pack else self.lib.vetrast_unpack_moments
         abi.check(call(self.ctx, C.byref(a), self._stream()), "convert_moments")
 
+    def dropout(self, x, p, seed, step=0, residual=None, out=None, device_step=None):
+        """x with a share p of its elements left out and the others scaled, plus a residual (vetrast_dropout). Contiguous CUDA tensors of one
+        type; device_step: int64 [1] on the GPU, added to step."""
+        y = torch.empty_like(x) if out is None else out
+        a = abi.DropoutArgs()
+        for name, t in (("x", x), ("residual", residual), ("y", y)):
+            if t is not None:
+                assert t.is_cuda and t.is_contiguous() and t.dtype == x.dtype and t.numel() == x.numel(), name
+                setattr(a, name, t.data_ptr())
+        a.n, a.type, a.p, a.seed, a.step = x.numel(), _DTYPES[x.dtype], p, seed, step
+        if device_step is not None:
+            assert device_step.is_cuda and device_step.dtype == torch.int64 and device_step.numel() == 1
+            a.device_step = device_step.data_ptr()
+        abi.check(self.lib.vetrast_dropout(self.ctx, C.byref(a), self._stream()), "dropout")
+        return y
+
     def lift_error(self, cell_bb_min, cell_bb_length, cell_value, cell_access_count, view, poses_se3, intrinsics,
                    loss_image, border_pixels=abi.LIFT_BORDER_PIXELS, workspace=None, static_scratch=False):
         """Adds the error image of one view to the grid cells its pixels fall in, in place on cell_value (float32 [n]

@@ -3,58 +3,17 @@
 
 #include <cstring>
 #include <limits>
-#include <map>
 #include <utility>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
+
+#include "calls.h"
 
 namespace vet_amd
 {
 namespace
 {
 constexpr int64_t kBlock = VETRAST_MOMENT_BLOCK;
-
-void check(int st, const char* where)
-{
-    TORCH_CHECK(st == VETRAST_OK, "vetrast ", where, " failed: ", st, " (", vetrast_status_string(st), ")");
-}
-
-void* stream_on(const torch::Device& device)
-{
-    return (void*)c10::hip::getCurrentHIPStream(device.index()).stream();
-}
-
-bool capturing()
-{
-    return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
-}
-
-// What a host thread keeps. A context serves one host thread at a time and belongs to a device, a norm's workspace serves one stream of torch's.
-struct Kept
-{
-    std::map<int, vetrast_ctx*> contexts;
-    std::map<std::pair<int, void*>, torch::Tensor> workspaces;
-    ~Kept()
-    {
-        for (auto& c : contexts) vetrast_destroy(c.second);
-    }
-};
-Kept& kept()
-{
-    thread_local Kept k;
-    return k;
-}
-
-// The caller has made `device` the current one.
-vetrast_ctx* context_on(const torch::Device& device)
-{
-    vetrast_ctx*& ctx = kept().contexts[device.index()];
-    if (!ctx) check(vetrast_create(&ctx), "create");
-    return ctx;
-}
 
 // Zeroed memory for vetrast_gradient_norm, which leaves it zeroed where that counts. A captured call has its own, cleared in the graph, and
 // so has one on a stream that is not of torch's pool (its id is its handle): such a stream may be destroyed while its norm still runs,
@@ -71,36 +30,9 @@ torch::Tensor norm_workspace(const torch::Device& device, size_t bytes)
     return w;
 }
 
-int32_t type_of(const torch::Tensor& t, const char* what)
-{
-    switch (t.scalar_type())
-    {
-        case torch::kFloat32: return VETRAST_F32;
-        case torch::kBFloat16: return VETRAST_BF16;
-        case torch::kFloat16: return VETRAST_F16;
-        default: TORCH_CHECK(false, what, " must be float32, bfloat16 or float16, not ", t.scalar_type());
-    }
-}
-
-void check_on(const torch::Tensor& t, const torch::Device& device, const char* what)
-{
-    TORCH_CHECK(t.layout() == torch::kStrided && t.device() == device, what, " must be a strided tensor on ", device);
-}
-
-// The elements one behind the other in memory, whatever the order of dimensions.
-bool dense(const torch::Tensor& t)
-{
-    return t.is_contiguous() || t.is_non_overlapping_and_dense();
-}
-
 int64_t whole_blocks(int64_t n)
 {
     return (n + kBlock - 1) / kBlock * kBlock;
-}
-
-bool same_order(const torch::Tensor& a, const torch::Tensor& b)
-{
-    return (a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides();
 }
 
 // Whether two orders of memory are one: strides of dimensions of one element say nothing.

@@ -2,6 +2,7 @@
 // calling the C ABI of include/vetrast.h. See point_render.h for the reference lines each piece mirrors.
 #include "point_render.h"
 #include "adamw.h"
+#include "entries.h"
 #include "vet_adapter.h"
 
 #include <algorithm>
@@ -1311,6 +1312,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         },
         pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"));
     m.def("unpack_moments", &vet_amd::UnpackMoments, pybind11::arg("exp_avg"), pybind11::arg("exp_avg_sq"), pybind11::arg("block_scale"));
+    m.def("dropout", &vet_amd::Dropout, pybind11::arg("x"), pybind11::arg("p"), pybind11::arg("seed"), pybind11::arg("step") = 0,
+          pybind11::arg("residual") = pybind11::none(), pybind11::arg("device_step") = pybind11::none());
     m.def(
         "fill_scene_grid_with_loss",
         [](int batch, torch::Tensor bb_min, torch::Tensor bb_length, torch::Tensor value, torch::Tensor access_count,

@@ -97,6 +97,17 @@ def unpack_moments(exp_avg, exp_avg_sq, block_scale):
     return load().unpack_moments(exp_avg, exp_avg_sq, block_scale)
 
 
+def dropout(x, p, seed, step=0, residual=None, device_step=None):
+    """x with a share p of its elements left out and the others scaled by 1 / (1 - p), plus a residual of x's shape and type
+    (vetrast_dropout); differentiable in both. float32, bfloat16 or float16 on the GPU, any order of dimensions.
+
+    The mask is stored nowhere: it is a function of seed, step and an element's place in memory, which the backward pass evaluates again.
+    Give every layer a seed of its own and count steps. p counts in multiples of 2^-16. device_step: int64 [1] on the GPU, added to
+    step, for steps that are captured in a graph (AdamW(capturable=True).device_step goes up by itself); not to be written between a
+    forward pass and its backward pass."""
+    return load().dropout(x, p, seed, step, residual, device_step)
+
+
 def fill_scene_grid_with_loss(batch, cell_bb_min, cell_bb_length, cell_value, cell_access_count, views, poses_se3,
                               intrinsics, loss_img):
     """PointRendererCache::FillSceneGridWithLoss of the reference (src/lib/rendering/RenderForward.cu:763-791): adds
