@@ -509,6 +509,58 @@ typedef struct vetrast_dropout_args
 } vetrast_dropout_args;
 int vetrast_dropout(vetrast_ctx* ctx, const vetrast_dropout_args* args, void* stream);
 
+/* ---- Eviction ------------------------------------------------------------------------------------------------------
+ * A scene (or a cache) that may hold `budget` entries keeps those that gave most. vetrast_select_kept says which ones, from
+ * the weights they have accumulated; vetrast_keep_rows takes the rows of a list of tensors along.
+ *
+ * Of a row's first length[row] entries the last `recent` ones stay whatever their scores (points that were added a moment
+ * ago have had no time to gather weight), and of those in front of them the budget - recent with the highest scores, of
+ * equal ones those with the lowest numbers. +0 and -0 are equal, a NaN is below everything. A row of at most `budget` entries
+ * keeps them all. The entries that are kept are given in ascending order, the order of a cloud in memory, and behind them
+ * -1. Only the first length[row] scores of a row are read. */
+typedef struct vetrast_select_args
+{
+    const float* score;    /* device [rows][n], a row every row_stride elements */
+    int64_t row_stride;    /* >= n */
+    const int32_t* length; /* optional, device [rows]: entries of a row, taken as 0 below 0 and as n above n. NULL: n */
+    int32_t* index;        /* device [rows][budget]; overwritten */
+    int32_t* count;        /* device [rows]: entries kept, min(length, budget); overwritten */
+    int32_t rows, n;       /* >= 0 */
+    int32_t budget;        /* >= 0; may be more than n */
+    int32_t recent;        /* 0 .. budget */
+    void* workspace;       /* device, 16-byte aligned; its contents before and after the call do not matter */
+    size_t workspace_bytes;
+} vetrast_select_args;
+size_t vetrast_select_kept_workspace_bytes(int32_t rows, int32_t n); /* 0 for rows that one workgroup takes */
+int vetrast_select_kept(vetrast_ctx* ctx, const vetrast_select_args* args, void* stream);
+
+/* dst[o][k] = src[o][index[r][k]] for a list of tensors, entries being rows of row_bytes bytes of any kind; o counts what
+ * lies outside the dimension of the entries (the channels of a planar texture [C,N]; heads), and the outers of a tensor share
+ * the rows of indices evenly: r = o / (outers / index_rows). An index that is negative or not below n leaves zeros. dst is
+ * contiguous and must overlap neither a source nor another dst. Few launches whatever the length of the list (one for up to
+ * 32 tensors). */
+typedef struct vetrast_keep_tensor
+{
+    const void* src;
+    void* dst;               /* [outers][kept][row_bytes] */
+    int64_t outers;          /* a multiple of index_rows; at most 2^31 - 1 */
+    int64_t n;               /* entries of an outer, at most 2^31 - 1 */
+    int64_t row_bytes;       /* 1 .. 2^30 */
+    int64_t src_outer_bytes; /* from one outer to the next, and from one entry to the next; >= 0 */
+    int64_t src_row_bytes;
+} vetrast_keep_tensor;
+typedef struct vetrast_keep_args
+{
+    const vetrast_keep_tensor* tensors; /* host [num_tensors] */
+    int32_t num_tensors;
+    int32_t index_rows;      /* >= 1 */
+    int32_t kept;            /* >= 0, indices of a row */
+    int32_t reserved;
+    int64_t index_row_stride; /* elements, >= kept */
+    const int32_t* index;     /* device [index_rows][kept] */
+} vetrast_keep_args;
+int vetrast_keep_rows(vetrast_ctx* ctx, const vetrast_keep_args* args, void* stream);
+
 /* Error lifting: adds the per-pixel error of one rendered view to every cell of the scene grid whose projection covers
  * the pixel. Replaces PointRendererCache::FillSceneGridWithLoss and its kernel FillSceneGridWithLossRasterize
  * (src/lib/rendering/RenderForward.cu:605-632,639-791; called once per view of a batch in the epoch before points are

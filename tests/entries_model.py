@@ -38,3 +38,32 @@ def dropout(x, p, seed, step, residual=None):
     out = dropout_bits(x.size, seed, step) < t
     y = np.where(out, 0.0, x.astype(np.float64) * (65536.0 / (65536 - t) if t < 65536 else 0.0))
     return (y if residual is None else y + residual.astype(np.float64)), out
+
+
+def select_kept(score, budget, recent=0, length=None):
+    """score: [rows, n]. Indices [rows, budget] and counts [rows]."""
+    rows, n = score.shape
+    index, count = np.full((rows, budget), -1, np.int64), np.zeros(rows, np.int64)
+    for row in range(rows):
+        m = n if length is None else min(max(int(length[row]), 0), n)
+        s = score[row, :m].astype(np.float64)
+        if m <= budget:
+            kept = np.arange(m)
+        else:
+            free = m - recent
+            order = np.lexsort((np.arange(free), -np.where(np.isnan(s[:free]), -np.inf, s[:free]), np.isnan(s[:free])))
+            kept = np.sort(np.r_[order[:budget - recent], np.arange(free, m)])
+        index[row, :len(kept)], count[row] = kept, len(kept)
+    return index, count
+
+
+def keep_rows(a, index, dim):
+    """a: an array, index: [K] or [rows, K]; rows of zeros where an index is none."""
+    if index.ndim == 2:
+        return np.stack([keep_rows(x, i, dim - 1) for x, i in zip(a, index)]) if len(index) else a[:, :0]
+    there = (index >= 0) & (index < a.shape[dim])
+    if a.shape[dim] == 0:
+        return np.zeros(a.shape[:dim] + (len(index),) + a.shape[dim + 1:], a.dtype)
+    out = np.take(a, np.where(there, index, 0), axis=dim)
+    out[(slice(None),) * dim + (~there,)] = 0
+    return out

@@ -11,6 +11,7 @@ from tests import entries_model as em
 from vet_amd import abi, torch_ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CONTEXT = C.create_string_buffer(1 << 16)  # refusals come before anything reads it
 AT = 1 << 20  # an address that is never read: these calls are refused before
 
 
@@ -56,14 +57,14 @@ def args(**changes):
                                      dict(x=None), dict(y=None), dict(x=AT + 2), dict(y=AT + 66), dict(residual=AT + 1), dict(device_step=AT + 4),
                                      dict(y=AT + 60), dict(y=AT - 4), dict(residual=AT + 68)])
 def test_refusals(changes):
-    lib, ctx = abi.load_library(), C.addressof(C.create_string_buffer(1 << 16))
+    lib, ctx = abi.load_library(), C.addressof(CONTEXT)
     assert lib.vetrast_dropout(ctx, C.byref(args(**changes)), None) == abi.ERR_INVALID_ARG
     assert lib.vetrast_dropout(None, C.byref(args()), None) == abi.ERR_INVALID_ARG
     assert lib.vetrast_dropout(ctx, None, None) == abi.ERR_INVALID_ARG
 
 
 def test_nothing_to_do_is_done():
-    lib, ctx = abi.load_library(), C.addressof(C.create_string_buffer(1 << 16))
+    lib, ctx = abi.load_library(), C.addressof(CONTEXT)
     assert lib.vetrast_dropout(ctx, C.byref(args(n=0, x=None, y=None)), None) == abi.OK
 
 

@@ -183,6 +183,28 @@ class DropoutArgs(C.Structure):
     ]
 
 
+class SelectArgs(C.Structure):
+    _fields_ = [
+        ("score", C.c_void_p), ("row_stride", C.c_int64), ("length", C.c_void_p), ("index", C.c_void_p), ("count", C.c_void_p),
+        ("rows", C.c_int32), ("n", C.c_int32), ("budget", C.c_int32), ("recent", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class KeepTensor(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p), ("dst", C.c_void_p), ("outers", C.c_int64), ("n", C.c_int64), ("row_bytes", C.c_int64),
+        ("src_outer_bytes", C.c_int64), ("src_row_bytes", C.c_int64),
+    ]
+
+
+class KeepArgs(C.Structure):
+    _fields_ = [
+        ("tensors", C.POINTER(KeepTensor)), ("num_tensors", C.c_int32), ("index_rows", C.c_int32), ("kept", C.c_int32), ("reserved", C.c_int32),
+        ("index_row_stride", C.c_int64), ("index", C.c_void_p),
+    ]
+
+
 class PackArgs(C.Structure):
     _fields_ = [
         ("num_points", C.c_int32),
@@ -276,6 +298,9 @@ SYMBOLS = {
     "vetrast_pack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
     "vetrast_unpack_moments": (C.c_int, [C.c_void_p, C.POINTER(MomentsArgs), C.c_void_p]),
     "vetrast_dropout": (C.c_int, [C.c_void_p, C.POINTER(DropoutArgs), C.c_void_p]),
+    "vetrast_select_kept_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
+    "vetrast_select_kept": (C.c_int, [C.c_void_p, C.POINTER(SelectArgs), C.c_void_p]),
+    "vetrast_keep_rows": (C.c_int, [C.c_void_p, C.POINTER(KeepArgs), C.c_void_p]),
     "vetrast_lift_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "vetrast_lift_workspace_bytes_for_image": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     "vetrast_lift_error": (C.c_int, [C.c_void_p, C.POINTER(LiftArgs), C.c_void_p]),

@@ -1,10 +1,36 @@
-// Elements of tensors of float32, bfloat16 and float16, eight to a thread.
+// Tables of tensors in a launch's arguments, and elements of tensors of float32, bfloat16 and float16, eight to a thread.
 #pragma once
 #include "common.h"
 
 namespace vetrast
 {
 constexpr uint32_t kOptimChunk = 8 * kBlock;  // elements of a workgroup
+
+// Tables hold up to 64 * GROUPS entries: lane k of a wave knows which chunk of the launch is the first of entries k, k + 64, ...
+template <int GROUPS>
+struct ChunkFinder
+{
+    uint32_t begins[GROUPS];
+    template <class Launch>
+    __device__ __forceinline__ explicit ChunkFinder(const Launch& a)
+    {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q)
+        {
+            const uint32_t k = q * kWave + threadIdx.x % kWave;
+            begins[q]        = k < a.entries ? a.e[k].begins() : 0xFFFFFFFFu;
+        }
+    }
+    // The entry of a chunk; all lanes of the wave take part.
+    __device__ __forceinline__ uint32_t operator()(uint32_t chunk) const
+    {
+        uint32_t k = 0;
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) k += (uint32_t)__popcll(__ballot(begins[q] <= chunk));
+        return k - 1u;
+    }
+};
+constexpr int finder_groups(int entries) { return (entries + kWave - 1) / kWave; }
 
 // As they lie in memory, 32 bytes or (16-bit types) 16. Loads of several arrays are under way before the first is looked at.
 struct RawEight

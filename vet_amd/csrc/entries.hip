@@ -2,10 +2,12 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <limits>
 
 #include "common.h"
 #include "context.h"
 #include "dropout_kernels.h"
+#include "evict_kernels.h"
 
 using namespace vetrast;
 
@@ -27,6 +29,62 @@ inline bool overlap(const void* a, const void* b, size_t bytes)
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x != y && (x < y ? y - x : x - y) < bytes;
 }
+// Rows of more entries than a workgroup holds are shared by several: 8 entries a thread each, or more where there are many workgroups.
+constexpr int kSelectShare    = 8 * kSelectThreads;
+constexpr int kSelectGroups   = 1024;   // workgroups of a row at most
+constexpr int kSelectGridRows = 32768;  // rows of a launch
+inline int select_share(int n)
+{
+    const int64_t groups = std::min<int64_t>(((int64_t)n + kSelectShare - 1) / kSelectShare, kSelectGroups);
+    return (int)((((int64_t)n + groups - 1) / groups + kSelectThreads - 1) / kSelectThreads * kSelectThreads);
+}
+inline int select_groups(int n) { return (int)(((int64_t)n + select_share(n) - 1) / select_share(n)); }
+inline size_t select_words(int n) { return kDigits * (size_t)kBins + 2 * (size_t)select_groups(n); }  // of a row
+
+void launch_select_row(const SelectPass& p, hipStream_t stream)
+{
+    const dim3 grid((uint32_t)p.rows), block(kSelectThreads);
+    const int items = (p.n + kSelectThreads - 1) / kSelectThreads;
+    if (items <= 1) hipLaunchKernelGGL((select_row_kernel<1>), grid, block, 0, stream, p);
+    else if (items <= 4) hipLaunchKernelGGL((select_row_kernel<4>), grid, block, 0, stream, p);
+    else if (items <= 12) hipLaunchKernelGGL((select_row_kernel<12>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((select_row_kernel<32>), grid, block, 0, stream, p);
+}
+
+void launch_select_rows(SelectPass p, char* workspace, hipStream_t stream)
+{
+    p.share  = select_share(p.n);
+    p.groups = select_groups(p.n);
+    const int rows        = p.rows;
+    const SelectPass all  = p;
+    for (int from = 0; from < rows; from += kSelectGridRows)
+    {
+        p           = all;
+        p.rows      = std::min(rows - from, kSelectGridRows);
+        p.score     = all.score + (int64_t)from * all.row_stride;
+        p.length    = all.length ? all.length + from : nullptr;
+        p.index     = all.index + (int64_t)from * all.budget;
+        p.count     = all.count + from;
+        p.histogram = reinterpret_cast<uint32_t*>(workspace) + (size_t)from * select_words(p.n);
+        p.counts    = reinterpret_cast<uint2*>(p.histogram + (size_t)p.rows * kDigits * kBins);
+        const size_t words = (size_t)p.rows * kDigits * kBins;
+        const dim3 grid((uint32_t)p.groups, (uint32_t)p.rows), block(kSelectThreads);
+        hipLaunchKernelGGL(select_clear_kernel, dim3((uint32_t)std::min<size_t>((words + kBlock - 1) / kBlock, 2048)), dim3(kBlock), 0, stream, p.histogram, words);
+        hipLaunchKernelGGL((select_digit_kernel<0>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((select_digit_kernel<1>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((select_digit_kernel<2>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL(select_count_kernel, grid, block, 0, stream, p);
+        hipLaunchKernelGGL(select_place_kernel, grid, block, 0, stream, p);
+    }
+}
+
+// Bytes from a tensor's first to behind its last.
+inline uint64_t stretch(int64_t outers, int64_t n, int64_t outer_bytes, int64_t row_bytes, int64_t bytes)
+{
+    return (uint64_t)(outers - 1) * (uint64_t)outer_bytes + (uint64_t)(n - 1) * (uint64_t)row_bytes + (uint64_t)bytes;
+}
+constexpr int64_t kKeepMost       = (int64_t)1 << 30;  // units of an entry's outer: places in it are 32 bits
+constexpr int64_t kKeepGroupsMost = (int64_t)1 << 22;  // workgroups of an entry, and with those in front twice that: a launch's threads are 32 bits
 }  // namespace
 
 extern "C" {
@@ -55,6 +113,120 @@ int vetrast_dropout(vetrast_ctx* ctx, const vetrast_dropout_args* a, void* strea
         else if (a->type == VETRAST_BF16) launch_dropout<VETRAST_BF16>(l, stream);
         else launch_dropout<VETRAST_F16>(l, stream);
     }
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+size_t vetrast_select_kept_workspace_bytes(int32_t rows, int32_t n)
+{
+    if (rows <= 0 || n <= kSelectRowMost) return 0;
+    return (size_t)rows * select_words(n) * sizeof(uint32_t);
+}
+
+int vetrast_select_kept(vetrast_ctx* ctx, const vetrast_select_args* a, void* stream_)
+{
+    if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
+    if (a->rows < 0 || a->n < 0 || a->budget < 0 || a->recent < 0 || a->recent > a->budget || a->row_stride < a->n) return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->score, 4) || !aligned_to(a->length, 4) || !aligned_to(a->index, 4) || !aligned_to(a->count, 4) || !aligned_to(a->workspace, 16))
+        return VETRAST_ERR_INVALID_ARG;
+    if (a->rows == 0) return VETRAST_OK;
+    if (!a->count || (a->budget > 0 && !a->index) || (a->n > 0 && !a->score)) return VETRAST_ERR_INVALID_ARG;
+    const size_t need = vetrast_select_kept_workspace_bytes(a->rows, a->n);
+    if (need > 0 && !a->workspace) return VETRAST_ERR_INVALID_ARG;
+    if (a->workspace_bytes < need) return VETRAST_ERR_WORKSPACE_SMALL;
+    SelectPass p;
+    p.score      = a->score;
+    p.row_stride = a->row_stride;
+    p.length     = a->length;
+    p.index      = a->index;
+    p.count      = a->count;
+    p.rows       = a->rows;
+    p.n          = a->n;
+    p.budget     = a->budget;
+    p.recent     = a->recent;
+    p.histogram  = nullptr;
+    p.counts     = nullptr;
+    p.share = p.groups = 0;
+    hipStream_t stream = (hipStream_t)stream_;
+    if (need == 0) launch_select_row(p, stream);
+    else launch_select_rows(p, static_cast<char*>(a->workspace), stream);
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+int vetrast_keep_rows(vetrast_ctx* ctx, const vetrast_keep_args* a, void* stream_)
+{
+    if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
+    if (a->num_tensors < 0 || (a->num_tensors > 0 && !a->tensors) || a->index_rows < 1 || a->kept < 0 || a->index_row_stride < a->kept)
+        return VETRAST_ERR_INVALID_ARG;
+    if (!aligned_to(a->index, 4) || (a->kept > 0 && !a->index)) return VETRAST_ERR_INVALID_ARG;
+    constexpr int64_t kMost = std::numeric_limits<int32_t>::max(), kFar = (int64_t)1 << 47;
+    bool any = false;
+    for (int k = 0; k < a->num_tensors; ++k)
+    {
+        const vetrast_keep_tensor& t = a->tensors[k];
+        if (t.outers < 0 || t.outers > kMost || t.outers % a->index_rows != 0 || t.n < 0 || t.n > kMost) return VETRAST_ERR_INVALID_ARG;
+        if (t.row_bytes < 1 || t.row_bytes > kKeepMost || t.src_outer_bytes < 0 || t.src_row_bytes < 0) return VETRAST_ERR_INVALID_ARG;
+        if (t.outers == 0 || a->kept == 0) continue;
+        any = true;
+        if (!t.dst || (t.n > 0 && !t.src)) return VETRAST_ERR_INVALID_ARG;
+        // no memory is as long as this; products below stay within 64 bits
+        if ((double)t.outers * a->kept * t.row_bytes > (double)kFar || (double)t.outers * t.src_outer_bytes > (double)kFar ||
+            (double)t.n * t.src_row_bytes > (double)kFar)
+            return VETRAST_ERR_INVALID_ARG;
+        if (t.n == 0) continue;
+        const uint64_t from = reinterpret_cast<uintptr_t>(t.src), to = reinterpret_cast<uintptr_t>(t.dst);
+        const uint64_t there = stretch(t.outers, t.n, t.src_outer_bytes, t.src_row_bytes, t.row_bytes);
+        const uint64_t here  = (uint64_t)t.outers * (uint64_t)a->kept * (uint64_t)t.row_bytes;
+        if (from < to + here && to < from + there) return VETRAST_ERR_INVALID_ARG;
+    }
+    if (!any) return VETRAST_OK;
+    hipStream_t stream = (hipStream_t)stream_;
+    KeepLaunch l;
+    l.entries = l.total = 0;
+    const auto launch = [&] {
+        if (l.entries > 0) hipLaunchKernelGGL(keep_rows_kernel, dim3(l.total), dim3(kBlock), 0, stream, l);
+        l.entries = l.total = 0;
+    };
+    for (int k = 0; k < a->num_tensors; ++k)
+    {
+        const vetrast_keep_tensor& t = a->tensors[k];
+        if (t.outers == 0 || a->kept == 0) continue;
+        uint64_t bits = reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst) | (uint64_t)t.row_bytes | 16;
+        if (t.n > 1) bits |= (uint64_t)t.src_row_bytes;
+        if (t.outers > 1) bits |= (uint64_t)t.src_outer_bytes;
+        const uint32_t unit_log = (uint32_t)__builtin_ctzll(bits);
+        const int64_t units = t.row_bytes >> unit_log, per_index = t.outers / a->index_rows;
+        const int64_t rows_at_once = std::max<int64_t>(kKeepMost / units, 1);
+        for (int64_t row = 0; row < a->kept; row += rows_at_once)
+        {
+            const int64_t rows   = std::min<int64_t>(a->kept - row, rows_at_once);
+            const int64_t chunks = (rows * units + kKeepChunk - 1) / kKeepChunk, outers_at_once = std::max<int64_t>(kKeepGroupsMost / chunks, 1);
+            for (int64_t outer = 0; outer < t.outers; outer += outers_at_once)
+            {
+                const int64_t outers = std::min(t.outers - outer, outers_at_once);
+                if (l.entries == (uint32_t)kKeepEntries || l.total + outers * chunks > 2 * kKeepGroupsMost) launch();
+                KeepEntry& e   = l.e[l.entries++];
+                e.src          = static_cast<const char*>(t.src) + outer * t.src_outer_bytes;
+                e.dst          = static_cast<char*>(t.dst) + (outer * a->kept + row) * t.row_bytes;
+                e.src_outer    = t.src_outer_bytes;
+                e.src_row      = t.src_row_bytes;
+                e.dst_outer    = a->kept * t.row_bytes;
+                e.index        = a->index + (outer / per_index) * a->index_row_stride + row;
+                e.index_stride = a->index_row_stride;
+                e.per_index    = (uint32_t)per_index;
+                e.outer_in_row = (uint32_t)(outer % per_index);
+                e.kept         = (uint32_t)rows;
+                e.units        = (uint32_t)units;
+                e.n            = (uint32_t)t.n;
+                e.chunks       = (uint32_t)chunks;
+                e.first_chunk  = l.total;
+                e.unit_log     = unit_log;
+                l.total += (uint32_t)(outers * chunks);
+            }
+        }
+    }
+    launch();
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;
 }

@@ -14,32 +14,6 @@ constexpr int kMomentBlock       = VETRAST_MOMENT_BLOCK;
 constexpr uint32_t kMomentMargin = 0x100100;  // see code_base
 static_assert(kWaveChunk % kMomentBlock == 0 && kMomentBlock == 16 * 8, "16 lanes of 8 elements hold a block");
 
-// Tables hold up to 64 * GROUPS entries: lane k of a wave knows which chunk of the launch is the first of entries k, k + 64, ...
-template <int GROUPS>
-struct ChunkFinder
-{
-    uint32_t begins[GROUPS];
-    template <class Launch>
-    __device__ __forceinline__ explicit ChunkFinder(const Launch& a)
-    {
-#pragma unroll
-        for (int q = 0; q < GROUPS; ++q)
-        {
-            const uint32_t k = q * kWave + threadIdx.x % kWave;
-            begins[q]        = k < a.entries ? a.e[k].begins() : 0xFFFFFFFFu;
-        }
-    }
-    // The entry of a chunk; all lanes of the wave take part.
-    __device__ __forceinline__ uint32_t operator()(uint32_t chunk) const
-    {
-        uint32_t k = 0;
-#pragma unroll
-        for (int q = 0; q < GROUPS; ++q) k += (uint32_t)__popcll(__ballot(begins[q] <= chunk));
-        return k - 1u;
-    }
-};
-constexpr int finder_groups(int entries) { return (entries + kWave - 1) / kWave; }
-
 // ---- random bits -------------------------------------------------------------------------------------------------------
 
 // A step's key: two rounds of a 64-bit mixing function (the finalizer of splitmix64) over seed and step.

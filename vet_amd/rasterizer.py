@@ -423,6 +423,43 @@ class Rasterizer:
         abi.check(self.lib.vetrast_dropout(self.ctx, C.byref(a), self._stream()), "dropout")
         return y
 
+    def select_kept(self, score, budget, recent=0, length=None, workspace=None):
+        """Indices [rows, budget] and counts [rows] of the entries a budget keeps (vetrast_select_kept). score: float32 [rows, n], a row's
+        scores one behind the other."""
+        rows, n = score.shape
+        assert score.is_cuda and score.dtype == torch.float32 and (n <= 1 or score.stride(1) == 1)
+        index, count = (torch.empty(s, dtype=torch.int32, device=score.device) for s in ((rows, budget), (rows,)))
+        a = abi.SelectArgs()
+        a.score, a.row_stride, a.index, a.count = score.data_ptr(), score.stride(0) if rows > 1 else n, index.data_ptr(), count.data_ptr()
+        a.rows, a.n, a.budget, a.recent = rows, n, budget, recent
+        if length is not None:
+            assert length.is_cuda and length.dtype == torch.int32 and length.is_contiguous() and length.numel() == rows
+            a.length = length.data_ptr()
+        need = self.lib.vetrast_select_kept_workspace_bytes(rows, n)
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=score.device)
+        if workspace is not None:
+            assert workspace.is_cuda and workspace.is_contiguous() and workspace.dtype == torch.uint8
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        abi.check(self.lib.vetrast_select_kept(self.ctx, C.byref(a), self._stream()), "select_kept")
+        return index, count
+
+    def keep_rows(self, tensors, index):
+        """Entries `index` [index_rows, kept] of a list of contiguous tensors [outers, n, ...] (vetrast_keep_rows)."""
+        ts, a = (abi.KeepTensor * max(len(tensors), 1))(), abi.KeepArgs()
+        assert index.is_cuda and index.dtype == torch.int32 and index.is_contiguous() and index.dim() == 2
+        out = []
+        for t, x in zip(ts, tensors):
+            assert x.is_cuda and x.is_contiguous() and x.dim() >= 2
+            out.append(torch.empty((x.shape[0], index.shape[1]) + x.shape[2:], dtype=x.dtype, device=x.device))
+            t.src, t.dst, t.outers, t.n = x.data_ptr(), out[-1].data_ptr(), x.shape[0], x.shape[1]
+            t.row_bytes = x[0, 0].numel() * x.element_size() if x.numel() else 1
+            t.src_row_bytes, t.src_outer_bytes = t.row_bytes, t.row_bytes * t.n
+        a.tensors, a.num_tensors, a.index_rows, a.kept = ts, len(tensors), index.shape[0], index.shape[1]
+        a.index, a.index_row_stride = index.data_ptr(), index.shape[1]
+        abi.check(self.lib.vetrast_keep_rows(self.ctx, C.byref(a), self._stream()), "keep_rows")
+        return out
+
     def lift_error(self, cell_bb_min, cell_bb_length, cell_value, cell_access_count, view, poses_se3, intrinsics,
                    loss_image, border_pixels=abi.LIFT_BORDER_PIXELS, workspace=None, static_scratch=False):
         """Adds the error image of one view to the grid cells its pixels fall in, in place on cell_value (float32 [n]

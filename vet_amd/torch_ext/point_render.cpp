@@ -1314,6 +1314,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("unpack_moments", &vet_amd::UnpackMoments, pybind11::arg("exp_avg"), pybind11::arg("exp_avg_sq"), pybind11::arg("block_scale"));
     m.def("dropout", &vet_amd::Dropout, pybind11::arg("x"), pybind11::arg("p"), pybind11::arg("seed"), pybind11::arg("step") = 0,
           pybind11::arg("residual") = pybind11::none(), pybind11::arg("device_step") = pybind11::none());
+    m.def("select_kept", &vet_amd::SelectKept, pybind11::arg("score"), pybind11::arg("budget"), pybind11::arg("recent") = 0,
+          pybind11::arg("length") = pybind11::none());
+    m.def("keep_rows", &vet_amd::KeepRows, pybind11::arg("tensors"), pybind11::arg("index"), pybind11::arg("dims"));
     m.def(
         "fill_scene_grid_with_loss",
         [](int batch, torch::Tensor bb_min, torch::Tensor bb_length, torch::Tensor value, torch::Tensor access_count,

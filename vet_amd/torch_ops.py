@@ -108,6 +108,23 @@ def dropout(x, p, seed, step=0, residual=None, device_step=None):
     return load().dropout(x, p, seed, step, residual, device_step)
 
 
+def select_kept(score, budget, recent=0, length=None):
+    """Which entries a budget keeps, by the weight they have accumulated (vetrast_select_kept): the last `recent` ones of a row whatever
+    their scores, else those with the highest scores, of equal ones those in front; a NaN is below everything.
+
+    score: float32 [N], or [rows, N] with rows of their own (heads); length: int32 [rows], entries of a row, the others are not read.
+    Returns (index, count): int32 [budget] or [rows, budget], ascending, -1 behind the last one, and int32 [rows]. Nothing waits for
+    the device."""
+    return load().select_kept(score, int(budget), int(recent), length)
+
+
+def keep_rows(tensors, index, dims):
+    """The rows that go with select_kept's indices, of a list of tensors of any type (vetrast_keep_rows): tensor k's entries lie along
+    dimension dims[k]; with indices [rows, K] every tensor's first dimension is that of the rows. An index that is negative or beyond the end
+    leaves zeros. The results are contiguous and have no history."""
+    return load().keep_rows(list(tensors), index, list(dims))
+
+
 def fill_scene_grid_with_loss(batch, cell_bb_min, cell_bb_length, cell_value, cell_access_count, views, poses_se3,
                               intrinsics, loss_img):
     """PointRendererCache::FillSceneGridWithLoss of the reference (src/lib/rendering/RenderForward.cu:763-791): adds
