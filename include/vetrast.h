@@ -266,6 +266,13 @@ typedef struct vetrast_forward_args
      * same array. NULL = the call interleaves for itself, into the workspace. No counterpart in the reference, which
      * reads the planar tensors per channel (src/lib/rendering/RenderForward.cu:1338-1342). */
     const float* packed_descriptors;
+    /* Optional: drop-out of points without a mask in memory, instead of `dropout` (which must be NULL then). Point i is skipped in view b
+     * where vetrast_dropout would leave out element b * num_points + i, with p = point_dropout, seed = dropout_seed and step =
+     * dropout_step (+ *dropout_device_step, device, where it isn't NULL: for calls that are captured in a graph). What a backward
+     * pass is handed has to be what the forward pass had, *dropout_device_step included. 0: none. */
+    double point_dropout;
+    uint64_t dropout_seed, dropout_step;
+    const int64_t* dropout_device_step;
 } vetrast_forward_args;
 
 /* Arguments of the backward pass. Replaces BlendPointCloudBackward's inputs and its seven returned tensors
@@ -290,6 +297,22 @@ typedef struct vetrast_backward_args
                                     vetrast_params.allow_distortion is set, else stay 0; overwritten */
     float* grad_intrinsics_count; /* device [num_cameras]: fragments / 1024 per camera row; required with grad_intrinsics */
 } vetrast_backward_args;
+
+/* What every point gave to the pixels of a render: weight[i] = decay * weight[i] + the sum, over the views, layers and pixels in which a
+ * fragment of point i was blended, of its weight there, the transmittance in front of it times its alpha (its confidence; with the 2x2
+ * splat times the corner's weight; in FUZZY_BLEND its share of the bucket's). That is the derivative of the sum of all pixels of one
+ * channel by the point's descriptor. Accumulated over renders it says which points a budget should keep (vetrast_select_kept).
+ * Sums are formed in float32 in a fixed order, without atomics. No counterpart in the reference, which removes points by their
+ * confidence alone (src/apps/train.cpp:727-741). */
+typedef struct vetrast_point_weights_args
+{
+    vetrast_forward_args fwd; /* same values as passed to vetrast_forward, with save_for_backward = 1; workspace and inputs unchanged
+                                 since. The backward scratch of the workspace is written: not between or during other calls on it */
+    float* weight;            /* device [N] */
+    float decay;              /* finite, >= 0; 0: the old values are not read */
+    int32_t reserved;
+} vetrast_point_weights_args;
+int vetrast_point_weights(vetrast_ctx* ctx, const vetrast_point_weights_args* args, void* stream);
 
 /* Create / destroy a context bound to the current HIP device. The context owns only a few HIP events. */
 int vetrast_create(vetrast_ctx** out_ctx);

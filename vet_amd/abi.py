@@ -257,6 +257,7 @@ class ForwardArgs(C.Structure):
         ("out_weight", C.c_void_p * MAX_LAYERS),
         ("point_order", C.c_void_p),
         ("packed_descriptors", C.c_void_p),
+        ("point_dropout", C.c_double), ("dropout_seed", C.c_uint64), ("dropout_step", C.c_uint64), ("dropout_device_step", C.c_void_p),
     ]
 
 
@@ -276,6 +277,10 @@ class BackwardArgs(C.Structure):
     ]
 
 
+class PointWeightsArgs(C.Structure):
+    _fields_ = [("fwd", ForwardArgs), ("weight", C.c_void_p), ("decay", C.c_float), ("reserved", C.c_int32)]
+
+
 # Every symbol include/vetrast.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "vetrast_create": (C.c_int, [C.POINTER(C.c_void_p)]),
@@ -288,6 +293,7 @@ SYMBOLS = {
     "vetrast_forward_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "vetrast_forward": (C.c_int, [C.c_void_p, C.POINTER(ForwardArgs), C.c_void_p]),
     "vetrast_backward": (C.c_int, [C.c_void_p, C.POINTER(BackwardArgs), C.c_void_p]),
+    "vetrast_point_weights": (C.c_int, [C.c_void_p, C.POINTER(PointWeightsArgs), C.c_void_p]),
     "vetrast_packed_descriptor_bytes": (C.c_size_t, [C.c_int32]),
     "vetrast_pack_descriptors": (C.c_int, [C.c_void_p, C.POINTER(PackArgs), C.c_void_p]),
     "vetrast_adam_step": (C.c_int, [C.c_void_p, C.POINTER(AdamArgs), C.c_void_p]),

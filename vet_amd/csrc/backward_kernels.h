@@ -1664,10 +1664,12 @@ __device__ __forceinline__ double wave_sum_terms(const double (&term_values)[kCa
 // Distortion's 16 more sums and the 2x2 splat together have the registers of four waves: with five, 60 bytes a lane went to memory
 // and came back in every layer for one view and 116 for several, 1080p 225 against 126 us, four crops 243 against 153. With
 // one hit per layer, distortion and several views five waves and 28 bytes are the better: four views of 960x540 182 against 195 us.
-constexpr int gather_waves(int hits, bool distort) { return hits == 4 && distort ? 4 : 5; }
+// DROP: points are left out by random bits, one register more, which the variants with several views do not have: these calls have variants
+// of their own, with the registers of a wave less.
+constexpr int gather_waves(int hits, bool distort, bool drop) { return (hits == 4 && distort ? 4 : 5) - (drop ? 1 : 0); }
 constexpr int kGatherLayers = 2;
-template <int C, int HITS, bool DISTORT = false, bool MANY = false>
-__global__ void __launch_bounds__(kBlock, gather_waves(HITS, DISTORT)) gather_point_gradients_kernel(GatherPass a)
+template <int C, int HITS, bool DISTORT = false, bool MANY = false, bool DROP = false>
+__global__ void __launch_bounds__(kBlock, gather_waves(HITS, DISTORT, DROP)) gather_point_gradients_kernel(GatherPass a)
 {
     constexpr int kLayers = HITS == 1 ? kGatherLayers : 1, kSlots = kLayers * HITS;
     // corners whose pixels' upstream gradients are asked for together: all of them, or two where several views leave no registers
@@ -1686,6 +1688,9 @@ __global__ void __launch_bounds__(kBlock, gather_waves(HITS, DISTORT)) gather_po
     const float4 wp     = alive ? a.vp.position[i] : make_float4(0.f, 0.f, 0.f, 0.f);
     // skipped in every view alike (viewer cut-off), or in this view (drop-out mask)
     const bool never = !alive || point_is_skipped_in_all_views(a.vp, i);
+    uint32_t left_out = 0u;  // by random bits, a bit for each view
+    if constexpr (DROP)
+        for (int view = 0; view < view_count; ++view) left_out |= point_is_left_out(a.vp, view, i) ? 1u << view : 0u;
   for (int view = 0; view < view_count; ++view)
   {
     const float* dropout       = a.vp.dropout ? a.vp.dropout + (size_t)view * a.dropout_stride : nullptr;
@@ -1704,7 +1709,7 @@ __global__ void __launch_bounds__(kBlock, gather_waves(HITS, DISTORT)) gather_po
     // (a position further outside the image than the coarsest layer's border pixels reach has no fragment in any
     // layer, see bin_scatter_kernel: most of the cloud, for a crop)
     const float reach = (float)(1 << (a.vp.ly.L - 1)) + 1.f;
-    if (!never && !(dropout && dropout[i] == 1.f) && project_point(cam, wp, p) && p.ipx >= -reach &&
+    if (!never && !(dropout && dropout[i] == 1.f) && !(DROP && (left_out >> view & 1u)) && project_point(cam, wp, p) && p.ipx >= -reach &&
         p.ipx <= (float)a.vp.ly.w[0] + reach && p.ipy >= -reach && p.ipy <= (float)a.vp.ly.h[0] + reach)
     {
         // view-space position again, for the projection Jacobian (same expressions as project_point)

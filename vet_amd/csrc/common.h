@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../include/vetrast.h"
+#include "dropout_bits.h"
 
 namespace vetrast
 {
@@ -180,6 +181,8 @@ struct ViewPass
     const int32_t* index;
     const float* confidence;
     const float* dropout;  // already offset to this view, or null
+    DropoutBits dropout_bits;  // or the same from random bits: of element dropout_first + point, where the threshold isn't 0
+    uint64_t dropout_first;
     const DeviceView* view;
     LayerTable ly;
     int N;
@@ -505,4 +508,34 @@ __device__ __forceinline__ TilePixel tile_pixel(const TileMap& tm, const LayerTa
     return r;
 }
 
+// The viewer's confidence cut-off: the same verdict in every view of a call.
+__device__ __forceinline__ bool point_is_skipped_in_all_views(const ViewPass& a, int i)
+{
+    if (a.viewer_only)
+    {
+        const int ti = a.index ? a.index[i] : i;
+        float c      = a.confidence[ti];
+        if (a.confidence_activation) c = sigmoid_canon(a.confidence_scale * c);
+        if (c < a.stability_cutoff) return true;
+    }
+    return false;
+}
+
+// Drop-out by random bits, in the view that lies `view` views behind the one that `a` is about.
+__device__ __forceinline__ bool point_is_left_out(const ViewPass& a, int view, int i)
+{
+    return dropped_out(a.dropout_bits, dropout_step(a.dropout_bits), a.dropout_first + (uint64_t)view * (uint64_t)a.N + (uint64_t)i);
+}
+
+// The drop-out of that view, from the caller's mask or from random bits.
+__device__ __forceinline__ bool point_is_dropped(const ViewPass& a, int view, int i)
+{
+    if (a.dropout && a.dropout[(size_t)view * (size_t)a.N + i] == 1.f) return true;
+    return a.dropout_bits.threshold != 0u && point_is_left_out(a, view, i);
+}
+
+__device__ __forceinline__ bool point_is_skipped(const ViewPass& a, int i)
+{
+    return point_is_dropped(a, 0, i) || point_is_skipped_in_all_views(a, i);
+}
 }  // namespace vetrast

@@ -239,11 +239,4 @@ __device__ __forceinline__ RawEight from_floats(const float* x, uint32_t type)
     r.a = make_uint4(w[0], w[1], w[2], w[3]);
     return r;
 }
-
-__device__ __forceinline__ uint32_t exclusive_or(uint32_t a, uint32_t b, uint32_t c)  // of three, in one instruction
-{
-    uint32_t x;
-    asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x96" : "=v"(x) : "v"(a), "v"(b), "v"(c));
-    return x;
-}
 }  // namespace vetrast

@@ -8,8 +8,26 @@
 #include "context.h"
 #include "dropout_kernels.h"
 #include "evict_kernels.h"
+#include "weight_kernels.h"
 
 using namespace vetrast;
+
+namespace vetrast
+{
+void launch_fragment_weights(const WeightPass& pass, int hits, bool fuzzy, int views, hipStream_t stream)
+{
+    const dim3 grid(pass.group_base[pass.ly.L], (uint32_t)views), block(kBlock);
+    if (fuzzy) hipLaunchKernelGGL(fragment_weights_fuzzy_kernel, grid, block, 0, stream, pass);
+    else if (hits == 1) hipLaunchKernelGGL((fragment_weights_kernel<1>), grid, block, 0, stream, pass);
+    else hipLaunchKernelGGL((fragment_weights_kernel<4>), grid, block, 0, stream, pass);
+}
+void launch_point_weights(const PointWeightPass& pass, int hits, hipStream_t stream)
+{
+    const dim3 grid((uint32_t)((pass.vp.N + kBlock - 1) / kBlock)), block(kBlock);
+    if (hits == 1) hipLaunchKernelGGL((point_weights_kernel<1>), grid, block, 0, stream, pass);
+    else hipLaunchKernelGGL((point_weights_kernel<4>), grid, block, 0, stream, pass);
+}
+}  // namespace vetrast
 
 namespace
 {

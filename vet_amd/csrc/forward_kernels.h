@@ -167,25 +167,6 @@ __global__ void __launch_bounds__(kBlock) prepare_views_kernel(PrepareViewsArgs 
     views[first_view + k] = v;
 }
 
-// The viewer's confidence cut-off: the same verdict in every view of a call.
-__device__ __forceinline__ bool point_is_skipped_in_all_views(const ViewPass& a, int i)
-{
-    if (a.viewer_only)
-    {
-        const int ti = a.index ? a.index[i] : i;
-        float c      = a.confidence[ti];
-        if (a.confidence_activation) c = sigmoid_canon(a.confidence_scale * c);
-        if (c < a.stability_cutoff) return true;
-    }
-    return false;
-}
-
-__device__ __forceinline__ bool point_is_skipped(const ViewPass& a, int i)
-{
-    if (a.dropout && a.dropout[i] == 1.f) return true;  // this view's drop-out mask
-    return point_is_skipped_in_all_views(a, i);
-}
-
 // ---- binning ---------------------------------------------------------------------------------------------------------
 // The reference counts every (point, layer) hit with one global atomic on its pixel, fills the lists with a second one
 // (CountingPrepassMulti / CollectMulti, src/lib/rendering/RenderForward.cu:806-905,1011-1096) and then sorts every

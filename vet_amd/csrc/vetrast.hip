@@ -22,6 +22,7 @@
 #include "lift_kernels.h"
 #include "optim_kernels.h"
 #include "region_rule.h"
+#include "weight_pass.h"
 
 using namespace vetrast;
 
@@ -188,6 +189,8 @@ int validate_forward(const vetrast_forward_args* a, vetrast_workspace_layout* la
     }
     if (((uintptr_t)a->workspace % kAlign) != 0 || ((uintptr_t)a->position % 16) != 0) return VETRAST_ERR_INVALID_ARG;
     if (((uintptr_t)a->packed_descriptors % 32) != 0) return VETRAST_ERR_INVALID_ARG;
+    if (!(a->point_dropout >= 0.0 && a->point_dropout <= 1.0) || (a->point_dropout > 0.0 && a->dropout) || !aligned_to(a->dropout_device_step, 8))
+        return VETRAST_ERR_INVALID_ARG;
     st = vetrast_workspace_layout_for_mode(a->num_points, a->num_views, p.num_layers, w, h, p.render_mode, lay);
     if (st != VETRAST_OK) return st;
     const size_t need = a->save_for_backward ? lay->total_bytes : lay->forward_only_bytes;
@@ -280,6 +283,8 @@ ViewPass make_view_pass(const vetrast_forward_args* a, const vetrast_workspace_l
     vp.index            = a->index;
     vp.confidence       = a->confidence;
     vp.dropout          = a->dropout ? a->dropout + (size_t)b * a->num_points : nullptr;
+    vp.dropout_bits     = dropout_bits(a->point_dropout, a->dropout_seed, a->dropout_step, a->dropout_device_step);
+    vp.dropout_first    = (uint64_t)b * (uint64_t)a->num_points;
     vp.view             = ws_ptr<DeviceView>(a->workspace, lay.views_base) + b;
     vp.ly               = ly;
     vp.N                = a->num_points;
@@ -1227,17 +1232,18 @@ int vetrast_backward(vetrast_ctx* ctx, const vetrast_backward_args* g, void* str
             // cameras with distortion switched on take the variant that carries the distortion Jacobians
             auto launch = [&](auto c_tag, auto hits_tag) {
                 constexpr int kC = decltype(c_tag)::value, kHits = decltype(hits_tag)::value;
-                if (gp.view_count > 1)
-                {
-                    if (p.allow_distortion)
-                        hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, true, true>), grid, blk, 0, stream, gp);
+                auto with_views = [&](auto distort_tag, auto drop_tag) {
+                    constexpr bool kDistort = decltype(distort_tag)::value, kDrop = decltype(drop_tag)::value;
+                    if (gp.view_count > 1)
+                        hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, kDistort, true, kDrop>), grid, blk, 0, stream, gp);
                     else
-                        hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, false, true>), grid, blk, 0, stream, gp);
-                }
-                else if (p.allow_distortion)
-                    hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, true>), grid, blk, 0, stream, gp);
-                else
-                    hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, false>), grid, blk, 0, stream, gp);
+                        hipLaunchKernelGGL((gather_point_gradients_kernel<kC, kHits, kDistort, false, kDrop>), grid, blk, 0, stream, gp);
+                };
+                const bool drop = gp.vp.dropout_bits.threshold != 0u;
+                if (p.allow_distortion && drop) with_views(std::true_type{}, std::true_type{});
+                else if (p.allow_distortion) with_views(std::true_type{}, std::false_type{});
+                else if (drop) with_views(std::false_type{}, std::true_type{});
+                else with_views(std::false_type{}, std::false_type{});
             };
             auto with_channels = [&](auto hits_tag) {
                 switch (C)
@@ -1307,6 +1313,76 @@ int vetrast_backward(vetrast_ctx* ctx, const vetrast_backward_args* g, void* str
                                background_rows_count, C, g->grad_background, g->grad_confidence, 0, v > 0 ? 1 : 0,
                                p.texture_abs ? a->background : nullptr);
         }
+    }
+    VET_HIP(ctx, hipGetLastError());
+    return VETRAST_OK;
+}
+
+int vetrast_point_weights(vetrast_ctx* ctx, const vetrast_point_weights_args* g, void* stream_)
+{
+    if (!ctx || !g) return VETRAST_ERR_INVALID_ARG;
+    const vetrast_forward_args* a = &g->fwd;
+    vetrast_workspace_layout lay;
+    const int st = validate_forward(a, &lay, /*for_backward=*/true);
+    if (st != VETRAST_OK) return st;
+    if (!a->save_for_backward || !(g->decay >= 0.f) || !std::isfinite(g->decay)) return VETRAST_ERR_INVALID_ARG;
+    if (a->num_points == 0) return VETRAST_OK;
+    if (!g->weight || !aligned_to(g->weight, 4)) return VETRAST_ERR_INVALID_ARG;
+    const vetrast_params& p = a->params;
+    hipStream_t stream      = (hipStream_t)stream_;
+    const int N = a->num_points, B = a->num_views, L = p.num_layers, hits = hits_of_mode(p.render_mode), lanes = std::max(1, lay.view_lanes);
+    const bool fuzzy        = p.render_mode == VETRAST_RENDER_FUZZY_BLEND;
+    void* ws                = a->workspace;
+    WeightPass f;
+    f.ly                    = make_call_layer_table(a->views[0].w, a->views[0].h, L, (int64_t)N * hits, p.expected_fragments);
+    f.index                 = a->index;
+    f.confidence            = a->confidence;
+    f.confidence_activation = p.confidence_activation;
+    f.confidence_scale      = p.confidence_scale;
+    f.N                     = N;
+    f.K                     = p.debug_max_list_length;
+    f.point_major           = views_see_little(p, N, hits) ? 1 : 0;
+    f.depth_accept          = p.depth_accept_blend;
+    f.group_base[0]         = 0;
+    for (int l = 0; l < VETRAST_MAX_LAYERS; ++l)
+    {
+        f.parts[l] = 1;
+        if (l >= L) continue;
+        const uint32_t tiles = f.ly.tile_base[l + 1] - f.ly.tile_base[l];
+        f.parts[l]           = fuzzy ? 1u : weight_parts((double)N * hits, tiles);
+        f.group_base[l + 1]  = f.group_base[l] + tiles * f.parts[l];
+    }
+    float* scratch = ws_ptr<float>(ws, lay.partial_base);
+    for (int first = 0; first < B; first += lanes)
+    {
+        const int count = std::min(B, first + lanes) - first;
+        for (int k = 0; k < count; ++k)
+        {
+            const int b     = first + k;
+            WeightView& v   = f.view[k];
+            v.offsets       = ws_ptr<uint32_t>(ws, lay.offsets_base + lay.offsets_stride * b);
+            v.kept          = ws_ptr<uint32_t>(ws, lay.kept_base + lay.kept_stride * b);
+            v.fragments     = ws_ptr<uint64_t>(ws, lay.fragments_base + lay.fragments_stride * b);
+            v.transmittance = ws_ptr<float>(ws, lay.transmittance_base + lay.transmittance_stride * b);
+            v.projected     = lay.projected_stride ? ws_ptr<float2>(ws, lay.projected_base + lay.projected_stride * b) : nullptr;
+            v.weights       = ws_ptr<float>(ws, lay.partial_base + lay.lane_scratch_stride * k);
+        }
+        launch_fragment_weights(f, hits, fuzzy, count, stream);
+        PointWeightPass s;
+        s.vp              = make_view_pass(a, lay, f.ly, first);
+        s.list_is_cut     = ws_ptr<uint8_t>(ws, lay.cut_flags_base + lay.cut_flags_stride * first);
+        s.last_key        = ws_ptr<uint64_t>(ws, lay.last_key_base + lay.last_key_stride * first);
+        s.weights         = scratch;
+        s.flags_stride    = lay.cut_flags_stride;
+        s.last_key_stride = lay.last_key_stride / sizeof(uint64_t);
+        s.weights_stride  = lay.lane_scratch_stride / sizeof(float);
+        s.view_count      = count;
+        s.K               = f.K;
+        s.point_major     = f.point_major;
+        s.decay           = g->decay;
+        s.accumulate      = first > 0 ? 1 : 0;
+        s.sum             = g->weight;
+        launch_point_weights(s, hits, stream);
     }
     VET_HIP(ctx, hipGetLastError());
     return VETRAST_OK;

@@ -234,10 +234,12 @@ class Rasterizer:
         return lay
 
     def forward(self, dev: DeviceScene, params: abi.Params = None, save_for_backward=True, workspace=None,
-                out=None, want_weight=False, point_order=None, packed=None) -> ForwardResult:
+                out=None, want_weight=False, point_order=None, packed=None, point_dropout=0.0, dropout_seed=0, dropout_step=0,
+                dropout_device_step=None) -> ForwardResult:
         """point_order: optional int32 device tensor [N], a permutation: the order the binning pass walks the points in.
         packed: optional float32 device tensor [N,8] from pack_descriptors: the call reads the descriptor records from
-        it instead of interleaving them itself."""
+        it instead of interleaving them itself. point_dropout, dropout_seed, dropout_step, dropout_device_step: drop-out of points
+        without a mask (vetrast_forward_args)."""
         scene = dev.scene
         params = params or make_params(scene)
         lay = self.layout(scene, params.render_mode)
@@ -271,8 +273,22 @@ class Rasterizer:
             assert packed.dtype == torch.float32 and packed.is_cuda and packed.is_contiguous()
             assert packed.numel() == 8 * scene.num_points
             args.packed_descriptors = packed.data_ptr()
+        args.point_dropout, args.dropout_seed, args.dropout_step = point_dropout, dropout_seed, dropout_step
+        if dropout_device_step is not None:
+            assert dropout_device_step.is_cuda and dropout_device_step.dtype == torch.int64 and dropout_device_step.numel() == 1
+            args.dropout_device_step = dropout_device_step.data_ptr()
         abi.check(self.lib.vetrast_forward(self.ctx, C.byref(args), self._stream()), "forward")
-        return ForwardResult(out, masks, workspace, lay, args, (views, dev, params, point_order, packed), weights)
+        return ForwardResult(out, masks, workspace, lay, args, (views, dev, params, point_order, packed, dropout_device_step), weights)
+
+    def point_weights(self, fwd: ForwardResult, weight, decay=1.0):
+        """Adds what every point gave to the pixels of a render to `weight` (float32 [N], in place), whose old values are multiplied by
+        `decay` first (vetrast_point_weights). fwd: a forward call with save_for_backward."""
+        assert weight.is_cuda and weight.is_contiguous() and weight.dtype == torch.float32 and weight.numel() == fwd.args.num_points
+        a = abi.PointWeightsArgs()
+        C.memmove(C.byref(a.fwd), C.byref(fwd.args), C.sizeof(abi.ForwardArgs))
+        a.weight, a.decay = weight.data_ptr(), decay
+        abi.check(self.lib.vetrast_point_weights(self.ctx, C.byref(a), self._stream()), "point_weights")
+        return weight
 
     def pack_descriptors(self, dev: DeviceScene, params: abi.Params, out=None) -> torch.Tensor:
         """The descriptor records [N,8] of the scene's texture and confidence under `params` (vetrast_pack_descriptors),

@@ -66,6 +66,12 @@ void check_f32_cuda(const torch::Tensor& t, const char* name)
                 " must be a contiguous float32 tensor on the GPU");
 }
 
+// Points are left out without a mask.
+bool random_dropout(const NeuralRenderInfo* info)
+{
+    return info->train && info->params.dropout > 0 && info->params.dropout_seed >= 0;
+}
+
 // Fills the part of the argument struct that forward and backward share. `info->images` must outlive the call.
 vetrast_forward_args make_forward_args(NeuralRenderInfo* info, const torch::Tensor& texture,
                                        const torch::Tensor& background_color, const torch::Tensor& points,
@@ -116,6 +122,19 @@ vetrast_forward_args make_forward_args(NeuralRenderInfo* info, const torch::Tens
     RenderParams prm         = info->params;
     prm.num_texture_channels = (int)texture.size(0);
     a.params                 = to_abi_params(prm, info->num_layers);
+    if (random_dropout(info))
+    {
+        a.point_dropout = info->params.dropout;
+        a.dropout_seed  = (uint64_t)info->params.dropout_seed;
+        a.dropout_step  = (uint64_t)info->params.dropout_step;
+        const torch::Tensor& count = info->dropout_device_step;
+        if (count.defined())
+        {
+            TORCH_CHECK(count.device() == points.device() && count.scalar_type() == torch::kInt64 && count.numel() == 1,
+                        "dropout_device_step is one int64 on the points' GPU");
+            a.dropout_device_step = count.data_ptr<int64_t>();
+        }
+    }
     return a;
 }
 
@@ -325,7 +344,7 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
 
     // dropout mask per view, PointRenderer.cu:461-468 (the mask is 1 where a point is dropped)
     torch::Tensor dropout;
-    if (info->train && info->params.dropout > 0) dropout = torch::empty({B, N}, f32).bernoulli_(info->params.dropout);
+    if (info->train && info->params.dropout > 0 && !random_dropout(info)) dropout = torch::empty({B, N}, f32).bernoulli_(info->params.dropout);
 
     if (info->params.size_bins_from_history)
         info->cache->ExpectedFragments(info->params.expected_fragments, N, L, info->images[0].w, info->images[0].h,
@@ -343,6 +362,13 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
     const bool need_backward =
         ctx != nullptr && info->grad_mode && (texture.requires_grad() || background_color.requires_grad() || points.requires_grad() ||
                            confidence.requires_grad() || pose_tangents.requires_grad() || intrinsics.requires_grad());
+    const torch::Tensor& point_weight = info->point_weight;
+    if (point_weight.defined())
+    {
+        check_f32_cuda(point_weight, "point_weight");
+        TORCH_CHECK(point_weight.device() == points.device() && point_weight.numel() == N, "point_weight must have one element for each point, on their GPU");
+        TORCH_CHECK(!point_weight.requires_grad(), "point_weight is written in place and must not require a gradient");
+    }
     // Kept descriptor records only serve calls without a backward pass. The interleave inside a call is also what
     // brings the rows into the last-level cache for the gathers of the backward pass: measured with kept records, the
     // forward call is 9 us faster and the backward call 12 us slower at 2 M points.
@@ -362,9 +388,9 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
     }
     else
     {
-        auto& ws = info->cache->eval_workspace;
-        if (!ws.defined() || ws.numel() < (int64_t)lay.forward_only_bytes || ws.device() != points.device())
-            ws = torch::empty({(int64_t)lay.forward_only_bytes}, u8);
+        auto& ws           = info->cache->eval_workspace;
+        const int64_t need = (int64_t)(point_weight.defined() ? lay.total_bytes : lay.forward_only_bytes);
+        if (!ws.defined() || ws.numel() < need || ws.device() != points.device()) ws = torch::empty({need}, u8);
         workspace = ws;
     }
 
@@ -395,7 +421,7 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
     }
     a.workspace         = workspace.data_ptr();
     a.workspace_bytes   = (size_t)workspace.numel();
-    a.save_for_backward = need_backward ? 1 : 0;
+    a.save_for_backward = need_backward || point_weight.defined() ? 1 : 0;
     const torch::Tensor& order = info->cache->PointOrderFor(points);
     a.point_order              = order.defined() ? order.data_ptr<int32_t>() : nullptr;
     check_status(vetrast_forward(info->cache->ctx, &a, current_stream()), "forward");
@@ -403,6 +429,12 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
     {
         info->cache->FinishIntrinsicsCheck();  // may throw: nothing of this call has been handed out yet
         info->cache->NoteDeviceFlags(workspace, lay);
+    }
+    if (point_weight.defined())
+    {
+        vetrast_point_weights_args w{a, point_weight.data_ptr<float>(), info->point_weight_decay, 0};
+        check_status(vetrast_point_weights(info->cache->ctx, &w, current_stream()), "point_weights");
+        if (!point_weight.is_inference()) point_weight.unsafeGetTensorImpl()->bump_version();
     }
     if (info->cache->keep_layer_weights) info->cache->layer_weights = std::move(weights);
     if (info->params.size_bins_from_history)
@@ -416,7 +448,10 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
         saved.insert(saved.end(), out.begin(), out.end());
         if (dropout.defined()) saved.push_back(dropout);
         if (t_index.defined()) saved.push_back(t_index);
+        const bool counted = random_dropout(info) && info->dropout_device_step.defined();
+        if (counted) saved.push_back(info->dropout_device_step);  // noticed there if somebody has written it meanwhile
         ctx->save_for_backward(saved);
+        ctx->saved_data["counted"]     = counted;
         ctx->saved_data["has_dropout"] = dropout.defined();
         ctx->saved_data["has_index"]   = t_index.defined();
         ctx->saved_data["points_need_grad"] = points.requires_grad();
@@ -452,7 +487,7 @@ torch::autograd::variable_list PointRender::backward(torch::autograd::AutogradCo
     const bool has_dropout   = ctx->saved_data["has_dropout"].toBool();
     const bool has_index     = ctx->saved_data["has_index"].toBool();
     constexpr int kFixed     = 7;
-    TORCH_CHECK((int)saved.size() == kFixed + L + (has_dropout ? 1 : 0) + (has_index ? 1 : 0),
+    TORCH_CHECK((int)saved.size() == kFixed + L + (has_dropout ? 1 : 0) + (has_index ? 1 : 0) + (ctx->saved_data["counted"].toBool() ? 1 : 0),
                 "unexpected number of saved tensors");  // PointRenderer.cu:1163-1164
     TORCH_CHECK((int)grad_output.size() >= L, "expected one upstream gradient per layer");  // PointRenderer.cu:1158-1159
     torch::Tensor workspace = saved[0], texture = saved[1], background_color = saved[2], points = saved[3],
@@ -970,7 +1005,10 @@ std::vector<torch::Tensor> blend_point_cloud(torch::Tensor texture, torch::Tenso
                                              torch::Tensor pose_tangents, torch::Tensor intrinsics,
                                              torch::Tensor confidence, torch::Tensor poses_se3, torch::Tensor t_index,
                                              std::vector<std::vector<double>> views, int num_layers, bool train,
-                                             pybind11::dict params, pybind11::object environment)
+                                             pybind11::dict params, pybind11::object environment,
+                                             const std::optional<torch::Tensor>& point_weight, double point_weight_decay,
+                                             int64_t dropout_seed, int64_t dropout_step,
+                                             const std::optional<torch::Tensor>& dropout_device_step)
 {
     using namespace vet_amd;
     if (!g_cache) g_cache = std::make_shared<PointRendererCache>();
@@ -1007,6 +1045,11 @@ std::vector<torch::Tensor> blend_point_cloud(torch::Tensor texture, torch::Tenso
     }
     RenderParams& p = nri.params;
     p.dropout       = 0.f;
+    p.dropout_seed  = dropout_seed;
+    p.dropout_step  = dropout_step;
+    if (dropout_device_step.has_value()) nri.dropout_device_step = *dropout_device_step;
+    if (point_weight.has_value()) nri.point_weight = *point_weight;
+    nri.point_weight_decay = (float)point_weight_decay;
     bool super_sampling = false, cat_masks_to_color = false, cat_env_to_color = false, no_envmap_at_points = true;
     for (auto item : params)
     {
@@ -1451,6 +1494,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("points"), pybind11::arg("pose_tangents"), pybind11::arg("intrinsics"), pybind11::arg("confidence"),
           pybind11::arg("poses_se3"), pybind11::arg("t_index"), pybind11::arg("views"), pybind11::arg("num_layers"),
           pybind11::arg("train"), pybind11::arg("params"), pybind11::arg("environment") = pybind11::none(),
+          pybind11::arg("point_weight") = pybind11::none(), pybind11::arg("point_weight_decay") = 1.0, pybind11::arg("dropout_seed") = -1,
+          pybind11::arg("dropout_step") = 0, pybind11::arg("dropout_device_step") = pybind11::none(),
           "BlendPointCloud(NeuralRenderInfo*) of the reference, with the scene passed as tensors; `environment`, a "
           "callable (layers[l][b] weight tensors) -> L tensors, routes the call through the render module's "
           "environment-map branch");

@@ -26,6 +26,11 @@ struct RenderParams
 {
     bool check_normal                  = false;
     float dropout                      = 0.25f;
+    // Not in the reference. From 0 on: points are left out by random bits that the kernels find out by themselves, a function of this seed, of
+    // dropout_step (count it up from step to step) and of NeuralRenderInfo::dropout_device_step (vetrast_forward_args.point_dropout),
+    // instead of a mask [B,N] that torch's generator draws and that is kept for the backward pass.
+    int64_t dropout_seed               = -1;
+    int64_t dropout_step               = 0;
     float drop_out_radius_threshold    = 0.6f;
     float K_gradient_factor            = 0.5f;
     float distortion_gradient_factor   = 0.005f;  // src/lib/data/Settings.h:54
@@ -232,6 +237,12 @@ class NeuralRenderInfo : public torch::CustomClassHolder
     int current_epoch        = 0;
     void* timer_system       = nullptr;  // accepted for signature parity; per-kernel times come from vetrast_scope_times
     PointRendererCache* cache = nullptr;
+    // Not in the reference. Where defined, float32 [N]: what every point gave to the pixels of this call (vetrast_point_weights) is added to it, its
+    // old values times point_weight_decay. What SelectKept (entries.h) takes.
+    torch::Tensor point_weight;
+    float point_weight_decay = 1.f;
+    // Where defined, int64 [1] on the GPU: added to RenderParams::dropout_step. Not to be written between a forward pass and its backward pass.
+    torch::Tensor dropout_device_step;
 };
 
 struct PointRender : public torch::autograd::Function<PointRender>

@@ -21,7 +21,8 @@ def load():
 
 
 def blend_point_cloud(texture, background_color, points, pose_tangents, intrinsics, confidence, poses_se3, t_index,
-                      views, num_layers, train=False, environment=None, **params):
+                      views, num_layers, train=False, environment=None, point_weight=None, point_weight_decay=1.0, dropout_seed=-1,
+                      dropout_step=0, dropout_device_step=None, **params):
     """BlendPointCloud of the reference (src/lib/rendering/PointRenderer.h:53) on tensors; differentiable.
 
     views: list of (w, h, image_index, camera_index, camera_model, crop fx,fy,cx,cy,s, rot r00,r01,r10,r11).
@@ -32,12 +33,17 @@ def blend_point_cloud(texture, background_color, points, pose_tangents, intrinsi
     (src/lib/rendering/RenderModule.cpp:129-202): it gets layers[l][b] = the [1,1,h_l,w_l] per-pixel transmittance left
     behind the points and returns L tensors [B,C_env,h_l,w_l]; they are added to the images (masked with
     no_envmap_at_points, the default) or appended as channels (cat_env_to_color). Needs output_background_mask.
+    point_weight: float32 [N], to which what every point gave to the pixels of this call is added in place, its old values times
+    point_weight_decay (vetrast_point_weights); what select_kept takes.
+    dropout_seed: from 0 on, the points that `dropout` leaves out in training are a function of seed, dropout_step and dropout_device_step (int64 [1] on the
+    GPU, or None), without a mask in memory; negative: torch's generator draws a mask.
     """
     if t_index is None:
         t_index = _no_index
     return load().blend_point_cloud(texture, background_color, points, pose_tangents, intrinsics, confidence, poses_se3,
                                     t_index, [list(map(float, v)) for v in views], int(num_layers), bool(train),
-                                    {k: float(v) for k, v in params.items()}, environment)
+                                    {k: float(v) for k, v in params.items()}, environment, point_weight, float(point_weight_decay),
+                                    int(dropout_seed), int(dropout_step), dropout_device_step)
 
 
 def adapter_selftest(texture, background_color, points, pose_tangents, intrinsics, confidence, poses_se3, views,
