@@ -1341,16 +1341,17 @@ int vetrast_point_weights(vetrast_ctx* ctx, const vetrast_point_weights_args* g,
     f.confidence_scale      = p.confidence_scale;
     f.N                     = N;
     f.K                     = p.debug_max_list_length;
-    f.point_major           = views_see_little(p, N, hits) ? 1 : 0;
     f.depth_accept          = p.depth_accept_blend;
-    f.group_base[0]         = 0;
+    f.share_base[0]    = 0;
     for (int l = 0; l < VETRAST_MAX_LAYERS; ++l)
     {
-        f.parts[l] = 1;
+        f.parts[l] = f.shares[l] = 0;
+        f.share_base[l + 1] = f.share_base[l];
         if (l >= L) continue;
         const uint32_t tiles = f.ly.tile_base[l + 1] - f.ly.tile_base[l];
-        f.parts[l]           = fuzzy ? 1u : weight_parts((double)N * hits, tiles);
-        f.group_base[l + 1]  = f.group_base[l] + tiles * f.parts[l];
+        f.parts[l]           = weight_parts((double)N * hits, tiles);
+        f.shares[l]          = (tiles * f.parts[l] + kXcds * (kBlock / kWave) - 1) / (kXcds * (kBlock / kWave));
+        f.share_base[l + 1] += f.shares[l];
     }
     float* scratch = ws_ptr<float>(ws, lay.partial_base);
     for (int first = 0; first < B; first += lanes)
@@ -1364,21 +1365,19 @@ int vetrast_point_weights(vetrast_ctx* ctx, const vetrast_point_weights_args* g,
             v.kept          = ws_ptr<uint32_t>(ws, lay.kept_base + lay.kept_stride * b);
             v.fragments     = ws_ptr<uint64_t>(ws, lay.fragments_base + lay.fragments_stride * b);
             v.transmittance = ws_ptr<float>(ws, lay.transmittance_base + lay.transmittance_stride * b);
-            v.projected     = lay.projected_stride ? ws_ptr<float2>(ws, lay.projected_base + lay.projected_stride * b) : nullptr;
-            v.weights       = ws_ptr<float>(ws, lay.partial_base + lay.lane_scratch_stride * k);
+            v.slots         = ws_ptr<float>(ws, lay.partial_base + lay.lane_scratch_stride * k);
         }
         launch_fragment_weights(f, hits, fuzzy, count, stream);
         PointWeightPass s;
         s.vp              = make_view_pass(a, lay, f.ly, first);
         s.list_is_cut     = ws_ptr<uint8_t>(ws, lay.cut_flags_base + lay.cut_flags_stride * first);
         s.last_key        = ws_ptr<uint64_t>(ws, lay.last_key_base + lay.last_key_stride * first);
-        s.weights         = scratch;
+        s.slots           = scratch;
         s.flags_stride    = lay.cut_flags_stride;
         s.last_key_stride = lay.last_key_stride / sizeof(uint64_t);
-        s.weights_stride  = lay.lane_scratch_stride / sizeof(float);
+        s.slots_stride    = lay.lane_scratch_stride / sizeof(float);
         s.view_count      = count;
-        s.K               = f.K;
-        s.point_major     = f.point_major;
+        s.fuzzy           = fuzzy ? 1 : 0;
         s.decay           = g->decay;
         s.accumulate      = first > 0 ? 1 : 0;
         s.sum             = g->weight;
