@@ -115,13 +115,16 @@ __global__ void __launch_bounds__(kSelectThreads) select_row_kernel(SelectPass a
     const RowRange r   = row_range(a, row);
     const float* score = a.score + (int64_t)row * a.row_stride;
     int32_t* index     = a.index + (int64_t)row * a.budget;
+    float raw[ITEMS];
     uint32_t key[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
     {
         const int i = k * kSelectThreads + (int)threadIdx.x;
-        key[k]      = i < r.range ? score_key(score[i]) : 0u;
+        raw[k]      = r.range > 0 ? score[min(i, r.range - 1)] : 0.f;  // without branches, so that all are under way before the first is looked at
     }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) key[k] = score_key(raw[k]);
     uint32_t prefix = 0, mask = 0, left = (uint32_t)r.need;
     if (r.range > 0 && r.need > 0)
     {

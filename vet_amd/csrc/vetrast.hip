@@ -1349,7 +1349,7 @@ int vetrast_point_weights(vetrast_ctx* ctx, const vetrast_point_weights_args* g,
         f.share_base[l + 1] = f.share_base[l];
         if (l >= L) continue;
         const uint32_t tiles = f.ly.tile_base[l + 1] - f.ly.tile_base[l];
-        f.parts[l]           = weight_parts((double)N * hits, tiles);
+        f.parts[l]           = weight_parts((double)N * hits, tiles, hits);
         f.shares[l]          = (tiles * f.parts[l] + kXcds * (kBlock / kWave) - 1) / (kXcds * (kBlock / kWave));
         f.share_base[l + 1] += f.shares[l];
     }
