@@ -57,26 +57,24 @@ inline bool overlap(const void* a, const void* b, size_t bytes)
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x != y && (x < y ? y - x : x - y) < bytes;
 }
-// Rows of more entries than a workgroup holds are shared by several: 8 entries a thread each, or more where there are many workgroups.
-constexpr int kSelectShare    = 8 * kSelectThreads;
+// Rows of more entries than a workgroup holds are shared by several: a piece of 8 entries a thread each, or more where there are many.
 constexpr int kSelectGroups   = 1024;   // workgroups of a row at most
 constexpr int kSelectGridRows = 32768;  // rows of a launch
 inline int select_share(int n)
 {
-    const int64_t groups = std::min<int64_t>(((int64_t)n + kSelectShare - 1) / kSelectShare, kSelectGroups);
-    return (int)((((int64_t)n + groups - 1) / groups + kSelectThreads - 1) / kSelectThreads * kSelectThreads);
+    const int64_t pieces = ((int64_t)n + kSharePiece - 1) / kSharePiece;
+    return (int)((pieces + kSelectGroups - 1) / kSelectGroups) * kSharePiece;
 }
 inline int select_groups(int n) { return (int)(((int64_t)n + select_share(n) - 1) / select_share(n)); }
 inline size_t select_words(int n) { return kDigits * (size_t)kBins + 2 * (size_t)select_groups(n); }  // of a row
 
 void launch_select_row(const SelectPass& p, hipStream_t stream)
 {
-    const dim3 grid((uint32_t)p.rows), block(kSelectThreads);
-    const int items = (p.n + kSelectThreads - 1) / kSelectThreads;
-    if (items <= 1) hipLaunchKernelGGL((select_row_kernel<1>), grid, block, 0, stream, p);
-    else if (items <= 4) hipLaunchKernelGGL((select_row_kernel<4>), grid, block, 0, stream, p);
-    else if (items <= 12) hipLaunchKernelGGL((select_row_kernel<12>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((select_row_kernel<32>), grid, block, 0, stream, p);
+    const dim3 grid((uint32_t)p.rows);
+    if (p.n <= 4 * kBlock) hipLaunchKernelGGL((select_row_kernel<kBlock, 1>), grid, dim3(kBlock), 0, stream, p);
+    else if (p.n <= 4 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 1>), grid, dim3(kSelectThreads), 0, stream, p);
+    else if (p.n <= 12 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 3>), grid, dim3(kSelectThreads), 0, stream, p);
+    else hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 8>), grid, dim3(kSelectThreads), 0, stream, p);
 }
 
 void launch_select_rows(SelectPass p, char* workspace, hipStream_t stream)

@@ -10,7 +10,6 @@
 namespace vetrast
 {
 constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves   = kSelectThreads / kWave;
 constexpr int kDigits        = 3;
 constexpr uint32_t kBins     = 2048;
 constexpr int kSelectRowMost = 32 * kSelectThreads;  // entries of a row that one workgroup holds in registers
@@ -38,7 +37,7 @@ struct SelectPass
     // rows of several workgroups
     uint32_t* histogram;  // [rows][kDigits][kBins]
     uint2* counts;        // [rows][groups]: above the threshold, at it
-    int share, groups;    // entries of a workgroup (a multiple of kSelectThreads), workgroups of a row
+    int share, groups;    // entries of a workgroup (a multiple of kSharePiece), workgroups of a row
 };
 
 // What a row is asked for: `need` of its first `range` entries, and all from there to `length`.
@@ -56,14 +55,17 @@ __device__ __forceinline__ RowRange row_range(const SelectPass& a, int row)
     return r;
 }
 
+// A thread has groups of four neighbouring entries: entry 4 * (group * THREADS + thread) + k.
+template <int THREADS>
 struct SelectRoom
 {
     uint32_t bins[kBins];
-    uint32_t sums[kSelectWaves];
+    uint32_t sums[THREADS / kWave];
     uint32_t bin, left;
 };
 
 // Inclusive sum over the workgroup's threads; all take part.
+template <int THREADS>
 __device__ __forceinline__ uint32_t group_inclusive_scan(uint32_t v, uint32_t* sums)
 {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -72,124 +74,194 @@ __device__ __forceinline__ uint32_t group_inclusive_scan(uint32_t v, uint32_t* s
     __syncthreads();
     uint32_t before = 0;
 #pragma unroll
-    for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? sums[w] : 0u;
+    for (int w = 0; w < THREADS / kWave; ++w) before += w < wave ? sums[w] : 0u;
     return v + before;
 }
 
-// From the counts of two neighbouring bins a thread, the bin that the need-th largest lies in, and how many of it are needed
-// (room.bin, room.left). need is at least 1 and at most the sum of all.
-__device__ __forceinline__ void find_bin(SelectRoom& room, uint32_t upper, uint32_t lower, uint32_t need)
+// The bin that the need-th largest lies in, and how many of it are needed (room.bin, room.left), from the counts in `bins` (room.bins, or those in
+// memory). need is at least 1 and at most the sum of all.
+template <int THREADS>
+__device__ __forceinline__ void find_bin(SelectRoom<THREADS>& room, const uint32_t* bins, uint32_t need)
 {
-    const uint32_t sum = group_inclusive_scan(upper + lower, room.sums), before = sum - upper - lower;
-    if (before < need && need <= sum)
+    constexpr uint32_t kEach = kBins / THREADS;
+    const uint32_t top       = kBins - kEach * (threadIdx.x + 1);  // the lowest of this thread's bins
+    uint32_t counts[kEach], sum = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) counts[k] = bins[top + k];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) sum += counts[k];
+    const uint32_t end = group_inclusive_scan<THREADS>(sum, room.sums);
+    if (end - sum < need && need <= end)
     {
-        const bool first = need <= before + upper;
-        room.bin         = kBins - 1 - 2 * threadIdx.x - (first ? 0 : 1);
-        room.left        = need - before - (first ? 0 : upper);
+        uint32_t before = end - sum;
+#pragma unroll
+        for (int k = kEach - 1; k >= 0; --k)
+        {
+            if (before < need && need <= before + counts[k]) room.bin = top + k, room.left = need - before;
+            before += counts[k];
+        }
     }
     __syncthreads();
 }
 
-// Counts one key in the histogram. A third of a cloud may be seen by no view: equal scores of zero would queue up at one address.
-__device__ __forceinline__ void count_key(SelectRoom& room, bool there, uint32_t key, int digit)
+template <int THREADS>
+__device__ __forceinline__ void clear_bins(SelectRoom<THREADS>& room)
 {
-    const bool zero      = there && key == kZeroKey;
-    const uint64_t zeros = __ballot(zero);
-    if (zeros && threadIdx.x % kWave == 0) atomicAdd(&room.bins[digit_of(kZeroKey, digit)], (uint32_t)__popcll(zeros));
-    if (there && !zero) atomicAdd(&room.bins[digit_of(key, digit)], 1u);
+#pragma unroll
+    for (uint32_t k = 0; k < kBins; k += THREADS) room.bins[k + threadIdx.x] = 0u;
+    __syncthreads();
 }
 
-__device__ __forceinline__ void clear_bins(SelectRoom& room)
+// Scores that two thirds of a scene's points may share, as no view has seen them, are counted by the thread and not in LDS, where they would queue up at one address.
+__device__ __forceinline__ void count_key(uint32_t* bins, uint32_t& zeros, bool there, uint32_t key, int digit)
 {
-    room.bins[threadIdx.x] = room.bins[threadIdx.x + kSelectThreads] = 0u;
+    const bool zero = key == kZeroKey;
+    zeros += there && zero;
+    if (there && !zero) atomicAdd(&bins[digit_of(key, digit)], 1u);
+}
+__device__ __forceinline__ void count_zeros(uint32_t* bins, uint32_t zeros, int digit)
+{
+    zeros = wave_inclusive_scan(zeros, 0);
+    if (threadIdx.x % kWave == kWave - 1 && zeros) atomicAdd(&bins[digit_of(kZeroKey, digit)], zeros);
+}
+
+// Four neighbouring scores, the first of them entry i; those from `end` on are some others of the row (end is at least 1).
+__device__ __forceinline__ void load_scores(const float* score, int i, int end, float* raw)
+{
+    if (i + 4 <= end)
+    {
+        const uint4 x = load_four(reinterpret_cast<const char*>(score + i));
+        raw[0] = __uint_as_float(x.x), raw[1] = __uint_as_float(x.y), raw[2] = __uint_as_float(x.z), raw[3] = __uint_as_float(x.w);
+    }
+    else
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[k] = score[min(i + k, end - 1)];
+    }
+}
+
+// Places of the entries that stay, in order. key: GROUPS groups of four a thread, of entries first + ..., those from `last` on are not counted; threshold and
+// left: as found; larger, equal: entries above and at the threshold in front of these.
+template <int THREADS, int GROUPS>
+__device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], int first, int last, uint32_t threshold, uint32_t left, uint32_t larger, uint32_t equal,
+                                            int32_t* index, uint32_t (&totals)[GROUPS * (THREADS / kWave)])
+{
+    constexpr int kWaves = THREADS / kWave;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    uint32_t counts[GROUPS], ends[GROUPS];  // of a thread's four: above the threshold in the lower half, at it in the upper
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+    {
+        const int i = first + 4 * (g * THREADS + (int)threadIdx.x);
+        counts[g]   = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const bool there = i + k < last;
+            counts[g] += there && key[4 * g + k] > threshold ? 1u : 0u;
+            counts[g] += there && key[4 * g + k] == threshold ? 1u << 16 : 0u;
+        }
+        ends[g] = wave_inclusive_scan(counts[g], lane);
+        if (lane == kWave - 1) totals[g * kWaves + wave] = ends[g];
+    }
     __syncthreads();
+    // (at most 32768 entries: neither half runs over)
+    if (wave == 0)
+    {
+        uint32_t before = 0;
+#pragma unroll
+        for (int t = 0; t < GROUPS * kWaves; t += kWave)
+        {
+            const uint32_t own = t + lane < GROUPS * kWaves ? totals[t + lane] : 0u, end = wave_inclusive_scan(own, lane);
+            if (t + lane < GROUPS * kWaves) totals[t + lane] = before + end - own;
+            before += (uint32_t)__builtin_amdgcn_readlane((int)end, kWave - 1);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+    {
+        const int i             = first + 4 * (g * THREADS + (int)threadIdx.x);
+        const uint32_t in_front = totals[g * kWaves + wave] + ends[g] - counts[g];
+        uint32_t more = larger + (in_front & 0xFFFFu), same = equal + (in_front >> 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const bool there = i + k < last, above = there && key[4 * g + k] > threshold, at = there && key[4 * g + k] == threshold;
+            if (above || (at && same < left)) index[more + min(same, left)] = i + k;
+            more += above, same += at;
+        }
+    }
 }
 
 // One workgroup for a row, its keys in registers.
-template <int ITEMS>
-__global__ void __launch_bounds__(kSelectThreads) select_row_kernel(SelectPass a)
+template <int THREADS, int GROUPS>
+__global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 {
-    __shared__ SelectRoom room;
-    __shared__ uint32_t places[ITEMS * kSelectWaves + 1];
-    const int row = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    __shared__ SelectRoom<THREADS> room;
+    __shared__ uint32_t totals[GROUPS * (THREADS / kWave)];
+    const int row      = blockIdx.x;
     const RowRange r   = row_range(a, row);
     const float* score = a.score + (int64_t)row * a.row_stride;
     int32_t* index     = a.index + (int64_t)row * a.budget;
-    float raw[ITEMS];
-    uint32_t key[ITEMS];
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-    {
-        const int i = k * kSelectThreads + (int)threadIdx.x;
-        raw[k]      = r.range > 0 ? score[min(i, r.range - 1)] : 0.f;  // without branches, so that all are under way before the first is looked at
-    }
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) key[k] = score_key(raw[k]);
-    uint32_t prefix = 0, mask = 0, left = (uint32_t)r.need;
     if (r.range > 0 && r.need > 0)
     {
+        float raw[4 * GROUPS];
+        uint32_t key[4 * GROUPS];
+        const int mine = 4 * (int)threadIdx.x;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            if (4 * g * THREADS < r.range) load_scores(score, 4 * g * THREADS + mine, r.range, raw + 4 * g);  // (the same branch in all threads)
+#pragma unroll
+        for (int k = 0; k < 4 * GROUPS; ++k) key[k] = score_key(raw[k]);
+        uint32_t threshold = 0, mask = 0, left = (uint32_t)r.need;
+#pragma unroll
         for (int digit = 0; digit < kDigits; ++digit)
         {
             clear_bins(room);
+            uint32_t zeros = 0;
 #pragma unroll
-            for (int k = 0; k < ITEMS; ++k)
-            {
-                const int i = k * kSelectThreads + (int)threadIdx.x;
-                count_key(room, i < r.range && (key[k] & mask) == prefix, key[k], digit);
-            }
+            for (int g = 0; g < GROUPS; ++g)
+                if (4 * g * THREADS < r.range)
+                {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        count_key(room.bins, zeros, 4 * g * THREADS + mine + k < r.range && (key[4 * g + k] & mask) == threshold, key[4 * g + k], digit);
+                }
+            count_zeros(room.bins, zeros, digit);
             __syncthreads();
-            find_bin(room, room.bins[kBins - 1 - 2 * threadIdx.x], room.bins[kBins - 2 - 2 * threadIdx.x], left);
+            find_bin(room, room.bins, left);
             left = room.left;
-            prefix |= room.bin << digit_shift(digit);
+            threshold |= room.bin << digit_shift(digit);
             mask |= (digit == 2 ? 1023u : 2047u) << digit_shift(digit);
             __syncthreads();
         }
-        // places: entries above the threshold in front of a wave's 64 (lower half), entries at it (upper half)
-        uint64_t above[ITEMS], at[ITEMS];
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k)
-        {
-            const int i = k * kSelectThreads + (int)threadIdx.x;
-            above[k]    = __ballot(i < r.range && key[k] > prefix);
-            at[k]       = __ballot(i < r.range && key[k] == prefix);
-            if (lane == 0) places[k * kSelectWaves + wave] = (uint32_t)__popcll(above[k]) | (uint32_t)__popcll(at[k]) << 16;
-        }
-        __syncthreads();
-        const uint32_t mine = threadIdx.x < (uint32_t)(ITEMS * kSelectWaves) ? places[threadIdx.x] : 0u;
-        const uint32_t sum  = group_inclusive_scan(mine, room.sums);
-        if (threadIdx.x < (uint32_t)(ITEMS * kSelectWaves)) places[threadIdx.x] = sum - mine;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k)
-        {
-            const int i             = k * kSelectThreads + (int)threadIdx.x;
-            const uint32_t in_front = places[k * kSelectWaves + wave];
-            const auto below = [](uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
-            const uint32_t larger = (in_front & 0xFFFFu) + below(above[k]), equal = (in_front >> 16) + below(at[k]);
-            const bool stays      = i < r.range && (key[k] > prefix || (key[k] == prefix && equal < left));
-            if (stays) index[larger + min(equal, left)] = i;
-        }
+        give_places<THREADS, GROUPS>(key, 0, r.range, threshold, left, 0, 0, index, totals);
     }
     const int selected = min(r.need, r.range), total = selected + r.length - r.range;
-    for (int i = (int)threadIdx.x; i < a.budget - selected; i += kSelectThreads) index[selected + i] = i < r.length - r.range ? r.range + i : -1;
+    for (int i = (int)threadIdx.x; i < a.budget - selected; i += THREADS) index[selected + i] = i < r.length - r.range ? r.range + i : -1;
     if (threadIdx.x == 0) a.count[row] = total;
 }
 
 // ---- rows of several workgroups: a launch for each digit, one that counts and one that gives places ---------------------------
+
+constexpr int kShareGroups = 2;  // groups of four of a thread under way at once
+constexpr int kSharePiece  = 4 * kShareGroups * kSelectThreads;
 
 __global__ void __launch_bounds__(kBlock) select_clear_kernel(uint32_t* p, size_t n)
 {
     for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) p[i] = 0u;
 }
 
+using SharedRoom = SelectRoom<kSelectThreads>;
+
 // The threshold's digits in front of `digits`, from the histograms that are there, and how many at it are needed.
-__device__ __forceinline__ uint32_t known_digits(const SelectPass& a, SelectRoom& room, int row, int digits, uint32_t& left)
+__device__ __forceinline__ uint32_t known_digits(const SelectPass& a, SharedRoom& room, int row, int digits, uint32_t& left)
 {
     uint32_t prefix = 0;
     for (int digit = 0; digit < digits; ++digit)
     {
-        const uint2 pair = reinterpret_cast<const uint2*>(a.histogram + ((size_t)row * kDigits + digit) * kBins)[kBins / 2 - 1 - threadIdx.x];
-        find_bin(room, pair.y, pair.x, left);
+        find_bin(room, a.histogram + ((size_t)row * kDigits + digit) * kBins, left);
         left = room.left;
         prefix |= room.bin << digit_shift(digit);
         __syncthreads();
@@ -197,106 +269,138 @@ __device__ __forceinline__ uint32_t known_digits(const SelectPass& a, SelectRoom
     return prefix;
 }
 
+// A piece of a share: keys of kShareGroups groups of four a thread, from entry `base` on. Loads come first.
+struct Piece
+{
+    float raw[4 * kShareGroups];
+    __device__ __forceinline__ Piece(const float* score, int base, int last)
+    {
+#pragma unroll
+        for (int g = 0; g < kShareGroups; ++g) load_scores(score, base + 4 * (g * kSelectThreads + (int)threadIdx.x), last, raw + 4 * g);
+    }
+    __device__ __forceinline__ static int entry(int base, int k) { return base + 4 * (k / 4 * kSelectThreads + (int)threadIdx.x) + k % 4; }
+};
+
 template <int DIGIT>
 __global__ void __launch_bounds__(kSelectThreads) select_digit_kernel(SelectPass a)
 {
-    __shared__ SelectRoom room;
+    __shared__ SharedRoom room;
     const int row    = blockIdx.y;
     const RowRange r = row_range(a, row);
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     if (r.need <= 0 || first >= last) return;
-    uint32_t left         = (uint32_t)r.need;
-    const uint32_t prefix = known_digits(a, room, row, DIGIT, left);
-    const uint32_t mask   = DIGIT == 0 ? 0u : ~0u << digit_shift(DIGIT - 1);
-    clear_bins(room);
     const float* score = a.score + (int64_t)row * a.row_stride;
-    for (int base = first; base < last; base += kSelectThreads)
+    uint32_t left = (uint32_t)r.need, zeros = 0, prefix = 0;
+    constexpr uint32_t kMask = DIGIT == 0 ? 0u : ~0u << digit_shift(DIGIT == 0 ? 0 : DIGIT - 1);
+    for (int base = first; base < last; base += kSharePiece)
     {
-        const int i        = base + (int)threadIdx.x;
-        const uint32_t key = i < last ? score_key(score[i]) : 0u;
-        count_key(room, i < last && (key & mask) == prefix, key, DIGIT);
+        const Piece piece(score, base, last);
+        if (base == first)  // while the loads are under way
+        {
+            prefix = known_digits(a, room, row, DIGIT, left);
+            clear_bins(room);
+        }
+#pragma unroll
+        for (int k = 0; k < 4 * kShareGroups; ++k)
+        {
+            const uint32_t key = score_key(piece.raw[k]);
+            count_key(room.bins, zeros, Piece::entry(base, k) < last && (key & kMask) == prefix, key, DIGIT);
+        }
     }
+    count_zeros(room.bins, zeros, DIGIT);
     __syncthreads();
     uint32_t* histogram = a.histogram + ((size_t)row * kDigits + DIGIT) * kBins;
 #pragma unroll
-    for (uint32_t k = 0; k < 2; ++k)
+    for (uint32_t k = 0; k < kBins; k += kSelectThreads)
     {
-        const uint32_t bin = threadIdx.x + k * kSelectThreads, v = room.bins[bin];
-        if (v) atomicAdd(&histogram[bin], v);
+        const uint32_t v = room.bins[k + threadIdx.x];
+        if (v) atomicAdd(&histogram[k + threadIdx.x], v);
     }
 }
 
 __global__ void __launch_bounds__(kSelectThreads) select_count_kernel(SelectPass a)
 {
-    __shared__ SelectRoom room;
+    __shared__ SharedRoom room;
     const int row    = blockIdx.y;
     const RowRange r = row_range(a, row);
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     uint32_t above = 0, at = 0;
     if (r.need > 0 && first < last)
     {
-        uint32_t left         = (uint32_t)r.need;
-        const uint32_t prefix = known_digits(a, room, row, kDigits, left);
-        const float* score    = a.score + (int64_t)row * a.row_stride;
-        for (int i = first + (int)threadIdx.x; i < last; i += kSelectThreads)
+        const float* score = a.score + (int64_t)row * a.row_stride;
+        uint32_t left = (uint32_t)r.need, prefix = 0;
+        for (int base = first; base < last; base += kSharePiece)
         {
-            const uint32_t key = score_key(score[i]);
-            above += key > prefix;
-            at += key == prefix;
+            const Piece piece(score, base, last);
+            if (base == first) prefix = known_digits(a, room, row, kDigits, left);
+#pragma unroll
+            for (int k = 0; k < 4 * kShareGroups; ++k)
+            {
+                const uint32_t key = score_key(piece.raw[k]);
+                const bool there   = Piece::entry(base, k) < last;
+                above += there && key > prefix;
+                at += there && key == prefix;
+            }
         }
     }
-    above = group_inclusive_scan(above, room.sums);
+    above = group_inclusive_scan<kSelectThreads>(above, room.sums);
     __syncthreads();
-    at = group_inclusive_scan(at, room.sums);
+    at = group_inclusive_scan<kSelectThreads>(at, room.sums);
     if (threadIdx.x == kSelectThreads - 1) a.counts[(size_t)row * a.groups + blockIdx.x] = make_uint2(above, at);
 }
 
 __global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass a)
 {
-    __shared__ SelectRoom room;
-    __shared__ uint32_t totals[2][kSelectWaves];
-    const int row    = blockIdx.y, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    __shared__ SharedRoom room;
+    __shared__ uint32_t totals[kShareGroups * (kSelectThreads / kWave)];
+    const int row    = blockIdx.y;
     const RowRange r = row_range(a, row);
     int32_t* index   = a.index + (int64_t)row * a.budget;
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     if (r.need > 0 && first < last)
     {
-        uint32_t left         = (uint32_t)r.need;
-        const uint32_t prefix = known_digits(a, room, row, kDigits, left);
-        // what the workgroups in front have
-        uint2 sum = make_uint2(0, 0);
-        for (int g = (int)threadIdx.x; g < (int)blockIdx.x; g += kSelectThreads)
-        {
-            const uint2 c = a.counts[(size_t)row * a.groups + g];
-            sum.x += c.x, sum.y += c.y;
-        }
-        sum.x = group_inclusive_scan(sum.x, room.sums);
-        __syncthreads();
-        sum.y = group_inclusive_scan(sum.y, room.sums);
-        if (threadIdx.x == kSelectThreads - 1) room.bin = sum.x, room.left = sum.y;
-        __syncthreads();
-        uint32_t larger = room.bin, equal = room.left;
         const float* score = a.score + (int64_t)row * a.row_stride;
-        for (int base = first; base < last; base += kSelectThreads)
+        uint32_t left = (uint32_t)r.need, prefix = 0, larger = 0, equal = 0;
+        for (int base = first; base < last; base += kSharePiece)
         {
-            const int i          = base + (int)threadIdx.x;
-            const uint32_t key   = i < last ? score_key(score[i]) : 0u;
-            const uint64_t above = __ballot(i < last && key > prefix), at = __ballot(i < last && key == prefix);
-            if (lane == 0) totals[0][wave] = (uint32_t)__popcll(above), totals[1][wave] = (uint32_t)__popcll(at);
-            __syncthreads();
-            uint32_t more = 0, same = 0, all_more = 0, all_same = 0;
-#pragma unroll
-            for (int w = 0; w < kSelectWaves; ++w)
+            const Piece piece(score, base, last);
+            if (base == first)
             {
-                more += w < wave ? totals[0][w] : 0u, same += w < wave ? totals[1][w] : 0u;
-                all_more += totals[0][w], all_same += totals[1][w];
+                // what the workgroups in front have
+                uint2 sum = make_uint2(0, 0);
+                for (int g = (int)threadIdx.x; g < (int)blockIdx.x; g += kSelectThreads)
+                {
+                    const uint2 c = a.counts[(size_t)row * a.groups + g];
+                    sum.x += c.x, sum.y += c.y;
+                }
+                prefix = known_digits(a, room, row, kDigits, left);
+                sum.x  = group_inclusive_scan<kSelectThreads>(sum.x, room.sums);
+                __syncthreads();
+                sum.y = group_inclusive_scan<kSelectThreads>(sum.y, room.sums);
+                if (threadIdx.x == kSelectThreads - 1) room.bin = sum.x, room.left = sum.y;
+                __syncthreads();
+                larger = room.bin, equal = room.left;
             }
-            const auto below = [](uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
-            const uint32_t before_more = larger + more + below(above), before_same = equal + same + below(at);
-            const bool stays           = i < last && (key > prefix || (key == prefix && before_same < left));
-            if (stays) index[before_more + min(before_same, left)] = i;
-            larger += all_more, equal += all_same;
+            uint32_t key[4 * kShareGroups];
+#pragma unroll
+            for (int k = 0; k < 4 * kShareGroups; ++k) key[k] = score_key(piece.raw[k]);
+            give_places<kSelectThreads, kShareGroups>(key, base, last, prefix, left, larger, equal, index, totals);
+            if (base + kSharePiece >= last) break;
+            // this piece's own, for the next one
+            uint32_t above = 0, at = 0;
+#pragma unroll
+            for (int k = 0; k < 4 * kShareGroups; ++k)
+            {
+                above += key[k] > prefix;
+                at += key[k] == prefix;
+            }
             __syncthreads();
+            above = group_inclusive_scan<kSelectThreads>(above, room.sums);
+            __syncthreads();
+            at = group_inclusive_scan<kSelectThreads>(at, room.sums);
+            if (threadIdx.x == kSelectThreads - 1) room.bin = above, room.left = at;
+            __syncthreads();
+            larger += room.bin, equal += room.left;
         }
     }
     // the entries that stay in any case, and what is left of the row
