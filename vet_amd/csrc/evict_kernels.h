@@ -14,14 +14,15 @@ constexpr int kDigits        = 3;
 constexpr uint32_t kBins     = 2048;
 constexpr int kSelectRowMost = 32 * kSelectThreads;  // entries of a row that one workgroup holds in registers
 
-// Larger for larger scores. Both zeros are one, a NaN is below everything.
+// Larger for larger scores. Both zeros are one, a NaN is below everything, and below that is what stands for no entry: no more are asked for than there
+// are, so that the threshold is above it.
 __device__ __forceinline__ uint32_t score_key(float score)
 {
     const uint32_t b = __float_as_uint(score + 0.f);
     const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return score == score ? k : 0u;
+    return score == score ? k : 1u;
 }
-constexpr uint32_t kZeroKey = 0x80000000u;
+constexpr uint32_t kNoKey = 0u, kZeroKey = 0x80000000u;
 
 __device__ __forceinline__ constexpr int digit_shift(int digit) { return digit == 0 ? 21 : digit == 1 ? 10 : 0; }
 __device__ __forceinline__ uint32_t digit_of(uint32_t key, int digit) { return digit == 2 ? key & 1023u : (key >> digit_shift(digit)) & 2047u; }
@@ -36,6 +37,7 @@ struct SelectPass
     int rows, n, budget, recent;
     // rows of several workgroups
     uint32_t* histogram;  // [rows][kDigits][kBins]
+    uint2* known;         // [rows][kDigits]: the threshold's digits so far, and how many entries at it are needed
     uint2* counts;        // [rows][groups]: above the threshold, at it
     int share, groups;    // entries of a workgroup (a multiple of kSharePiece), workgroups of a row
 };
@@ -113,11 +115,10 @@ __device__ __forceinline__ void clear_bins(SelectRoom<THREADS>& room)
 }
 
 // Scores that two thirds of a scene's points may share, as no view has seen them, are counted by the thread and not in LDS, where they would queue up at one address.
-__device__ __forceinline__ void count_key(uint32_t* bins, uint32_t& zeros, bool there, uint32_t key, int digit)
+__device__ __forceinline__ void count_key(uint32_t* bins, uint32_t& zeros, bool matches, uint32_t key, int digit)
 {
-    const bool zero = key == kZeroKey;
-    zeros += there && zero;
-    if (there && !zero) atomicAdd(&bins[digit_of(key, digit)], 1u);
+    zeros += matches && key == kZeroKey;
+    if (matches && key != kZeroKey && key != kNoKey) atomicAdd(&bins[digit_of(key, digit)], 1u);
 }
 __device__ __forceinline__ void count_zeros(uint32_t* bins, uint32_t zeros, int digit)
 {
@@ -125,7 +126,7 @@ __device__ __forceinline__ void count_zeros(uint32_t* bins, uint32_t zeros, int 
     if (threadIdx.x % kWave == kWave - 1 && zeros) atomicAdd(&bins[digit_of(kZeroKey, digit)], zeros);
 }
 
-// Four neighbouring scores, the first of them entry i; those from `end` on are some others of the row (end is at least 1).
+// Four neighbouring scores, the first of them entry i, as they lie in memory; those from `end` on are some others of the row (end is at least 1).
 __device__ __forceinline__ void load_scores(const float* score, int i, int end, float* raw)
 {
     if (i + 4 <= end)
@@ -139,11 +140,17 @@ __device__ __forceinline__ void load_scores(const float* score, int i, int end, 
         for (int k = 0; k < 4; ++k) raw[k] = score[min(i + k, end - 1)];
     }
 }
+// Their keys.
+__device__ __forceinline__ void keys_of(const float* raw, int i, int end, uint32_t* key)
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) key[k] = i + k < end ? score_key(raw[k]) : kNoKey;
+}
 
-// Places of the entries that stay, in order. key: GROUPS groups of four a thread, of entries first + ..., those from `last` on are not counted; threshold and
-// left: as found; larger, equal: entries above and at the threshold in front of these.
+// Places of the entries that stay, in order. key: GROUPS groups of four a thread, of entries first + ...; threshold and left: as found; larger, equal:
+// entries above and at the threshold in front of these.
 template <int THREADS, int GROUPS>
-__device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], int first, int last, uint32_t threshold, uint32_t left, uint32_t larger, uint32_t equal,
+__device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], int first, uint32_t threshold, uint32_t left, uint32_t larger, uint32_t equal,
                                             int32_t* index, uint32_t (&totals)[GROUPS * (THREADS / kWave)])
 {
     constexpr int kWaves = THREADS / kWave;
@@ -152,15 +159,9 @@ __device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], i
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
     {
-        const int i = first + 4 * (g * THREADS + (int)threadIdx.x);
-        counts[g]   = 0;
+        counts[g] = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-        {
-            const bool there = i + k < last;
-            counts[g] += there && key[4 * g + k] > threshold ? 1u : 0u;
-            counts[g] += there && key[4 * g + k] == threshold ? 1u << 16 : 0u;
-        }
+        for (int k = 0; k < 4; ++k) counts[g] += key[4 * g + k] > threshold ? 1u : key[4 * g + k] == threshold ? 1u << 16 : 0u;
         ends[g] = wave_inclusive_scan(counts[g], lane);
         if (lane == kWave - 1) totals[g * kWaves + wave] = ends[g];
     }
@@ -187,7 +188,7 @@ __device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], i
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
-            const bool there = i + k < last, above = there && key[4 * g + k] > threshold, at = there && key[4 * g + k] == threshold;
+            const bool above = key[4 * g + k] > threshold, at = key[4 * g + k] == threshold;
             if (above || (at && same < left)) index[more + min(same, left)] = i + k;
             more += above, same += at;
         }
@@ -206,14 +207,21 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
     int32_t* index     = a.index + (int64_t)row * a.budget;
     if (r.range > 0 && r.need > 0)
     {
-        float raw[4 * GROUPS];
         uint32_t key[4 * GROUPS];
-        const int mine = 4 * (int)threadIdx.x;
+        {
+            float raw[4 * GROUPS];
+            const int mine = 4 * (int)threadIdx.x;
+            // (the same branches in all threads)
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-            if (4 * g * THREADS < r.range) load_scores(score, 4 * g * THREADS + mine, r.range, raw + 4 * g);  // (the same branch in all threads)
+            for (int g = 0; g < GROUPS; ++g)
+                if (4 * g * THREADS < r.range) load_scores(score, 4 * g * THREADS + mine, r.range, raw + 4 * g);
 #pragma unroll
-        for (int k = 0; k < 4 * GROUPS; ++k) key[k] = score_key(raw[k]);
+            for (int g = 0; g < GROUPS; ++g)
+            {
+                key[4 * g] = key[4 * g + 1] = key[4 * g + 2] = key[4 * g + 3] = kNoKey;
+                if (4 * g * THREADS < r.range) keys_of(raw + 4 * g, 4 * g * THREADS + mine, r.range, key + 4 * g);
+            }
+        }
         uint32_t threshold = 0, mask = 0, left = (uint32_t)r.need;
 #pragma unroll
         for (int digit = 0; digit < kDigits; ++digit)
@@ -225,8 +233,7 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
                 if (4 * g * THREADS < r.range)
                 {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        count_key(room.bins, zeros, 4 * g * THREADS + mine + k < r.range && (key[4 * g + k] & mask) == threshold, key[4 * g + k], digit);
+                    for (int k = 0; k < 4; ++k) count_key(room.bins, zeros, (key[4 * g + k] & mask) == threshold, key[4 * g + k], digit);
                 }
             count_zeros(room.bins, zeros, digit);
             __syncthreads();
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
             mask |= (digit == 2 ? 1023u : 2047u) << digit_shift(digit);
             __syncthreads();
         }
-        give_places<THREADS, GROUPS>(key, 0, r.range, threshold, left, 0, 0, index, totals);
+        give_places<THREADS, GROUPS>(key, 0, threshold, left, 0, 0, index, totals);
     }
     const int selected = min(r.need, r.range), total = selected + r.length - r.range;
     for (int i = (int)threadIdx.x; i < a.budget - selected; i += THREADS) index[selected + i] = i < r.length - r.range ? r.range + i : -1;
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 
 // ---- rows of several workgroups: a launch for each digit, one that counts and one that gives places ---------------------------
 
-constexpr int kShareGroups = 2;  // groups of four of a thread under way at once
+constexpr int kShareGroups = 3;  // groups of four of a thread under way at once (5.5 M entries: 54 us of the launches, with 2 61, with 4 60)
 constexpr int kSharePiece  = 4 * kShareGroups * kSelectThreads;
 
 __global__ void __launch_bounds__(kBlock) select_clear_kernel(uint32_t* p, size_t n)
@@ -255,21 +262,24 @@ __global__ void __launch_bounds__(kBlock) select_clear_kernel(uint32_t* p, size_
 
 using SharedRoom = SelectRoom<kSelectThreads>;
 
-// The threshold's digits in front of `digits`, from the histograms that are there, and how many at it are needed.
-__device__ __forceinline__ uint32_t known_digits(const SelectPass& a, SharedRoom& room, int row, int digits, uint32_t& left)
+// The threshold's digits in front of DIGITS, and how many at it are needed. The last of them comes from the histogram of the launch before, the others
+// this launch finds in memory, and leaves what it knows there for the next one.
+template <int DIGITS>
+__device__ __forceinline__ uint2 known_digits(const SelectPass& a, SharedRoom& room, int row, int need)
 {
-    uint32_t prefix = 0;
-    for (int digit = 0; digit < digits; ++digit)
+    uint2 known = make_uint2(0, (uint32_t)need);
+    if constexpr (DIGITS > 1) known = a.known[(size_t)row * kDigits + DIGITS - 2];
+    if constexpr (DIGITS > 0)
     {
-        find_bin(room, a.histogram + ((size_t)row * kDigits + digit) * kBins, left);
-        left = room.left;
-        prefix |= room.bin << digit_shift(digit);
+        find_bin(room, a.histogram + ((size_t)row * kDigits + DIGITS - 1) * kBins, known.y);
+        known = make_uint2(known.x | room.bin << digit_shift(DIGITS - 1), room.left);
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.known[(size_t)row * kDigits + DIGITS - 1] = known;
         __syncthreads();
     }
-    return prefix;
+    return known;
 }
 
-// A piece of a share: keys of kShareGroups groups of four a thread, from entry `base` on. Loads come first.
+// A piece of a share: kShareGroups groups of four a thread, from entry `base` on. Loads come first.
 struct Piece
 {
     float raw[4 * kShareGroups];
@@ -278,7 +288,11 @@ struct Piece
 #pragma unroll
         for (int g = 0; g < kShareGroups; ++g) load_scores(score, base + 4 * (g * kSelectThreads + (int)threadIdx.x), last, raw + 4 * g);
     }
-    __device__ __forceinline__ static int entry(int base, int k) { return base + 4 * (k / 4 * kSelectThreads + (int)threadIdx.x) + k % 4; }
+    __device__ __forceinline__ void keys(int base, int last, uint32_t* key) const
+    {
+#pragma unroll
+        for (int g = 0; g < kShareGroups; ++g) keys_of(raw + 4 * g, base + 4 * (g * kSelectThreads + (int)threadIdx.x), last, key + 4 * g);
+    }
 };
 
 template <int DIGIT>
@@ -290,22 +304,20 @@ __global__ void __launch_bounds__(kSelectThreads) select_digit_kernel(SelectPass
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     if (r.need <= 0 || first >= last) return;
     const float* score = a.score + (int64_t)row * a.row_stride;
-    uint32_t left = (uint32_t)r.need, zeros = 0, prefix = 0;
+    uint32_t zeros = 0, prefix = 0;
     constexpr uint32_t kMask = DIGIT == 0 ? 0u : ~0u << digit_shift(DIGIT == 0 ? 0 : DIGIT - 1);
     for (int base = first; base < last; base += kSharePiece)
     {
         const Piece piece(score, base, last);
         if (base == first)  // while the loads are under way
         {
-            prefix = known_digits(a, room, row, DIGIT, left);
+            prefix = known_digits<DIGIT>(a, room, row, r.need).x;
             clear_bins(room);
         }
+        uint32_t key[4 * kShareGroups];
+        piece.keys(base, last, key);
 #pragma unroll
-        for (int k = 0; k < 4 * kShareGroups; ++k)
-        {
-            const uint32_t key = score_key(piece.raw[k]);
-            count_key(room.bins, zeros, Piece::entry(base, k) < last && (key & kMask) == prefix, key, DIGIT);
-        }
+        for (int k = 0; k < 4 * kShareGroups; ++k) count_key(room.bins, zeros, (key[k] & kMask) == prefix, key[k], DIGIT);
     }
     count_zeros(room.bins, zeros, DIGIT);
     __syncthreads();
@@ -328,18 +340,18 @@ __global__ void __launch_bounds__(kSelectThreads) select_count_kernel(SelectPass
     if (r.need > 0 && first < last)
     {
         const float* score = a.score + (int64_t)row * a.row_stride;
-        uint32_t left = (uint32_t)r.need, prefix = 0;
+        uint32_t prefix = 0;
         for (int base = first; base < last; base += kSharePiece)
         {
             const Piece piece(score, base, last);
-            if (base == first) prefix = known_digits(a, room, row, kDigits, left);
+            if (base == first) prefix = known_digits<kDigits>(a, room, row, r.need).x;
+            uint32_t key[4 * kShareGroups];
+            piece.keys(base, last, key);
 #pragma unroll
             for (int k = 0; k < 4 * kShareGroups; ++k)
             {
-                const uint32_t key = score_key(piece.raw[k]);
-                const bool there   = Piece::entry(base, k) < last;
-                above += there && key > prefix;
-                at += there && key == prefix;
+                above += key[k] > prefix;
+                at += key[k] == prefix;
             }
         }
     }
@@ -360,7 +372,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass
     if (r.need > 0 && first < last)
     {
         const float* score = a.score + (int64_t)row * a.row_stride;
-        uint32_t left = (uint32_t)r.need, prefix = 0, larger = 0, equal = 0;
+        const uint2 known     = a.known[(size_t)row * kDigits + kDigits - 1];
+        const uint32_t prefix = known.x, left = known.y;
+        uint32_t larger = 0, equal = 0;
         for (int base = first; base < last; base += kSharePiece)
         {
             const Piece piece(score, base, last);
@@ -373,8 +387,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass
                     const uint2 c = a.counts[(size_t)row * a.groups + g];
                     sum.x += c.x, sum.y += c.y;
                 }
-                prefix = known_digits(a, room, row, kDigits, left);
-                sum.x  = group_inclusive_scan<kSelectThreads>(sum.x, room.sums);
+                sum.x = group_inclusive_scan<kSelectThreads>(sum.x, room.sums);
                 __syncthreads();
                 sum.y = group_inclusive_scan<kSelectThreads>(sum.y, room.sums);
                 if (threadIdx.x == kSelectThreads - 1) room.bin = sum.x, room.left = sum.y;
@@ -382,9 +395,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass
                 larger = room.bin, equal = room.left;
             }
             uint32_t key[4 * kShareGroups];
-#pragma unroll
-            for (int k = 0; k < 4 * kShareGroups; ++k) key[k] = score_key(piece.raw[k]);
-            give_places<kSelectThreads, kShareGroups>(key, base, last, prefix, left, larger, equal, index, totals);
+            piece.keys(base, last, key);
+            give_places<kSelectThreads, kShareGroups>(key, base, prefix, left, larger, equal, index, totals);
             if (base + kSharePiece >= last) break;
             // this piece's own, for the next one
             uint32_t above = 0, at = 0;
