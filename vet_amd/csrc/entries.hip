@@ -229,7 +229,8 @@ int vetrast_keep_rows(vetrast_ctx* ctx, const vetrast_keep_args* a, void* stream
         for (int64_t row = 0; row < a->kept; row += rows_at_once)
         {
             const int64_t rows   = std::min<int64_t>(a->kept - row, rows_at_once);
-            const int64_t chunks = (rows * units + kKeepChunk - 1) / kKeepChunk, outers_at_once = std::max<int64_t>(kKeepGroupsMost / chunks, 1);
+            const int64_t chunk  = unit_log == 2 && units == 1 && t.n > 0 ? kKeepWords : kKeepChunk;
+            const int64_t chunks = (rows * units + chunk - 1) / chunk, outers_at_once = std::max<int64_t>(kKeepGroupsMost / chunks, 1);
             for (int64_t outer = 0; outer < t.outers; outer += outers_at_once)
             {
                 const int64_t outers = std::min(t.outers - outer, outers_at_once);
@@ -250,6 +251,7 @@ int vetrast_keep_rows(vetrast_ctx* ctx, const vetrast_keep_args* a, void* stream
                 e.chunks       = (uint32_t)chunks;
                 e.first_chunk  = l.total;
                 e.unit_log     = unit_log;
+                e.units_log    = (units & (units - 1)) == 0 ? (uint32_t)__builtin_ctzll((uint64_t)units) : 32u;
                 l.total += (uint32_t)(outers * chunks);
             }
         }
