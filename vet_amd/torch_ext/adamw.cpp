@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include "calls.h"
+#include "entries.h"
 
 namespace vet_amd
 {
@@ -479,6 +480,121 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
         exp_avg.narrow(0, slots_[k].first, slots_[k].n).copy_(kept[0][k].as_strided({slots_[k].n}, {1}));
         exp_avg_sq.narrow(0, slots_[k].first, slots_[k].n).copy_(kept[1][k].as_strided({slots_[k].n}, {1}));
     }
+}
+
+void AdamW::keep_rows(const std::vector<torch::Tensor>& params, const torch::Tensor& index, const std::vector<int64_t>& dims)
+{
+    torch::NoGradGuard no_grad;
+    c10::DeviceGuard guard(device_);
+    TORCH_CHECK(params.size() == dims.size(), "AdamW: ", params.size(), " parameters, but dimensions of ", dims.size());
+    TORCH_CHECK(index.defined() && index.dim() == 1, "AdamW: keep_rows takes one row of indices, int32 [K]");
+    TORCH_CHECK(!options_.capturable && !capturing(), "AdamW: parameters cannot change their size with capturable, nor in a captured call");
+    check_state();
+    use_on_stream();
+    follow_parameters();
+    const bool eight  = options_.moment_bits == 8;
+    const auto bytes  = torch::TensorOptions(device_).dtype(torch::kUInt8);
+    const auto floats = torch::TensorOptions(device_).dtype(torch::kFloat32);
+    std::vector<size_t> chosen;
+    for (auto& p : params)
+    {
+        size_t k = 0;
+        while (k < slots_.size() && !slots_[k].param.is_same(p)) ++k;
+        TORCH_CHECK(k < slots_.size(), "AdamW: keep_rows takes parameters of this optimiser");
+        for (size_t other : chosen) TORCH_CHECK(other != k, "AdamW: a parameter is in the list twice");
+        check_on(p, device_, "AdamW: parameters");
+        TORCH_CHECK(p.is_contiguous() && slots_[k].rows && p.sizes() == slots_[k].sizes, "AdamW: keep_rows takes contiguous parameters");
+        TORCH_CHECK(!p.is_inference(), "AdamW: a parameter made in inference mode cannot change its size");
+        chosen.push_back(k);
+    }
+    // Everything that goes with the entries, in one call: a parameter, its moments and its master.
+    std::vector<torch::Tensor> all;
+    std::vector<int64_t> all_dims;
+    for (size_t j = 0; j < chosen.size(); ++j)
+    {
+        const Slot& s    = slots_[chosen[j]];
+        const auto state = [&](const torch::Tensor& flat, int64_t first) { all.push_back(flat.narrow(0, first, s.n).view(s.sizes)); };
+        all.push_back(s.param.detach());
+        if (eight)
+        {
+            torch::Tensor m = torch::empty({s.n}, floats), v = torch::empty({s.n}, floats);
+            const std::vector<vetrast_moment_tensor> list{{m.data_ptr<float>(), v.data_ptr<float>(), s.n, s.first}};
+            const vetrast_moments_args a = moments_args(list, exp_avg, exp_avg_sq, block_scale);
+            check(vetrast_unpack_moments(context_on(device_), &a, stream_on(device_)), "unpack_moments");
+            state(m, 0);
+            state(v, 0);
+        }
+        else
+        {
+            state(exp_avg, s.first);
+            state(exp_avg_sq, s.first);
+        }
+        if (master.defined()) state(master, s.first);
+        all_dims.insert(all_dims.end(), master.defined() ? 4 : 3, dims[j]);
+    }
+    const std::vector<torch::Tensor> kept = KeepRows(all, index, all_dims);
+    const size_t each                     = master.defined() ? 4 : 3;
+    // A new layout aside, as lay_out makes it.
+    std::vector<Slot> slots = slots_;
+    std::vector<int64_t> of(slots.size(), -1);  // a slot's place in `kept`
+    for (size_t j = 0; j < chosen.size(); ++j)
+    {
+        of[chosen[j]] = (int64_t)(j * each);
+        Slot& s       = slots[chosen[j]];
+        s.n           = kept[j * each].numel();
+        s.sizes       = kept[j * each].sizes().vec();
+        s.strides     = kept[j * each].strides().vec();
+        s.rows        = true;
+    }
+    int64_t at = 0;
+    for (auto& s : slots)
+    {
+        s.first = at;
+        at += whole_blocks(s.n);
+    }
+    torch::Tensor m = torch::zeros({at}, eight ? bytes : floats), v = torch::zeros({at}, eight ? bytes : floats), scales, masters;
+    if (eight) scales = torch::zeros({at / kBlock, 2}, bytes);
+    if (master.defined()) masters = torch::zeros({at}, floats);
+    std::vector<vetrast_moment_tensor> packed;
+    for (size_t k = 0; k < slots.size(); ++k)
+    {
+        const Slot &s = slots[k], &old = slots_[k];
+        if (s.n == 0) continue;
+        if (of[k] < 0)
+        {
+            const int64_t n = whole_blocks(s.n);
+            m.narrow(0, s.first, n).copy_(exp_avg.narrow(0, old.first, n));
+            v.narrow(0, s.first, n).copy_(exp_avg_sq.narrow(0, old.first, n));
+            if (eight) scales.narrow(0, s.first / kBlock, n / kBlock).copy_(block_scale.narrow(0, old.first / kBlock, n / kBlock));
+            if (masters.defined()) masters.narrow(0, s.first, n).copy_(master.narrow(0, old.first, n));
+            continue;
+        }
+        const torch::Tensor* mine = kept.data() + of[k];
+        if (eight) packed.push_back({mine[1].data_ptr<float>(), mine[2].data_ptr<float>(), s.n, s.first});
+        else
+        {
+            m.narrow(0, s.first, s.n).copy_(mine[1].view({s.n}));
+            v.narrow(0, s.first, s.n).copy_(mine[2].view({s.n}));
+        }
+        if (masters.defined()) masters.narrow(0, s.first, s.n).copy_(mine[3].view({s.n}));
+    }
+    if (!packed.empty())
+    {
+        const vetrast_moments_args a = moments_args(packed, m, v, scales);
+        check(vetrast_pack_moments(context_on(device_), &a, stream_on(device_)), "pack_moments");
+    }
+    for (size_t j = 0; j < chosen.size(); ++j)
+    {
+        torch::Tensor& p = slots[chosen[j]].param;
+        p.mutable_grad().reset();
+        p.set_data(kept[j * each]);
+    }
+    slots_.swap(slots);
+    exp_avg     = std::move(m);
+    exp_avg_sq  = std::move(v);
+    block_scale = std::move(scales);
+    master      = std::move(masters);
+    elements_   = at;
 }
 
 void AdamW::reload_master()

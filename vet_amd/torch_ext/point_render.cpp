@@ -1335,6 +1335,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
              pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
         .def("load_moments", pybind11::overload_cast<const Tensors&, const Tensors&, const std::vector<int64_t>&>(&AdamW::load_moments),
              pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"), pybind11::arg("step"))
+        .def("keep_rows", &AdamW::keep_rows, pybind11::arg("params"), pybind11::arg("index"), pybind11::arg("dims"))
         .def("reload_master", &AdamW::reload_master)
         .def_readonly("exp_avg", &AdamW::exp_avg)
         .def_readonly("exp_avg_sq", &AdamW::exp_avg_sq)
