@@ -66,7 +66,7 @@ inline int select_share(int n)
     return (int)((pieces + kSelectGroups - 1) / kSelectGroups) * kSharePiece;
 }
 inline int select_groups(int n) { return (int)(((int64_t)n + select_share(n) - 1) / select_share(n)); }
-inline size_t select_words(int n) { return kDigits * (size_t)kBins + 2 * kDigits + 2 * (size_t)select_groups(n); }  // of a row
+inline size_t select_words(int n) { return kDigits * (size_t)kBins + 2 + 2 * kDigits + 2 * (size_t)select_groups(n); }  // of a row
 
 void launch_select_row(const SelectPass& p, hipStream_t stream)
 {
@@ -92,9 +92,10 @@ void launch_select_rows(SelectPass p, char* workspace, hipStream_t stream)
         p.index     = all.index + (int64_t)from * all.budget;
         p.count     = all.count + from;
         p.histogram = reinterpret_cast<uint32_t*>(workspace) + (size_t)from * select_words(p.n);
-        p.known     = reinterpret_cast<uint2*>(p.histogram + (size_t)p.rows * kDigits * kBins);
+        p.zeros     = p.histogram + (size_t)p.rows * kDigits * kBins;
+        p.known     = reinterpret_cast<uint2*>(p.zeros + 2 * (size_t)p.rows);
         p.counts    = p.known + (size_t)p.rows * kDigits;
-        const size_t words = (size_t)p.rows * kDigits * kBins;
+        const size_t words = (size_t)p.rows * (kDigits * kBins + 1);  // histograms and zeros
         const dim3 grid((uint32_t)p.groups, (uint32_t)p.rows), block(kSelectThreads);
         hipLaunchKernelGGL(select_clear_kernel, dim3((uint32_t)std::min<size_t>((words + kBlock - 1) / kBlock, 2048)), dim3(kBlock), 0, stream, p.histogram, words);
         hipLaunchKernelGGL((select_digit_kernel<0>), grid, block, 0, stream, p);
@@ -172,6 +173,7 @@ int vetrast_select_kept(vetrast_ctx* ctx, const vetrast_select_args* a, void* st
     p.budget     = a->budget;
     p.recent     = a->recent;
     p.histogram  = nullptr;
+    p.zeros      = nullptr;
     p.known      = nullptr;
     p.counts     = nullptr;
     p.share = p.groups = 0;
