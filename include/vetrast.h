@@ -548,8 +548,8 @@ typedef struct vetrast_select_args
     const int32_t* length; /* optional, device [rows]: entries of a row, taken as 0 below 0 and as n above n. NULL: n */
     int32_t* index;        /* device [rows][budget]; overwritten */
     int32_t* count;        /* device [rows]: entries kept, min(length, budget); overwritten */
-    int32_t rows, n;       /* >= 0 */
-    int32_t budget;        /* >= 0; may be more than n */
+    int32_t rows, n;       /* >= 0; n at most 2^30 */
+    int32_t budget;        /* 0 .. 2^30; may be more than n */
     int32_t recent;        /* 0 .. budget */
     void* workspace;       /* device, 16-byte aligned; its contents before and after the call do not matter */
     size_t workspace_bytes;

@@ -109,3 +109,15 @@ def test_the_model():
     index, count = em.select_kept(np.array([[1.0, 2, 3]] * 4), 2, length=[0, 1, 2, 9])
     assert index.tolist() == [[-1, -1], [0, -1], [0, 1], [1, 2]] and count.tolist() == [0, 1, 2, 2]
     assert em.keep_rows(np.arange(6).reshape(2, 3), np.array([2, -1, 0, 3]), 1).tolist() == [[2, 0, 0, 0], [5, 0, 3, 0]]
+
+
+@pytest.mark.parametrize("changes", [dict(budget=2 ** 30 + 1), dict(budget=2 ** 31 - 1), dict(n=2 ** 30 + 1, row_stride=2 ** 31, workspace_bytes=2 ** 62),
+                                     dict(n=2 ** 31 - 1, row_stride=2 ** 31, workspace_bytes=2 ** 62)])
+def test_select_refuses_rows_whose_places_pass_32_bits(changes):
+    lib, ctx = lib_and_context()
+    assert lib.vetrast_select_kept(ctx, C.byref(select_args(**changes)), None) == abi.ERR_INVALID_ARG
+
+
+def test_the_calls_on_tensors_refuse_a_budget_that_passes_32_bits():
+    with pytest.raises(RuntimeError, match="budget"):
+        torch_ops.select_kept(torch.zeros(5), 2 ** 30 + 1)

@@ -95,6 +95,29 @@ def test_rows_behind_one_another_beyond_32_bits():
     assert index[n - 1].tolist() == [7, n - 2, n - 1] and index[n - 2].tolist() == [1, 7, n - 1]
 
 
+def test_more_rows_than_threads_have_numbers():
+    """Rows of one workgroup each, more than a launch takes."""
+    rows = 2 ** 21 + 7
+    s = torch.zeros(rows, 3, device="cuda")
+    s[:, 1] = 1
+    s[rows - 2, 0] = 2
+    index, count = torch_ops.select_kept(s, 2, recent=1)
+    assert (count == 2).all() and (index[:, 1] == 2).all()
+    assert (index[:rows - 2, 0] == 1).all() and index[rows - 2, 0] == 0 and index[rows - 1, 0] == 1
+
+
+def test_the_longest_row_and_a_budget_beyond_it():
+    n = 2 ** 30
+    s = torch.zeros(n, device="cuda")
+    s[5], s[n - 2], s[n // 2] = 1, 1, -1
+    index, count = torch_ops.select_kept(s, 4, recent=1)
+    assert index.tolist() == [0, 5, n - 2, n - 1] and count.item() == 4
+    index, count = torch_ops.select_kept(s[:70_000], 2 ** 28 + 3)
+    assert count.item() == 70_000 and torch.equal(index[:70_000], torch.arange(70_000, dtype=torch.int32, device="cuda")) and (index[70_000:] == -1).all()
+    index, count = torch_ops.select_kept(s[:7], 2 ** 26 + 3)
+    assert count.item() == 7 and index[:7].tolist() == list(range(7)) and (index[7:] == -1).all()
+
+
 def test_the_rasterizer_class(rasterizer):
     for n in (100, 50_000):
         s = scores(3, n, "weights")

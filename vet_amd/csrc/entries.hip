@@ -57,9 +57,11 @@ inline bool overlap(const void* a, const void* b, size_t bytes)
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x != y && (x < y ? y - x : x - y) < bytes;
 }
-// Rows of more entries than a workgroup holds are shared by several: a piece of 8 entries a thread each, or more where there are many.
-constexpr int kSelectGroups   = 1024;   // workgroups of a row at most
-constexpr int kSelectGridRows = 32768;  // rows of a launch
+// Rows of more entries than a workgroup holds are shared by several: a piece of 12 entries a thread each, or more where there are many.
+constexpr int kSelectGroups   = 1024;     // workgroups of a row at most
+constexpr int kSelectGridRows = 32768;    // rows of a launch
+constexpr int kSelectRows     = 1 << 21;  // ... where each is one workgroup: a launch's threads are counted in 32 bits
+constexpr int kSelectMost     = 1 << 30;  // scores of a row, and a budget: places stay within 32 bits with a piece behind them
 inline int select_share(int n)
 {
     const int64_t pieces = ((int64_t)n + kSharePiece - 1) / kSharePiece;
@@ -68,13 +70,22 @@ inline int select_share(int n)
 inline int select_groups(int n) { return (int)(((int64_t)n + select_share(n) - 1) / select_share(n)); }
 inline size_t select_words(int n) { return kDigits * (size_t)kBins + 2 + 2 * kDigits + 2 * (size_t)select_groups(n); }  // of a row
 
-void launch_select_row(const SelectPass& p, hipStream_t stream)
+void launch_select_row(SelectPass p, hipStream_t stream)
 {
-    const dim3 grid((uint32_t)p.rows);
-    if (p.n <= 4 * kBlock) hipLaunchKernelGGL((select_row_kernel<kBlock, 1>), grid, dim3(kBlock), 0, stream, p);
-    else if (p.n <= 4 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 1>), grid, dim3(kSelectThreads), 0, stream, p);
-    else if (p.n <= 12 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 3>), grid, dim3(kSelectThreads), 0, stream, p);
-    else hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 8>), grid, dim3(kSelectThreads), 0, stream, p);
+    const SelectPass all = p;
+    for (int64_t from = 0; from < all.rows; from += kSelectRows)
+    {
+        p.rows   = (int)std::min<int64_t>(all.rows - from, kSelectRows);
+        p.score  = all.score + from * all.row_stride;
+        p.length = all.length ? all.length + from : nullptr;
+        p.index  = all.index + from * all.budget;
+        p.count  = all.count + from;
+        const dim3 grid((uint32_t)p.rows);
+        if (p.n <= 4 * kBlock) hipLaunchKernelGGL((select_row_kernel<kBlock, 1>), grid, dim3(kBlock), 0, stream, p);
+        else if (p.n <= 4 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 1>), grid, dim3(kSelectThreads), 0, stream, p);
+        else if (p.n <= 12 * kSelectThreads) hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 3>), grid, dim3(kSelectThreads), 0, stream, p);
+        else hipLaunchKernelGGL((select_row_kernel<kSelectThreads, 8>), grid, dim3(kSelectThreads), 0, stream, p);
+    }
 }
 
 void launch_select_rows(SelectPass p, char* workspace, hipStream_t stream)
@@ -83,13 +94,13 @@ void launch_select_rows(SelectPass p, char* workspace, hipStream_t stream)
     p.groups = select_groups(p.n);
     const int rows        = p.rows;
     const SelectPass all  = p;
-    for (int from = 0; from < rows; from += kSelectGridRows)
+    for (int64_t from = 0; from < rows; from += kSelectGridRows)
     {
         p           = all;
-        p.rows      = std::min(rows - from, kSelectGridRows);
-        p.score     = all.score + (int64_t)from * all.row_stride;
+        p.rows      = (int)std::min<int64_t>(rows - from, kSelectGridRows);
+        p.score     = all.score + from * all.row_stride;
         p.length    = all.length ? all.length + from : nullptr;
-        p.index     = all.index + (int64_t)from * all.budget;
+        p.index     = all.index + from * all.budget;
         p.count     = all.count + from;
         p.histogram = reinterpret_cast<uint32_t*>(workspace) + (size_t)from * select_words(p.n);
         p.zeros     = p.histogram + (size_t)p.rows * kDigits * kBins;
@@ -154,7 +165,9 @@ size_t vetrast_select_kept_workspace_bytes(int32_t rows, int32_t n)
 int vetrast_select_kept(vetrast_ctx* ctx, const vetrast_select_args* a, void* stream_)
 {
     if (!ctx || !a) return VETRAST_ERR_INVALID_ARG;
-    if (a->rows < 0 || a->n < 0 || a->budget < 0 || a->recent < 0 || a->recent > a->budget || a->row_stride < a->n) return VETRAST_ERR_INVALID_ARG;
+    if (a->rows < 0 || a->n < 0 || a->budget < 0 || a->recent < 0 || a->recent > a->budget || a->row_stride < a->n || a->n > kSelectMost ||
+        a->budget > kSelectMost)
+        return VETRAST_ERR_INVALID_ARG;
     if (!aligned_to(a->score, 4) || !aligned_to(a->length, 4) || !aligned_to(a->index, 4) || !aligned_to(a->count, 4) || !aligned_to(a->workspace, 16))
         return VETRAST_ERR_INVALID_ARG;
     if (a->rows == 0) return VETRAST_OK;

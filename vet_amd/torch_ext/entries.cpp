@@ -138,13 +138,13 @@ torch::Tensor Dropout(const torch::Tensor& x, double p, uint64_t seed, uint64_t 
 
 std::tuple<torch::Tensor, torch::Tensor> SelectKept(const torch::Tensor& score, int64_t budget, int64_t recent, const std::optional<torch::Tensor>& length)
 {
-    constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
-    TORCH_CHECK(budget >= 0 && budget <= kMost, "select_kept: a budget is not below 0 and fits 32 bits, it is ", budget);
+    constexpr int64_t kMost = (int64_t)1 << 30, kRows = std::numeric_limits<int32_t>::max();
+    TORCH_CHECK(budget >= 0 && budget <= kMost, "select_kept: a budget lies in [0, 2^30], not at ", budget);
     TORCH_CHECK(recent >= 0 && recent <= budget, "select_kept: recent lies in [0, budget], not at ", recent);
     TORCH_CHECK(score.defined() && score.is_cuda() && score.layout() == torch::kStrided && score.scalar_type() == torch::kFloat32,
                 "select_kept: score must be a float32 tensor on the GPU");
     TORCH_CHECK(score.dim() == 1 || score.dim() == 2, "select_kept: score is [N] or [rows, N]");
-    TORCH_CHECK(score.size(0) <= kMost && score.size(-1) <= kMost, "select_kept: rows and entries fit 32 bits");
+    TORCH_CHECK(score.size(-1) <= kMost && (score.dim() == 1 || score.size(0) <= kRows), "select_kept: a row has at most 2^30 scores, and rows are counted in 32 bits");
     c10::DeviceGuard guard(score.device());
     torch::NoGradGuard no_grad;
     const bool one      = score.dim() == 1;
@@ -220,6 +220,8 @@ std::vector<torch::Tensor> KeepRows(const std::vector<torch::Tensor>& tensors, c
     torch::NoGradGuard no_grad;
     const bool one           = index.dim() == 1;
     const int64_t kept       = index.size(-1), rows = one ? 1 : index.size(0);
+    constexpr int64_t kMost  = std::numeric_limits<int32_t>::max();
+    TORCH_CHECK(kept <= kMost && rows <= kMost && (int64_t)tensors.size() <= kMost, "keep_rows: indices, their rows and tensors are counted in 32 bits");
     const bool apart         = (kept <= 1 || index.stride(-1) == 1) && (one || rows <= 1 || index.stride(0) >= kept);
     const torch::Tensor at   = apart ? index : index.contiguous();
     std::vector<torch::Tensor> out, gathered;
