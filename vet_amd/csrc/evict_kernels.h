@@ -41,6 +41,7 @@ struct SelectPass
     uint2* known;         // [rows][kDigits]: see Known
     uint2* counts;        // [rows][groups]: above the threshold, at it
     int share, groups;    // entries of a workgroup (a multiple of kSharePiece), workgroups of a row
+    int shares;           // of a workgroup that counts digits
 };
 
 // What a row is asked for: `need` of its first `range` entries, and all from there to `length`.
@@ -154,10 +155,10 @@ __device__ __forceinline__ void keys_of(const float* raw, int i, int end, uint32
 }
 
 // Places of the entries that stay, in order. key: GROUPS groups of four a thread, of entries first + ...; threshold and left: as found; larger, equal:
-// entries above and at the threshold in front of these.
+// entries above and at the threshold in front of these, for the last thread afterwards with these; index: of place `base`.
 template <int THREADS, int GROUPS>
-__device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], int first, uint32_t threshold, uint32_t left, uint32_t larger, uint32_t equal,
-                                            int32_t* index, uint32_t (&totals)[GROUPS * (THREADS / kWave)])
+__device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], int first, uint32_t threshold, uint32_t left, uint32_t& larger, uint32_t& equal,
+                                            int32_t* index, uint32_t base, uint32_t (&totals)[GROUPS * (THREADS / kWave)])
 {
     constexpr int kWaves = THREADS / kWave;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -185,20 +186,22 @@ __device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], i
         }
     }
     __syncthreads();
+    uint32_t more = 0, same = 0;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
     {
         const int i             = first + 4 * (g * THREADS + (int)threadIdx.x);
         const uint32_t in_front = totals[g * kWaves + wave] + ends[g] - counts[g];
-        uint32_t more = larger + (in_front & 0xFFFFu), same = equal + (in_front >> 16);
+        more = larger + (in_front & 0xFFFFu), same = equal + (in_front >> 16);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
             const bool above = key[4 * g + k] > threshold, at = key[4 * g + k] == threshold;
-            if (above || (at && same < left)) index[more + min(same, left)] = i + k;
+            if (above || (at && same < left)) index[more + min(same, left) - base] = i + k;
             more += above, same += at;
         }
     }
+    larger = more, equal = same;
 }
 
 // One workgroup for a row, its keys in registers.
@@ -255,7 +258,8 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
             mask |= (digit == 2 ? 1023u : 2047u) << digit_shift(digit);
             __syncthreads();
         }
-        give_places<THREADS, GROUPS>(key, 0, threshold, left, 0, 0, index, totals);
+        uint32_t larger = 0, equal = 0;
+        give_places<THREADS, GROUPS>(key, 0, threshold, left, larger, equal, index, 0, totals);
     }
     const int selected = min(r.need, r.range), total = selected + r.length - r.range;
     for (int i = (int)threadIdx.x; i < a.budget - selected; i += THREADS) index[selected + i] = i < r.length - r.range ? r.range + i : -1;
@@ -264,15 +268,18 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 
 // ---- rows of several workgroups: a launch for each digit, one that counts and one that gives places ---------------------------
 
-constexpr int kShareGroups = 3;  // groups of four of a thread under way at once (5.5 M entries: 54 us of the launches, with 2 61, with 4 60)
-constexpr int kSharePiece  = 4 * kShareGroups * kSelectThreads;
+// Workgroups of 512: a row of 40 k entries takes 20.0 us of all launches, 64 rows of 131 k 48.5, one of 5.5 M 34.5 (with 1024 threads 23.8, 62 and
+// 34.8; with 256 19.9, 48 and 39). Three groups of four of a thread under way at once (5.5 M entries: with 2 7 us more).
+constexpr int kShareThreads = 512;
+constexpr int kShareGroups  = 3;
+constexpr int kSharePiece  = 4 * kShareGroups * kShareThreads;
 
 __global__ void __launch_bounds__(kBlock) select_clear_kernel(uint32_t* p, size_t n)
 {
     for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) p[i] = 0u;
 }
 
-using SharedRoom = SelectRoom<kSelectThreads>;
+using SharedRoom = SelectRoom<kShareThreads>;
 
 // What is known of a row's threshold: its digits so far, how many entries at it are needed, and whether it is whole (as it is after the first digit
 // where the budget ends among scores of zero).
@@ -314,17 +321,87 @@ struct Piece
     __device__ __forceinline__ Piece(const float* score, int base, int last)
     {
 #pragma unroll
-        for (int g = 0; g < kShareGroups; ++g) load_scores(score, base + 4 * (g * kSelectThreads + (int)threadIdx.x), last, raw + 4 * g);
+        for (int g = 0; g < kShareGroups; ++g) load_scores(score, base + 4 * (g * kShareThreads + (int)threadIdx.x), last, raw + 4 * g);
     }
     __device__ __forceinline__ void keys(int base, int last, uint32_t* key) const
     {
 #pragma unroll
-        for (int g = 0; g < kShareGroups; ++g) keys_of(raw + 4 * g, base + 4 * (g * kSelectThreads + (int)threadIdx.x), last, key + 4 * g);
+        for (int g = 0; g < kShareGroups; ++g) keys_of(raw + 4 * g, base + 4 * (g * kShareThreads + (int)threadIdx.x), last, key + 4 * g);
     }
 };
 
+// Entries above and at the threshold, of a share.
+__device__ __forceinline__ void leave_counts(const SelectPass& a, SharedRoom& room, int row, int share, uint32_t above, uint32_t at)
+{
+    __syncthreads();
+    above = group_inclusive_scan<kShareThreads>(above, room.sums);
+    __syncthreads();
+    at = group_inclusive_scan<kShareThreads>(at, room.sums);
+    if (threadIdx.x == kShareThreads - 1) a.counts[(size_t)row * a.groups + share] = make_uint2(above, at);
+}
+__device__ __forceinline__ void count_piece(const uint32_t (&key)[4 * kShareGroups], uint32_t threshold, uint32_t& above, uint32_t& at)
+{
+#pragma unroll
+    for (int k = 0; k < 4 * kShareGroups; ++k)
+    {
+        above += key[k] > threshold;
+        at += key[k] == threshold;
+    }
+}
+
+// Workgroups take several shares, since each adds its histogram to the row's, at addresses that all of them want. Where the threshold is whole after the
+// first digit the second launch counts what select_count_kernel otherwise does.
 template <int DIGIT>
-__global__ void __launch_bounds__(kSelectThreads) select_digit_kernel(SelectPass a)
+__global__ void __launch_bounds__(kShareThreads) select_digit_kernel(SelectPass a)
+{
+    __shared__ SharedRoom room;
+    const int row    = blockIdx.y;
+    const RowRange r = row_range(a, row);
+    const int first = (int)blockIdx.x * a.shares * a.share, last = (int)min((int64_t)r.range, (int64_t)first + (int64_t)a.shares * a.share);
+    if (r.need <= 0 || first >= last) return;
+    const float* score = a.score + (int64_t)row * a.row_stride;
+    uint32_t zeros = 0;
+    Known known = {0u, 0u, false};
+    constexpr uint32_t kMask = DIGIT == 0 ? 0u : ~0u << digit_shift(DIGIT == 0 ? 0 : DIGIT - 1);
+    uint32_t above = 0, at = 0;
+    for (int base = first; base < last; base += kSharePiece)
+    {
+        const Piece piece(score, base, last);
+        if (base == first)  // while the loads are under way
+        {
+            known = known_digits<DIGIT>(a, room, row, r.need);
+            if (DIGIT > 1 && known.whole) return;
+            if (!known.whole) clear_bins(room);
+        }
+        uint32_t key[4 * kShareGroups];
+        piece.keys(base, last, key);
+        if (DIGIT == 1 && known.whole)
+        {
+            count_piece(key, known.digits, above, at);
+            if (base + kSharePiece >= last || (base + kSharePiece - first) % a.share == 0)
+            {
+                leave_counts(a, room, row, base / a.share, above, at);
+                above = at = 0;
+            }
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < 4 * kShareGroups; ++k) count_key(room.bins, zeros, (key[k] & kMask) == known.digits, key[k], DIGIT);
+    }
+    if (DIGIT == 1 && known.whole) return;
+    count_zeros(room, zeros, DIGIT);
+    __syncthreads();
+    if (DIGIT == 0 && threadIdx.x == 0 && room.zeros) atomicAdd(&a.zeros[row], room.zeros);
+    uint32_t* histogram = a.histogram + ((size_t)row * kDigits + DIGIT) * kBins;
+#pragma unroll
+    for (uint32_t k = 0; k < kBins; k += kShareThreads)
+    {
+        const uint32_t v = room.bins[k + threadIdx.x];
+        if (v) atomicAdd(&histogram[k + threadIdx.x], v);
+    }
+}
+
+__global__ void __launch_bounds__(kShareThreads) select_count_kernel(SelectPass a)
 {
     __shared__ SharedRoom room;
     const int row    = blockIdx.y;
@@ -332,79 +409,38 @@ __global__ void __launch_bounds__(kSelectThreads) select_digit_kernel(SelectPass
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     if (r.need <= 0 || first >= last) return;
     const float* score = a.score + (int64_t)row * a.row_stride;
-    uint32_t zeros = 0, prefix = 0;
-    constexpr uint32_t kMask = DIGIT == 0 ? 0u : ~0u << digit_shift(DIGIT == 0 ? 0 : DIGIT - 1);
+    uint32_t threshold = 0, above = 0, at = 0;
     for (int base = first; base < last; base += kSharePiece)
     {
         const Piece piece(score, base, last);
-        if (base == first)  // while the loads are under way
+        if (base == first)
         {
-            const Known known = known_digits<DIGIT>(a, room, row, r.need);
+            const Known known = known_digits<kDigits>(a, room, row, r.need);
             if (known.whole) return;
-            prefix = known.digits;
-            clear_bins(room);
+            threshold = known.digits;
         }
         uint32_t key[4 * kShareGroups];
         piece.keys(base, last, key);
-#pragma unroll
-        for (int k = 0; k < 4 * kShareGroups; ++k) count_key(room.bins, zeros, (key[k] & kMask) == prefix, key[k], DIGIT);
+        count_piece(key, threshold, above, at);
     }
-    count_zeros(room, zeros, DIGIT);
-    __syncthreads();
-    if (DIGIT == 0 && threadIdx.x == 0 && room.zeros) atomicAdd(&a.zeros[row], room.zeros);
-    uint32_t* histogram = a.histogram + ((size_t)row * kDigits + DIGIT) * kBins;
-#pragma unroll
-    for (uint32_t k = 0; k < kBins; k += kSelectThreads)
-    {
-        const uint32_t v = room.bins[k + threadIdx.x];
-        if (v) atomicAdd(&histogram[k + threadIdx.x], v);
-    }
+    leave_counts(a, room, row, (int)blockIdx.x, above, at);
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_count_kernel(SelectPass a)
+// A piece's entries are put together in LDS first, so that a wave's stores are neighbours (5.5 M entries, 4.1 M kept: 34.5 us of all launches, not 36.1).
+__global__ void __launch_bounds__(kShareThreads) select_place_kernel(SelectPass a)
 {
     __shared__ SharedRoom room;
-    const int row    = blockIdx.y;
-    const RowRange r = row_range(a, row);
-    const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
-    uint32_t above = 0, at = 0;
-    if (r.need > 0 && first < last)
-    {
-        const float* score = a.score + (int64_t)row * a.row_stride;
-        uint32_t prefix = 0;
-        for (int base = first; base < last; base += kSharePiece)
-        {
-            const Piece piece(score, base, last);
-            if (base == first) prefix = known_digits<kDigits>(a, room, row, r.need).digits;
-            uint32_t key[4 * kShareGroups];
-            piece.keys(base, last, key);
-#pragma unroll
-            for (int k = 0; k < 4 * kShareGroups; ++k)
-            {
-                above += key[k] > prefix;
-                at += key[k] == prefix;
-            }
-        }
-    }
-    above = group_inclusive_scan<kSelectThreads>(above, room.sums);
-    __syncthreads();
-    at = group_inclusive_scan<kSelectThreads>(at, room.sums);
-    if (threadIdx.x == kSelectThreads - 1) a.counts[(size_t)row * a.groups + blockIdx.x] = make_uint2(above, at);
-}
-
-__global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass a)
-{
-    __shared__ SharedRoom room;
-    __shared__ uint32_t totals[kShareGroups * (kSelectThreads / kWave)];
+    __shared__ uint32_t totals[kShareGroups * (kShareThreads / kWave)];
+    __shared__ int32_t placed[kSharePiece];
     const int row    = blockIdx.y;
     const RowRange r = row_range(a, row);
     int32_t* index   = a.index + (int64_t)row * a.budget;
     const int first = (int)blockIdx.x * a.share, last = min(r.range, first + a.share);
     if (r.need > 0 && first < last)
     {
-        const float* score = a.score + (int64_t)row * a.row_stride;
-        const Known known     = unpack_known(a.known[(size_t)row * kDigits + kDigits - 1]);
-        const uint32_t prefix = known.digits, left = known.left;
+        const float* score   = a.score + (int64_t)row * a.row_stride;
+        const Known known    = unpack_known(a.known[(size_t)row * kDigits + kDigits - 1]);
+        const uint32_t left  = known.left;
         uint32_t larger = 0, equal = 0;
         for (int base = first; base < last; base += kSharePiece)
         {
@@ -413,42 +449,32 @@ __global__ void __launch_bounds__(kSelectThreads) select_place_kernel(SelectPass
             {
                 // what the workgroups in front have
                 uint2 sum = make_uint2(0, 0);
-                for (int g = (int)threadIdx.x; g < (int)blockIdx.x; g += kSelectThreads)
+                for (int g = (int)threadIdx.x; g < (int)blockIdx.x; g += kShareThreads)
                 {
                     const uint2 c = a.counts[(size_t)row * a.groups + g];
                     sum.x += c.x, sum.y += c.y;
                 }
-                sum.x = group_inclusive_scan<kSelectThreads>(sum.x, room.sums);
+                sum.x = group_inclusive_scan<kShareThreads>(sum.x, room.sums);
                 __syncthreads();
-                sum.y = group_inclusive_scan<kSelectThreads>(sum.y, room.sums);
-                if (threadIdx.x == kSelectThreads - 1) room.bin = sum.x, room.left = sum.y;
+                sum.y = group_inclusive_scan<kShareThreads>(sum.y, room.sums);
+                if (threadIdx.x == kShareThreads - 1) room.bin = sum.x, room.left = sum.y;
                 __syncthreads();
-                larger = room.bin, equal = room.left;
             }
+            larger = room.bin, equal = room.left;
             uint32_t key[4 * kShareGroups];
             piece.keys(base, last, key);
-            give_places<kSelectThreads, kShareGroups>(key, base, prefix, left, larger, equal, index, totals);
-            if (base + kSharePiece >= last) break;
-            // this piece's own, for the next one
-            uint32_t above = 0, at = 0;
-#pragma unroll
-            for (int k = 0; k < 4 * kShareGroups; ++k)
-            {
-                above += key[k] > prefix;
-                at += key[k] == prefix;
-            }
+            const uint32_t from = larger + min(equal, left);
+            give_places<kShareThreads, kShareGroups>(key, base, known.digits, left, larger, equal, placed, from, totals);
+            if (threadIdx.x == kShareThreads - 1) room.bin = larger, room.left = equal;
             __syncthreads();
-            above = group_inclusive_scan<kSelectThreads>(above, room.sums);
-            __syncthreads();
-            at = group_inclusive_scan<kSelectThreads>(at, room.sums);
-            if (threadIdx.x == kSelectThreads - 1) room.bin = above, room.left = at;
-            __syncthreads();
-            larger += room.bin, equal += room.left;
+            const uint32_t to = room.bin + min(room.left, left);
+            for (uint32_t i = from + threadIdx.x; i < to; i += kShareThreads) index[i] = placed[i - from];
+            // (the next piece's are written behind two barriers)
         }
     }
     // the entries that stay in any case, and what is left of the row
     const int selected = min(r.need, r.range), behind = a.budget - selected;
-    for (int64_t i = (int64_t)blockIdx.x * kSelectThreads + threadIdx.x; i < behind; i += (int64_t)gridDim.x * kSelectThreads)
+    for (int64_t i = (int64_t)blockIdx.x * kShareThreads + threadIdx.x; i < behind; i += (int64_t)gridDim.x * kShareThreads)
         index[selected + i] = i < r.length - r.range ? r.range + (int)i : -1;
     if (blockIdx.x == 0 && threadIdx.x == 0) a.count[row] = selected + r.length - r.range;
 }
