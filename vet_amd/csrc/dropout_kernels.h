@@ -17,7 +17,11 @@ struct DropoutPass
 };
 
 // y = scale * x where x is kept, else 0, plus the residual: one rounding to the type. What is left out is not looked at, so that an
-// infinity or a NaN there leaves nothing behind. A thread takes eight elements.
+// infinity or a NaN there leaves nothing behind.
+//
+// A thread takes the eight elements of one evaluation of the generator, one load of 16 bytes for types of 16 bits; the evaluation lies
+// between the loads and the first use of what they bring. Memory bounds it: 66 M float16 with a residual take 69 us, 5.8 TB/s, 16.8 M bf16 18
+// with a residual and 13.4 without. Below about 1 M elements a call is its launch, 4 us.
 template <int TYPE, bool RESIDUAL>
 __global__ void __launch_bounds__(kBlock) dropout_kernel(DropoutPass a)
 {

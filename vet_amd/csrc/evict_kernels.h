@@ -204,7 +204,8 @@ __device__ __forceinline__ void give_places(const uint32_t (&key)[4 * GROUPS], i
     larger = more, equal = same;
 }
 
-// One workgroup for a row, its keys in registers.
+// One workgroup for a row, its keys in registers: what it costs is instructions, barriers and atomics in LDS, one after the other. A row of 20 k scores takes
+// 14.7 us, 11 where the budget ends among zeros; 64 rows of 8193 7.5.
 template <int THREADS, int GROUPS>
 __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 {
@@ -267,6 +268,8 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 }
 
 // ---- rows of several workgroups: a launch for each digit, one that counts and one that gives places ---------------------------
+// A launch is the barrier between workgroups. Five passes over the scores, most of them from the last-level cache: 5.5 M take 34.6 us, of
+// which 10 are the first digit, 7 the counts, 11 the places and 7 launches that find nothing to do (45 where the budget does not end among zeros).
 
 // Workgroups of 512: a row of 40 k entries takes 20.0 us of all launches, 64 rows of 131 k 48.5, one of 5.5 M 34.5 (with 1024 threads 23.8, 62 and
 // 34.8; with 256 19.9, 48 and 39). Three groups of four of a thread under way at once (5.5 M entries: with 2 7 us more).
@@ -517,8 +520,9 @@ __device__ __forceinline__ Unit nothing(const Unit&)
     return 0;
 }
 
-// A workgroup goes through kKeepChunk units of an outer. Loads are made by all threads, of an entry that is there, so that none waits for a
-// branch around another.
+// A workgroup goes through kKeepChunk units of an outer, units being the largest that size, strides and addresses allow (16 bytes at most). Loads are made by
+// all threads, of an entry that is there, so that none waits for a branch around another. Memory bounds it: keys and values of 64 heads, 2048 of 8193
+// entries of 256 bytes, 26.6 us, 5.1 TB/s.
 template <class Unit>
 __device__ __forceinline__ void keep_units(const KeepEntry& e, const int32_t* index, const char* src, char* dst, uint32_t begin)
 {
@@ -551,7 +555,8 @@ __device__ __forceinline__ void keep_units(const KeepEntry& e, const int32_t* in
     }
 }
 
-// Entries of one unit of 4 bytes, planes of floats mostly: a thread takes four neighbouring ones at a time. (The last four of an outer may be taken twice.)
+// Entries of one unit of 4 bytes, planes of floats mostly: a thread takes four neighbouring ones at a time, whose indices and results are 16 bytes (a scene of
+// 2 M points, 353 MB, 72 us, 4.9 TB/s; unit by unit 92). The last four of an outer may be taken twice.
 __device__ __forceinline__ void keep_words(const KeepEntry& e, const int32_t* index, const char* src, char* dst, uint32_t begin)
 {
     const uint32_t end = e.kept;
