@@ -67,6 +67,17 @@ def test_a_cloud():
     check(scores(1, 2_000_003, "plain")[0], 5, 2)
 
 
+def test_long_rows_that_end_anywhere():
+    """Workgroups with several shares, some of them empty; rows beside one another whose budget ends among zeros and elsewhere."""
+    n = 2_000_003
+    length = torch.tensor([n, 1_234_567, 6144 * 4 + 1, 17, 1_600_000], dtype=torch.int32, device="cuda")
+    s = torch.cat([scores(3, n, "weights"), scores(1, n, "plain"), scores(1, n, "ties")])
+    s[1, :700_000] = 0
+    for budget, recent in ((20_000, 0), (1_000_000, 333), (1_500_000, 100_000)):
+        check(s, budget, recent, length)
+        check(s.flip(0), budget, recent, length)
+
+
 def test_many_rows():
     check(scores(70_001, 3, "ties"), 2, 1)
     s = scores(300, 1000, "plain")
