@@ -95,6 +95,22 @@ def test_the_definition(mode, rasterizer):
         assert want.sum() > 0 or scene.num_points == 1
 
 
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("K, views", [(8, 1), (8, 5), (-1, 1)])
+def test_many_points(mode, K, views, rasterizer):
+    """So many that the call clears a place for each of them instead of finding their pixels again."""
+    scene = synthetic.tiny_scene(num_points=140_000, w=96, h=64, num_layers=2, K=K, seed=11, num_views=views)
+    scene.dropout = (np.random.default_rng(11).random((views, 140_000)) < 0.2).astype(np.float32)
+    params = make_params(scene, render_mode=mode)
+    res = rasterizer.forward(DeviceScene(scene), params)
+    want, roundings = definition(res, scene, params)
+    start = torch.rand(scene.num_points, device="cuda")
+    close(rasterizer.point_weights(res, start.clone(), 0.75), want, roundings, start.double().cpu().numpy(), 0.75)
+    got = rasterizer.point_weights(res, torch.full_like(start, float("nan")), 0.0)
+    close(got, want, roundings)
+    assert torch.equal(got, rasterizer.point_weights(res, torch.empty_like(start), 0.0))
+
+
 @pytest.mark.parametrize("mode", [1, 3])
 def test_it_is_a_gradient(mode, rasterizer):
     """The sum of all pixels of a channel has these sums as its gradient with respect to that channel's descriptors, which the backward pass

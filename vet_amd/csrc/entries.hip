@@ -17,7 +17,7 @@ namespace vetrast
 void launch_fragment_weights(const WeightPass& pass, int hits, bool fuzzy, int views, hipStream_t stream)
 {
     const dim3 block(kBlock);
-    if (hits == 1)
+    if (slots_are_cleared(hits, pass.N))
     {
         const size_t n = ((size_t)pass.N * pass.ly.L + 3) / 4;
         hipLaunchKernelGGL(clear_slots_kernel, dim3((uint32_t)std::min<size_t>((n + kBlock - 1) / kBlock, 8192), (uint32_t)views), block, 0, stream, pass, n);
@@ -34,8 +34,9 @@ void launch_fragment_weights(const WeightPass& pass, int hits, bool fuzzy, int v
 void launch_point_weights(const PointWeightPass& pass, int hits, hipStream_t stream)
 {
     const dim3 grid((uint32_t)((pass.vp.N + kBlock - 1) / kBlock)), block(kBlock);
-    if (hits == 1) hipLaunchKernelGGL(point_weights_cleared_kernel, grid, block, 0, stream, pass);
-    else hipLaunchKernelGGL(point_weights_kernel, grid, block, 0, stream, pass);
+    if (slots_are_cleared(hits, pass.vp.N)) hipLaunchKernelGGL(point_weights_cleared_kernel, grid, block, 0, stream, pass);
+    else if (hits == 1) hipLaunchKernelGGL((point_weights_kernel<1>), grid, block, 0, stream, pass);
+    else hipLaunchKernelGGL((point_weights_kernel<4>), grid, block, 0, stream, pass);
 }
 }  // namespace vetrast
 

@@ -8,8 +8,7 @@
 // These stores bound it, at 110 to 125 G a second: 1920x1080 with 2 M points has 4.6 M fragments, 36 us, beside 6.6 to clear the slots and 12 for
 // the points; four 512x512 crops of the 2x2 splat have 9.0 M, 81 us, and the points 69, of which 27 to find out that no view sees a point. (A
 // point's four corners in one store, if they met on the chip, would take 22 us off the crops before the work of letting them meet. 20 k points:
-// three launches, 9 us. Finding pixels again instead of clearing slots, with one hit per layer: 20 k points 1.4 us less, 200 k 0.4 to
-// 0.8 more, 2 M 10 more.)
+// two launches, 8 us.)
 #pragma once
 #include "weight_pass.h"
 
@@ -178,8 +177,9 @@ __global__ void __launch_bounds__(kBlock) point_weights_cleared_kernel(PointWeig
     add_weight(a, i, sum);
 }
 
-// 2x2 splat: a thread finds its point's pixels again, and out whether its fragments there were blended, in the way of the gradients' pass. (Zeroed slots
-// would be 64 bytes a point and view, most of which a crop does not see.)
+// Slots are not cleared (slots_are_cleared): a thread finds its point's pixels again, and out whether its fragments there were blended, in the way of the
+// gradients' pass. (With the 2x2 splat zeroed slots would be 64 bytes a point and view, most of which a crop does not see.)
+template <int HITS>
 __global__ void __launch_bounds__(kBlock) point_weights_kernel(PointWeightPass a)
 {
     const int i = blockIdx.x * kBlock + threadIdx.x, N = a.vp.N;
@@ -195,14 +195,25 @@ __global__ void __launch_bounds__(kBlock) point_weights_kernel(PointWeightPass a
         const DeviceView& cam = a.vp.view[view];
         const uint8_t* is_cut = a.list_is_cut + (size_t)view * a.flags_stride;
         const uint64_t* last  = a.last_key + (size_t)view * a.last_key_stride;
-        const float4* slots   = reinterpret_cast<const float4*>(a.slots + (size_t)view * a.slots_stride);
+        const float* slots    = a.slots + (size_t)view * a.slots_stride;
         Projected p;
         if (surely_outside(cam, (float)ly.w[0], (float)ly.h[0], reach, wp) || point_is_dropped(a.vp, view, i) || !project_point(cam, wp, p)) continue;
         if (!(p.ipx >= -reach && p.ipx <= (float)ly.w[0] + reach && p.ipy >= -reach && p.ipy <= (float)ly.h[0] + reach)) continue;
-        const uint64_t key = (uint64_t)__float_as_uint(p.z) << 32 | (uint32_t)i << 2;
+        const uint64_t key = (uint64_t)__float_as_uint(p.z) << 32 | (HITS == 1 ? (uint32_t)i : (uint32_t)i << 2);
         for (int l = 0; l < ly.L; ++l, p.ipx *= 0.5f, p.ipy *= 0.5f, p.radius *= 0.5f)
         {
             if (a.vp.drop_by_radius && p.radius < a.vp.radius_threshold) break;
+            if constexpr (HITS == 1)
+            {
+                const float fx   = rintf(p.ipx), fy = rintf(p.ipy);
+                const bool in    = fx >= 0.f && fx < (float)ly.w[l] && fy >= 0.f && fy < (float)ly.h[l];
+                const uint32_t x = in ? (uint32_t)(int)fx : 0u, y = in ? (uint32_t)(int)fy : 0u;
+                const uint32_t q = ly.base[l] + (y / kTile * (uint32_t)ly.tiles_x[l] + x / kTile) * kTilePixels + y % kTile * kTile + x % kTile;
+                const bool cut   = is_cut[q] != 0;
+                const float T    = slots[(size_t)l * N + i];
+                if (in && (!cut || key <= last[q])) sum += a.fuzzy ? T : conf * T;
+                continue;
+            }
             // pixel number = part of its column + part of its row (tile_pixel)
             const float fx = floorf(p.ipx), fy = floorf(p.ipy), sx = p.ipx - fx, sy = p.ipy - fy;
             const int x = (int)fx, y = (int)fy, w = ly.w[l], h = ly.h[l];
@@ -225,7 +236,7 @@ __global__ void __launch_bounds__(kBlock) point_weights_kernel(PointWeightPass a
                 kept[c] = in_x[c & 1] && in_y[c >> 1];
                 cut[c]  = is_cut[of_x[c & 1] + of_y[c >> 1]] != 0;
             }
-            const float4 slot = slots[(size_t)l * N + i];
+            const float4 slot = reinterpret_cast<const float4*>(slots)[(size_t)l * N + i];
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (kept[c] && cut[c]) kept[c] = (key | (uint32_t)c) <= last[of_x[c & 1] + of_y[c >> 1]];

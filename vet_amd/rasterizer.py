@@ -224,7 +224,7 @@ class Rasterizer:
 
     @staticmethod
     def _stream():
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))  # 3 us less than a Stream object
 
     def layout(self, scene: Scene, render_mode=abi.RENDER_FULL_BLEND) -> abi.WorkspaceLayout:
         lay = abi.WorkspaceLayout()
