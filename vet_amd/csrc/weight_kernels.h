@@ -5,8 +5,8 @@
 // points multiply it with their alpha and add up in a fixed order, so that results do not depend on the order of atomics. A fragment is one
 // scattered store; its alpha the point has at hand.
 //
-// These stores bound it, at 110 to 125 G a second: 1920x1080 with 2 M points has 4.6 M fragments, 36 us, beside 6.6 to clear the slots and 12 for
-// the points; four 512x512 crops of the 2x2 splat have 9.0 M, 81 us, and the points 69, of which 27 to find out that no view sees a point. (A
+// These stores bound it, at 117 to 127 G a second: 1920x1080 with 2 M points has 4.6 M fragments, 36 us, beside 6.6 to clear the slots and 11 for
+// the points; four 512x512 crops of the 2x2 splat have 9.0 M, 77 us, and the points 68, of which 27 to find out that no view sees a point. (A
 // point's four corners in one store, if they met on the chip, would take 22 us off the crops before the work of letting them meet. 20 k points:
 // two launches, 8 us.)
 #pragma once
@@ -21,14 +21,16 @@ __global__ void __launch_bounds__(kBlock) clear_slots_kernel(WeightPass a, size_
 }
 
 // A wave takes the 256 pixels of a tile, whose lists are one stretch of the fragments: a lane takes a fragment, whichever pixel's it is. Tiles
-// with long lists are shared by several waves, each of which takes every `parts`-th 256 fragments. Where a list was not blended to its
+// with long lists are shared by several waves, each of which takes every `parts`-th 128 fragments. Where a list was not blended to its
 // end, a bit in LDS is turned over where a pixel's blended fragments begin and where they end: a fragment was blended if an odd number of bits
 // up to its own is set. Neighbouring tiles of a layer go to one XCD: their fragments are of the same blocks of points, whose slots then come
-// together in one L2. (To find a fragment's pixel by a search over the lanes took 14 lane exchanges for 64 fragments.)
+// together in one L2, and are not driven out by lists that are read once (loaded the ordinary way 1080p takes 1.5 us more). (To find a
+// fragment's pixel by a search over the lanes took 14 lane exchanges for 64 fragments.)
 template <int HITS>
 __global__ void __launch_bounds__(kBlock) fragment_weights_kernel(WeightPass a)
 {
-    constexpr uint32_t kEach = 4, kWindow = kEach * kWave;  // fragments of a lane under way at once
+    // fragments of a lane under way at once (four crops 146.8 us of the call, with 1 147.3, with 4 151, with 8 162; 1080p 53.4, 54.0, 53.7)
+    constexpr uint32_t kEach = 2, kWindow = kEach * kWave;
     __shared__ uint32_t turns[kBlock / kWave][kWindow / 32];
     const uint32_t xcd = blockIdx.x % kXcds, group = blockIdx.x / kXcds, lane = threadIdx.x % kWave;
     int l = 0;
@@ -95,8 +97,8 @@ __global__ void __launch_bounds__(kBlock) fragment_weights_kernel(WeightPass a)
         for (uint32_t k = 0; k < kEach; ++k)
             if (blended[k])
             {
-                low[k] = (uint32_t)v.fragments[base + k * kWave + lane];
-                T[k]   = v.transmittance[base + k * kWave + lane];
+                low[k] = (uint32_t)__builtin_nontemporal_load(v.fragments + base + k * kWave + lane);
+                T[k]   = __builtin_nontemporal_load(v.transmittance + base + k * kWave + lane);
             }
 #pragma unroll
         for (uint32_t k = 0; k < kEach; ++k)

@@ -46,18 +46,18 @@ struct PointWeightPass
     float* sum;                  // [N]
 };
 
-// Waves that share a tile of a layer, from an upper bound of its fragments (every point lands in the layer). A wave then has 256 at most with one hit
-// per layer (1080p, 2 M points: 36 us of the pass, with 1024 57, for the waves of the fullest tiles are the last), and 1024 with the 2x2 splat, with
-// which mostly crops are rendered, that see a part of the points (four 512x512 crops: 81 us, with 256 and four times as many waves, most of them
-// without a fragment, 89).
+// Waves that share a tile of a layer, from an upper bound of its fragments (every point lands in the layer). A wave then has 128 at most with one hit
+// per layer, all of them under way at once, for the waves of the fullest tiles are the last (1080p: 500 k points 22.3 us of the call, with 256 25.3,
+// with 1024 50.5; 2 M 53.4, 53.1 and 77), and 1024 with the 2x2 splat, with which mostly crops are rendered, that see a part of the points (four
+// 512x512 crops: 147 us, with 256 and four times as many waves, most of them without a fragment, 155, with 4096 155).
 inline uint32_t weight_parts(double fragments, uint32_t tiles, int hits)
 {
-    return (uint32_t)std::min(std::max(std::ceil(fragments / tiles / (hits == 1 ? 256.0 : 1024.0)), 1.0), 64.0);
+    return (uint32_t)std::min(std::max(std::ceil(fragments / tiles / (hits == 1 ? 128.0 : 1024.0)), 1.0), 64.0);
 }
 
 // Whether slots are cleared for points without a fragment, and points read them without looking where they are. With one hit per layer, and where there are
 // many points: 2 M at 1080p 54.8 us (finding pixels again 65), 200 k 18.1 (18.8), 400 k in one layer of 256x256 13.7 (15.2); for few ones it
-// is a launch too many, 100 k 12.8 us (12.4), 20 k 9.6 (8.2), and 12.4 of the host (9.7).
+// is a launch too many, 100 k 12.8 us (12.4), 20 k 9.6 (8.2).
 inline bool slots_are_cleared(int hits, int points) { return hits == 1 && points > 131072; }
 
 // entries.hip
