@@ -588,6 +588,9 @@ void AdamW::keep_rows(const std::vector<torch::Tensor>& params, const torch::Ten
         torch::Tensor& p = slots[chosen[j]].param;
         p.mutable_grad().reset();
         p.set_data(kept[j * each]);
+        // A leaf's node expects gradients of the size that the leaf had when the node was made, and lives as long as any graph of it: graphs from here
+        // on get a node of their own. (Hooks are the tensor's, not the node's.)
+        torch::autograd::impl::set_grad_accumulator(p, {});
     }
     slots_.swap(slots);
     exp_avg     = std::move(m);
