@@ -74,6 +74,15 @@ vetrast_moments_args moments_args(const std::vector<vetrast_moment_tensor>& list
 {
     return {list.data(), (int32_t)list.size(), 0, m.data_ptr<uint8_t>(), v.data_ptr<uint8_t>(), scale.data_ptr<uint8_t>()};
 }
+
+// On the node of a leaf that has other entries than when the node was made.
+struct RefuseGradients : torch::autograd::FunctionPreHook
+{
+    torch::autograd::variable_list operator()(const torch::autograd::variable_list&) override
+    {
+        TORCH_CHECK(false, "a parameter has other entries since AdamW.keep_rows: a graph from before cannot be differentiated");
+    }
+};
 }  // namespace
 
 AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
@@ -588,8 +597,12 @@ void AdamW::keep_rows(const std::vector<torch::Tensor>& params, const torch::Ten
         torch::Tensor& p = slots[chosen[j]].param;
         p.mutable_grad().reset();
         p.set_data(kept[j * each]);
+        // Graphs from before have saved other entries, at places that mean others now. Where they have saved nothing their gradients are refused when
+        // they come to the leaf's node.
+        p.unsafeGetTensorImpl()->bump_version();  // (set_data does not)
+        if (const auto node = torch::autograd::impl::try_get_grad_accumulator(p)) node->add_pre_hook(std::make_unique<RefuseGradients>());
         // A leaf's node expects gradients of the size that the leaf had when the node was made, and lives as long as any graph of it: graphs from here
-        // on get a node of their own. (Hooks are the tensor's, not the node's.)
+        // on get a node of their own. (A tensor's hooks are the tensor's, not the node's.)
         torch::autograd::impl::set_grad_accumulator(p, {});
     }
     slots_.swap(slots);

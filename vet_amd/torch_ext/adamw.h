@@ -65,7 +65,7 @@ class AdamW
     // Parameters shrink to the entries `index` (int32 [K], as SelectKept gives them; one below 0 or beyond the end leaves zeros) along dims[k], and
     // their moments and masters with them: a scene that loses points trains on. Their gradients are dropped, counts stay, and the other parameters
     // keep their state. params: contiguous parameters of this optimiser. 8-bit moments are rounded to nearest once more. Not with capturable, whose captured
-    // steps would go on with what was there. Nothing changes if it throws.
+    // steps would go on with what was there. Graphs of these parameters from before can no longer be differentiated. Nothing changes if it throws.
     void keep_rows(const std::vector<torch::Tensor>& params, const torch::Tensor& index, const std::vector<int64_t>& dims);
     // Masters are read from the parameters again (after a checkpoint was loaded into these).
     void reload_master();

@@ -81,7 +81,8 @@ def AdamW(groups, beta1=0.9, beta2=0.999, eps=1e-8, moment_bits=32, master_weigh
     layout() -> [(first element, elements)] in the flat state tensors exp_avg, exp_avg_sq, block_scale and master; moments() ->
     both as flat float32; load_moments(exp_avgs, exp_avg_sqs, n or a list of counts), reload_master().
     keep_rows(params, index, dims): contiguous parameters shrink to the entries `index` (int32 [K], see select_kept) along their dimension,
-    with their moments and masters; their gradients are dropped, counts stay. Not with capturable."""
+    with their moments and masters; their gradients are dropped, counts stay, and graphs of them from before can no longer be differentiated. Not with
+    capturable."""
     return load().AdamW([(list(g[0]), float(g[1]), float(g[2]) if len(g) > 2 else 0.0) for g in groups], beta1, beta2, eps,
                         int(moment_bits), bool(master_weights), bool(stochastic_rounding), int(seed), bool(capturable))
 
