@@ -60,6 +60,19 @@ def test_a_render_from_before_is_refused(kept):
     assert texture.grad.shape == (4, kept) and position.grad.shape == (kept, 4) and all(torch.isfinite(t).all() for t in (texture, confidence, position))
 
 
+@pytest.mark.parametrize("points, channels", [(650, 4), (900, 3), (1200, 4)])
+def test_a_render_whose_tensors_were_exchanged_is_refused(points, channels):
+    """As a program may do it by itself; torch does not see it."""
+    scene = synthetic.tiny_scene(num_points=900, seed=5)
+    other = synthetic.tiny_scene(num_points=points, channels=channels, seed=6)
+    texture, confidence, position, call = render(scene)
+    loss = call()
+    for t, a in ((texture, other.texture), (confidence, other.confidence.reshape(1, -1)), (position, other.position)):
+        t.data = torch.from_numpy(a).cuda()
+    with pytest.raises(RuntimeError, match="rendered with 900 points of 4 channels"):
+        loss.backward()
+
+
 @pytest.mark.parametrize("kept", [60, 41])
 def test_a_graph_that_has_saved_nothing_is_refused_too(kept):
     p = torch.randn(60, 4, device="cuda", requires_grad=True)

@@ -458,6 +458,7 @@ torch::autograd::variable_list PointRender::forward(torch::autograd::AutogradCon
         ctx->saved_data["pose_need_grad"]   = pose_tangents.requires_grad();
         ctx->saved_data["intr_need_grad"]   = intrinsics.requires_grad();
         ctx->saved_data["num_poses"]        = (int64_t)poses_se3.size(0);
+        ctx->saved_data["num_points"]       = N;
     }
     // With add_depth_to_network the output list carries L depth tensors behind the images
     // (src/lib/rendering/PointRenderer.cu:1061-1066). The blend modes never write them: they are the zero-filled
@@ -498,6 +499,10 @@ torch::autograd::variable_list PointRender::backward(torch::autograd::AutogradCo
     vetrast_backward_args g;
     std::memset(&g, 0, sizeof(g));
     g.fwd = make_forward_args(info, texture, background_color, points, intrinsics, confidence, dropout, poses_se3, t_index);
+    // The workspace is laid out for what was rendered. Data that was exchanged (set_data, .data) does not tell torch.
+    const int64_t rendered_points = ctx->saved_data["num_points"].toInt(), rendered_channels = saved[kFixed].size(1);
+    TORCH_CHECK(points.size(0) == rendered_points && texture.size(0) == rendered_channels, "this graph was rendered with ", rendered_points, " points of ",
+                rendered_channels, " channels, its tensors have ", points.size(0), " of ", texture.size(0), " now");
     std::vector<torch::Tensor> grads(L);
     for (int l = 0; l < L; ++l)
     {
