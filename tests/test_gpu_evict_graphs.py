@@ -104,3 +104,24 @@ def test_training_goes_on_while_a_graph_from_before_lives():
     assert torch.equal(p.grad, 2 * p.detach()) and seen == [(41, 4), (41, 4)]
     assert torch.isfinite(before)
     opt.step()
+
+
+def test_in_inference_mode():
+    """An eviction needs no gradients; what it leaves is trained on."""
+    torch.manual_seed(3)
+    start = torch.randn(60, 4, device="cuda")
+    results = []
+    for mode in (torch.no_grad, torch.inference_mode):
+        p, q = start.clone().requires_grad_(True), torch.ones(5, device="cuda", requires_grad=True)
+        opt = torch_ops.AdamW([([p, q], 0.1)])
+        for k in range(3):
+            opt.zero_grad()
+            ((p * p).sum() + (q * q).sum()).backward()
+            opt.step()
+            if k == 1:
+                with mode():
+                    opt.keep_rows([p], some(60, 41), [0])
+                assert not p.is_inference() and not opt.exp_avg.is_inference() and p.is_leaf and p.requires_grad
+        opt.load_moments([torch.zeros_like(p), torch.zeros_like(q)], [torch.zeros_like(p), torch.zeros_like(q)], 0)
+        results.append(p.detach())
+    assert torch.equal(*results)

@@ -6,6 +6,7 @@
 #include <utility>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/InferenceMode.h>
 
 #include "calls.h"
 #include "entries.h"
@@ -493,6 +494,7 @@ void AdamW::load_moments(const std::vector<torch::Tensor>& exp_avgs, const std::
 
 void AdamW::keep_rows(const std::vector<torch::Tensor>& params, const torch::Tensor& index, const std::vector<int64_t>& dims)
 {
+    c10::InferenceMode inference(false);  // what is made here is trained on, also where the caller evaluates
     torch::NoGradGuard no_grad;
     c10::DeviceGuard guard(device_);
     TORCH_CHECK(params.size() == dims.size(), "AdamW: ", params.size(), " parameters, but dimensions of ", dims.size());
