@@ -125,3 +125,21 @@ def test_in_inference_mode():
         opt.load_moments([torch.zeros_like(p), torch.zeros_like(q)], [torch.zeros_like(p), torch.zeros_like(q)], 0)
         results.append(p.detach())
     assert torch.equal(*results)
+
+
+def test_on_another_stream_than_the_parameters_own():
+    """The old entries are read there, and their memory is not given out before that."""
+    n = 1 << 20
+    p = torch.randn(n, 4, device="cuda", requires_grad=True)
+    opt = torch_ops.AdamW([([p], 0.1)])
+    p.grad = torch.ones_like(p)
+    index = some(n, n // 2 + 1)
+    want = p.detach().index_select(0, index.long())
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(50_000_000)
+        opt.keep_rows([p], index, [0])
+    taken = [torch.full((n, 4), float("nan"), device="cuda") for _ in range(4)]  # what an allocation at once would get
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(p.detach(), want) and torch.isnan(taken[0]).all()

@@ -597,6 +597,9 @@ void AdamW::keep_rows(const std::vector<torch::Tensor>& params, const torch::Ten
     for (size_t j = 0; j < chosen.size(); ++j)
     {
         torch::Tensor& p = slots[chosen[j]].param;
+        // (what is let go may be memory of another stream, which must not give it out before this one has read it)
+        for (const torch::Tensor& old : {p.detach(), p.grad()})
+            if (old.defined() && old.layout() == torch::kStrided && old.numel() > 0) old.record_stream(*stream_);
         p.mutable_grad().reset();
         p.set_data(kept[j * each]);
         // Graphs from before have saved other entries, at places that mean others now. Where they have saved nothing their gradients are refused when
