@@ -358,6 +358,8 @@ void AdamW::step(bool zero_grad, const std::optional<torch::Tensor>& grad_scale)
         a.grad_scale = x.data_ptr<float>() + x.numel() - 1;
     }
     check(vetrast_adamw_step(context_on(device_), &a, stream_on(device_)), "adamw_step");
+    // the kernel counted: a backward pass that has saved the count (dropout by a step on the device) would go by another one
+    if (device_step.defined() && !device_step.is_inference()) device_step.unsafeGetTensorImpl()->bump_version();
     for (auto& s : slots_)
     {
         const torch::Tensor& grad = s.param.grad();

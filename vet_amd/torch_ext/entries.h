@@ -17,7 +17,7 @@ namespace vet_amd
 // is a function of seed, step and an element's place in memory (a tensor with gaps is made contiguous first), and nothing is kept for the
 // backward pass. Give every layer a seed of its own and count steps.
 // device_step: int64 [1] on the GPU, added to `step` (AdamW::device_step, say), for steps that are captured in a graph. The backward
-// pass reads it again: it must not be written between the two.
+// pass reads it again: it must not be written between the two, which is noticed and refused unless a replayed graph has done it.
 torch::Tensor Dropout(const torch::Tensor& x, double p, uint64_t seed, uint64_t step = 0, const std::optional<torch::Tensor>& residual = std::nullopt,
                       const std::optional<torch::Tensor>& device_step = std::nullopt);
 

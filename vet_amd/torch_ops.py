@@ -113,7 +113,7 @@ def dropout(x, p, seed, step=0, residual=None, device_step=None):
     The mask is stored nowhere: it is a function of seed, step and an element's place in memory, which the backward pass evaluates again.
     Give every layer a seed of its own and count steps. p counts in multiples of 2^-16. device_step: int64 [1] on the GPU, added to
     step, for steps that are captured in a graph (AdamW(capturable=True).device_step goes up by itself); not to be written between a
-    forward pass and its backward pass."""
+    forward pass and its backward pass (refused, unless a replayed graph has done it)."""
     return load().dropout(x, p, seed, step, residual, device_step)
 
 
