@@ -42,3 +42,21 @@ def test_a_step_of_the_optimiser_is_noticed_by_a_render():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         sum(o.sum() for o in outs).backward()
+
+
+def test_the_rates_factor_is_no_count():
+    """It lies beside the count, and says nothing about masks."""
+    opt = optimiser()
+    x = torch.randn(3000, device="cuda", requires_grad=True)
+    y = torch_ops.dropout(x, 0.3, seed=2, device_step=opt.device_step)
+    opt.lr_factor.fill_(0.5)
+    y.sum().backward()
+    factor, _ = em.dropout(np.ones(3000), 0.3, 2, 0)
+    assert np.abs(x.grad.cpu().numpy() - factor).max() <= 2.0 ** -23 * 2
+    y = torch_ops.dropout(x, 0.3, seed=2, device_step=opt.device_step)
+    opt.set_step(7)
+    assert opt.steps() == [7] and opt.lr_factor.item() == 0.5
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        assert optimiser().steps() == [0]

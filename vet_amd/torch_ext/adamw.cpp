@@ -121,6 +121,7 @@ AdamW::AdamW(std::vector<Group> groups, Options options) : options_(options)
         device_step         = device_state_.narrow(0, 0, 8).view(torch::kInt64);
         lr_factor           = device_state_.narrow(0, 8, 4).view(torch::kFloat32);
         lr_factor.fill_(1.0);
+        if (!device_step.is_inference()) device_step = device_step.variable_data();  // with a version of its own: the factor is no count
     }
 }
 
