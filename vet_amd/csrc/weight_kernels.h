@@ -14,10 +14,16 @@
 
 namespace vetrast
 {
+// Cleared slots hold what no fragment leaves, a NaN with all bits set: a zero there would be multiplied by the confidence of a point that nobody sees, which
+// may be infinite or a NaN. A fragment whose T is that NaN leaves another one.
+constexpr uint32_t kNoFragment = 0xFFFFFFFFu;
+__device__ __forceinline__ bool has_fragment(float slot) { return __float_as_uint(slot) != kNoFragment; }
+__device__ __forceinline__ float for_slot(float x) { return has_fragment(x) ? x : __uint_as_float(0x7FC00000u); }
+
 __global__ void __launch_bounds__(kBlock) clear_slots_kernel(WeightPass a, size_t n)
 {
-    float4* slots = reinterpret_cast<float4*>(a.view[blockIdx.y].slots);
-    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) slots[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint4* slots = reinterpret_cast<uint4*>(a.view[blockIdx.y].slots);
+    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) slots[i] = make_uint4(kNoFragment, kNoFragment, kNoFragment, kNoFragment);
 }
 
 // A wave takes the 256 pixels of a tile, whose lists are one stretch of the fragments: a lane takes a fragment, whichever pixel's it is. Tiles
@@ -105,7 +111,7 @@ __global__ void __launch_bounds__(kBlock) fragment_weights_kernel(WeightPass a)
         {
             if (!blended[k]) continue;
             const uint32_t id = HITS == 1 ? low[k] : low[k] >> 2;
-            if (id < (uint32_t)a.N) v.slots[((size_t)l * a.N + id) * HITS + (HITS == 1 ? 0u : low[k] & 3u)] = T[k];
+            if (id < (uint32_t)a.N) v.slots[((size_t)l * a.N + id) * HITS + (HITS == 1 ? 0u : low[k] & 3u)] = HITS == 1 ? for_slot(T[k]) : T[k];
         }
     }
 }
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(kBlock) fragment_weights_fuzzy_kernel(WeightPa
         return a.confidence_activation ? sigmoid_canon(a.confidence_scale * c) : c;
     };
     const auto store = [&](int id, float w) {
-        if ((uint32_t)id < (uint32_t)a.N) v.slots[(size_t)l * a.N + id] = w;
+        if ((uint32_t)id < (uint32_t)a.N) v.slots[(size_t)l * a.N + id] = for_slot(w);
     };
     uint32_t m  = 0;
     float sum   = 0.f;
@@ -161,7 +167,7 @@ __device__ __forceinline__ void add_weight(const PointWeightPass& a, int i, floa
     else a.sum[i] = (a.decay != 0.f ? a.decay * a.sum[i] : 0.f) + sum;
 }
 
-// Slots of points without a fragment are zeros.
+// Slots of points without a fragment say so.
 __global__ void __launch_bounds__(kBlock) point_weights_cleared_kernel(PointWeightPass a)
 {
     const int i = blockIdx.x * kBlock + threadIdx.x, N = a.vp.N, L = a.vp.ly.L;
@@ -172,9 +178,9 @@ __global__ void __launch_bounds__(kBlock) point_weights_cleared_kernel(PointWeig
     {
         float T[VETRAST_MAX_LAYERS];
 #pragma unroll
-        for (int l = 0; l < VETRAST_MAX_LAYERS; ++l) T[l] = l < L ? a.slots[(size_t)view * a.slots_stride + (size_t)l * N + i] : 0.f;
+        for (int l = 0; l < VETRAST_MAX_LAYERS; ++l) T[l] = l < L ? a.slots[(size_t)view * a.slots_stride + (size_t)l * N + i] : __uint_as_float(kNoFragment);
 #pragma unroll
-        for (int l = 0; l < VETRAST_MAX_LAYERS; ++l) sum += alpha * T[l];
+        for (int l = 0; l < VETRAST_MAX_LAYERS; ++l) sum += has_fragment(T[l]) ? alpha * T[l] : 0.f;
     }
     add_weight(a, i, sum);
 }
