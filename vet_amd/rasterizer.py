@@ -4,6 +4,7 @@ This is what tests and bench.py drive. It adds no arithmetic of its own and has 
 built HIP library every call raises.
 """
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import List, Optional
 
@@ -462,16 +463,19 @@ class Rasterizer:
 
     def keep_rows(self, tensors, index):
         """Entries `index` [index_rows, kept] of a list of contiguous tensors [outers, n, ...] (vetrast_keep_rows)."""
-        ts, a = (abi.KeepTensor * max(len(tensors), 1))(), abi.KeepArgs()
+        ts, a, count = (abi.KeepTensor * max(len(tensors), 1))(), abi.KeepArgs(), 0
         assert index.is_cuda and index.dtype == torch.int32 and index.is_contiguous() and index.dim() == 2
         out = []
-        for t, x in zip(ts, tensors):
+        for x in tensors:
             assert x.is_cuda and x.is_contiguous() and x.dim() >= 2
             out.append(torch.empty((x.shape[0], index.shape[1]) + x.shape[2:], dtype=x.dtype, device=x.device))
+            if out[-1].numel() == 0:
+                continue
+            t, count = ts[count], count + 1
             t.src, t.dst, t.outers, t.n = x.data_ptr(), out[-1].data_ptr(), x.shape[0], x.shape[1]
-            t.row_bytes = x[0, 0].numel() * x.element_size() if x.numel() else 1
+            t.row_bytes = math.prod(x.shape[2:]) * x.element_size()  # also where there are no entries, whose rows are zeros
             t.src_row_bytes, t.src_outer_bytes = t.row_bytes, t.row_bytes * t.n
-        a.tensors, a.num_tensors, a.index_rows, a.kept = ts, len(tensors), index.shape[0], index.shape[1]
+        a.tensors, a.num_tensors, a.index_rows, a.kept = ts, count, index.shape[0], index.shape[1]
         a.index, a.index_row_stride = index.data_ptr(), index.shape[1]
         abi.check(self.lib.vetrast_keep_rows(self.ctx, C.byref(a), self._stream()), "keep_rows")
         return out
