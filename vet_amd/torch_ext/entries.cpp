@@ -104,11 +104,13 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction>
 };
 }  // namespace
 
-torch::Tensor Dropout(const torch::Tensor& x, double p, uint64_t seed, uint64_t step, const std::optional<torch::Tensor>& residual,
+// (A view that negates what lies in memory is made a tensor of its own here and below; kernels read memory.)
+torch::Tensor Dropout(const torch::Tensor& given, double p, uint64_t seed, uint64_t step, const std::optional<torch::Tensor>& residual,
                       const std::optional<torch::Tensor>& device_step)
 {
     TORCH_CHECK(p >= 0.0 && p <= 1.0, "dropout: p lies in [0, 1], not ", p);
-    TORCH_CHECK(x.defined() && x.is_cuda() && x.layout() == torch::kStrided, "dropout: x must be a strided tensor on the GPU");
+    TORCH_CHECK(given.defined() && given.is_cuda() && given.layout() == torch::kStrided, "dropout: x must be a strided tensor on the GPU");
+    const torch::Tensor x = given.resolve_neg();
     type_of(x, "dropout: x");
     torch::Tensor added, counted;
     if (residual.has_value() && residual->defined())
@@ -116,12 +118,14 @@ torch::Tensor Dropout(const torch::Tensor& x, double p, uint64_t seed, uint64_t 
         added = *residual;
         check_on(added, x.device(), "dropout: residual");
         TORCH_CHECK(added.scalar_type() == x.scalar_type() && added.sizes() == x.sizes(), "dropout: the residual must have the type and shape of x");
+        added = added.resolve_neg();
     }
     if (device_step.has_value() && device_step->defined())
     {
         counted = *device_step;
         check_on(counted, x.device(), "dropout: device_step");
         TORCH_CHECK(counted.scalar_type() == torch::kInt64 && counted.numel() == 1, "dropout: device_step is one int64");
+        TORCH_CHECK(!counted.is_neg(), "dropout: device_step is read where it lies and cannot be a negative view");
     }
     if (torch::GradMode::is_enabled() && (x.requires_grad() || (added.defined() && added.requires_grad())))
     {
@@ -136,17 +140,18 @@ torch::Tensor Dropout(const torch::Tensor& x, double p, uint64_t seed, uint64_t 
     return dropout_call(x, added, counted, p, seed, step);
 }
 
-std::tuple<torch::Tensor, torch::Tensor> SelectKept(const torch::Tensor& score, int64_t budget, int64_t recent, const std::optional<torch::Tensor>& length)
+std::tuple<torch::Tensor, torch::Tensor> SelectKept(const torch::Tensor& given, int64_t budget, int64_t recent, const std::optional<torch::Tensor>& length)
 {
     constexpr int64_t kMost = (int64_t)1 << 30, kRows = std::numeric_limits<int32_t>::max();
     TORCH_CHECK(budget >= 0 && budget <= kMost, "select_kept: a budget lies in [0, 2^30], not at ", budget);
     TORCH_CHECK(recent >= 0 && recent <= budget, "select_kept: recent lies in [0, budget], not at ", recent);
-    TORCH_CHECK(score.defined() && score.is_cuda() && score.layout() == torch::kStrided && score.scalar_type() == torch::kFloat32,
+    TORCH_CHECK(given.defined() && given.is_cuda() && given.layout() == torch::kStrided && given.scalar_type() == torch::kFloat32,
                 "select_kept: score must be a float32 tensor on the GPU");
-    TORCH_CHECK(score.dim() == 1 || score.dim() == 2, "select_kept: score is [N] or [rows, N]");
-    TORCH_CHECK(score.size(-1) <= kMost && (score.dim() == 1 || score.size(0) <= kRows), "select_kept: a row has at most 2^30 scores, and rows are counted in 32 bits");
-    c10::DeviceGuard guard(score.device());
+    TORCH_CHECK(given.dim() == 1 || given.dim() == 2, "select_kept: score is [N] or [rows, N]");
+    TORCH_CHECK(given.size(-1) <= kMost && (given.dim() == 1 || given.size(0) <= kRows), "select_kept: a row has at most 2^30 scores, and rows are counted in 32 bits");
+    c10::DeviceGuard guard(given.device());
     torch::NoGradGuard no_grad;
+    const torch::Tensor score = given.resolve_neg();
     const bool one      = score.dim() == 1;
     const int64_t rows  = one ? 1 : score.size(0), n = score.size(-1);
     // rows may lie further apart, their scores not, and they must not be one row seen many times
@@ -159,7 +164,7 @@ std::tuple<torch::Tensor, torch::Tensor> SelectKept(const torch::Tensor& score, 
     {
         check_on(*length, score.device(), "select_kept: length");
         TORCH_CHECK(length->scalar_type() == torch::kInt32 && length->numel() == rows, "select_kept: length is int32, one for each row");
-        lengths = length->contiguous();
+        lengths = length->resolve_neg().contiguous();
     }
     const size_t bytes      = vetrast_select_kept_workspace_bytes((int32_t)rows, (int32_t)n);
     torch::Tensor workspace = torch::empty({(int64_t)bytes}, ints.dtype(torch::kUInt8));
@@ -223,7 +228,7 @@ std::vector<torch::Tensor> KeepRows(const std::vector<torch::Tensor>& tensors, c
     constexpr int64_t kMost  = std::numeric_limits<int32_t>::max();
     TORCH_CHECK(kept <= kMost && rows <= kMost && (int64_t)tensors.size() <= kMost, "keep_rows: indices, their rows and tensors are counted in 32 bits");
     const bool apart         = (kept <= 1 || index.stride(-1) == 1) && (one || rows <= 1 || index.stride(0) >= kept);
-    const torch::Tensor at   = apart ? index : index.contiguous();
+    const torch::Tensor at   = apart ? index.resolve_neg() : index.contiguous();
     std::vector<torch::Tensor> out, gathered;
     std::vector<vetrast_keep_tensor> list;
     for (size_t k = 0; k < tensors.size(); ++k)

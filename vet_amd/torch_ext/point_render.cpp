@@ -62,8 +62,8 @@ vetrast_params to_abi_params(const RenderParams& p, int num_layers)
 
 void check_f32_cuda(const torch::Tensor& t, const char* name)
 {
-    TORCH_CHECK(t.defined() && t.is_cuda() && t.scalar_type() == torch::kFloat32 && t.is_contiguous(), name,
-                " must be a contiguous float32 tensor on the GPU");
+    TORCH_CHECK(t.defined() && t.is_cuda() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() && !t.is_neg(), name,
+                " must be a contiguous float32 tensor on the GPU, and no negative view");
 }
 
 // Points are left out without a mask.
@@ -130,8 +130,8 @@ vetrast_forward_args make_forward_args(NeuralRenderInfo* info, const torch::Tens
         const torch::Tensor& count = info->dropout_device_step;
         if (count.defined())
         {
-            TORCH_CHECK(count.device() == points.device() && count.scalar_type() == torch::kInt64 && count.numel() == 1,
-                        "dropout_device_step is one int64 on the points' GPU");
+            TORCH_CHECK(count.device() == points.device() && count.scalar_type() == torch::kInt64 && count.numel() == 1 && !count.is_neg(),
+                        "dropout_device_step is one int64 on the points' GPU, and no negative view");
             a.dropout_device_step = count.data_ptr<int64_t>();
         }
     }
