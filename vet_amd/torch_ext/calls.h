@@ -3,8 +3,10 @@
 #include <torch/torch.h>
 
 #include <map>
+#include <unordered_set>
 #include <utility>
 
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -26,6 +28,37 @@ inline void* stream_on(const torch::Device& device)
 inline bool capturing()
 {
     return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
+// A backward pass waits for the streams of the nodes that it comes to. In a capture each of them has to take part in it: torch otherwise records an
+// event on a stream outside, and the process ends when the capture does. A leaf's node lives as long as any graph of that leaf, so one of an eager
+// pass that still lives is what a captured pass would come to. What leads to `node` is looked at here, where an error can still be given.
+inline void check_captured_gradients(const std::shared_ptr<torch::autograd::Node>& node, const c10::Stream& here, const char* what)
+{
+    const auto captured = [&](const c10::Stream& stream) {
+        if (stream == here) return true;
+        const hipStream_t handle      = c10::hip::HIPStreamMasqueradingAsCUDA(stream).stream();
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return handle != nullptr && hipStreamIsCapturing(handle, &status) == hipSuccess && status == hipStreamCaptureStatusActive;  // forked within the capture
+    };
+    std::vector<std::shared_ptr<torch::autograd::Node>> nodes{node};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!nodes.empty())
+    {
+        const auto next = std::move(nodes.back());
+        nodes.pop_back();
+        if (!next || !seen.insert(next.get()).second) continue;
+        const auto stream = next->stream();
+        TORCH_CHECK(!stream.has_value() || captured(*stream), what, ": an eager graph of a tensor that is differentiated in this captured call still lives (on another stream): ",
+                    "drop it before the capture, or detach");
+        for (const auto& edge : next->next_edges()) nodes.push_back(edge.function);
+    }
+}
+inline void check_captured_gradients(const torch::Tensor& t, const char* what)
+{
+    if (!t.requires_grad()) return;
+    check_captured_gradients(t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t),
+                             c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap(), what);
 }
 
 // What a host thread keeps. A context serves one host thread at a time and belongs to a device, a norm's workspace serves one stream of torch's.

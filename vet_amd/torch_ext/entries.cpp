@@ -3,9 +3,6 @@
 
 #include <cstring>
 #include <limits>
-#include <unordered_set>
-
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include "calls.h"
 
@@ -45,28 +42,6 @@ torch::Tensor dropout_call(const torch::Tensor& x, const torch::Tensor& residual
     if (device_step.defined()) a.device_step = device_step.data_ptr<int64_t>();
     check(vetrast_dropout(context_on(x.device()), &a, stream_on(x.device())), "dropout");
     return y;
-}
-
-// A backward pass ends with a wait for the streams of the nodes that it came to. In a capture each of them has to be the one that is
-// captured: torch otherwise records an event on a stream outside the capture, and the process ends when the capture does. A leaf's node
-// lives as long as any graph of that leaf, so one of an eager pass that still lives is what a captured pass would come to. What leads to
-// `t` is looked at here, where an error can still be given.
-void check_captured_gradients(const torch::Tensor& t, const char* what)
-{
-    if (!t.defined() || !t.requires_grad()) return;
-    const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
-    std::vector<std::shared_ptr<torch::autograd::Node>> nodes{t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t)};
-    std::unordered_set<torch::autograd::Node*> seen;
-    while (!nodes.empty())
-    {
-        const auto node = std::move(nodes.back());
-        nodes.pop_back();
-        if (!node || !seen.insert(node.get()).second) continue;
-        const auto stream = node->stream();
-        TORCH_CHECK(!stream.has_value() || *stream == here, what, ": an eager graph of a tensor that is differentiated in this captured call still lives (on another stream): ",
-                    "drop it before the capture, or detach");
-        for (const auto& edge : node->next_edges()) nodes.push_back(edge.function);
-    }
 }
 
 struct DropoutFunction : public torch::autograd::Function<DropoutFunction>
@@ -132,7 +107,7 @@ torch::Tensor Dropout(const torch::Tensor& given, double p, uint64_t seed, uint6
         if (capturing())
         {
             check_captured_gradients(x, "dropout");
-            check_captured_gradients(added, "dropout");
+            if (added.defined()) check_captured_gradients(added, "dropout");
         }
         const auto maybe = [](const torch::Tensor& t) { return t.defined() ? std::optional(t) : std::nullopt; };
         return DropoutFunction::apply(x, maybe(added), maybe(counted), p, (int64_t)seed, (int64_t)step);
