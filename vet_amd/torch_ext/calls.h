@@ -1,8 +1,10 @@
 // What the tensor calls of this directory share: contexts, streams and what is asked of tensors.
 #pragma once
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/torch.h>
 
 #include <map>
+#include <unordered_map>
 #include <unordered_set>
 #include <utility>
 
@@ -32,8 +34,11 @@ inline bool capturing()
 
 // A backward pass waits for the streams of the nodes that it comes to. In a capture each of them has to take part in it: torch otherwise records an
 // event on a stream outside, and the process ends when the capture does. A leaf's node lives as long as any graph of that leaf, so one of an eager
-// pass that still lives is what a captured pass would come to. What leads to `node` is looked at here, where an error can still be given.
-inline void check_captured_gradients(const std::shared_ptr<torch::autograd::Node>& node, const c10::Stream& here, const char* what)
+// pass that still lives is what a captured pass would come to. What leads to `node` is looked at here, where an error can still be given; with `asked`
+// (of the backward pass under way) only what that pass comes to.
+using AskedNodes = std::unordered_map<torch::autograd::Node*, torch::autograd::GraphTask::ExecInfo>;
+inline void check_captured_gradients(const std::shared_ptr<torch::autograd::Node>& node, const c10::Stream& here, const char* what,
+                                     const AskedNodes* asked = nullptr)
 {
     const auto captured = [&](const c10::Stream& stream) {
         if (stream == here) return true;
@@ -48,6 +53,11 @@ inline void check_captured_gradients(const std::shared_ptr<torch::autograd::Node
         const auto next = std::move(nodes.back());
         nodes.pop_back();
         if (!next || !seen.insert(next.get()).second) continue;
+        if (asked && !asked->empty())  // (empty: all that there are)
+        {
+            const auto info = asked->find(next.get());
+            if (info == asked->end() || !info->second.should_execute()) continue;
+        }
         const auto stream = next->stream();
         TORCH_CHECK(!stream.has_value() || captured(*stream), what, ": an eager graph of a tensor that is differentiated in this captured call still lives (on another stream): ",
                     "drop it before the capture, or detach");

@@ -2,6 +2,7 @@
 // calling the C ABI of include/vetrast.h. See point_render.h for the reference lines each piece mirrors.
 #include "point_render.h"
 #include "adamw.h"
+#include "calls.h"
 #include "entries.h"
 #include "vet_adapter.h"
 
@@ -485,6 +486,10 @@ torch::autograd::variable_list PointRender::backward(torch::autograd::AutogradCo
     NeuralRenderInfo* info   = info_value.toCustomClass<NeuralRenderInfo>().get();
     const int L              = info->num_layers;
     auto saved               = ctx->get_saved_variables();
+    if (capturing())
+        for (const auto& edge : torch::autograd::get_current_node()->next_edges())
+            check_captured_gradients(edge.function, c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(saved[0].device().index()).unwrap(), "PointRender",
+                                     torch::autograd::get_current_graph_task_exec_info());
     const bool has_dropout   = ctx->saved_data["has_dropout"].toBool();
     const bool has_index     = ctx->saved_data["has_index"].toBool();
     constexpr int kFixed     = 7;
