@@ -301,8 +301,8 @@ typedef struct vetrast_backward_args
 /* What every point gave to the pixels of a render: weight[i] = decay * weight[i] + the sum, over the views, layers and pixels in which a
  * fragment of point i was blended, of its weight there, the transmittance in front of it times its alpha (its confidence; with the 2x2
  * splat times the corner's weight; in FUZZY_BLEND its share of the bucket's). That is the derivative of the sum of all pixels of one
- * channel by the point's descriptor. Accumulated over renders it says which points a budget should keep (vetrast_select_kept).
- * Sums are formed in float32 in a fixed order, without atomics. No counterpart in the reference, which removes points by their
+ * channel by the point's descriptor; a point without a fragment adds nothing, whatever its confidence. Accumulated over renders it says which points a budget should keep (vetrast_select_kept).
+ * Sums are formed in float32 in a fixed order, without atomics, and kept so from call to call. No counterpart in the reference, which removes points by their
  * confidence alone (src/apps/train.cpp:727-741). */
 typedef struct vetrast_point_weights_args
 {

@@ -118,7 +118,7 @@ __device__ __forceinline__ void clear_bins(SelectRoom<THREADS>& room)
     __syncthreads();
 }
 
-// Scores that two thirds of a scene's points may share, as no view has seen them, are counted by the thread and not in LDS, where they would queue up at one address.
+// Scores that a third of a scene's points may share, as no view has seen them, are counted by the thread and not in LDS, where they would queue up at one address.
 __device__ __forceinline__ void count_key(uint32_t* bins, uint32_t& zeros, bool matches, uint32_t key, int digit)
 {
     zeros += matches && key == kZeroKey;
@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(THREADS) select_row_kernel(SelectPass a)
 
 // ---- rows of several workgroups: a launch for each digit, one that counts and one that gives places ---------------------------
 // A launch is the barrier between workgroups. Five passes over the scores, most of them from the last-level cache: 5.5 M take 34.6 us, of
-// which 10 are the first digit, 7 the counts, 11 the places and 7 launches that find nothing to do (45 where the budget does not end among zeros).
+// which 10 are the first digit, 7 the counts, 11 the places, 2 to clear, and 6 two launches that learn from the ones before that nothing is left to
+// count: 2 and 4.4, with the first piece of every workgroup loaded by then, which in the second is the whole row (45 in all where the budget does
+// not end among zeros).
 
 // Workgroups of 512: a row of 40 k entries takes 20.0 us of all launches, 64 rows of 131 k 48.5, one of 5.5 M 34.5 (with 1024 threads 23.8, 62 and
 // 34.8; with 256 19.9, 48 and 39). Three groups of four of a thread under way at once (5.5 M entries: with 2 7 us more).

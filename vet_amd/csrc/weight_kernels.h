@@ -5,7 +5,7 @@
 // points multiply it with their alpha and add up in a fixed order, so that results do not depend on the order of atomics. A fragment is one
 // scattered store; its alpha the point has at hand.
 //
-// These stores bound it, at 117 to 127 G a second: 1920x1080 with 2 M points has 4.6 M fragments, 36 us, beside 6.6 to clear the slots and 11 for
+// These stores bound it, at 117 to 127 G a second: 1920x1080 with 2 M points has 4.6 M fragments, 37 us, beside 6.7 to clear the slots and 11 for
 // the points; four 512x512 crops of the 2x2 splat have 9.0 M, 77 us, and the points 68, of which 27 to find out that no view sees a point. (A
 // point's four corners in one store, if they met on the chip, would take 22 us off the crops before the work of letting them meet. 20 k points:
 // two launches, 8 us.)
